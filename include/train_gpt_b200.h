@@ -216,6 +216,33 @@ int64_t tg_rmsnorm_bwd_static_max_scratch_bytes(void);
 int tg_rmsnorm_bwd_static(const void* x, const void* gamma, const void* g, float eps, void* dx,
                           void* dgamma, int64_t rows, int64_t cols, void* stream);
 
+/* ---- a block with a norm on both sides -------------------------------------------- */
+
+/* No counterpart in the reference.  The junction between two such blocks: the norm behind a block (branch is its output), a gate,
+ * the scaled residual add, and the norm before the next block, in one pass:
+ *   x_new = bf16(residual_scale * x + G * (branch * rsqrt(mean(branch^2) + eps) * post))
+ *   h     = bf16(x_new * rsqrt(mean(x_new^2) + eps) * pre), and its 1 x 128 e4m3 form (q, scales) as tg_quantize_rowwise's
+ * in float32 between the roundings.
+ *   x, branch, x_new, h [rows, cols] bf16, post, pre [cols] bf16, cols % 8 == 0, cols <= 8192 (else TG_ERR_TOO_LARGE)
+ *   gate     bf16: [cols] for TG_GATE_CHANNEL, [rows] for TG_GATE_TOKEN; ignored for TG_GATE_NONE (G = 1)
+ *   q, scales both or neither (then h is required); cols % 128 == 0 with them.  h may be NULL with them.
+ *   x_new may be the buffer of x or of branch. */
+#define TG_GATE_NONE 0
+#define TG_GATE_CHANNEL 1
+#define TG_GATE_TOKEN 2
+int tg_sandwich_norm_fwd(const void* x, const void* branch, const void* post, const void* pre, const void* gate, int gate_kind,
+                         float residual_scale, float eps, void* x_new, void* h, void* q, float* scales, int64_t rows, int64_t cols,
+                         void* stream);
+
+/* Its backward pass from the gradients of x_new and of h (either may be NULL: zero), both factors recomputed from x_new and branch.
+ *   dx, dbranch [rows, cols] bf16; dpost, dpre [cols] bf16; dgate like gate, or NULL where it is not wanted.  Outputs overlap no input.
+ *   scratch  tg_sandwich_norm_bwd_scratch_bytes(rows, cols) bytes, 16-byte aligned, contents undefined on entry and exit.
+ * Deterministic (no atomics). */
+int64_t tg_sandwich_norm_bwd_scratch_bytes(int64_t rows, int64_t cols);
+int tg_sandwich_norm_bwd(const void* x_new, const void* branch, const void* post, const void* pre, const void* gate, int gate_kind,
+                         float residual_scale, float eps, const void* g_new, const void* g_h, void* dx, void* dbranch, void* dpost,
+                         void* dpre, void* dgate, void* scratch, int64_t rows, int64_t cols, void* stream);
+
 /* ---- capped-logit cross-entropy --------------------------------------------------- */
 
 /* train-gpt model.py:97 (`cap * tanh(logits / cap)`, bf16, every op rounding) followed by
@@ -240,6 +267,47 @@ int tg_softcap_ce_fwd(const void* logits, const int32_t* targets, float cap, voi
 int tg_softcap_ce_bwd(const void* tanh_in, const int32_t* targets, const float* lse, const float* gscale,
                       float cap, void* dlogits, int64_t rows, int64_t vocab, int64_t ld_tanh, int64_t ld_d,
                       void* stream);
+
+/* ---- distillation from a teacher's top logits --------------------------------------- */
+
+/* No counterpart in the reference (nor have the two below).  With z = cap * tanh(x / cap) of a row's logits x (train-gpt
+ * model.py:97, here in float32 throughout), the k largest logits in descending order, equal ones by index (-0 is 0, a NaN is
+ * above all), their log-probabilities at a temperature and the log of the probability that all others share:
+ *   ids      int32 [rows, k]
+ *   logp     float32 [rows, k]: z[id] / T - log sum_i exp(z_i / T)
+ *   log_rest float32 [rows]: log sum_{i not in ids} exp(z_i / T) - log sum_i exp(z_i / T); -inf if k == vocab
+ *   logits   bf16 [rows, ld], row r at logits + r * ld, any alignment of 2 bytes.  The 16-byte pieces of memory that hold
+ *            elements of a row are read whole.
+ *   1 <= k <= vocab, k <= TG_TOP_LOGITS_MAX and vocab <= 2^20 (else TG_ERR_TOO_LARGE); 2^-10 <= cap <= 64, 0 < T <= 1024,
+ *   cap / T <= 64 (else TG_ERR_SHAPE): sums of exp(z / T) are taken without a running maximum.
+ * Results do not depend on scheduling. */
+#define TG_TOP_LOGITS_MAX 256
+int tg_top_logits(const void* logits, float cap, float temperature, int32_t* ids, float* logp, float* log_rest, int64_t rows,
+                  int64_t vocab, int64_t ld, int k, void* stream);
+
+/* A student's loss against a teacher's top logits, and its gradient, from one read of the student's logits.  Per row, with
+ * s = z / T, q = softmax(s), q1 = softmax(z), p_j = exp(logp_j), K the named logits and q_R = sum_{i not in K} q_i:
+ *   weight T^2 [ sum_j p_j (logp_j - log q[id_j]) + p_R (log_rest - log q_R) ] + (1 - weight) (-log q1[target])
+ * Terms whose probability is 0 are 0.  An id outside [0, vocab) is no entry (its logp is not read) and a target outside it no
+ * target: rows of padding have ids and targets of -1, and log_rest 0.  An id that occurs twice is one logit with both
+ * probabilities.  The probabilities of a row need not sum to 1. */
+typedef struct tg_distill_args {
+  const void* logits;      /* bf16 [rows, ld], as tg_top_logits takes them                                        */
+  const void* ids;         /* int32 [rows, k], or int64 with ids_64; k may be 0                                    */
+  const float* logp;       /* [rows, k]                                                                            */
+  const float* log_rest;   /* [rows], or NULL: p_R = 0                                                             */
+  const void* targets;     /* int32 [rows], or int64 with targets_64, or NULL: no such term                        */
+  int ids_64, targets_64;
+  float cap, temperature, weight;   /* limits of cap and T as in tg_top_logits; 0 <= weight <= 1                   */
+  void* dlogits;           /* bf16 [rows, ld] or NULL: gscale / rows * d(sum of the rows' losses)/dlogits; not the logits'
+                              buffer, and as far from a 16-byte boundary as they are (else TG_ERR_ALIGN)           */
+  const float* gscale;     /* device float or NULL for 1                                                           */
+  int only_if_scaled;      /* the launch does nothing where *gscale is 1                                           */
+  float* row_loss;         /* [rows] or NULL                                                                       */
+  int64_t rows, vocab, ld;
+  int k;                   /* <= TG_TOP_LOGITS_MAX                                                                 */
+} tg_distill_args;
+int tg_softcap_distill(const tg_distill_args* args, void* stream);
 
 /* ---- optimiser step --------------------------------------------------------------- */
 

@@ -34,6 +34,15 @@ class GemmArgs(C.Structure):
     ]
 
 
+class DistillArgs(C.Structure):
+    """struct tg_distill_args"""
+    _fields_ = [
+        ("logits", _p), ("ids", _p), ("logp", _p), ("log_rest", _p), ("targets", _p), ("ids_64", _i), ("targets_64", _i),
+        ("cap", _f), ("temperature", _f), ("weight", _f), ("dlogits", _p), ("gscale", _p), ("only_if_scaled", _i), ("row_loss", _p),
+        ("rows", _i64), ("vocab", _i64), ("ld", _i64), ("k", _i),
+    ]
+
+
 # every symbol include/train_gpt_b200.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "tg_version": (_i, []),
@@ -55,8 +64,13 @@ SYMBOLS = {
     "tg_rmsnorm_bwd_add": (_i, [_p, _p, _p, _p, _f, _p, _p, _p, _i64, _i64, _p]),
     "tg_rmsnorm_bwd_static_max_scratch_bytes": (_i64, []),
     "tg_rmsnorm_bwd_static": (_i, [_p, _p, _p, _f, _p, _p, _i64, _i64, _p]),
+    "tg_sandwich_norm_fwd": (_i, [_p, _p, _p, _p, _p, _i, _f, _f, _p, _p, _p, _p, _i64, _i64, _p]),
+    "tg_sandwich_norm_bwd_scratch_bytes": (_i64, [_i64, _i64]),
+    "tg_sandwich_norm_bwd": (_i, [_p, _p, _p, _p, _p, _i, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _p]),
     "tg_softcap_ce_fwd": (_i, [_p, _p, _f, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "tg_softcap_ce_bwd": (_i, [_p, _p, _p, _p, _f, _p, _i64, _i64, _i64, _i64, _p]),
+    "tg_top_logits": (_i, [_p, _f, _f, _p, _p, _p, _i64, _i64, _i64, _i, _p]),
+    "tg_softcap_distill": (_i, [C.POINTER(DistillArgs), _p]),
     "tg_sumsq_scratch_bytes": (_i64, []),
     "tg_sumsq_bf16": (_i, [_p, _i64, _p, _p, _p]),
     "tg_adamw_bf16": (_i, [_p, _p, _p, _p, _i64, _f, _f, _f, _f, _f, _p, _p, _p]),

@@ -13,6 +13,7 @@
 #include <dlfcn.h>
 #include <torch/csrc/autograd/engine.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
@@ -260,7 +261,242 @@ Pair rmsnorm_bwd(const Tensor& x_, const Tensor& gamma_, const Tensor& g_, doubl
   return {dx, dgamma};
 }
 
+// contiguous, and at a 16-byte boundary
+Tensor need16(const Tensor& t_, at::ScalarType dt, const char* name) {
+  const Tensor t = need(t_, dt, name);
+  return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0 ? t : t.clone();
+}
+void need_device(const Tensor& t, const Tensor& like, const char* name) {
+  if (t.device() != like.device()) throw py::value_error(cat(name, " is on ", t.device().str(), ", not on ", like.device().str()));
+}
+
+// The arguments that both directions of the junction take.
+struct Junction {
+  Tensor y, post, pre, gate;
+  int kind = TG_GATE_NONE;
+  int64_t d = 0, rows = 0;
+};
+Junction junction(const Tensor& x, const char* x_name, const Tensor& branch, const Tensor& post, const Tensor& pre, const std::optional<Tensor>& gate) {
+  Junction j;
+  if (x.dim() == 0) throw py::value_error(cat(x_name, " must have at least one dimension"));
+  j.d = x.size(-1);
+  if (branch.sizes() != x.sizes()) throw py::value_error(cat(x_name, " shape ", x.sizes(), " != branch shape ", branch.sizes()));
+  need_gamma(post, j.d);
+  need_gamma(pre, j.d);
+  if (j.d % 8 || j.d == 0 || j.d > 8192) throw py::value_error(cat("D=", j.d, " must be a multiple of 8 and at most 8192"));
+  if (gate) {
+    auto per_token = with_last(x, 1);
+    if (gate->dim() == 1 && gate->size(0) == j.d) j.kind = TG_GATE_CHANNEL;
+    else if (gate->sizes() == at::IntArrayRef(per_token)) j.kind = TG_GATE_TOKEN;
+    else throw py::value_error(cat("gate shape ", gate->sizes(), " is neither ", at::IntArrayRef({j.d}), " (per channel) nor ", at::IntArrayRef(per_token), " (per token)"));
+  }
+  j.y = need16(branch, at::kBFloat16, "branch");
+  j.post = need16(post, at::kBFloat16, "post_scale");
+  j.pre = need16(pre, at::kBFloat16, "scale");
+  if (gate) j.gate = need16(*gate, at::kBFloat16, "gate");
+  const std::pair<const Tensor*, const char*> all[] = {{&j.y, "branch"}, {&j.post, "post_scale"}, {&j.pre, "scale"}, {&j.gate, "gate"}};
+  for (const auto& [t, n] : all)
+    if (t->defined()) need_device(*t, x, n);
+  j.rows = x.numel() / j.d;
+  return j;
+}
+
+struct Sandwich {
+  Tensor x_new, h, q, s;
+};
+
+Sandwich sandwich_norm_fwd(const Tensor& x_, const Tensor& branch, const Tensor& post, const Tensor& pre, double eps, const std::optional<Tensor>& gate,
+                           double residual_scale, bool want_h, bool want_q) {
+  const Junction j = junction(x_, "x", branch, post, pre, gate);
+  if (want_q) need_tiles(j.d);
+  const Tensor x = need16(x_, at::kBFloat16, "x");
+  if (!want_q && !want_h) throw py::value_error("nothing to compute: neither the quantised nor the bf16 output is wanted");
+  const c10::cuda::CUDAGuard guard(x.device());
+  Sandwich o;
+  o.x_new = empty_as(x);
+  if (want_h) o.h = empty_as(x);
+  if (want_q) {
+    o.q = empty(x.sizes(), kF8, x);
+    o.s = empty(with_last(x, j.d / kTile), at::kFloat, x);
+  }
+  if (j.rows == 0) return o;
+  check(api.tg_sandwich_norm_fwd(ptr(x), ptr(j.y), ptr(j.post), ptr(j.pre), ptr(j.gate), j.kind, float(residual_scale), float(eps), ptr(o.x_new),
+                                 ptr(o.h), ptr(o.q), fptr(o.s), j.rows, j.d, cur_stream()),
+        "tg_sandwich_norm_fwd");
+  return o;
+}
+
+// dx, dbranch, dpost, dpre, dgate (undefined without a gate); either gradient may be undefined: zero
+std::array<Tensor, 5> sandwich_norm_bwd(const Tensor& x_new_, const Tensor& branch, const Tensor& post, const Tensor& pre, double eps,
+                                        const Tensor& g_new_, const Tensor& g_h_, const std::optional<Tensor>& gate, double residual_scale) {
+  const Junction j = junction(x_new_, "x_new", branch, post, pre, gate);
+  const Tensor x_new = need16(x_new_, at::kBFloat16, "x_new");
+  auto gradient = [&](const Tensor& g, const char* name) {
+    if (!g.defined()) return g;
+    if (g.sizes() != x_new.sizes()) throw py::value_error(cat(name, " and x_new shapes differ"));
+    need_device(g, x_new, name);
+    return need16(g, at::kBFloat16, name);
+  };
+  const Tensor g_new = gradient(g_new_, "g_new"), g_h = gradient(g_h_, "g_h");
+  const c10::cuda::CUDAGuard guard(x_new.device());
+  std::array<Tensor, 5> out = {empty_as(x_new), empty_as(x_new), empty({j.d}, at::kBFloat16, x_new), empty({j.d}, at::kBFloat16, x_new), Tensor()};
+  if (j.gate.defined()) out[4] = empty_as(j.gate);
+  Tensor scratch = empty({std::max<int64_t>(api.tg_sandwich_norm_bwd_scratch_bytes(j.rows, j.d), 16)}, at::kByte, x_new);
+  check(api.tg_sandwich_norm_bwd(ptr(x_new), ptr(j.y), ptr(j.post), ptr(j.pre), ptr(j.gate), j.kind, float(residual_scale), float(eps), ptr(g_new),
+                                 ptr(g_h), ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(out[3]), ptr(out[4]), ptr(scratch), j.rows, j.d, cur_stream()),
+        "tg_sandwich_norm_bwd");
+  return out;
+}
+
 // ---- loss ---------------------------------------------------------------------------------------------------------
+
+// Logits as rows of one pitch: as they lie where the last axis has unit stride and the others collapse, copied otherwise.
+struct LogitRows {
+  Tensor t;
+  int64_t rows = 0, vocab = 0, ld = 0;
+};
+void need_vocabulary(const Tensor& logits) {
+  if (logits.dim() == 0) throw py::value_error("logits must have at least one dimension");
+  if (logits.size(-1) == 0) throw py::value_error("logits of no vocabulary");
+}
+LogitRows logit_rows(const Tensor& logits) {
+  if (!logits.is_cuda()) throw std::runtime_error("logits must be a CUDA tensor (there is no CPU path)");
+  if (logits.scalar_type() != at::kBFloat16) throw py::type_error(cat("logits must be torch.bfloat16, got ", dtype_name(logits.scalar_type())));
+  LogitRows r;
+  r.vocab = logits.size(-1);
+  r.rows = logits.numel() / r.vocab;
+  r.t = logits;
+  r.ld = r.vocab;
+  if (r.rows == 0 || logits.is_contiguous()) return r;
+  bool lies = logits.stride(-1) == 1;
+  int64_t pitch = 0, next = 0;                 // of the rows; what the next axis outwards has to step by
+  for (int64_t i = logits.dim() - 2; i >= 0; --i) {
+    if (logits.size(i) == 1) continue;
+    if (pitch == 0) pitch = logits.stride(i);
+    else lies = lies && logits.stride(i) == next;
+    next = logits.stride(i) * logits.size(i);
+  }
+  if (lies && (pitch >= r.vocab || pitch == 0)) r.ld = std::max(pitch, r.vocab);
+  else r.t = logits.contiguous();
+  return r;
+}
+
+void need_temperature(double cap, double temperature) {
+  if (!(cap >= 0x1p-10 && cap <= 64.0)) throw py::value_error(cat("cap=", cap, " must be between 2^-10 and 64"));
+  if (!(temperature > 0 && temperature <= 1024.0 && cap <= 64.0 * temperature))
+    throw py::value_error(cat("temperature=", temperature, " must be positive, at most 1024 and at least cap / 64"));
+}
+void need_top(int64_t k, int64_t vocab) {
+  if (k > TG_TOP_LOGITS_MAX) throw py::value_error(cat("k=", k, " must be at most ", TG_TOP_LOGITS_MAX));
+  if (vocab > 1 << 20) throw py::value_error(cat("vocabulary of ", vocab, " must be at most ", 1 << 20));
+}
+
+std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& logits, double cap, int64_t k, double temperature) {
+  need_vocabulary(logits);
+  need_temperature(cap, temperature);
+  if (k < 1 || k > logits.size(-1)) throw py::value_error(cat("k=", k, " must be between 1 and the vocabulary's ", logits.size(-1)));
+  need_top(k, logits.size(-1));
+  const LogitRows x = logit_rows(logits);
+  const c10::cuda::CUDAGuard guard(x.t.device());
+  Tensor ids = empty(with_last(logits, k), at::kInt, x.t), logp = empty(with_last(logits, k), at::kFloat, x.t);
+  Tensor rest = empty(logits.sizes().slice(0, logits.dim() - 1), at::kFloat, x.t);
+  if (x.rows == 0) return {ids, logp, rest};
+  check(api.tg_top_logits(ptr(x.t), float(cap), float(temperature), static_cast<int32_t*>(ptr(ids)), fptr(logp), fptr(rest), x.rows, x.vocab, x.ld,
+                          int(k), cur_stream()),
+        "tg_top_logits");
+  return {ids, logp, rest};
+}
+
+// The student's loss: what both of its directions are called with.
+struct Distill {
+  LogitRows x;
+  Tensor ids, logp, log_rest, targets;
+  double cap = 0, temperature = 1, weight = 1;
+
+  // the rows' losses into `row_loss` and the gradient into `d` (like x.t, of its pitch), where they are defined
+  void run(const Tensor& d, const Tensor& gscale, bool only_if_scaled, const Tensor& row_loss) const {
+    tg_distill_args a = {};
+    a.logits = ptr(x.t);
+    a.ids = ptr(ids);
+    a.logp = fptr(logp);
+    a.log_rest = fptr(log_rest);
+    a.targets = ptr(targets);
+    a.ids_64 = ids.scalar_type() == at::kLong;
+    a.targets_64 = targets.defined() && targets.scalar_type() == at::kLong;
+    a.cap = float(cap);
+    a.temperature = float(temperature);
+    a.weight = float(weight);
+    a.dlogits = ptr(d);
+    a.gscale = fptr(gscale);
+    a.only_if_scaled = only_if_scaled;
+    a.row_loss = fptr(row_loss);
+    a.rows = x.rows;
+    a.vocab = x.vocab;
+    a.ld = x.ld;
+    a.k = int(ids.size(-1));
+    check(api.tg_softcap_distill(&a, cur_stream()), "tg_softcap_distill");
+  }
+  // memory for the gradient: rows of the logits' pitch, seen in the logits' shape
+  Tensor gradient(at::IntArrayRef shape) const {
+    if (x.ld == x.vocab) return empty(shape, at::kBFloat16, x.t);
+    std::vector<int64_t> strides(shape.size());
+    int64_t step = x.ld;
+    for (int64_t i = int64_t(shape.size()) - 2; i >= 0; --i) {
+      strides[size_t(i)] = step;
+      step *= shape[size_t(i)];
+    }
+    strides.back() = 1;
+    return empty({x.rows, x.ld}, at::kBFloat16, x.t).as_strided(shape, strides);
+  }
+};
+
+Tensor need_index(const Tensor& t, const char* name) {
+  if (!t.is_cuda()) throw std::runtime_error(cat(name, " must be a CUDA tensor (there is no CPU path)"));
+  if (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong)
+    throw py::type_error(cat(name, " must be torch.int32 or torch.int64, got ", dtype_name(t.scalar_type())));
+  return t.contiguous();
+}
+
+Distill distill_args(const Tensor& logits, const Tensor& ids, const Tensor& logp, const std::optional<Tensor>& log_rest, double cap,
+                     const std::optional<Tensor>& targets, double temperature, double weight) {
+  need_vocabulary(logits);
+  const auto leading = logits.sizes().slice(0, logits.dim() - 1);
+  if (ids.dim() != logits.dim() || ids.sizes().slice(0, ids.dim() - 1) != leading)
+    throw py::value_error(cat("logits ", logits.sizes(), " and teacher ids ", ids.sizes(), " do not match"));
+  if (logp.sizes() != ids.sizes()) throw py::value_error(cat("teacher logp ", logp.sizes(), " and ids ", ids.sizes(), " do not match"));
+  if (log_rest && log_rest->sizes() != leading)
+    throw py::value_error(cat("logits ", logits.sizes(), " and teacher log_rest ", log_rest->sizes(), " do not match"));
+  if (targets && targets->sizes() != leading)
+    throw py::value_error(cat("logits ", logits.sizes(), " and target_ids ", targets->sizes(), " do not match"));
+  need_temperature(cap, temperature);
+  if (!(weight >= 0.0 && weight <= 1.0)) throw py::value_error(cat("weight=", weight, " must be between 0 and 1"));
+  if (weight < 1.0 && !targets) throw py::value_error("weight below 1 needs target_ids");
+  need_top(ids.size(-1), logits.size(-1));
+  Distill a;
+  a.x = logit_rows(logits);
+  a.ids = need_index(ids, "teacher ids");
+  a.logp = need(logp, at::kFloat, "teacher logp");
+  if (log_rest) a.log_rest = need(*log_rest, at::kFloat, "teacher log_rest");
+  if (targets) a.targets = need_index(*targets, "target_ids");
+  const std::pair<const Tensor*, const char*> all[] = {{&a.ids, "teacher ids"}, {&a.logp, "teacher logp"}, {&a.log_rest, "teacher log_rest"}, {&a.targets, "target_ids"}};
+  for (const auto& [t, n] : all)
+    if (t->defined()) need_device(*t, logits, n);
+  a.cap = cap;
+  a.temperature = temperature;
+  a.weight = weight;
+  return a;
+}
+
+std::pair<Tensor, Tensor> softcap_distill(const Tensor& logits, const Tensor& ids, const Tensor& logp, const std::optional<Tensor>& log_rest, double cap,
+                                          const std::optional<Tensor>& targets, double temperature, double weight, bool want_grad) {
+  Distill a = distill_args(logits, ids, logp, log_rest, cap, targets, temperature, weight);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  if (want_grad && (reinterpret_cast<uintptr_t>(ptr(a.x.t)) & 15u)) a.x = logit_rows(a.x.t.clone(at::MemoryFormat::Contiguous));
+  Tensor row_loss = empty(logits.sizes().slice(0, logits.dim() - 1), at::kFloat, logits), d;
+  if (want_grad) d = a.gradient(logits.sizes());
+  if (a.x.rows > 0) a.run(d, Tensor(), false, row_loss);
+  return {row_loss, d};
+}
 
 std::tuple<Tensor, Tensor, Tensor> softcap_ce_fwd(const Tensor& logits_, const Tensor& targets, double cap, bool want_tanh) {
   Tensor logits = need(logits_, at::kBFloat16, "logits");
@@ -911,6 +1147,138 @@ Tensor capped_cross_entropy(const Tensor& logits_, const Tensor& target_ids, dou
   return loss;
 }
 
+// What a node hands back where a second derivative could be asked for (create_graph): values whose own derivative is an error.
+variable_list once_differentiable(variable_list&& out, const Node& node, const char* what) {
+  if (!at::GradMode::is_enabled()) return std::move(out);
+  const std::string message = cat(what, " is differentiable once");
+  for (Tensor& t : out) {
+    if (!t.defined()) continue;
+    t = t.detach();
+    torch::autograd::set_history(t, std::make_shared<torch::autograd::Error>(message, torch::autograd::edge_list(node.next_edges())));
+  }
+  return std::move(out);
+}
+
+// The student's loss.  As capped_cross_entropy: the forward makes the gradient for an upstream gradient of 1, another one is
+// seen on the device and the gradient made again from the inputs with it (scaled, where those were overwritten in between).
+struct CappedDistillationBackward : public Node {
+  Distill args;
+  Tensor d;
+  std::vector<int64_t> shape;
+  std::vector<uint32_t> versions;
+  bool given = false;                        // `d` has been handed out: it is no longer this node's own
+  std::string name() const override { return "CappedDistillationBackward"; }
+  std::vector<uint32_t> versions_now() const {
+    std::vector<uint32_t> v;
+    for (const Tensor* t : {&args.x.t, &args.ids, &args.logp, &args.log_rest, &args.targets})
+      if (t->defined()) v.push_back(t->_version());
+    return v;
+  }
+  void release_variables() override {
+    args = Distill();
+    d = Tensor();
+  }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(1);
+    if (!grads[0].defined()) return out;
+    if (!d.defined()) backward_twice();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor g = grads[0].to(at::kFloat).contiguous();
+      const c10::cuda::CUDAGuard guard(d.device());
+      if (versions_now() != versions) {
+        out[0] = (d * g).to(at::kBFloat16);
+      } else {
+        const bool again = given;
+        if (again) d = args.gradient(shape);
+        if (args.x.rows > 0) args.run(d, g, !again, Tensor());
+        given = true;
+        out[0] = d;
+      }
+    }
+    return once_differentiable(std::move(out), *this, "capped_distillation");
+  }
+};
+
+Tensor capped_distillation(const Tensor& logits, const Tensor& ids, const Tensor& logp, const std::optional<Tensor>& log_rest, double cap,
+                           const std::optional<Tensor>& targets, double temperature, double weight) {
+  Distill a = distill_args(logits, ids, logp, log_rest, cap, targets, temperature, weight);
+  const bool track = at::GradMode::is_enabled() && logits.requires_grad();
+  const c10::cuda::CUDAGuard guard(logits.device());
+  Tensor loss, d;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    if (track && (reinterpret_cast<uintptr_t>(ptr(a.x.t)) & 15u)) a.x = logit_rows(a.x.t.clone(at::MemoryFormat::Contiguous));
+    if (track) d = a.gradient(logits.sizes());
+    const Tensor row_loss = empty({a.x.rows}, at::kFloat, logits);
+    if (a.x.rows > 0) {
+      a.run(d, Tensor(), false, row_loss);
+      loss = mean_of(row_loss);
+    } else {
+      loss = row_loss.mean();
+    }
+  }
+  if (!track) return loss;
+  std::shared_ptr<CappedDistillationBackward> node(new CappedDistillationBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(logits));
+  for (Tensor* t : {&a.x.t, &a.ids, &a.logp, &a.log_rest, &a.targets})
+    if (t->defined()) *t = t->detach();      // (shares the version counter)
+  node->args = a;
+  node->versions = node->versions_now();
+  node->d = d;
+  node->shape.assign(logits.sizes().begin(), logits.sizes().end());
+  torch::autograd::set_history(loss, node);
+  return loss;
+}
+
+struct SandwichNormBackward : public Node {
+  SavedVariable x_new, branch, post, pre, gate;
+  bool has_gate = false;
+  double eps = 0, residual_scale = 1;
+  std::string name() const override { return "SandwichNormBackward"; }
+  void release_variables() override {
+    for (SavedVariable* v : {&x_new, &branch, &post, &pre, &gate}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(5);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const Tensor x = x_new.unpack(shared_from_this()), y = branch.unpack(), a = post.unpack(), b = pre.unpack();
+    const std::optional<Tensor> g = has_gate ? std::optional<Tensor>(gate.unpack()) : std::nullopt;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto bf16 = [](const Tensor& t) { return t.defined() ? to(t, at::kBFloat16) : t; };
+      auto d = sandwich_norm_bwd(x, y, a, b, eps, bf16(grads[0]), bf16(grads[1]), g, residual_scale);
+      for (size_t i = 0; i < 5; ++i) out[i] = std::move(d[i]);
+    }
+    return once_differentiable(std::move(out), *this, "sandwich_norm");
+  }
+};
+
+Sandwich sandwich_norm(const Tensor& x, const Tensor& branch, const Tensor& post, const Tensor& pre, double eps, const std::optional<Tensor>& gate,
+                       double residual_scale, bool want_q) {
+  bool track = x.requires_grad() || branch.requires_grad() || post.requires_grad() || pre.requires_grad() || (gate && gate->requires_grad());
+  track = track && at::GradMode::is_enabled();
+  Sandwich o;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    o = sandwich_norm_fwd(x, branch, post, pre, eps, gate, residual_scale, true, want_q);
+  }
+  if (!track) return o;
+  std::shared_ptr<SandwichNormBackward> node(new SandwichNormBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(x, branch, post, pre, gate ? *gate : Tensor()));
+  node->branch = SavedVariable(branch, false);
+  node->post = SavedVariable(post, false);
+  node->pre = SavedVariable(pre, false);
+  node->has_gate = gate.has_value();
+  if (gate) node->gate = SavedVariable(*gate, false);
+  node->eps = eps;
+  node->residual_scale = residual_scale;
+  torch::autograd::set_history(o.x_new, node);
+  torch::autograd::set_history(o.h, node);
+  node->x_new = SavedVariable(o.x_new, true);
+  return o;
+}
+
 // ---- bindings -------------------------------------------------------------------------------------------------------
 
 Tensor or_none(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
@@ -943,6 +1311,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           return py::make_tuple(o.sum, o.q, o.s, o.y);
         });
   m.def("rmsnorm_bwd", &rmsnorm_bwd);
+  m.def("sandwich_norm_fwd", [](const Tensor& x, const Tensor& branch, const Tensor& post, const Tensor& pre, double eps, const std::optional<Tensor>& gate,
+                                double residual_scale, bool want_h, bool want_q) {
+    const Sandwich o = sandwich_norm_fwd(x, branch, post, pre, eps, gate, residual_scale, want_h, want_q);
+    return py::make_tuple(o.x_new, o.h, o.q, o.s);
+  });
+  m.def("sandwich_norm_bwd", [](const Tensor& x_new, const Tensor& branch, const Tensor& post, const Tensor& pre, double eps, const std::optional<Tensor>& g_new,
+                                const std::optional<Tensor>& g_h, const std::optional<Tensor>& gate, double residual_scale) {
+    const auto d = sandwich_norm_bwd(x_new, branch, post, pre, eps, or_none(g_new), or_none(g_h), gate, residual_scale);
+    return py::make_tuple(d[0], d[1], d[2], d[3], d[4]);
+  });
+  m.def("top_logits", &top_logits);
+  m.def("softcap_distill", &softcap_distill);
+  m.def("sandwich_norm", [](const Tensor& x, const Tensor& branch, const Tensor& post, const Tensor& pre, double eps, const std::optional<Tensor>& gate,
+                            double residual_scale, bool want_q) -> py::object {
+    const Sandwich o = sandwich_norm(x, branch, post, pre, eps, gate, residual_scale, want_q);
+    return want_q ? py::object(py::make_tuple(o.x_new, o.h, o.q, o.s)) : py::object(py::make_tuple(o.x_new, o.h));
+  });
+  m.def("capped_distillation", &capped_distillation);
   m.def("softcap_ce_fwd", &softcap_ce_fwd);
   m.def("softcap_ce_bwd", &softcap_ce_bwd);
   m.def("sumsq", &sumsq);

@@ -1,0 +1,570 @@
+// The junction between two blocks of a network whose blocks have a norm on both sides, as one kernel each way:
+//
+//     x' = bf16(alpha x + G (y * rsqrt(mean y^2 + eps) * post)),   h = bf16(x' * rsqrt(mean x'^2 + eps) * pre)
+//
+// y is the block's output, x the residual stream, G a gate per channel or per token (or 1), h what the next block reads -- in bf16 and,
+// where an FP8 linear reads it, in 1 x 128 e4m3 tiles (fp8.py:39-47 on the bf16 h).  x' is rounded before it is normalised: it is what the
+// stream keeps, and what the backward pass computes from.  All else is float32, rounded once.
+//
+// Backward, for the gradients g of x' and gh of h, with r and s the two norms' factors (r of x', s of y):
+//     a = gh pre,  d = g + r (a - x' r^2 mean(a x')),  dx = alpha d,  dpre = sum_rows r gh x'
+//     t = d post (gate per channel: times the gate),  dy = G s (t - y s^2 mean(t y)),  C = sum_rows G s d y
+//     dpost = C (times the gate per channel),  dgate per channel = C post,  per token = s sum_columns t y
+//
+// A pass of either is bound by memory (8 bytes an element forward, 12 backward), so each is one read of its inputs: rows are staged
+// through shared memory by cp.async, the next ones on their way while one is worked on.  Every lane reads only the 16-byte pieces that
+// it fetched itself, so the warps of a row meet only at its sums, of which there are two rounds.
+#include <algorithm>
+#include <atomic>
+
+#include "common.cuh"
+#include "host_api.h"
+#include "norm.cuh"
+
+namespace tg {
+
+// ---- N sums over a row at once; `red` holds N floats per warp of the block.  Two rounds a row with a buffer of their own each: a warp
+// that writes one of the next row has passed the other's barrier, which every warp of the row reaches after reading the first.
+template <int N, int WPR, int WARPS>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[WARPS], int warp, int lane) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+  if constexpr (WPR > 1) {
+    if (lane == 0) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) red[n][warp] = v[n];
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / WPR), "n"(WPR * 32) : "memory");   // this row's warps only
+    const int g0 = (warp / WPR) * WPR;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      v[n] = red[n][g0];
+#pragma unroll
+      for (int i = 1; i < WPR; ++i) v[n] += red[n][g0 + i];
+    }
+  }
+}
+
+struct SandwichVectors {
+  const __nv_bfloat16 *post, *pre, *gate;
+  int gate_kind;
+};
+
+// post (times the gate per channel) and pre, widened to float, in two planes each (columns 8i..8i+3 of every piece, then 8i+4..8i+7): a
+// warp's 16-byte reads of either plane are contiguous
+__device__ __forceinline__ void fill_planes(const SandwichVectors& v, float4* s_w, float4* s_pre, int pieces) {
+  for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
+    const uint4 a = reinterpret_cast<const uint4*>(v.post)[i], b = reinterpret_cast<const uint4*>(v.pre)[i];
+    float4 lo = make_float4(bf16lo(a.x), bf16hi(a.x), bf16lo(a.y), bf16hi(a.y));
+    float4 hi = make_float4(bf16lo(a.z), bf16hi(a.z), bf16lo(a.w), bf16hi(a.w));
+    if (v.gate_kind == TG_GATE_CHANNEL) {      // (a product of two bf16 values is exact)
+      const uint4 g = reinterpret_cast<const uint4*>(v.gate)[i];
+      lo = make_float4(lo.x * bf16lo(g.x), lo.y * bf16hi(g.x), lo.z * bf16lo(g.y), lo.w * bf16hi(g.y));
+      hi = make_float4(hi.x * bf16lo(g.z), hi.y * bf16hi(g.z), hi.z * bf16lo(g.w), hi.w * bf16hi(g.w));
+    }
+    s_w[i] = lo;
+    s_w[pieces + i] = hi;
+    s_pre[i] = make_float4(bf16lo(b.x), bf16hi(b.x), bf16lo(b.y), bf16hi(b.y));
+    s_pre[pieces + i] = make_float4(bf16lo(b.z), bf16hi(b.z), bf16lo(b.w), bf16hi(b.w));
+  }
+}
+__device__ __forceinline__ void plane8(const float4* s, int pieces, int piece, float2 (&v)[4]) {
+  const float4 a = s[piece], b = s[pieces + piece];
+  v[0] = make_float2(a.x, a.y);
+  v[1] = make_float2(a.z, a.w);
+  v[2] = make_float2(b.x, b.y);
+  v[3] = make_float2(b.z, b.w);
+}
+__device__ __forceinline__ void unpack8(const uint4& w, float2 (&v)[4]) {
+  v[0] = bf16x2_unpack(w.x);
+  v[1] = bf16x2_unpack(w.y);
+  v[2] = bf16x2_unpack(w.z);
+  v[3] = bf16x2_unpack(w.w);
+}
+__device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
+
+// ---- forward -----------------------------------------------------------------------------------------------------
+
+struct SandwichFwd {
+  const __nv_bfloat16 *x, *y;
+  SandwichVectors v;
+  float alpha, eps;
+  __nv_bfloat16 *x_new, *h;
+  uint8_t* q;
+  float* scales;
+  int64_t rows;
+  int cols;
+};
+
+// x' of a piece
+__device__ __forceinline__ uint4 junction8(const uint4& xw, const uint4& yw, const float2 (&w)[4], float alpha, float rg) {
+  float2 x[4], y[4];
+  unpack8(xw, x);
+  unpack8(yw, y);
+  uint4 o;
+  uint32_t* op = &o.x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 n = __fmul2_rn(__fmul2_rn(y[j], splat(rg)), w[j]);
+    const float2 t = __ffma2_rn(splat(alpha), x[j], n);
+    op[j] = pack_bf16x2(t.x, t.y);
+  }
+  return o;
+}
+__device__ __forceinline__ uint4 normed8(const uint4& xw, const float2 (&g)[4], float r) {
+  float2 x[4];
+  unpack8(xw, x);
+  uint4 o;
+  uint32_t* op = &o.x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 t = __fmul2_rn(__fmul2_rn(x[j], splat(r)), g[j]);
+    op[j] = pack_bf16x2(t.x, t.y);
+  }
+  return o;
+}
+
+constexpr int sw_fwd_warps(int wpr) { return wpr == 8 ? 16 : 8; }
+
+template <int NCHUNK, int WPR, bool FULL>
+__global__ void __launch_bounds__(sw_fwd_warps(WPR) * 32) sandwich_fwd_kernel(const SandwichFwd p) {
+  constexpr int WARPS = sw_fwd_warps(WPR), RPB = WARPS / WPR, kRowBytes = NCHUNK * 512, kSlotBytes = 2 * kRowBytes;
+  __shared__ float s_red[2][1][WARPS];
+  extern __shared__ float4 s_w[];              // planes of w and pre, then [warps][2][x row | y row]
+  const int cols = p.cols, pieces = cols / 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col_base = (warp % WPR) * (NCHUNK * 256) + lane * 8;
+  float4* s_pre = s_w + 2 * pieces;
+  const uint32_t slot0 = uint32_t(__cvta_generic_to_shared(s_w)) + uint32_t(cols) * 8u + uint32_t(warp) * 2u * kSlotBytes + uint32_t(lane) * 16u;
+  grid_trigger();
+  grid_wait();
+  fill_planes(p.v, s_w, s_pre, pieces);
+  __syncthreads();
+
+  const int64_t stride = int64_t(gridDim.x) * RPB;
+  int64_t row = int64_t(blockIdx.x) * RPB + warp / WPR;
+  auto prefetch = [&](int64_t r, int slot) {
+    if (r < p.rows) {
+#pragma unroll
+      for (int c = 0; c < NCHUNK; ++c) {
+        const int col = col_base + c * 256;
+        if (FULL || col < cols) {
+          cp_async16(slot0 + slot * kSlotBytes + c * 512, p.x + r * cols + col);
+          cp_async16(slot0 + slot * kSlotBytes + kRowBytes + c * 512, p.y + r * cols + col);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");   // an empty group keeps the wait count uniform
+  };
+  prefetch(row, 0);
+  for (int it = 0; row < p.rows; row += stride, ++it) {
+    const uint32_t base = slot0 + (it & 1) * kSlotBytes;
+    prefetch(row + stride, (it & 1) ^ 1);
+    const float gate = p.v.gate_kind == TG_GATE_TOKEN ? __bfloat162float(p.v.gate[row]) : 1.0f;
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    float part[NCHUNK];
+#pragma unroll
+    for (int c = 0; c < NCHUNK; ++c) part[c] = (FULL || col_base + c * 256 < cols) ? sumsq8(lds128(base + kRowBytes + c * 512)) : 0.f;
+    float ss[1] = {tree_sum(part)};
+    row_sums<1, WPR, WARPS>(ss, s_red[0], warp, lane);
+    const float rg = __frsqrt_rn(__fdiv_rn(ss[0], float(cols)) + p.eps) * gate;
+
+    uint4 xo[NCHUNK];
+#pragma unroll
+    for (int c = 0; c < NCHUNK; ++c) {
+      const int col = col_base + c * 256;
+      xo[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (FULL || col < cols) {
+        float2 w[4];
+        plane8(s_w, pieces, col >> 3, w);
+        xo[c] = junction8(lds128(base + c * 512), lds128(base + kRowBytes + c * 512), w, p.alpha, rg);
+        *reinterpret_cast<uint4*>(p.x_new + row * cols + col) = xo[c];
+      }
+      part[c] = sumsq8(xo[c]);
+    }
+    ss[0] = tree_sum(part);
+    row_sums<1, WPR, WARPS>(ss, s_red[1], warp, lane);
+    const float r = __frsqrt_rn(__fdiv_rn(ss[0], float(cols)) + p.eps);
+
+    constexpr int G = pow2_at_least(NCHUNK);
+    uint32_t amax_bits[G];
+#pragma unroll
+    for (int u = NCHUNK; u < G; ++u) amax_bits[u] = 0u;
+#pragma unroll
+    for (int c = 0; c < NCHUNK; ++c) {
+      const int col = col_base + c * 256;
+      amax_bits[c] = 0u;
+      if (FULL || col < cols) {
+        float2 g[4];
+        plane8(s_pre, pieces, col >> 3, g);
+        xo[c] = normed8(xo[c], g, r);
+        if (p.h != nullptr) *reinterpret_cast<uint4*>(p.h + row * cols + col) = xo[c];
+        amax_bits[c] = absmax8_h(xo[c]);
+      }
+    }
+    if (p.q == nullptr) continue;
+    float s[G], inv[G], s_mine;
+    bool fin;
+    tile_scales_own<G>(exchange_tile_amax<G>(amax_bits), s, inv, s_mine, fin);
+    {
+      const int j = lane & 15;
+      const int col = col_base - lane * 8 + j * 256 + (lane & 16) * 8;     // first column of the tile this lane computed
+      if (j < NCHUNK && (FULL || col < cols)) p.scales[row * (cols / kTile) + col / kTile] = s_mine;
+    }
+    uint8_t* qp = p.q + row * cols + col_base;
+#pragma unroll
+    for (int c = 0; c < NCHUNK; ++c)
+      if (FULL || col_base + c * 256 < cols) *reinterpret_cast<uint2*>(qp + c * 256) = fin ? quantize8_sr(xo[c], s[c], inv[c]) : quantize8(xo[c], s[c]);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// ---- backward ----------------------------------------------------------------------------------------------------
+
+struct SandwichBwd {
+  const __nv_bfloat16 *x_new, *y;
+  SandwichVectors v;
+  float alpha, eps;
+  const __nv_bfloat16 *g_new, *g_h;            // either may be NULL: zero
+  __nv_bfloat16 *dx, *dy, *dgate_token;
+  float* partial;                              // [blocks][2][cols]: sums of r gh x', and C
+  int64_t rows;
+  int cols;
+};
+
+constexpr int sw_bwd_warps(int) { return 8; }
+constexpr int kSwBwdSlots = 2;
+
+template <int NCHUNK, int WPR, bool FULL>
+__global__ void __launch_bounds__(sw_bwd_warps(WPR) * 32) sandwich_bwd_kernel(const SandwichBwd p) {
+  constexpr int WARPS = sw_bwd_warps(WPR), RPB = WARPS / WPR, SLOTS = kSwBwdSlots, kRowBytes = NCHUNK * 512, kSlotBytes = 4 * kRowBytes;
+  __shared__ float s_red3[3][WARPS], s_red1[1][WARPS];
+  extern __shared__ float4 s_w[];              // planes of w and pre, then [warps][slots][x' | y | g | gh]
+  const int cols = p.cols, pieces = cols / 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col_base = (warp % WPR) * (NCHUNK * 256) + lane * 8;
+  float4* s_pre = s_w + 2 * pieces;
+  const uint32_t slot0 = uint32_t(__cvta_generic_to_shared(s_w)) + uint32_t(cols) * 8u + uint32_t(warp) * SLOTS * kSlotBytes + uint32_t(lane) * 16u;
+  const float inv_d = __fdiv_rn(1.0f, float(cols));
+  const bool has_g = p.g_new != nullptr, has_h = p.g_h != nullptr, token = p.v.gate_kind == TG_GATE_TOKEN;
+  grid_wait();
+  fill_planes(p.v, s_w, s_pre, pieces);
+  __syncthreads();
+
+  float2 acc_p[NCHUNK][4], acc_c[NCHUNK][4];
+#pragma unroll
+  for (int c = 0; c < NCHUNK; ++c)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc_p[c][j] = acc_c[c][j] = splat(0.f);
+
+  const int64_t stride = int64_t(gridDim.x) * RPB;
+  int64_t row = int64_t(blockIdx.x) * RPB + warp / WPR;
+  auto prefetch = [&](int64_t r, int slot) {
+    if (r < p.rows) {
+      const uint32_t dst = slot0 + uint32_t(slot) * kSlotBytes;
+#pragma unroll
+      for (int c = 0; c < NCHUNK; ++c) {
+        const int col = col_base + c * 256;
+        if (FULL || col < cols) {
+          const int64_t at = r * cols + col;
+          cp_async16(dst + c * 512, p.x_new + at);
+          cp_async16(dst + kRowBytes + c * 512, p.y + at);
+          if (has_g) cp_async16(dst + 2 * kRowBytes + c * 512, p.g_new + at);
+          if (has_h) cp_async16(dst + 3 * kRowBytes + c * 512, p.g_h + at);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int s = 0; s < SLOTS - 1; ++s) prefetch(row + s * stride, s);
+  int slot = 0, slot_in = SLOTS - 1;
+  for (; row < p.rows; row += stride) {
+    const uint32_t xs = slot0 + uint32_t(slot) * kSlotBytes, ys = xs + kRowBytes, gs = ys + kRowBytes, hs = gs + kRowBytes;
+    prefetch(row + (SLOTS - 1) * stride, slot_in);    // into the slot that the previous row has left
+    const float gate = token ? __bfloat162float(p.v.gate[row]) : 1.0f;
+    asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 1) : "memory");
+    slot_in = slot;
+    if (++slot == SLOTS) slot = 0;
+
+    // ---- sums of x'^2, a x' and y^2
+    float sums[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < NCHUNK; ++c) {
+      const int col = col_base + c * 256;
+      if (!(FULL || col < cols)) continue;
+      const uint4 xw = lds128(xs + c * 512);
+      sums[0] += sumsq8(xw);
+      sums[2] += sumsq8(lds128(ys + c * 512));
+      if (has_h) {
+        float2 x[4], g[4], m[4];
+        unpack8(xw, x);
+        unpack8(lds128(hs + c * 512), g);
+        plane8(s_pre, pieces, col >> 3, m);
+        float2 t = splat(0.f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t = __ffma2_rn(__fmul2_rn(g[j], m[j]), x[j], t);
+        sums[1] += t.x + t.y;
+      }
+    }
+    row_sums<3, WPR, WARPS>(sums, s_red3, warp, lane);
+    const float r = __frsqrt_rn(__fmaf_rn(sums[0], inv_d, p.eps)), s = __frsqrt_rn(__fmaf_rn(sums[2], inv_d, p.eps));
+    const float nm = -(r * r) * (sums[1] * inv_d);    // d = g + r (a + x' nm)
+
+    // ---- d, dx, the sum of t y
+    float2 d[NCHUNK][4];
+    float sum4[1] = {0.f};
+#pragma unroll
+    for (int c = 0; c < NCHUNK; ++c) {
+      const int col = col_base + c * 256;
+      if (!(FULL || col < cols)) continue;
+      float2 x[4], y[4], g[4], gh[4], m[4];
+      unpack8(lds128(xs + c * 512), x);
+      unpack8(has_g ? lds128(gs + c * 512) : zero, g);
+      unpack8(has_h ? lds128(hs + c * 512) : zero, gh);
+      plane8(s_pre, pieces, col >> 3, m);
+      uint4 o;
+      uint32_t* op = &o.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = __fmul2_rn(gh[j], m[j]);
+        d[c][j] = __ffma2_rn(splat(r), __ffma2_rn(x[j], splat(nm), a), g[j]);
+        acc_p[c][j] = __ffma2_rn(__fmul2_rn(x[j], splat(r)), gh[j], acc_p[c][j]);
+        const float2 t = __fmul2_rn(d[c][j], splat(p.alpha));
+        op[j] = pack_bf16x2(t.x, t.y);
+      }
+      *reinterpret_cast<uint4*>(p.dx + row * cols + col) = o;
+      unpack8(lds128(ys + c * 512), y);
+      plane8(s_w, pieces, col >> 3, m);
+      float2 t = splat(0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t = __ffma2_rn(__fmul2_rn(d[c][j], m[j]), y[j], t);
+      sum4[0] += t.x + t.y;
+    }
+    row_sums<1, WPR, WARPS>(sum4, s_red1, warp, lane);
+    if (token && p.dgate_token != nullptr && lane == 0 && warp % WPR == 0) p.dgate_token[row] = __float2bfloat16_rn(s * sum4[0]);
+    const float gsr = gate * s, nm2 = -(s * s) * (sum4[0] * inv_d);
+
+    // ---- dy and C
+#pragma unroll
+    for (int c = 0; c < NCHUNK; ++c) {
+      const int col = col_base + c * 256;
+      if (!(FULL || col < cols)) continue;
+      float2 y[4], m[4];
+      unpack8(lds128(ys + c * 512), y);
+      plane8(s_w, pieces, col >> 3, m);
+      uint4 o;
+      uint32_t* op = &o.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc_c[c][j] = __ffma2_rn(__fmul2_rn(y[j], splat(gsr)), d[c][j], acc_c[c][j]);
+        const float2 t = __fmul2_rn(splat(gsr), __ffma2_rn(y[j], splat(nm2), __fmul2_rn(d[c][j], m[j])));
+        op[j] = pack_bf16x2(t.x, t.y);
+      }
+      *reinterpret_cast<uint4*>(p.dy + row * cols + col) = o;
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+  grid_trigger();          // the reduction's blocks may take the places of this kernel's as they leave
+  // the block's rows added up in order over the (now idle) planes, then published
+  __syncthreads();
+  float* s_sum = reinterpret_cast<float*>(s_w);
+  for (int i = threadIdx.x; i < 2 * cols; i += blockDim.x) s_sum[i] = 0.f;
+  __syncthreads();
+  for (int turn = 0; turn < RPB; ++turn) {
+    if (warp / WPR == turn) {
+#pragma unroll
+      for (int c = 0; c < NCHUNK; ++c) {
+        const int col = col_base + c * 256;
+        if (!(FULL || col < cols)) continue;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+          float4* dst = reinterpret_cast<float4*>(s_sum + which * cols + col);
+          float4 a = dst[0], b = dst[1];
+          const float2(&v)[4] = which ? acc_c[c] : acc_p[c];
+          a.x += v[0].x; a.y += v[0].y; a.z += v[1].x; a.w += v[1].y;
+          b.x += v[2].x; b.y += v[2].y; b.z += v[3].x; b.w += v[3].y;
+          dst[0] = a; dst[1] = b;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  float* out = p.partial + int64_t(blockIdx.x) * 2 * cols;
+  for (int i = threadIdx.x; i < 2 * cols; i += blockDim.x) out[i] = s_sum[i];
+}
+
+// Column sums of the blocks' partial ones, 32 columns a block, warp w those of blocks w, w + 32, ...: an order that the number of blocks
+// alone fixes.  dpre is the first sum; dpost and the gate's gradient come from the second.
+struct SandwichReduce {
+  const float* partial;
+  SandwichVectors v;
+  __nv_bfloat16 *dpost, *dpre, *dgate;
+  int blocks, cols;
+};
+__global__ void __launch_bounds__(1024) sandwich_reduce_kernel(const SandwichReduce p) {
+  __shared__ float s_part[2][32][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  grid_wait();
+  float a = 0.f, b = 0.f;
+  if (col < p.cols) {
+#pragma unroll 4
+    for (int i = warp; i < p.blocks; i += 32) {
+      const float* at = p.partial + int64_t(i) * 2 * p.cols + col;
+      a += __ldcg(at);
+      b += __ldcg(at + p.cols);
+    }
+  }
+  s_part[0][warp][lane] = a;
+  s_part[1][warp][lane] = b;
+  __syncthreads();
+  if (warp < 2 && col < p.cols) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) t += s_part[warp][w][lane];
+    if (warp == 0) {
+      p.dpre[col] = __float2bfloat16_rn(t);
+    } else {
+      const bool channel = p.v.gate_kind == TG_GATE_CHANNEL;
+      p.dpost[col] = __float2bfloat16_rn(channel ? t * __bfloat162float(p.v.gate[col]) : t);
+      if (channel && p.dgate != nullptr) p.dgate[col] = __float2bfloat16_rn(t * __bfloat162float(p.v.post[col]));
+    }
+  }
+}
+
+// ---- launches ----------------------------------------------------------------------------------------------------
+
+struct SandwichGeom {
+  int nchunk, wpr;
+};
+// 1, 2 or 4 pieces of 256 columns a warp up to 1024 columns, then two, four or eight warps with three or four each.
+static bool sandwich_geom(int64_t cols, SandwichGeom* g) {
+  if (cols <= 0 || cols > 8192) return false;
+  const int chunks = int((cols + 255) / 256);
+  g->wpr = chunks <= 4 ? 1 : chunks <= 8 ? 2 : chunks <= 16 ? 4 : 8;
+  g->nchunk = g->wpr == 1 ? pow2_at_least(chunks) : chunks <= 3 * g->wpr ? 3 : 4;
+  return true;
+}
+
+template <int NC, int WPR, bool FULL>
+static int launch_sandwich_fwd(const SandwichFwd& a, cudaStream_t st) {
+  static std::atomic<bool> done[64];
+  auto kern = sandwich_fwd_kernel<NC, WPR, FULL>;
+  constexpr int warps = sw_fwd_warps(WPR), stage = warps * 2 * NC * 1024, most = WPR * NC * 256 * 8 + stage;
+  static_assert(most + 1024 <= 227 * 1024, "row slots exceed shared memory");
+  if (int rc = allow_smem(kern, most, done)) return rc;
+  const int smem = a.cols * 8 + stage, per_sm = std::max(1, std::min((227 * 1024) / (smem + 1280), 3));
+  const int64_t need = (a.rows + warps / WPR - 1) / (warps / WPR);
+  const int blocks = int(std::min<int64_t>(need, int64_t(sm_count()) * per_sm));
+  TG_CUDA_CHECK(launch_early(kern, blocks, warps * 32, smem, st, a));
+  return TG_OK;
+}
+
+static int sandwich_bwd_blocks(int64_t rows, const SandwichGeom& g) {
+  const int rpb = sw_bwd_warps(g.wpr) / g.wpr;
+  return int(std::min<int64_t>((rows + rpb - 1) / rpb, sm_count()));
+}
+template <int NC, int WPR, bool FULL>
+static int launch_sandwich_bwd(const SandwichBwd& a, int blocks, cudaStream_t st) {
+  static std::atomic<bool> done[64];
+  auto kern = sandwich_bwd_kernel<NC, WPR, FULL>;
+  constexpr int warps = sw_bwd_warps(WPR), stage = warps * kSwBwdSlots * NC * 2048, most = WPR * NC * 256 * 8 + stage;
+  static_assert(most + 1024 <= 227 * 1024, "row slots exceed shared memory");
+  if (int rc = allow_smem(kern, most, done)) return rc;
+  TG_CUDA_CHECK(launch_early(kern, blocks, warps * 32, a.cols * 8 + stage, st, a));
+  return TG_OK;
+}
+
+#define TG_SANDWICH_CASES(CALL)                                                                    \
+  if (g.wpr == 1) {                                                                                \
+    if (g.nchunk == 1) return full ? CALL(1, 1, true) : CALL(1, 1, false);                         \
+    if (g.nchunk == 2) return full ? CALL(2, 1, true) : CALL(2, 1, false);                         \
+    return full ? CALL(4, 1, true) : CALL(4, 1, false);                                            \
+  }                                                                                                \
+  if (g.wpr == 2) {                                                                                \
+    if (g.nchunk == 3) return full ? CALL(3, 2, true) : CALL(3, 2, false);                         \
+    return full ? CALL(4, 2, true) : CALL(4, 2, false);                                            \
+  }                                                                                                \
+  if (g.wpr == 4) {                                                                                \
+    if (g.nchunk == 3) return full ? CALL(3, 4, true) : CALL(3, 4, false);                         \
+    return full ? CALL(4, 4, true) : CALL(4, 4, false);                                            \
+  }                                                                                                \
+  if (g.nchunk == 3) return full ? CALL(3, 8, true) : CALL(3, 8, false);                           \
+  return full ? CALL(4, 8, true) : CALL(4, 8, false);
+
+static int launch_fwd_case(const SandwichGeom& g, const SandwichFwd& a, cudaStream_t st) {
+  const bool full = a.cols == g.wpr * g.nchunk * 256;
+#define TG_CALL(N, W, F) launch_sandwich_fwd<N, W, F>(a, st)
+  TG_SANDWICH_CASES(TG_CALL)
+#undef TG_CALL
+}
+static int launch_bwd_case(const SandwichGeom& g, const SandwichBwd& a, int blocks, cudaStream_t st) {
+  const bool full = a.cols == g.wpr * g.nchunk * 256;
+#define TG_CALL(N, W, F) launch_sandwich_bwd<N, W, F>(a, blocks, st)
+  TG_SANDWICH_CASES(TG_CALL)
+#undef TG_CALL
+}
+
+static bool gate_ok(const void* gate, int kind) {
+  return kind == TG_GATE_NONE || ((kind == TG_GATE_CHANNEL || kind == TG_GATE_TOKEN) && gate != nullptr);
+}
+static bool gate_aligned(const void* gate, int kind) { return kind != TG_GATE_CHANNEL || aligned16(gate); }
+
+}  // namespace tg
+
+using namespace tg;
+
+extern "C" int tg_sandwich_norm_fwd(const void* x, const void* branch, const void* post, const void* pre, const void* gate, int gate_kind,
+                                    float residual_scale, float eps, void* x_new, void* h, void* q, float* scales, int64_t rows,
+                                    int64_t cols, void* stream) {
+  if (rows < 0 || cols <= 0 || cols % 8 != 0 || !gate_ok(gate, gate_kind) || post == nullptr || pre == nullptr || x_new == nullptr) return TG_ERR_SHAPE;
+  if ((q == nullptr) != (scales == nullptr) || (q == nullptr && h == nullptr) || (q != nullptr && cols % kTile != 0)) return TG_ERR_SHAPE;
+  SandwichGeom g;
+  if (!sandwich_geom(cols, &g)) return TG_ERR_TOO_LARGE;
+  if (rows == 0) return TG_OK;
+  if (!aligned16(x) || !aligned16(branch) || !aligned16(post) || !aligned16(pre) || !gate_aligned(gate, gate_kind) || !aligned16(x_new) ||
+      !aligned16(h) || !aligned16(q))
+    return TG_ERR_ALIGN;
+  if (int rc = check_arch()) return rc;
+  using B = const __nv_bfloat16*;
+  const SandwichFwd a = {B(x), B(branch), {B(post), B(pre), B(gate), gate_kind}, residual_scale, eps, static_cast<__nv_bfloat16*>(x_new),
+                         static_cast<__nv_bfloat16*>(h), static_cast<uint8_t*>(q), scales, rows, int(cols)};
+  return launch_fwd_case(g, a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int64_t tg_sandwich_norm_bwd_scratch_bytes(int64_t rows, int64_t cols) {
+  SandwichGeom g;
+  if (rows <= 0 || !sandwich_geom(cols, &g)) return 0;
+  return int64_t(sandwich_bwd_blocks(rows, g)) * 2 * cols * int64_t(sizeof(float));
+}
+
+extern "C" int tg_sandwich_norm_bwd(const void* x_new, const void* branch, const void* post, const void* pre, const void* gate, int gate_kind,
+                                    float residual_scale, float eps, const void* g_new, const void* g_h, void* dx, void* dbranch, void* dpost,
+                                    void* dpre, void* dgate, void* scratch, int64_t rows, int64_t cols, void* stream) {
+  if (rows < 0 || cols <= 0 || cols % 8 != 0 || !gate_ok(gate, gate_kind) || post == nullptr || pre == nullptr || dpost == nullptr || dpre == nullptr)
+    return TG_ERR_SHAPE;
+  SandwichGeom g;
+  if (!sandwich_geom(cols, &g)) return TG_ERR_TOO_LARGE;
+  if (!aligned16(x_new) || !aligned16(branch) || !aligned16(post) || !aligned16(pre) || !gate_aligned(gate, gate_kind) || !aligned16(g_new) ||
+      !aligned16(g_h) || !aligned16(dx) || !aligned16(dbranch) || !aligned16(scratch))
+    return TG_ERR_ALIGN;
+  if (int rc = check_arch()) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {
+    for (void* v : {dpost, dpre, gate_kind == TG_GATE_CHANNEL ? dgate : nullptr})
+      if (v != nullptr) TG_CUDA_CHECK(cudaMemsetAsync(v, 0, size_t(cols) * 2, st));
+    return TG_OK;
+  }
+  using B = const __nv_bfloat16*;
+  using M = __nv_bfloat16*;
+  const int blocks = sandwich_bwd_blocks(rows, g);
+  const SandwichVectors v = {B(post), B(pre), B(gate), gate_kind};
+  const SandwichBwd a = {B(x_new), B(branch), v, residual_scale, eps, B(g_new), B(g_h), M(dx), M(dbranch), gate_kind == TG_GATE_TOKEN ? M(dgate) : nullptr,
+                         static_cast<float*>(scratch), rows, int(cols)};
+  if (int rc = launch_bwd_case(g, a, blocks, st)) return rc;
+  const SandwichReduce red = {static_cast<const float*>(scratch), v, M(dpost), M(dpre), gate_kind == TG_GATE_CHANNEL ? M(dgate) : nullptr, blocks, int(cols)};
+  TG_CUDA_CHECK(launch_if_short(true, sandwich_reduce_kernel, dim3(unsigned((cols + 31) / 32)), 1024, 0, st, red));
+  return TG_OK;
+}

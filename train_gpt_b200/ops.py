@@ -113,6 +113,21 @@ def rmsnorm_bwd(x, gamma, g, eps: float, addend=None):
     return _host().rmsnorm_bwd(x, gamma, g, eps, addend)
 
 
+# ---- the junction of blocks with a norm on both sides -------------------------------------
+
+def sandwich_norm_fwd(x, branch, post_scale, scale, eps: float, gate=None, residual_scale: float = 1.0, want_h: bool = True, want_q: bool = False):
+    """x_new = bf16(residual_scale x + G rms_norm(branch, post_scale)), h = rms_norm(x_new, scale), one pass; G is 1, a gate
+    per channel (D,) or per token (..., 1).  Returns (x_new, h or None, q or None, scales or None), q and scales the 1x128
+    e4m3 form of h."""
+    return _host().sandwich_norm_fwd(x, branch, post_scale, scale, eps, gate, residual_scale, want_h, want_q)
+
+
+def sandwich_norm_bwd(x_new, branch, post_scale, scale, eps: float, g_new=None, g_h=None, gate=None, residual_scale: float = 1.0):
+    """From the gradients of x_new and h (None: zero) and the saved x_new and branch:
+    (dx, dbranch, dpost_scale, dscale, dgate or None), all bf16."""
+    return _host().sandwich_norm_bwd(x_new, branch, post_scale, scale, eps, g_new, g_h, gate, residual_scale)
+
+
 # ---- capped-logit cross-entropy -----------------------------------------------------------
 
 def softcap_ce_fwd(logits, targets, cap: float, want_tanh: bool = True):
@@ -125,6 +140,22 @@ def softcap_ce_bwd(th, targets, lse, gscale, cap: float, in_place: bool = False)
     """Gradient of mean(nll) w.r.t. the uncapped logits; `gscale` is a float32 device scalar
     (or None for 1).  in_place=True overwrites `th` with the gradient."""
     return _host().softcap_ce_bwd(th, targets, lse, gscale, cap, in_place)
+
+
+# ---- distillation from a teacher's top logits ---------------------------------------------
+
+TOP_LOGITS_MAX = 256     # the most logits of a row that top_logits keeps and softcap_distill takes
+
+
+def top_logits(logits, cap: float, k: int, temperature: float = 1.0):
+    """(ids int32 (..., k), logp f32 (..., k), log_rest f32 (...)); see losses.top_logits."""
+    return _host().top_logits(logits, cap, k, temperature)
+
+
+def softcap_distill(logits, ids, logp, log_rest, cap: float, targets=None, temperature: float = 1.0, weight: float = 1.0, want_grad: bool = True):
+    """(the rows' losses f32 (...), the gradient of their MEAN w.r.t. the uncapped logits, bf16 like logits, or None); see
+    losses.capped_distillation."""
+    return _host().softcap_distill(logits, ids, logp, log_rest, cap, targets, temperature, weight, want_grad)
 
 
 # ---- optimiser ------------------------------------------------------------------------------

@@ -38,6 +38,7 @@ FFI_TARGETS = (
     "TgQuantizeRowwise", "TgQuantizeColwise", "TgQuantizeBlock128", "TgQuantizeRowcol", "TgQuantizeRowcolInto",
     "TgActQuantizeRowcol", "TgActQuantizeRowcolBwd",
     "TgRmsnormFwd", "TgRmsnormQuantFwd", "TgAddRmsnormQuantFwd", "TgRmsnormBwd", "TgRmsnormBwdAdd", "TgRmsnormBwdStatic",
+    "TgSandwichNormFwd", "TgSandwichNormQuantFwd", "TgSandwichNormBwd", "TgTopLogits", "TgSoftcapDistill",
     "TgSoftcapCeFwd", "TgSoftcapCeBwd", "TgSumsqBf16", "TgAdamwBf16",
     "TgGemmFwd", "TgGemmDgrad", "TgGemmWgrad",
 )

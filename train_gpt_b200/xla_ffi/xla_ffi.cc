@@ -33,6 +33,7 @@ using U32 = ffi::Buffer<ffi::U32>;
 using RBF16 = ffi::ResultBuffer<ffi::BF16>;
 using RF8 = ffi::ResultBuffer<ffi::F8E4M3FN>;
 using RF32 = ffi::ResultBuffer<ffi::F32>;
+using RS32 = ffi::ResultBuffer<ffi::S32>;
 using RU8 = ffi::ResultBuffer<ffi::U8>;
 using RU32 = ffi::ResultBuffer<ffi::U32>;
 
@@ -211,6 +212,74 @@ ffi::Error SoftcapCeBwd(cudaStream_t s, BF16 tanh_in, S32 targets, F32 lse, F32 
                "tg_softcap_ce_bwd");
 }
 
+// ---- the junction of blocks with a norm on both sides (no counterpart) -----------------------------
+
+// gate_kind: TG_GATE_NONE (pass any bf16 buffer), TG_GATE_CHANNEL (cols,) or TG_GATE_TOKEN (rows,)
+ffi::Error SandwichNormFwd(cudaStream_t s, BF16 x, BF16 branch, BF16 post, BF16 pre, BF16 gate, RBF16 x_new, RBF16 h, int32_t gate_kind,
+                           float residual_scale, float eps) {
+  int64_t rows, cols;
+  RowsCols(x, &rows, &cols);
+  return Check(tg_sandwich_norm_fwd(x.untyped_data(), branch.untyped_data(), post.untyped_data(), pre.untyped_data(), gate.untyped_data(), gate_kind,
+                                    residual_scale, eps, x_new->untyped_data(), h->untyped_data(), nullptr, nullptr, rows, cols, s),
+               "tg_sandwich_norm_fwd");
+}
+
+ffi::Error SandwichNormQuantFwd(cudaStream_t s, BF16 x, BF16 branch, BF16 post, BF16 pre, BF16 gate, RBF16 x_new, RBF16 h, RF8 q, RF32 scales,
+                                int32_t gate_kind, float residual_scale, float eps) {
+  int64_t rows, cols;
+  RowsCols(x, &rows, &cols);
+  return Check(tg_sandwich_norm_fwd(x.untyped_data(), branch.untyped_data(), post.untyped_data(), pre.untyped_data(), gate.untyped_data(), gate_kind,
+                                    residual_scale, eps, x_new->untyped_data(), h->untyped_data(), q->untyped_data(), scales->typed_data(), rows,
+                                    cols, s),
+               "tg_sandwich_norm_fwd");
+}
+
+// dgate has the gate's shape; scratch: tg_sandwich_norm_bwd_scratch_bytes(rows, cols) bytes that XLA plans
+ffi::Error SandwichNormBwd(cudaStream_t s, BF16 x_new, BF16 branch, BF16 post, BF16 pre, BF16 gate, BF16 g_new, BF16 g_h, RBF16 dx, RBF16 dbranch,
+                           RBF16 dpost, RBF16 dpre, RBF16 dgate, RU8 scratch, int32_t gate_kind, float residual_scale, float eps) {
+  int64_t rows, cols;
+  RowsCols(x_new, &rows, &cols);
+  if (static_cast<int64_t>(scratch->element_count()) < tg_sandwich_norm_bwd_scratch_bytes(rows, cols))
+    return ffi::Error(ffi::ErrorCode::kInvalidArgument, "TgSandwichNormBwd: scratch result smaller than tg_sandwich_norm_bwd_scratch_bytes");
+  return Check(tg_sandwich_norm_bwd(x_new.untyped_data(), branch.untyped_data(), post.untyped_data(), pre.untyped_data(), gate.untyped_data(), gate_kind,
+                                    residual_scale, eps, g_new.untyped_data(), g_h.untyped_data(), dx->untyped_data(), dbranch->untyped_data(),
+                                    dpost->untyped_data(), dpre->untyped_data(), dgate->untyped_data(), scratch->untyped_data(), rows, cols, s),
+               "tg_sandwich_norm_bwd");
+}
+
+// ---- distillation from a teacher's top logits (no counterpart) --------------------------------------
+
+// ids, logp (rows, k), log_rest (rows,)
+ffi::Error TopLogits(cudaStream_t s, BF16 logits, RS32 ids, RF32 logp, RF32 log_rest, float cap, float temperature) {
+  int64_t rows, vocab, k_rows, k;
+  RowsCols(logits, &rows, &vocab);
+  auto d = ids->dimensions();
+  k = d.size() ? d.back() : 0;
+  k_rows = k ? static_cast<int64_t>(ids->element_count()) / k : 0;
+  if (k_rows != rows || k > TG_TOP_LOGITS_MAX) return ffi::Error(ffi::ErrorCode::kInvalidArgument, "TgTopLogits: ids must be (rows, k)");
+  return Check(tg_top_logits(logits.untyped_data(), cap, temperature, ids->typed_data(), logp->typed_data(), log_rest->typed_data(), rows, vocab, vocab,
+                             static_cast<int>(k), s),
+               "tg_top_logits");
+}
+
+// The rows' losses and the gradient of their mean from one read of the logits: a custom_vjp's forward rule, whose backward rule
+// multiplies by the cotangent.  targets of -1 where there are none.
+ffi::Error SoftcapDistill(cudaStream_t s, BF16 logits, S32 ids, F32 logp, F32 log_rest, S32 targets, RF32 row_loss, RBF16 dlogits, float cap,
+                          float temperature, float weight) {
+  tg_distill_args a = {};
+  RowsCols(logits, &a.rows, &a.vocab);
+  auto d = ids.dimensions();
+  const int64_t k = d.size() ? d.back() : 0;
+  if (k > TG_TOP_LOGITS_MAX || static_cast<int64_t>(ids.element_count()) != a.rows * k || logp.element_count() != ids.element_count() ||
+      static_cast<int64_t>(log_rest.element_count()) != a.rows || static_cast<int64_t>(targets.element_count()) != a.rows)
+    return ffi::Error(ffi::ErrorCode::kInvalidArgument, "TgSoftcapDistill: ids and logp must be (rows, k), log_rest and targets (rows,)");
+  a.logits = logits.untyped_data(); a.ids = ids.untyped_data(); a.logp = logp.typed_data(); a.log_rest = log_rest.typed_data();
+  a.targets = targets.untyped_data(); a.cap = cap; a.temperature = temperature; a.weight = weight;
+  a.dlogits = dlogits->untyped_data(); a.row_loss = row_loss->typed_data();
+  a.ld = a.vocab; a.k = static_cast<int>(k);
+  return Check(tg_softcap_distill(&a, s), "tg_softcap_distill");
+}
+
 // ---- optimiser (train.py:114-123, 132-134) --------------------------------------------------------
 
 ffi::Error SumsqBf16(cudaStream_t s, BF16 x, RF32 out, RU8 scratch) {
@@ -347,3 +416,19 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(TgAdamwBf16, AdamwBf16,
 XLA_FFI_DEFINE_HANDLER_SYMBOL(TgGemmFwd, GemmFwd, TG_GEMM_BINDING("weight_gran"));
 XLA_FFI_DEFINE_HANDLER_SYMBOL(TgGemmDgrad, GemmDgrad, TG_GEMM_BINDING("weight_gran"));
 XLA_FFI_DEFINE_HANDLER_SYMBOL(TgGemmWgrad, GemmWgrad, TG_GEMM_BINDING("grad_gran"));
+XLA_FFI_DEFINE_HANDLER_SYMBOL(TgSandwichNormFwd, SandwichNormFwd,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Ret<BF16>().Ret<BF16>()
+                                  .Attr<int32_t>("gate_kind").Attr<float>("residual_scale").Attr<float>("eps"));
+XLA_FFI_DEFINE_HANDLER_SYMBOL(TgSandwichNormQuantFwd, SandwichNormQuantFwd,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Ret<BF16>().Ret<BF16>()
+                                  .Ret<F8>().Ret<F32>().Attr<int32_t>("gate_kind").Attr<float>("residual_scale").Attr<float>("eps"));
+XLA_FFI_DEFINE_HANDLER_SYMBOL(TgSandwichNormBwd, SandwichNormBwd,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<BF16>()
+                                  .Ret<BF16>().Ret<BF16>().Ret<BF16>().Ret<BF16>().Ret<BF16>().Ret<U8>()
+                                  .Attr<int32_t>("gate_kind").Attr<float>("residual_scale").Attr<float>("eps"));
+XLA_FFI_DEFINE_HANDLER_SYMBOL(TgTopLogits, TopLogits,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Ret<S32>().Ret<F32>().Ret<F32>().Attr<float>("cap")
+                                  .Attr<float>("temperature"));
+XLA_FFI_DEFINE_HANDLER_SYMBOL(TgSoftcapDistill, SoftcapDistill,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Arg<S32>().Arg<F32>().Arg<F32>().Arg<S32>().Ret<F32>().Ret<BF16>()
+                                  .Attr<float>("cap").Attr<float>("temperature").Attr<float>("weight"));
