@@ -17,6 +17,12 @@ import torch
 
 LAYER_KEYS = ("norm1", "wq", "wk", "wv", "wo", "norm2", "w_up", "w_down")      # model.py:33-42
 TOP_KEYS = ("embed", "pos", "final_norm")                                      # model.py:47-52
+SANDWICH_KEYS = ("post1", "post2", "gate1", "gate2")                           # of blocks with a norm on both sides, which the reference lacks
+
+
+def _layer_keys(layers):
+    """The keys of a layer's parameters: the reference's, and what of the sandwich norm's a model or a tree has."""
+    return LAYER_KEYS + tuple(k for k in SANDWICH_KEYS if k in layers)
 
 
 def _to_numpy(t: torch.Tensor) -> np.ndarray:
@@ -38,7 +44,7 @@ def _to_torch(a: np.ndarray, like: torch.Tensor) -> torch.Tensor:
 def params_tree(model) -> dict:
     """The reference's parameter pytree (model.py:46-54) from a `step.GPT`."""
     tree = {k: _to_numpy(getattr(model, k)) for k in TOP_KEYS}
-    tree["layers"] = {k: np.stack([_to_numpy(lp[k]) for lp in model.layers]) for k in LAYER_KEYS}
+    tree["layers"] = {k: np.stack([_to_numpy(lp[k]) for lp in model.layers]) for k in _layer_keys(model.layers[0] if model.layers else ())}
     tree["unembed"] = _to_numpy(model.unembed)
     return tree
 
@@ -81,7 +87,10 @@ def load_params(model, tree: dict) -> None:
         put(getattr(model, k), tree[k], k)
     layers = tree["layers"]
     n = len(model.layers)
-    for k in LAYER_KEYS:
+    keys = _layer_keys(model.layers[0] if model.layers else ())
+    if keys != _layer_keys(layers):
+        raise ValueError(f"checkpoint has layer parameters {_layer_keys(layers)}, the model {keys}")
+    for k in keys:
         if layers[k].shape[0] != n:
             raise ValueError(f"layers/{k}: checkpoint has {layers[k].shape[0]} layers, the model {n}")
         for i, lp in enumerate(model.layers):

@@ -17,6 +17,10 @@ layer and the norms run on this package's kernels through the reference's `mm` /
 Differences from model.py that the benchmark's training configuration asks for are switches: GELU
 (default there) or the reference's squared ReLU (model.py:72); learned positions, separate
 q/k/v, untied head, tanh logit cap 15 and the 0.02 / 0.02/sqrt(2L) init follow model.py.
+Beyond the reference: `block_norm="sandwich"` (a norm behind each branch too, with a gate and a scaled residual stream:
+kernels.sandwich_norm) and distillation (`GPT.top_logits` of a teacher, `Trainer.step(..., teacher=)` for its student:
+losses.capped_distillation).  Both run through autograd.
+
 No per-block rematerialisation (the reference's `use_remat` trades compute for memory; 180 GB
 does not need it at these sizes).
 """
@@ -52,6 +56,11 @@ class StepConfig:
     qkv: str = "fused"              # "fused": one dgrad GEMM contracts over the gradients of q, k and v (FP8 mm, norm "fused"); "separate"
     residual: str = "fused"         # "fused": the residual add runs inside the norm after it, its gradient fan-in inside that
                                     # norm's backward (norm "fused", FP8 mm, d_model <= 2048); "separate": elementwise adds
+    block_norm: str = "pre"         # "pre" (model.py:57-72); "sandwich": x = residual_scale x + G norm(branch), then the next block's norm, as one kernel
+    residual_gate: str = "none"     # G, with block_norm "sandwich": "none" (1), "channel" (a learned vector per junction), "token" (sigmoid(h w) of the branch's input h)
+    residual_scale: float = 1.0     # with block_norm "sandwich"
+    distill_temperature: float = 1.0    # Trainer.step(..., teacher=): the temperature that the teacher's log-probabilities were taken at,
+    distill_weight: float = 1.0         # and the weight of that loss; below 1 the targets' cross-entropy has the rest
     loss: str = "fused"             # "fused": one CUDA pass each way over the logits; "torch": op by op (CPU tests)
     optimizer: str = "fused"        # "fused": optim.ClippedAdamW (CUDA kernels); "torch": torch.optim.AdamW + tensor-op clip
     flat_parameters: bool = True    # optimizer "fused": a bucket's parameters and moments are slices of flat tensors, which the update walks
@@ -255,6 +264,12 @@ class GPT:
     """Parameters (bf16, model.py:19-54) and forward pass."""
 
     def __init__(self, cfg: StepConfig, device, seed: int = 0):
+        if cfg.block_norm not in ("pre", "sandwich"):
+            raise ValueError(f"unknown block_norm {cfg.block_norm!r}")
+        if cfg.residual_gate not in ("none", "channel", "token"):
+            raise ValueError(f"unknown residual_gate {cfg.residual_gate!r}")
+        if cfg.block_norm == "pre" and (cfg.residual_gate != "none" or cfg.residual_scale != 1.0):
+            raise ValueError("residual_gate and residual_scale need block_norm 'sandwich'")
         self.cfg = cfg
         g = torch.Generator(device=device).manual_seed(seed)
         std, proj_std = cfg.init_std, cfg.init_std / math.sqrt(2.0 * cfg.n_layers)   # model.py:21-22
@@ -274,6 +289,13 @@ class GPT:
                 "norm1": ones(d), "wq": normal((d, h)), "wk": normal((d, h)), "wv": normal((d, h)),
                 "wo": normal((h, d), proj_std), "norm2": ones(d), "w_up": normal((d, ff)),
                 "w_down": normal((ff, d), proj_std)})
+            if cfg.block_norm == "sandwich":
+                # a gate per channel starts where proj_std puts a branch's share (model.py:22); one per token at 1/2 (a zero projection)
+                gate = {"none": None, "channel": lambda: ones(d).detach() / math.sqrt(2.0 * cfg.n_layers),
+                        "token": lambda: torch.zeros((d, 1), device=device, dtype=torch.bfloat16)}[cfg.residual_gate]
+                self.layers[-1].update({"post1": ones(d), "post2": ones(d)})
+                if gate is not None:
+                    self.layers[-1].update({"gate1": torch.nn.Parameter(gate()), "gate2": torch.nn.Parameter(gate())})
         self.final_norm = ones(d)
         self.unembed = normal((d, cfg.vocab_size))
         self.exchange = None            # gradient buckets with a deferred exchange (data-parallel training): see _ExchangePoint
@@ -285,7 +307,7 @@ class GPT:
         out = [[self.unembed, self.final_norm]]
         for lp in reversed(self.layers):
             if qkv_side_by_side:
-                out.append([lp["norm1"], (lp["wq"], lp["wk"], lp["wv"]), lp["wo"], lp["norm2"], lp["w_up"], lp["w_down"]])
+                out.append([lp["norm1"], (lp["wq"], lp["wk"], lp["wv"]), *(v for n, v in lp.items() if n not in ("norm1", "wq", "wk", "wv"))])
             else:
                 out.append(list(lp.values()))
         out.append([self.embed, self.pos])
@@ -322,6 +344,23 @@ class GPT:
             return x * torch.rsqrt(var + c.rms_eps).to(x.dtype) * w, None           # kernels.py:32-33
         return kernels.rms_norm(x, w, c.rms_eps), None
 
+    def _junction(self, x, branch, h, gamma, lp, which, want_q=True):
+        """(new x, its norm, quantised norm) behind branch `which` of layer `lp`, whose input was h."""
+        c = self.cfg
+        gate = lp.get(f"gate{which}")
+        if c.residual_gate == "token":
+            gate = torch.sigmoid(h @ gate)
+        post = lp[f"post{which}"]
+        if c.norm == "torch_reference":
+            def rms(v, g):
+                return v * torch.rsqrt(v.float().pow(2).mean(-1, keepdim=True) + c.rms_eps).to(v.dtype) * g
+            n = rms(branch, post)
+            x = c.residual_scale * x + (n if gate is None else gate * n)
+            return x, rms(x, gamma), None
+        quantize = want_q and c.norm == "fused" and c.mm != "bf16"
+        out = kernels.sandwich_norm(x, branch, post, gamma, c.rms_eps, gate=gate, residual_scale=c.residual_scale, quantize=quantize)
+        return out[0], out[1], fp8.QuantizedActivation(*out[1:]) if quantize else None
+
     def _act(self, u):
         return F.gelu(u) if self.cfg.activation == "gelu" else F.relu(u) ** 2      # model.py:72
 
@@ -335,11 +374,14 @@ class GPT:
         fuse = c.residual == "fused" and c.norm == "fused" and c.mm != "bf16" and c.d_model <= ops.ADD_NORM_MAX_COLS
         branch = None
 
-        def norm_after(x, branch, gamma, want_q=True):
-            """(new x, h, quantised h) for `x = x + branch; h = norm(x)`; branch None: no add pending."""
+        def norm_after(x, branch, gamma, want_q=True, behind=None):
+            """(new x, h, quantised h) for `x = x + branch; h = norm(x)`; branch None: no add pending.  behind: the branch's
+            (input, layer, number), which a sandwich norm needs."""
             if branch is None:
                 h, hq = self._norm(x, gamma)
                 return x, h, hq
+            if c.block_norm == "sandwich":
+                return self._junction(x, branch, behind[0], gamma, behind[1], behind[2], want_q)
             if not fuse:
                 x = x + branch
                 h, hq = self._norm(x, gamma)
@@ -347,8 +389,9 @@ class GPT:
             out = _AddNormQuant.apply(x, branch, gamma, c.rms_eps, want_q)
             return out[0], out[1], (fp8.QuantizedActivation(out[1], out[2], out[3]) if want_q else None)
 
+        behind = None
         for lp in self.layers:
-            x, h, hq = norm_after(x, branch, lp["norm1"])                           # model.py:72 (layer before), :76
+            x, h, hq = norm_after(x, branch, lp["norm1"], behind=behind)            # model.py:72 (layer before), :76
             if c.qkv == "fused" and c.mm == "fp8" and hq is not None:
                 q, k, v = _QKV.apply(h, hq, lp["wq"], lp["wk"], lp["wv"])           # model.py:63-65
             else:
@@ -361,12 +404,13 @@ class GPT:
             # the attention output feeds one linear: both its quantised forms from one read when a backward pass follows
             oq = fp8.QuantizedActivation.both(o) if (c.mm == "fp8" and torch.is_grad_enabled() and o.shape[-1] % 128 == 0) else None
             branch = self._mm(o, lp["wo"], oq)
-            x, h, hq = norm_after(x, branch, lp["norm2"])                           # model.py:68, :77
+            x, h, hq = norm_after(x, branch, lp["norm2"], behind=(h, lp, 1))        # model.py:68, :77
             if c.mm == "fp8" and c.mlp == "fused":
                 branch = _FusedMLP.apply(h, hq, lp["w_up"], lp["w_down"], c.activation)
             else:
                 branch = self._mm(self._act(self._mm(h, lp["w_up"], hq)), lp["w_down"])
-        x, h, _ = norm_after(x, branch, self.final_norm, want_q=False)              # model.py:72, :93
+            behind = (h, lp, 2)
+        x, h, _ = norm_after(x, branch, self.final_norm, want_q=False, behind=behind)   # model.py:72, :93
         return h @ self.unembed                                                     # stays bf16 (bench_fp8_norm.py:86)
 
     def forward(self, ids):
@@ -378,6 +422,17 @@ class GPT:
             return losses.capped_cross_entropy(self.raw_logits(ids), targets, self.cfg.logit_cap)
         logits = self.forward(ids).float()                                          # losses.py:9
         return F.cross_entropy(logits.view(-1, logits.shape[-1]), targets.view(-1))  # losses.py:10-12
+
+    def top_logits(self, ids, k: int, temperature: float = 1.0):
+        """This model as a teacher: losses.TopLogits of every token, without a graph."""
+        with torch.no_grad():
+            return losses.top_logits(self.raw_logits(ids), self.cfg.logit_cap, k, temperature)
+
+    def distillation_loss(self, ids, targets, teacher):
+        """losses.capped_distillation of this model's logits with the configuration's temperature and weight."""
+        c = self.cfg
+        return losses.capped_distillation(self.raw_logits(ids), teacher, c.logit_cap, target_ids=targets if c.distill_weight < 1 else None,
+                                          temperature=c.distill_temperature, weight=c.distill_weight)
 
 
 class Trainer:
@@ -443,7 +498,7 @@ class Trainer:
         """The step as one native program (csrc/step.cpp) where every switch has its default value; None otherwise."""
         c, b = self.cfg, self.buckets
         h = c.n_heads * c.head_dim
-        if not (torch.device(self.device).type == "cuda" and c.mm == "fp8" and c.norm == "fused" and c.mlp == "fused" and c.qkv == "fused"
+        if not (torch.device(self.device).type == "cuda" and c.block_norm == "pre" and c.mm == "fp8" and c.norm == "fused" and c.mlp == "fused" and c.qkv == "fused"
                 and c.residual == "fused" and c.loss == "fused" and self._fused_opt and c.flat_parameters and c.direct_grads
                 and c.activation in ("gelu", "relu2") and c.d_model <= ops.ADD_NORM_MAX_COLS
                 and not (c.d_model % 128 or h % 128 or c.d_ff % 128)):
@@ -468,14 +523,14 @@ class Trainer:
             grads[id(m.unembed)], g_layers, [list(f) for f in self.opt._flat], self._params, self.opt._count,
             b.bucket_done if many else None, b.flush if many else None, b.finish if many else None)
 
-    def _eager_step(self, ids, targets):
-        if self._program is not None:
+    def _eager_step(self, ids, targets, teacher=None):
+        if self._program is not None and teacher is None:
             o = self.opt                          # read at every step: a schedule changes them
             out = self._program.step(ids, targets, o.lr, o.b1, o.b2, o.eps, o.wd, o.clip)
             if out is not None:                   # (None: a parameter is frozen or has a gradient hook)
                 return out
         self.buckets.zero()
-        loss = self.model.loss(ids, targets)
+        loss = self.model.loss(ids, targets) if teacher is None else self.model.distillation_loss(ids, targets, teacher)
         loss.backward()
         self.buckets.finish()
         if torch.device(self.device).type == "cuda":
@@ -497,8 +552,9 @@ class Trainer:
             return self.opt.state_tensors()
         return [t for st in self.opt.state.values() for t in st.values() if torch.is_tensor(t)]
 
-    def _capture(self, ids, targets):
+    def _capture(self, ids, targets, teacher=None):
         self._ids, self._tgt = ids.clone(), targets.clone()
+        self._teacher = None if teacher is None else losses.TopLogits(*(None if t is None else t.clone() for t in teacher))
         params = self.model.parameters()
         saved_p = [p.detach().clone() for p in params]
         saved_s = {id(t): t.clone() for t in self._opt_state_tensors()}
@@ -506,7 +562,7 @@ class Trainer:
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             for _ in range(2):                      # lazy initialisations (optimizer state, kernel attributes, NCCL)
-                self._eager_step(self._ids, self._tgt)
+                self._eager_step(self._ids, self._tgt, self._teacher)
         torch.cuda.current_stream().wait_stream(side)
         with torch.no_grad():
             for p, q in zip(params, saved_p):
@@ -519,16 +575,26 @@ class Trainer:
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            self._loss, self._gnorm = self._eager_step(self._ids, self._tgt)
+            self._loss, self._gnorm = self._eager_step(self._ids, self._tgt, self._teacher)
         self._graph = g
 
-    def step(self, ids, targets):
+    def step(self, ids, targets, teacher=None):
+        """One step on a batch; `teacher` (losses.TopLogits of it) makes the loss that of distillation.  A captured step
+        takes what its first call had: a teacher or none, of as many logits, with or without log_rest."""
         if not self._want_graph:
-            return self._eager_step(ids, targets)
+            return self._eager_step(ids, targets, teacher)
         if self._graph is None:
-            self._capture(ids, targets)
+            self._capture(ids, targets, teacher)
+        def form(t):
+            return None if t is None else tuple(None if v is None else (v.shape, v.dtype) for v in t)
+        if form(teacher) != form(self._teacher):
+            raise ValueError("a captured step takes a teacher of the form that it was captured with")
         self._ids.copy_(ids)
         self._tgt.copy_(targets)
+        if teacher is not None:
+            for kept, new in zip(self._teacher, teacher):
+                if kept is not None:
+                    kept.copy_(new)
         self._graph.replay()
         return self._loss, self._gnorm
 
