@@ -10,12 +10,12 @@
 
 #include "common.cuh"
 #include "host_api.h"
+#include "norm.cuh"
 
 namespace tg {
 
 constexpr int kDsMaxThreads = 512;
 constexpr int kDsMaxVocab = 1 << 20;
-constexpr int64_t kDsDynamicMax = 208 * 1024;       // of shared memory; up to 17 KB more are static
 constexpr int kTopMaxCandidates = 1024;
 constexpr float kDsLog2e = 1.4426950408889634f;
 
@@ -29,32 +29,66 @@ __device__ __forceinline__ float ds_rcp(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v));
   return e;
 }
+__device__ __forceinline__ float ds_lds(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
 
 // The cap.  u = 1 - tanh |x / c| = 2 / (1 + exp(2 |x| / c)) keeps its relative precision where tanh saturates, so that
-// sech^2(x / c) = u (2 - u) does too; z / T = sign(x) (c / T) (1 - u).
+// sech^2(x / c) = u (2 - u) does too; z / T = sign(x) (c / T) (1 - u).  Handed out as -u.
+//
+// Two ways to it.  Two approximations of the special function unit, an exponential and a reciprocal (a third one is the exponential of
+// z / T): 16 of them a clock and SM, so six clocks for 32 logits.  Or a table: x is a bf16 value, so between 2^-24 c, below
+// which z is as good as +-2^-24 c, and 16 c, from where on tanh is 1, it has 29 binades of 128 values.  A look-up of 32 random entries
+// takes 3.5 clocks of shared memory and leaves the special function unit two.
+constexpr int kCapBinadesBelow = 24, kCapBinades = 29;
+constexpr int kCapEntries = kCapBinades * 128 + 1;
+constexpr int kCapTableBytes = (kCapEntries * 4 + 15) / 16 * 16;
+
+template <bool TABLE>
 struct Cap {
   float k2;            // 2 log2(e) / c
   float zt;            // c log2(e) / T: z / T in powers of two is sign(x) zt (1 - u)
   float c, inv_c, inv_t;
-  __device__ __forceinline__ Cap(float cap, float temperature) {
+  uint32_t lo2, hi2;   // the table's first and last magnitude as bf16 bits, twice
+  uint32_t tab2;       // (its address) - 4 lo, twice: plus a pair of magnitudes times 4, two 16-bit addresses
+  __device__ __forceinline__ Cap(float cap, float temperature, void* table) {
     c = cap;
     inv_c = __fdiv_rn(1.0f, cap);
     inv_t = __fdiv_rn(1.0f, temperature);
     k2 = 2.0f * kDsLog2e * inv_c;
     zt = cap * kDsLog2e * inv_t;
+    if constexpr (TABLE) {
+      const uint32_t c_pow = (__float_as_uint(cap) >> 16) & 0x7f80u;     // 2^floor(log2 c)
+      const uint32_t lo = c_pow - (kCapBinadesBelow << 7), hi = lo + (kCapBinades << 7);
+      float* t = static_cast<float*>(table);
+      for (int i = threadIdx.x; i < kCapEntries; i += blockDim.x)
+        t[i] = __fdiv_rn(-2.0f, 1.0f + expf(2.0f * (__uint_as_float((lo + uint32_t(i)) << 16) * inv_c)));
+      lo2 = lo * 0x10001u;
+      hi2 = hi * 0x10001u;
+      tab2 = (uint32_t(__cvta_generic_to_shared(table)) - 4u * lo) * 0x10001u;
+    }
   }
-  // u of the two logits of a word
-  __device__ __forceinline__ float2 u2(uint32_t w) const {
-    const float2 a = __fmul2_rn(bf16x2_unpack(w & 0x7fff7fffu), make_float2(k2, k2));
-    const float2 d = __fadd2_rn(make_float2(ds_ex2(a.x), ds_ex2(a.y)), make_float2(1.f, 1.f));
-    const float2 r = make_float2(ds_rcp(d.x), ds_rcp(d.y));
-    return __fadd2_rn(r, r);
+  // -u of the two logits of a word.  `top` collects the largest magnitudes: the table has no NaN
+  __device__ __forceinline__ float2 minus_u(uint32_t w, uint32_t& top) const {
+    const uint32_t mag = w & 0x7fff7fffu;
+    if constexpr (TABLE) {
+      top = __vmaxu2(top, mag);
+      const uint32_t at = __vminu2(__vmaxu2(mag, lo2), hi2) * 4u + tab2;
+      return make_float2(ds_lds(at & 0xffffu), ds_lds(at >> 16));
+    } else {
+      const float2 a = __fmul2_rn(bf16x2_unpack(mag), make_float2(k2, k2));
+      const float2 d = __fadd2_rn(make_float2(ds_ex2(a.x), ds_ex2(a.y)), make_float2(1.f, 1.f));
+      return __fmul2_rn(make_float2(ds_rcp(d.x), ds_rcp(d.y)), make_float2(-2.f, -2.f));
+    }
   }
-  // s = sign(x) scale (1 - u), the capped logits in the units of `scale`
-  static __device__ __forceinline__ float2 signed2(uint32_t w, float2 u, float scale) {
+  static __device__ __forceinline__ bool is_nan(uint32_t top) { return TABLE && ((top & 0xffffu) > 0x7f80u || (top >> 16) > 0x7f80u); }
+  // sign(x) scale (1 - u), the capped logits in the units of `scale`
+  static __device__ __forceinline__ float2 capped2(uint32_t w, float2 minus_u, float scale) {
     const uint32_t b = __float_as_uint(scale);
     const float2 s = make_float2(__uint_as_float(b ^ ((w << 16) & 0x80000000u)), __uint_as_float(b ^ (w & 0x80000000u)));
-    return __ffma2_rn(make_float2(-u.x, -u.y), s, s);
+    return __ffma2_rn(minus_u, s, s);
   }
   // the few logits of a row whose own value counts (kept ones, the target) by CUDA's accurate functions
   __device__ __forceinline__ float z_over_t(float x) const { return __fmul_rn(c * tanhf(x * inv_c), inv_t); }
@@ -85,6 +119,13 @@ struct DsRow {
   }
 };
 
+// zeros in the place of a piece's elements that are not the row's
+__device__ __forceinline__ void clear_outside(uint4& w, uint32_t out) {
+  uint32_t* p = &w.x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) p[j] &= (out >> (2 * j) & 1u ? 0u : 0xffffu) | (out >> (2 * j + 1) & 1u ? 0u : 0xffff0000u);
+}
+
 __device__ __forceinline__ float ds_warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -103,11 +144,7 @@ __device__ __forceinline__ void ds_block_sum(float (&v)[N], float* s, int warps)
   }
   __syncthreads();
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    float t = 0.f;
-    for (int i = 0; i < warps; ++i) t += s[n * (kDsMaxThreads / 32) + i];
-    v[n] = t;
-  }
+  for (int n = 0; n < N; ++n) v[n] = ds_warp_sum(lane < warps ? s[n * (kDsMaxThreads / 32) + lane] : 0.f);
 }
 
 // log of part / (part + other), from the smaller of the two where the result is near 0
@@ -119,8 +156,10 @@ __device__ __forceinline__ float log_share(float part, float other) {
 // ---------------------------------------------------------------------------------------
 // The student's loss and its gradient.  One thread block per row.  First pass: the sum of exp(z / T) (and of exp(z)) over all logits that the
 // teacher does not name; those it does are marked in a bitmap, a byte per piece, and computed by one thread each.  Second pass: the gradient,
-// from the row as it lies in shared memory (or, of a vocabulary that does not fit there, read again), after which the threads of the named
+// from the row read again -- 600 rows of 100 KB are in work at a time, which the L2 holds -- after which the threads of the named
 // logits and the target write theirs over it.
+// EXPS: 1 where one sum does (one temperature, or one of the two losses), 2 for two exponentials, 3 and 4 where the second is the first one
+// squared once or twice (temperatures 2 and 4).
 // ---------------------------------------------------------------------------------------
 struct DistillArgs {
   const void* logits;
@@ -143,8 +182,9 @@ __device__ __forceinline__ int ds_index(const void* p, int is64, int64_t at, int
   return v >= 0 && v < vocab ? int(v) : -1;
 }
 
-template <bool TWO, bool GRAD, bool STAGED>
+template <int EXPS, bool GRAD, bool TABLE>
 __global__ void __launch_bounds__(kDsMaxThreads) softcap_distill_kernel(const DistillArgs p) {
+  constexpr bool TWO = EXPS > 1;
   grid_trigger();
   grid_wait();
   if (p.only_if_scaled && *p.gscale == 1.0f) return;
@@ -154,14 +194,24 @@ __global__ void __launch_bounds__(kDsMaxThreads) softcap_distill_kernel(const Di
   __shared__ float s_p[kDsMaxThreads];
   const int tid = int(threadIdx.x), nt = int(blockDim.x), warps = nt >> 5;
   const int map_words = (p.vocab + 14) / 8 / 4 + 1;
-  uint32_t* s_map = reinterpret_cast<uint32_t*>(s_ds);
-  const uint8_t* s_named = s_ds;
-  uint4* s_row = reinterpret_cast<uint4*>(s_ds + (map_words * 4 + 15) / 16 * 16);
+  const uint8_t* s_named = s_ds + (TABLE ? kCapTableBytes : 0);
+  uint32_t* s_map = reinterpret_cast<uint32_t*>(s_ds + (TABLE ? kCapTableBytes : 0));
   for (int i = tid; i < map_words; i += nt) s_map[i] = 0u;
-  const Cap cap(p.cap, p.temperature);
+  const Cap<TABLE> cap(p.cap, p.temperature, s_ds);
   const float z1 = p.cap * kDsLog2e;
   const float t = p.temperature, w_soft = p.weight, w_hard = 1.0f - p.weight;
   const float gs = GRAD ? (p.gscale != nullptr ? *p.gscale : 1.0f) * __fdiv_rn(1.0f, float(p.rows)) : 0.f;
+  // exp(z) of a pair, from its exp(z / T) or anew
+  auto second = [&](float2 e, uint32_t w, float2 nu) {
+    if constexpr (EXPS > 2) {
+#pragma unroll
+      for (int i = 2; i < EXPS; ++i) e = __fmul2_rn(e, e);
+      return e;
+    } else {
+      const float2 sz = Cap<TABLE>::capped2(w, nu, z1);
+      return make_float2(ds_ex2(sz.x), ds_ex2(sz.y));
+    }
+  };
   __syncthreads();
 
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
@@ -205,29 +255,31 @@ __global__ void __launch_bounds__(kDsMaxThreads) softcap_distill_kernel(const Di
 
     // ---- first pass
     float2 acc = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+    uint32_t top = 0u;
     const uint4* src = reinterpret_cast<const uint4*>(q.base);
     uint4 w0 = tid < q.pieces ? ld_stream_v4(src + tid) : make_uint4(0u, 0u, 0u, 0u);
     uint4 w1 = tid + nt < q.pieces ? ld_stream_v4(src + tid + nt) : make_uint4(0u, 0u, 0u, 0u);
     for (int i = tid; i < q.pieces; i += nt) {
-      const uint4 w = w0;
+      uint4 w = w0;
       w0 = w1;
       if (i + 2 * nt < q.pieces) w1 = ld_stream_v4(src + i + 2 * nt);
-      if (GRAD && STAGED) s_row[i] = w;
+      const uint32_t out = q.outside(i), skip = uint32_t(s_named[i]) | out;
+      if (out) clear_outside(w, out);
       const uint32_t wi[4] = {w.x, w.y, w.z, w.w};
-      const uint32_t skip = uint32_t(s_named[i]) | q.outside(i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 u = cap.u2(wi[j]);
-        const float2 s = Cap::signed2(wi[j], u, cap.zt);
+        const float2 nu = cap.minus_u(wi[j], top);
+        const float2 s = Cap<TABLE>::capped2(wi[j], nu, cap.zt);
         float2 e = make_float2(ds_ex2(s.x), ds_ex2(s.y));
         if (skip) {
           if (skip >> (2 * j) & 1u) e.x = 0.f;
           if (skip >> (2 * j + 1) & 1u) e.y = 0.f;
         }
         acc = __fadd2_rn(acc, e);
-        if (TWO) {
-          const float2 sz = Cap::signed2(wi[j], u, z1);
-          float2 e1 = make_float2(ds_ex2(sz.x), ds_ex2(sz.y));
+        if constexpr (EXPS > 2) {
+          acc1 = __fadd2_rn(acc1, second(e, wi[j], nu));
+        } else if constexpr (EXPS == 2) {
+          float2 e1 = second(e, wi[j], nu);
           if (skip) {
             if (skip >> (2 * j) & 1u) e1.x = 0.f;
             if (skip >> (2 * j + 1) & 1u) e1.y = 0.f;
@@ -236,6 +288,7 @@ __global__ void __launch_bounds__(kDsMaxThreads) softcap_distill_kernel(const Di
         }
       }
     }
+    if (Cap<TABLE>::is_nan(top)) acc.x = acc1.x = __int_as_float(0x7fffffff);
     float sums[TWO ? 5 : 3] = {acc.x + acc.y, first ? e_here : 0.f, prob};
     if constexpr (TWO) {
       sums[3] = acc1.x + acc1.y;
@@ -273,22 +326,24 @@ __global__ void __launch_bounds__(kDsMaxThreads) softcap_distill_kernel(const Di
       const float b = target >= 0 && w_hard != 0.f ? w_hard * __fdiv_rn(1.0f, total1) : 0.f;
       uint16_t* d_base = static_cast<uint16_t*>(p.d) + (q.base - static_cast<const uint16_t*>(p.logits));
       const float ab = TWO ? a : a + b;
-      const float2 a2 = make_float2(ab, ab), b2 = make_float2(b, b), gs2 = make_float2(gs, gs), two = make_float2(2.f, 2.f);
+      const float2 a2 = make_float2(ab, ab), b2 = make_float2(b, b), gs2 = make_float2(-gs, -gs), two = make_float2(2.f, 2.f);
+      w0 = tid < q.pieces ? ld_stream_v4(src + tid) : make_uint4(0u, 0u, 0u, 0u);
+      w1 = tid + nt < q.pieces ? ld_stream_v4(src + tid + nt) : make_uint4(0u, 0u, 0u, 0u);
       for (int i = tid; i < q.pieces; i += nt) {
-        const uint4 w = STAGED ? s_row[i] : ld_stream_v4(src + i);
+        const uint4 w = w0;
+        w0 = w1;
+        if (i + 2 * nt < q.pieces) w1 = ld_stream_v4(src + i + 2 * nt);
         const uint32_t wi[4] = {w.x, w.y, w.z, w.w};
         uint4 o;
         uint32_t* op = &o.x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 u = cap.u2(wi[j]);
-          const float2 s = Cap::signed2(wi[j], u, cap.zt);
-          float2 g = __fmul2_rn(a2, make_float2(ds_ex2(s.x), ds_ex2(s.y)));
-          if (TWO) {
-            const float2 sz = Cap::signed2(wi[j], u, z1);
-            g = __ffma2_rn(b2, make_float2(ds_ex2(sz.x), ds_ex2(sz.y)), g);
-          }
-          const float2 sech = __fmul2_rn(u, __fadd2_rn(two, make_float2(-u.x, -u.y)));
+          const float2 nu = cap.minus_u(wi[j], top);
+          const float2 s = Cap<TABLE>::capped2(wi[j], nu, cap.zt);
+          const float2 e = make_float2(ds_ex2(s.x), ds_ex2(s.y));
+          float2 g = __fmul2_rn(a2, e);
+          if (TWO) g = __ffma2_rn(b2, second(e, wi[j], nu), g);
+          const float2 sech = __fmul2_rn(nu, __fadd2_rn(two, nu));       // (negative, as is gs2)
           g = __fmul2_rn(g, __fmul2_rn(sech, gs2));
           op[j] = pack_bf16x2(g.x, g.y);
         }
@@ -323,12 +378,12 @@ __global__ void __launch_bounds__(kDsMaxThreads) softcap_distill_kernel(const Di
 }
 
 // ---------------------------------------------------------------------------------------
-// A teacher's top logits.  One thread block per row.  The first pass brings the row into shared memory and finds the largest logit of every
-// group (the even and the odd elements of a thread's pieces are a group each).  The k-th largest of the groups' maxima is a lower bound of the
-// k-th largest logit that few others reach: with 1024 groups about 1024 ln(1 / (1 - k / 1024)) logits.  The second pass collects those and sums
-// exp(z / T) of all others; each candidate then counts the candidates before it, which is its place.
-// Where the bound lets too many through (a row of equal logits, large ones side by side) the k-th largest logit is found by bisection on the
-// row's 16-bit keys, and its equals are taken in the row's order.
+// A teacher's top logits.  One thread block per row.  The first pass finds the largest logit of every group (the even and the odd elements
+// of a thread's pieces are a group each).  The k-th largest of the groups' maxima is a lower bound of the k-th largest logit
+// that few others reach: with 1024 groups about 1024 ln(1 / (1 - k / 1024)) logits.  The second pass, over the row as the L2 holds it, collects
+// those and sums exp(z / T) of all others.  Candidates are sorted by counting into bins of two keys, then within their bin.
+// Where the bound lets too many through (a row of equal logits, large ones side by side), or a NaN is among them, the k-th largest logit is found by
+// bisection on the row's 16-bit keys, and its equals are taken in the row's order.
 // ---------------------------------------------------------------------------------------
 struct TopArgs {
   const void* logits;
@@ -347,37 +402,50 @@ __device__ __forceinline__ uint32_t top_key(uint32_t bits) {
 }
 __device__ __forceinline__ uint32_t top_bits(uint32_t key) { return key >= 0x8000u ? key - 0x8000u : 0x8000u | (0x8000u - key); }
 
-template <bool STAGED>
+constexpr int kTopBins = 256;
+
+template <bool TABLE>
 __global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs p) {
   grid_trigger();
   grid_wait();
   extern __shared__ __align__(16) uint8_t s_ds[];
   __shared__ float s_red[2 * (kDsMaxThreads / 32)];
   __shared__ uint64_t s_cand[kTopMaxCandidates], s_sorted[kTopMaxCandidates];
-  __shared__ int s_count[2][kDsMaxThreads / 32], s_n;
-  uint4* s_row = reinterpret_cast<uint4*>(s_ds);
+  __shared__ __align__(16) int s_hist[kTopBins];
+  __shared__ int s_begin[kTopBins], s_count[2][kDsMaxThreads / 32], s_n;
+  __shared__ uint32_t s_bound;
   const int tid = int(threadIdx.x), nt = int(blockDim.x), warps = nt >> 5, lane = tid & 31, warp = tid >> 5;
-  const Cap cap(p.cap, p.temperature);
+  const Cap<TABLE> cap(p.cap, p.temperature, s_ds);
   const int k = p.k;
+  __syncthreads();
 
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const DsRow q(p.logits, row, p.ld, p.vocab);
     const uint4* src = reinterpret_cast<const uint4*>(q.base);
-    auto piece = [&](int i) { return STAGED ? s_row[i] : ld_stream_v4(src + i); };
-    // ---- first pass: the groups' maxima
-    uint32_t top[2] = {0u, 0u};
+    // ---- first pass: the groups' maxima (NaN aside), as keys; 0 for a group of none
+    uint32_t top[2];
     {
       uint4 w0 = tid < q.pieces ? ld_stream_v4(src + tid) : make_uint4(0u, 0u, 0u, 0u);
       uint4 w1 = tid + nt < q.pieces ? ld_stream_v4(src + tid + nt) : make_uint4(0u, 0u, 0u, 0u);
+      __nv_bfloat162 m = __halves2bfloat162(__ushort_as_bfloat16(0x7fff), __ushort_as_bfloat16(0x7fff));
       for (int i = tid; i < q.pieces; i += nt) {
-        const uint4 w = w0;
+        uint4 w = w0;
         w0 = w1;
         if (i + 2 * nt < q.pieces) w1 = ld_stream_v4(src + i + 2 * nt);
-        if (STAGED) s_row[i] = w;
-        const uint32_t wi[4] = {w.x, w.y, w.z, w.w}, skip = q.outside(i);
+        const uint32_t out = q.outside(i);
+        uint32_t* wi = &w.x;
+        if (out) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (!(skip >> j & 1u)) top[j & 1] = max(top[j & 1], top_key(j & 1 ? wi[j >> 1] >> 16 : wi[j >> 1] & 0xffffu));
+          for (int j = 0; j < 4; ++j) wi[j] |= (out >> (2 * j) & 1u ? 0x7fffu : 0u) | (out >> (2 * j + 1) & 1u ? 0x7fff0000u : 0u);   // NaN
+        }
+        const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(wi);
+        m = __hmax2(m, __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
+      }
+      const uint32_t bits = *reinterpret_cast<const uint32_t*>(&m);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t b = h ? bits >> 16 : bits & 0xffffu;
+        top[h] = (b & 0x7fffu) > 0x7f80u ? 0u : top_key(b);
       }
     }
     // how many of the block's `n`s there are (the same value in every thread); two buffers, so that one barrier a call does
@@ -386,85 +454,144 @@ __global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs
       n = __reduce_add_sync(0xffffffffu, n);
       if (lane == 0) s_count[turn][warp] = n;
       __syncthreads();
-      int c = 0;
-      for (int i = 0; i < warps; ++i) c += s_count[turn][i];
+      const int c = __reduce_add_sync(0xffffffffu, lane < warps ? s_count[turn][lane] : 0);
       turn ^= 1;
       return c;
     };
-    // the largest key that at least k of the groups reach (0: none)
-    uint32_t lo = 0u;
-    for (uint32_t bit = 0x8000u; bit != 0u; bit >>= 1)
-      if (count(int(top[0] >= (lo | bit)) + int(top[1] >= (lo | bit))) >= k) lo |= bit;
+    // ---- the bound: counts by distance from the largest, two keys a bin
+    uint32_t largest = __reduce_max_sync(0xffffffffu, max(top[0], top[1]));
+    if (lane == 0) s_count[turn][warp] = int(largest);
+    for (int i = tid; i < kTopBins; i += nt) s_hist[i] = 0;
+    __syncthreads();
+    largest = __reduce_max_sync(0xffffffffu, lane < warps ? uint32_t(s_count[turn][lane]) : 0u);
+    turn ^= 1;
+    auto bin = [&](uint32_t key) { return key > largest ? 0u : min((largest - key) >> 1, uint32_t(kTopBins - 1)); };
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (top[h] != 0u) atomicAdd(s_hist + bin(top[h]), 1);
+    __syncthreads();
+    // warp 0: the first bin at which the running count reaches `want` (kTopBins: none), or all bins' beginnings
+    auto scan = [&](int want, bool begins) {
+      int v[kTopBins / 32], sum = 0;
+#pragma unroll
+      for (int j = 0; j < kTopBins / 32; j += 4) {
+        const int4 b = reinterpret_cast<const int4*>(s_hist)[(lane * (kTopBins / 32) + j) / 4];
+        v[j] = b.x; v[j + 1] = b.y; v[j + 2] = b.z; v[j + 3] = b.w;
+      }
+#pragma unroll
+      for (int j = 0; j < kTopBins / 32; ++j) sum += v[j];
+      int before = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
+      }
+      before -= sum;
+      int found = kTopBins;
+#pragma unroll
+      for (int j = 0; j < kTopBins / 32; ++j) {
+        if (begins) s_begin[lane * (kTopBins / 32) + j] = before;
+        before += v[j];
+        if (before >= want && found == kTopBins) found = lane * (kTopBins / 32) + j;
+      }
+      return int(__reduce_min_sync(0xffffffffu, unsigned(found)));
+    };
+    if (warp == 0) {
+      const int b = scan(k, false);
+      // (the last bin has everything further down: no bound)
+      if (lane == 0) s_bound = b < kTopBins - 1 && largest > 2u * uint32_t(b) + 1u ? largest - 2u * uint32_t(b) - 1u : 0u;
+      if (lane == 0) s_n = 0;
+    }
+    __syncthreads();
+    uint32_t lo = s_bound;
+    if (lo == 0u) {
+      // the largest key that at least k of the groups reach (0: none)
+      for (uint32_t bit = 0x8000u; bit != 0u; bit >>= 1)
+        if (count(int(top[0] >= (lo | bit)) + int(top[1] >= (lo | bit))) >= k) lo |= bit;
+    }
 
-    // ---- second pass: candidates, and the sum of the others.  `strict`: equals of the bound are counted, not collected
-    float2 acc;
-    int equal;
-    auto collect = [&](uint32_t bound, bool strict) {
-      if (tid == 0) s_n = 0;
-      __syncthreads();
-      acc = make_float2(0.f, 0.f);
-      equal = 0;
+    // ---- second pass: candidates, and the sum of the others
+    float2 acc = make_float2(0.f, 0.f);
+    uint32_t nan = 0u;
+    {
+      const uint32_t bits = lo == 0u ? 0xff80u : top_bits(lo);           // (no bound: -inf)
+      const __nv_bfloat162 bound = __halves2bfloat162(__ushort_as_bfloat16(uint16_t(bits)), __ushort_as_bfloat16(uint16_t(bits)));
+      uint4 w0 = tid < q.pieces ? ld_stream_v4(src + tid) : make_uint4(0u, 0u, 0u, 0u);
+      uint4 w1 = tid + nt < q.pieces ? ld_stream_v4(src + tid + nt) : make_uint4(0u, 0u, 0u, 0u);
       for (int i = tid; i < q.pieces; i += nt) {
-        const uint4 w = piece(i);
-        const uint32_t wi[4] = {w.x, w.y, w.z, w.w}, skip = q.outside(i);
+        uint4 w = w0;
+        w0 = w1;
+        if (i + 2 * nt < q.pieces) w1 = ld_stream_v4(src + i + 2 * nt);
+        const uint32_t out = q.outside(i);
+        if (out) clear_outside(w, out);
+        const uint32_t wi[4] = {w.x, w.y, w.z, w.w};
+        uint32_t skip = out;
+        uint32_t ge[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ge[j] = __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&wi[j]), bound);
+        if (ge[0] | ge[1] | ge[2] | ge[3]) {
+          uint32_t hit = 0u;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) hit |= (ge[j] & 1u) << (2 * j) | (ge[j] >> 31) << (2 * j + 1);
+          hit &= ~out;
+          skip |= hit;
+          for (; hit != 0u; hit &= hit - 1u) {
+            const int at = __ffs(int(hit)) - 1, n = atomicAdd(&s_n, 1);
+            const uint32_t word = at < 4 ? (at < 2 ? wi[0] : wi[1]) : (at < 6 ? wi[2] : wi[3]);
+            if (n < kTopMaxCandidates)
+              s_cand[n] = uint64_t(top_key(at & 1 ? word >> 16 : word & 0xffffu)) << 32 | uint32_t(~uint32_t(i * 8 + at - q.off));
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 u = cap.u2(wi[j]);
-          const float2 s = Cap::signed2(wi[j], u, cap.zt);
+          const float2 s = Cap<TABLE>::capped2(wi[j], cap.minus_u(wi[j], nan), cap.zt);
           float2 e = make_float2(ds_ex2(s.x), ds_ex2(s.y));
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int at = 2 * j + h;
-            const uint32_t key = top_key(h ? wi[j] >> 16 : wi[j] & 0xffffu);
-            if (skip >> at & 1u) {
-              (h ? e.y : e.x) = 0.f;
-            } else if (key >= bound) {
-              (h ? e.y : e.x) = 0.f;
-              if (strict && key == bound) {
-                ++equal;
-              } else {
-                const int n = atomicAdd(&s_n, 1);
-                if (n < kTopMaxCandidates) s_cand[n] = uint64_t(key) << 32 | uint32_t(~uint32_t(i * 8 + at - q.off));
-              }
-            }
+          if (skip) {
+            if (skip >> (2 * j) & 1u) e.x = 0.f;
+            if (skip >> (2 * j + 1) & 1u) e.y = 0.f;
           }
           acc = __fadd2_rn(acc, e);
         }
       }
-      __syncthreads();
-      return s_n;
-    };
-    int n = collect(lo, false);
+    }
+    if (Cap<TABLE>::is_nan(nan)) acc.x = __int_as_float(0x7fffffff);
+    float others = acc.x + acc.y;
+    const bool odd = __syncthreads_or(isnan(others));
+    int n = s_n;
     float extra = 0.f;                         // the sum of candidates that are not kept
-    if (n > kTopMaxCandidates) {
+    if (n > kTopMaxCandidates || n < k || odd) {
       // the k-th largest key of the row
-      uint32_t key = lo;
-      for (uint32_t add = 0x8000u; add != 0u; add >>= 1) {
-        const uint32_t probe = key + add;
-        if (probe > 0xffffu) continue;
-        int c = 0;
-        for (int i = tid; i < q.pieces; i += nt) {
-          const uint4 w = piece(i);
-          const uint32_t wi[4] = {w.x, w.y, w.z, w.w}, skip = q.outside(i);
+      auto keys_of = [&](int i, auto&& f) {
+        const uint4 w = ld_stream_v4(src + i);
+        const uint32_t wi[4] = {w.x, w.y, w.z, w.w}, skip = q.outside(i);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) c += !(skip >> j & 1u) && top_key(j & 1 ? wi[j >> 1] >> 16 : wi[j >> 1] & 0xffffu) >= probe;
-        }
-        if (count(c) >= k) key = probe;
+        for (int j = 0; j < 8; ++j)
+          if (!(skip >> j & 1u)) f(j, top_key(j & 1 ? wi[j >> 1] >> 16 : wi[j >> 1] & 0xffffu));
+      };
+      uint32_t key = 0u;
+      for (uint32_t bit = 0x8000u; bit != 0u; bit >>= 1) {
+        int c = 0;
+        for (int i = tid; i < q.pieces; i += nt) keys_of(i, [&](int, uint32_t v) { c += v >= (key | bit); });
+        if (count(c) >= k) key |= bit;
       }
-      n = collect(key, true);                  // fewer than k
-      const int equals = count(equal), want = k - n;
+      if (tid == 0) s_n = 0;
+      __syncthreads();
+      // those above it, fewer than k; how many equal it; the sum of those below
+      int equal = 0;
+      others = 0.f;
+      for (int i = tid; i < q.pieces; i += nt)
+        keys_of(i, [&](int j, uint32_t v) {
+          if (v > key) s_cand[atomicAdd(&s_n, 1)] = uint64_t(v) << 32 | uint32_t(~uint32_t(i * 8 + j - q.off));
+          else if (v == key) ++equal;
+          else others += expf(cap.z_over_t(__uint_as_float(top_bits(v) << 16)));
+        });
+      const int equals = count(equal), above = s_n, want = k - above;
       // the first `want` of its equals: block after block of pieces, each thread's in its place by a prefix sum
       int have = 0;
       for (int i0 = 0; have < want; i0 += nt) {
         const int i = i0 + tid;
         uint32_t mine = 0u;
-        if (i < q.pieces) {
-          const uint4 w = piece(i);
-          const uint32_t wi[4] = {w.x, w.y, w.z, w.w}, skip = q.outside(i);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (!(skip >> j & 1u) && top_key(j & 1 ? wi[j >> 1] >> 16 : wi[j >> 1] & 0xffffu) == key) mine |= 1u << j;
-        }
+        if (i < q.pieces) keys_of(i, [&](int j, uint32_t v) { mine |= uint32_t(v == key) << j; });
         int before = __popc(mine);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -480,7 +607,7 @@ __global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs
         }
         turn ^= 1;
         for (; mine != 0u && at < want; mine &= mine - 1u, ++at)
-          s_cand[n + at] = uint64_t(key) << 32 | uint32_t(~uint32_t(i * 8 + __ffs(int(mine)) - 1 - q.off));
+          s_cand[above + at] = uint64_t(key) << 32 | uint32_t(~uint32_t(i * 8 + __ffs(int(mine)) - 1 - q.off));
         have += all;
       }
       __syncthreads();
@@ -488,16 +615,29 @@ __global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs
       n = k;
     }
     // ---- each candidate's place; from there on all in the order of places, so that results do not depend on that of the atomics
+    for (int i = tid; i < kTopBins; i += nt) s_hist[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += nt) atomicAdd(s_hist + bin(uint32_t(s_cand[i] >> 32)), 1);
+    __syncthreads();
+    if (warp == 0) scan(0, true);
+    __syncthreads();
     for (int i = tid; i < n; i += nt) {
-      const uint64_t mine = s_cand[i];
-      int r = 0;
-      for (int j = 0; j < n; ++j) r += s_cand[j] > mine;
-      s_sorted[r] = mine;
+      const uint64_t c = s_cand[i];
+      s_sorted[atomicAdd(s_begin + bin(uint32_t(c >> 32)), 1)] = c;      // (a bin's beginning becomes its end)
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += nt) {
+      const uint64_t mine = s_sorted[i];
+      const uint32_t b = bin(uint32_t(mine >> 32));
+      const int end = s_begin[b], begin = end - s_hist[b];
+      int r = begin;
+      for (int j = begin; j < end; ++j) r += s_sorted[j] > mine;
+      s_cand[r] = mine;
     }
     __syncthreads();
     float kept = 0.f, s = 0.f;
     for (int r = tid; r < n; r += nt) {
-      const float v = cap.z_over_t(__uint_as_float(top_bits(uint32_t(s_sorted[r] >> 32)) << 16));
+      const float v = cap.z_over_t(__uint_as_float(top_bits(uint32_t(s_cand[r] >> 32)) << 16));
       if (r < k) {
         s = v;
         kept = expf(v);
@@ -505,10 +645,10 @@ __global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs
         extra += expf(v);
       }
     }
-    float sums[2] = {acc.x + acc.y + extra, kept};
+    float sums[2] = {others + extra, kept};
     ds_block_sum(sums, s_red, warps);
     if (tid < k) {
-      p.ids[row * k + tid] = int32_t(~uint32_t(s_sorted[tid]));
+      p.ids[row * k + tid] = int32_t(~uint32_t(s_cand[tid]));
       p.logp[row * k + tid] = s - logf(sums[0] + sums[1]);
     }
     if (tid == 0) p.log_rest[row] = log_share(sums[0], sums[1]);
@@ -521,46 +661,64 @@ static int ds_threads(int64_t pieces, int least) {
   const int64_t want = std::max<int64_t>((pieces + 63) / 64 * 32, (least + 31) / 32 * 32);
   return int(std::min<int64_t>(std::max<int64_t>(want, 32), kDsMaxThreads));
 }
-static int64_t ds_row_bytes(int64_t vocab) { return (vocab + 14) / 8 * 16; }
 static int64_t ds_map_bytes(int64_t vocab) { return (((vocab + 14) / 8 / 4 + 1) * 4 + 15) / 16 * 16; }
 
-// Dynamic shared memory for `kern`, once per device and kernel.
+// Whether the logits that a block meets pay for its table.
+static bool ds_table(int64_t rows, int64_t vocab) { return std::max<int64_t>(1, rows / (2 * sm_count())) * vocab >= 16384; }
+
+// Blocks of nt threads that an SM holds of `kern`, whose registers and static shared memory are looked up once per device.
+struct DsKernelInfo {
+  std::atomic<int> registers[64];
+  std::atomic<int> smem[64];
+};
 template <typename K>
-static int ds_allow(K kern, std::atomic<bool> (&done)[64]) {
+static int ds_blocks(K kern, DsKernelInfo& info, int most_smem, int smem, int nt, int64_t rows, int* blocks) {
   int dev = 0;
   TG_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return TG_ERR_SHAPE;
-  if (!done[dev].load(std::memory_order_acquire)) {
-    TG_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kDsDynamicMax)));
-    done[dev].store(true, std::memory_order_release);
+  if (info.registers[dev].load(std::memory_order_acquire) == 0) {
+    cudaFuncAttributes a;
+    TG_CUDA_CHECK(cudaFuncGetAttributes(&a, kern));
+    TG_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem));
+    info.smem[dev].store(int(a.sharedSizeBytes), std::memory_order_relaxed);
+    info.registers[dev].store(a.numRegs, std::memory_order_release);
   }
+  const int per_warp = (info.registers[dev].load(std::memory_order_acquire) * 32 + 255) / 256 * 256;
+  const int64_t by_registers = 65536 / (int64_t(per_warp) * (nt / 32));
+  const int64_t by_smem = (228 * 1024) / (smem + info.smem[dev].load(std::memory_order_relaxed) + 1024);
+  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>({by_registers, by_smem, 2048 / nt, 32}));
+  *blocks = int(std::min<int64_t>(rows, sm_count() * per_sm));
   return TG_OK;
 }
 
-template <bool TWO, bool GRAD, bool STAGED>
+template <int EXPS, bool GRAD, bool TABLE>
+static int launch_distill(const DistillArgs& a, int nt, cudaStream_t st) {
+  static DsKernelInfo info;
+  auto kern = softcap_distill_kernel<EXPS, GRAD, TABLE>;
+  const int table = TABLE ? kCapTableBytes : 0, smem = int(ds_map_bytes(a.vocab)) + table;
+  int blocks;
+  if (int rc = ds_blocks(kern, info, int(ds_map_bytes(kDsMaxVocab)) + table, smem, nt, a.rows, &blocks)) return rc;
+  TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, kern, dim3(unsigned(blocks)), nt, size_t(smem), st, a));
+  return TG_OK;
+}
+template <int EXPS, bool GRAD>
 static int launch_distill(const DistillArgs& a, cudaStream_t st) {
-  static std::atomic<bool> done[64];
-  auto kern = softcap_distill_kernel<TWO, GRAD, STAGED>;
-  if (int rc = ds_allow(kern, done)) return rc;
-  const int64_t smem = ds_map_bytes(a.vocab) + (GRAD && STAGED ? ds_row_bytes(a.vocab) : 0);
   const int nt = ds_threads((a.vocab + 14) / 8, a.k);
-  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>({(227 * 1024) / (smem + 8 * 1024), 2048 / nt, 24}));
-  const int blocks = int(std::min<int64_t>(a.rows, int64_t(sm_count()) * per_sm));
-  TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, kern, dim3(unsigned(blocks)), nt, size_t(smem), st, a));
-  return TG_OK;
+  return ds_table(a.rows, a.vocab) ? launch_distill<EXPS, GRAD, true>(a, nt, st) : launch_distill<EXPS, GRAD, false>(a, nt, st);
 }
 
-template <bool STAGED>
-static int launch_top(const TopArgs& a, cudaStream_t st) {
-  static std::atomic<bool> done[64];
-  auto kern = top_logits_kernel<STAGED>;
-  if (int rc = ds_allow(kern, done)) return rc;
-  const int64_t smem = STAGED ? ds_row_bytes(a.vocab) : 0;
-  const int nt = ds_threads((a.vocab + 14) / 8, a.k);
-  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>({(227 * 1024) / (smem + 18 * 1024), 2048 / nt, 24}));
-  const int blocks = int(std::min<int64_t>(a.rows, int64_t(sm_count()) * per_sm));
-  TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, kern, dim3(unsigned(blocks)), nt, size_t(smem), st, a));
+template <bool TABLE>
+static int launch_top(const TopArgs& a, int nt, cudaStream_t st) {
+  static DsKernelInfo info;
+  const int smem = TABLE ? kCapTableBytes : 0;
+  int blocks;
+  if (int rc = ds_blocks(top_logits_kernel<TABLE>, info, smem, smem, nt, a.rows, &blocks)) return rc;
+  TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, top_logits_kernel<TABLE>, dim3(unsigned(blocks)), nt, size_t(smem), st, a));
   return TG_OK;
+}
+static int launch_top(const TopArgs& a, cudaStream_t st) {
+  const int nt = ds_threads((a.vocab + 14) / 8, a.k);
+  return ds_table(a.rows, a.vocab) ? launch_top<true>(a, nt, st) : launch_top<false>(a, nt, st);
 }
 
 static bool ds_cap_fits(float cap, float temperature) {
@@ -581,7 +739,7 @@ extern "C" int tg_top_logits(const void* logits, float cap, float temperature, i
   if (int rc = check_arch()) return rc;
   const TopArgs a = {logits, cap, temperature, ids, logp, log_rest, int(rows), int(vocab), k, ld};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return ds_row_bytes(vocab) <= kDsDynamicMax ? launch_top<true>(a, st) : launch_top<false>(a, st);
+  return launch_top(a, st);
 }
 
 extern "C" int tg_softcap_distill(const tg_distill_args* args, void* stream) {
@@ -598,12 +756,14 @@ extern "C" int tg_softcap_distill(const tg_distill_args* args, void* stream) {
   if (int rc = check_arch()) return rc;
   // one sum does where there is one temperature
   const bool soft = g.weight > 0.f, hard = g.weight < 1.f && g.targets != nullptr;
-  const bool two = soft && hard && g.temperature != 1.0f;
-  const DistillArgs a = {g.logits, g.ids, g.logp, g.log_rest, hard ? g.targets : nullptr, g.ids_64, g.targets_64, g.cap, soft ? g.temperature : 1.0f,
+  const float t = soft ? g.temperature : 1.0f;
+  const int exps = !(soft && hard) || t == 1.0f ? 1 : t == 2.0f ? 3 : t == 4.0f ? 4 : 2;
+  const DistillArgs a = {g.logits, g.ids, g.logp, g.log_rest, hard ? g.targets : nullptr, g.ids_64, g.targets_64, g.cap, t,
                          g.weight, g.dlogits, g.gscale, g.only_if_scaled, g.row_loss, int(g.rows), int(g.vocab), g.k, g.ld};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool staged = ds_map_bytes(g.vocab) + ds_row_bytes(g.vocab) <= kDsDynamicMax;
-  if (g.dlogits == nullptr) return two ? launch_distill<true, false, false>(a, st) : launch_distill<false, false, false>(a, st);
-  if (staged) return two ? launch_distill<true, true, true>(a, st) : launch_distill<false, true, true>(a, st);
-  return two ? launch_distill<true, true, false>(a, st) : launch_distill<false, true, false>(a, st);
+  const bool grad = g.dlogits != nullptr;
+  if (exps == 1) return grad ? launch_distill<1, true>(a, st) : launch_distill<1, false>(a, st);
+  if (exps == 2) return grad ? launch_distill<2, true>(a, st) : launch_distill<2, false>(a, st);
+  if (exps == 3) return grad ? launch_distill<3, true>(a, st) : launch_distill<3, false>(a, st);
+  return grad ? launch_distill<4, true>(a, st) : launch_distill<4, false>(a, st);
 }
