@@ -7,6 +7,7 @@
 // of its first and last piece that belong to other rows are read with them and take no part.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "host_api.h"
@@ -14,8 +15,9 @@
 
 namespace tg {
 
-constexpr int kDsMaxThreads = 512;
-constexpr int kDsMaxVocab = 1 << 20;
+constexpr int kDsMaxThreads = 512;                  // of a row
+constexpr int64_t kDsSmemMax = 227 * 1024;
+constexpr int kDsMaxVocab = 1 << 19;
 constexpr int kTopMaxCandidates = 1024;
 constexpr float kDsLog2e = 1.4426950408889634f;
 
@@ -31,65 +33,93 @@ __device__ __forceinline__ float ds_rcp(float v) {
 }
 __device__ __forceinline__ float ds_lds(uint32_t addr) {
   float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
   return v;
 }
 
 // The cap.  u = 1 - tanh |x / c| = 2 / (1 + exp(2 |x| / c)) keeps its relative precision where tanh saturates, so that
 // sech^2(x / c) = u (2 - u) does too; z / T = sign(x) (c / T) (1 - u).  Handed out as -u.
 //
-// Two ways to it.  Two approximations of the special function unit, an exponential and a reciprocal (a third one is the exponential of
-// z / T): 16 of them a clock and SM, so six clocks for 32 logits.  Or a table: x is a bf16 value, so between 2^-24 c, below
-// which z is as good as +-2^-24 c, and 16 c, from where on tanh is 1, it has 29 binades of 128 values.  A look-up of 32 random entries
-// takes 3.5 clocks of shared memory and leaves the special function unit two.
-constexpr int kCapBinadesBelow = 24, kCapBinades = 29;
+// Three approximations of the special function unit a logit (two exponentials and a reciprocal), 16 of them a clock and SM, are six clocks for 32
+// logits.  x is a bf16 value, though, and everything here a function of it: between 2^-22 c, below which z is as good as +-2^-22 c,
+// and 16 c, from where on tanh is 1, it has 27 binades of 128 values.  A table over those (of -u by the magnitude, 14 KB, or of E = exp(z / T)
+// by magnitude and sign, twice that) makes it a look-up, 3.5 clocks of shared memory for 32 random entries, and fewer instructions.
+// A quarter of the logits (the last word of four) goes the other way, so that both units work.
+enum { kTabU = 1, kTabE = 2 };
+constexpr int kCapBinadesBelow = 22, kCapBinades = 27;
 constexpr int kCapEntries = kCapBinades * 128 + 1;
 constexpr int kCapTableBytes = (kCapEntries * 4 + 15) / 16 * 16;
+constexpr int kCapSign = 4096;                                             // entries from the positive logits' to the negative ones'
+constexpr int cap_bytes(int table) { return table == 0 ? 0 : table == kTabU ? kCapTableBytes : kCapSign * 4 + kCapTableBytes; }
 
-template <bool TABLE>
+template <int TABLES>
 struct Cap {
   float k2;            // 2 log2(e) / c
   float zt;            // c log2(e) / T: z / T in powers of two is sign(x) zt (1 - u)
   float c, inv_c, inv_t;
-  uint32_t lo2, hi2;   // the table's first and last magnitude as bf16 bits, twice
-  uint32_t tab2;       // (its address) - 4 lo, twice: plus a pair of magnitudes times 4, two 16-bit addresses
-  __device__ __forceinline__ Cap(float cap, float temperature, void* table) {
+  uint32_t minus_lo2;  // minus the table's first magnitude as bf16 bits, twice
+  uint32_t tab2;       // its address, twice: plus a pair of entries times 4, two 16-bit addresses
+  __device__ __forceinline__ Cap(float cap, float temperature, void* tables) {
     c = cap;
     inv_c = __fdiv_rn(1.0f, cap);
     inv_t = __fdiv_rn(1.0f, temperature);
     k2 = 2.0f * kDsLog2e * inv_c;
     zt = cap * kDsLog2e * inv_t;
-    if constexpr (TABLE) {
+    if constexpr (TABLES != 0) {
       const uint32_t c_pow = (__float_as_uint(cap) >> 16) & 0x7f80u;     // 2^floor(log2 c)
-      const uint32_t lo = c_pow - (kCapBinadesBelow << 7), hi = lo + (kCapBinades << 7);
-      float* t = static_cast<float*>(table);
-      for (int i = threadIdx.x; i < kCapEntries; i += blockDim.x)
-        t[i] = __fdiv_rn(-2.0f, 1.0f + expf(2.0f * (__uint_as_float((lo + uint32_t(i)) << 16) * inv_c)));
-      lo2 = lo * 0x10001u;
-      hi2 = hi * 0x10001u;
-      tab2 = (uint32_t(__cvta_generic_to_shared(table)) - 4u * lo) * 0x10001u;
+      const uint32_t lo = c_pow - (kCapBinadesBelow << 7);
+      float* t = static_cast<float*>(tables);
+      for (int i = threadIdx.x; i < kCapEntries; i += blockDim.x) {
+        const float nu = __fdiv_rn(-2.0f, 1.0f + expf(2.0f * (__uint_as_float((lo + uint32_t(i)) << 16) * inv_c)));
+        if (TABLES & kTabU) t[i] = nu;
+        if (TABLES & kTabE) {
+          const float s = __fmaf_rn(nu, zt, zt);
+          t[i] = ds_ex2(s);
+          t[kCapSign + i] = ds_ex2(-s);
+        }
+      }
+      minus_lo2 = ((0x10000u - lo) & 0xffffu) * 0x10001u;
+      tab2 = uint32_t(__cvta_generic_to_shared(tables)) * 0x10001u;
     }
   }
-  // -u of the two logits of a word.  `top` collects the largest magnitudes: the table has no NaN
-  __device__ __forceinline__ float2 minus_u(uint32_t w, uint32_t& top) const {
-    const uint32_t mag = w & 0x7fff7fffu;
-    if constexpr (TABLE) {
-      top = __vmaxu2(top, mag);
-      const uint32_t at = __vminu2(__vmaxu2(mag, lo2), hi2) * 4u + tab2;
-      return make_float2(ds_lds(at & 0xffffu), ds_lds(at >> 16));
-    } else {
-      const float2 a = __fmul2_rn(bf16x2_unpack(mag), make_float2(k2, k2));
-      const float2 d = __fadd2_rn(make_float2(ds_ex2(a.x), ds_ex2(a.y)), make_float2(1.f, 1.f));
-      return __fmul2_rn(make_float2(ds_rcp(d.x), ds_rcp(d.y)), make_float2(-2.f, -2.f));
-    }
+  // two entries by magnitude, or by magnitude and sign
+  __device__ __forceinline__ float2 look_up(uint32_t w, bool by_sign) const {
+    uint32_t at = __viaddmin_s16x2_relu(w & 0x7fff7fffu, minus_lo2, uint32_t(kCapEntries - 1) * 0x10001u);   // max(min(mag - lo, last), 0)
+    if (by_sign) at |= (w >> 3) & 0x10001000u;
+    at = at * 4u + tab2;
+    return make_float2(ds_lds(at & 0xffffu), ds_lds(at >> 16));
   }
-  static __device__ __forceinline__ bool is_nan(uint32_t top) { return TABLE && ((top & 0xffffu) > 0x7f80u || (top >> 16) > 0x7f80u); }
+  __device__ __forceinline__ float2 direct_minus_u(uint32_t w) const {
+    const float2 a = __fmul2_rn(bf16x2_unpack(w & 0x7fff7fffu), make_float2(k2, k2));
+    const float2 d = __fadd2_rn(make_float2(ds_ex2(a.x), ds_ex2(a.y)), make_float2(1.f, 1.f));
+    return __fmul2_rn(make_float2(ds_rcp(d.x), ds_rcp(d.y)), make_float2(-2.f, -2.f));
+  }
   // sign(x) scale (1 - u), the capped logits in the units of `scale`
   static __device__ __forceinline__ float2 capped2(uint32_t w, float2 minus_u, float scale) {
     const uint32_t b = __float_as_uint(scale);
     const float2 s = make_float2(__uint_as_float(b ^ ((w << 16) & 0x80000000u)), __uint_as_float(b ^ (w & 0x80000000u)));
     return __ffma2_rn(minus_u, s, s);
   }
+  static __device__ __forceinline__ float2 ex2_2(float2 s) { return make_float2(ds_ex2(s.x), ds_ex2(s.y)); }
+  // -sech^2
+  static __device__ __forceinline__ float2 minus_sech2(float2 nu) { return __fmul2_rn(nu, __fadd2_rn(make_float2(2.f, 2.f), nu)); }
+
+  // Of the two logits of word J of a piece: -u, and E
+  template <int J>
+  __device__ __forceinline__ float2 minus_u(uint32_t w) const {
+    if constexpr ((TABLES & kTabU) && J != 3) return look_up(w, false);
+    else return direct_minus_u(w);
+  }
+  template <int J>
+  __device__ __forceinline__ float2 e(uint32_t w) const {
+    if constexpr ((TABLES & kTabE) && J != 3) return look_up(w, true);
+    else return ex2_2(capped2(w, minus_u<J>(w), zt));
+  }
+  // The table has no NaN: the largest magnitude of each half of the words that were looked up, and whether one was among them
+  static __device__ __forceinline__ uint32_t largest(const uint4& w) {
+    return TABLES == 0 ? 0u : __vimax3_u16x2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu, w.z & 0x7fff7fffu);
+  }
+  static __device__ __forceinline__ bool is_nan(uint32_t top) { return TABLES != 0 && ((top & 0xffffu) > 0x7f80u || (top >> 16) > 0x7f80u); }
   // the few logits of a row whose own value counts (kept ones, the target) by CUDA's accurate functions
   __device__ __forceinline__ float z_over_t(float x) const { return __fmul_rn(c * tanhf(x * inv_c), inv_t); }
   __device__ __forceinline__ float z(float x) const { return c * tanhf(x * inv_c); }
@@ -98,53 +128,110 @@ struct Cap {
     return u * (2.0f - u);
   }
 };
+// f(0, w.x), ... with the word's number as a constant
+template <typename F>
+__device__ __forceinline__ void four_words(const uint4& w, F&& f) {
+  f(std::integral_constant<int, 0>(), w.x);
+  f(std::integral_constant<int, 1>(), w.y);
+  f(std::integral_constant<int, 2>(), w.z);
+  f(std::integral_constant<int, 3>(), w.w);
+}
 
 // A row's 16-byte pieces.
 struct DsRow {
   const uint16_t* base;          // the 16-byte boundary at or below the row's start
   int off;                       // elements of the first piece that belong to what lies before the row
-  int pieces, end;               // pieces that hold any element of the row; the row's end, counted from base
+  int end;                       // the row's end, counted from base
   __device__ __forceinline__ DsRow(const void* logits, int64_t row, int64_t ld, int vocab) {
     const uint16_t* s = static_cast<const uint16_t*>(logits) + row * ld;
     off = int((reinterpret_cast<uintptr_t>(s) & 15u) >> 1);
     base = s - off;
     end = off + vocab;
-    pieces = (end + 7) >> 3;
+  }
+  // the pieces that are the row's as a whole: [first, last); one more may lie before them and one behind
+  __device__ __forceinline__ int first() const { return off != 0; }
+  __device__ __forceinline__ int last() const { return end >> 3; }
+  __device__ __forceinline__ const uint4* pieces() const { return reinterpret_cast<const uint4*>(base); }
+  // The elements of the other two, one for each of sixteen lanes: its place counted from base, or -1
+  __device__ __forceinline__ int edge(int lane) const {
+    if (lane < 8) return off != 0 && lane >= off && lane < end ? lane : -1;
+    const int e = last() * 8 + lane - 8;
+    return lane < 16 && last() >= first() && e >= off && e < end ? e : -1;
   }
   // which elements of piece i are not the row's, a bit each
   __device__ __forceinline__ uint32_t outside(int i) const {
     uint32_t m = i == 0 ? (1u << off) - 1u : 0u;
-    if (i == pieces - 1 && (end & 7)) m |= 0xffu & ~((1u << (end & 7)) - 1u);
+    if (i == last()) m |= 0xffu & ~((1u << (end & 7)) - 1u);
     return m;
   }
 };
 
-// zeros in the place of a piece's elements that are not the row's
-__device__ __forceinline__ void clear_outside(uint4& w, uint32_t out) {
-  uint32_t* p = &w.x;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) p[j] &= (out >> (2 * j) & 1u ? 0u : 0xffffu) | (out >> (2 * j + 1) & 1u ? 0u : 0xffff0000u);
-}
+// A thread's whole pieces of a row, every nt-th from its first one on: two of them are fetched by themselves, long before they are needed, and
+// two stay on their way.
+struct Pieces {
+  uint4 w0, w1;
+  __device__ __forceinline__ void fetch(const DsRow& q, int tid, int nt) {
+    const int i = q.first() + tid;
+    w0 = i < q.last() ? ld_stream_v4(q.pieces() + i) : make_uint4(0u, 0u, 0u, 0u);
+    w1 = i + nt < q.last() ? ld_stream_v4(q.pieces() + i + nt) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  // f(w, i) for each i below `end` (what is beyond the row's last is not read)
+  template <typename F>
+  __device__ __forceinline__ void each(const DsRow& q, int end, int tid, int nt, F&& f) {
+    const int last = q.last();
+    int i = q.first() + tid;
+    const uint4* p = q.pieces() + i + 2 * nt;
+#pragma unroll 1
+    for (; i < end; i += 2 * nt, p += 2 * nt) {
+      f(w0, i);
+      if (i + 2 * nt < last) w0 = ld_stream_v4(p);
+      if (i + nt < end) {
+        f(w1, i + nt);
+        if (i + 3 * nt < last) w1 = ld_stream_v4(p + nt);
+      }
+    }
+  }
+};
 
 __device__ __forceinline__ float ds_warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// Sums over the block of N values a thread, the same bits in every thread.  `s` holds N floats a warp; a barrier has to lie between two
-// uses of one `s`.
+// The threads that work on one row: a thread block, or one of two groups of a block that share its table.
+struct Group {
+  int index, tid, nt;
+  __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, %1;" ::"r"(1 + index), "r"(nt) : "memory"); }
+  __device__ __forceinline__ bool sync_or(bool v) const {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(uint32_t(v)), "r"(1 + index), "r"(nt) : "memory");
+    return r != 0u;
+  }
+};
+
+// Sums over a group of N values a thread, the same bits in every thread, in two halves with a barrier between them: each warp's into `s`
+// (N floats a warp), and those of the first `warps`.
 template <int N>
-__device__ __forceinline__ void ds_block_sum(float (&v)[N], float* s, int warps) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ void ds_warp_sums(float (&v)[N], float* s, int warp, bool wanted) {
+  if (!wanted) return;
 #pragma unroll
   for (int n = 0; n < N; ++n) v[n] = ds_warp_sum(v[n]);
-  if (lane == 0) {
+  if ((threadIdx.x & 31) == 0) {
 #pragma unroll
     for (int n = 0; n < N; ++n) s[n * (kDsMaxThreads / 32) + warp] = v[n];
   }
-  __syncthreads();
+}
+template <int N>
+__device__ __forceinline__ void ds_add_warps(float (&v)[N], const float* s, int warps) {
+  const int at = threadIdx.x & (kDsMaxThreads / 32 - 1);
 #pragma unroll
-  for (int n = 0; n < N; ++n) v[n] = ds_warp_sum(lane < warps ? s[n * (kDsMaxThreads / 32) + lane] : 0.f);
+  for (int n = 0; n < N; ++n) {
+    float t = at < warps ? s[n * (kDsMaxThreads / 32) + at] : 0.f;
+#pragma unroll
+    for (int o = kDsMaxThreads / 64; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    v[n] = t;
+  }
 }
 
 // log of part / (part + other), from the smaller of the two where the result is near 0
@@ -154,10 +241,15 @@ __device__ __forceinline__ float log_share(float part, float other) {
 }
 
 // ---------------------------------------------------------------------------------------
-// The student's loss and its gradient.  One thread block per row.  First pass: the sum of exp(z / T) (and of exp(z)) over all logits that the
-// teacher does not name; those it does are marked in a bitmap, a byte per piece, and computed by one thread each.  Second pass: the gradient,
-// from the row read again -- 600 rows of 100 KB are in work at a time, which the L2 holds -- after which the threads of the named
-// logits and the target write theirs over it.
+// The student's loss and its gradient.  A group of threads per row.  First pass: the sum of exp(z / T) (and of exp(z)) over all logits that the
+// teacher does not name.  Those it does are marked in a bitmap, a byte per piece, and computed by one thread each; what else is in a piece with a
+// mark is added by the thread of its lowest one, which is the same whatever the order of the marks was.  Second pass: the gradient, from the
+// row as the first has left it in shared memory, after which the threads of the named logits and the target write theirs over it.
+// (Read again instead -- a vocabulary that does not fit is -- a third of it comes from memory, with 444 rows of 100 KB and their gradients in
+// work: 8192 x 50304 with 64 logits 551 us, of which the second pass 330, however little it computes.)  Two rows of 50304 logits
+// fit on an SM only with one table for both, hence the groups.
+// A row has three barriers, and a chain of loads (an id, its logit) at its beginning: its first pieces and the next row's ids and logits are
+// fetched a phase ahead, and the next row as a whole comes as far as the L2 during the second pass.
 // EXPS: 1 where one sum does (one temperature, or one of the two losses), 2 for two exponentials, 3 and 4 where the second is the first one
 // squared once or twice (temperatures 2 and 4).
 // ---------------------------------------------------------------------------------------
@@ -175,213 +267,292 @@ struct DistillArgs {
   float* row_loss;
   int rows, vocab, k;
   int64_t ld;
+  int groups, group_bytes;                     // of a block; shared memory of each behind the table
 };
 
+// an id as it is given, and -1 for one outside the vocabulary
 __device__ __forceinline__ int ds_index(const void* p, int is64, int64_t at, int vocab) {
   const int64_t v = is64 ? static_cast<const int64_t*>(p)[at] : static_cast<const int32_t*>(p)[at];
   return v >= 0 && v < vocab ? int(v) : -1;
 }
 
-template <int EXPS, bool GRAD, bool TABLE>
-__global__ void __launch_bounds__(kDsMaxThreads) softcap_distill_kernel(const DistillArgs p) {
+constexpr int distill_table(int exps, bool grad) { return exps == 2 || grad ? kTabU : kTabE; }
+constexpr int ds_map_bytes(int64_t vocab) { return int(((vocab + 14) / 8 + 15) / 16 * 16); }
+constexpr int64_t ds_row_bytes(int64_t vocab) { return (vocab + 14) / 8 * 16; }
+
+template <int EXPS, bool GRAD, bool TABLE, bool STAGED>
+__global__ void __launch_bounds__(GRAD ? 2 * kDsMaxThreads : kDsMaxThreads / 2, GRAD ? 1 : 4) softcap_distill_kernel(const DistillArgs p) {
   constexpr bool TWO = EXPS > 1;
+  constexpr int TABLES = TABLE ? distill_table(EXPS, GRAD) : 0;
+  using C = Cap<TABLES>;
   grid_trigger();
   grid_wait();
   if (p.only_if_scaled && *p.gscale == 1.0f) return;
   extern __shared__ __align__(16) uint8_t s_ds[];
-  __shared__ float s_red[6 * (kDsMaxThreads / 32)], s_loss[kDsMaxThreads / 32];
-  __shared__ int s_ids[kDsMaxThreads];
-  __shared__ float s_p[kDsMaxThreads];
-  const int tid = int(threadIdx.x), nt = int(blockDim.x), warps = nt >> 5;
-  const int map_words = (p.vocab + 14) / 8 / 4 + 1;
-  const uint8_t* s_named = s_ds + (TABLE ? kCapTableBytes : 0);
-  uint32_t* s_map = reinterpret_cast<uint32_t*>(s_ds + (TABLE ? kCapTableBytes : 0));
-  for (int i = tid; i < map_words; i += nt) s_map[i] = 0u;
-  const Cap<TABLE> cap(p.cap, p.temperature, s_ds);
+  __shared__ float s_reds[2][5 * (kDsMaxThreads / 32)], s_losses[2][kDsMaxThreads / 32];
+  const C cap(p.cap, p.temperature, s_ds);
+  const int nt = int(blockDim.x) / p.groups, index = int(threadIdx.x) / nt;
+  const Group group = {index, int(threadIdx.x) - index * nt, nt};
+  const int tid = group.tid, warps = nt >> 5, lane = tid & 31, warp = tid >> 5;
+  float *const s_red = s_reds[index], *const s_loss = s_losses[index];
+  uint8_t* const s_mine = s_ds + cap_bytes(TABLES) + index * p.group_bytes;
+  const int map_bytes = ds_map_bytes(p.vocab);
+  uint32_t* const s_map = reinterpret_cast<uint32_t*>(s_mine);
+  const uint8_t* const s_named = s_mine;
+  uint4* const s_row = reinterpret_cast<uint4*>(s_mine + map_bytes);       // the row's whole pieces, each in a place of its thread's own
+  for (int i = tid; i < map_bytes / 4; i += nt) s_map[i] = 0u;
   const float z1 = p.cap * kDsLog2e;
   const float t = p.temperature, w_soft = p.weight, w_hard = 1.0f - p.weight;
   const float gs = GRAD ? (p.gscale != nullptr ? *p.gscale : 1.0f) * __fdiv_rn(1.0f, float(p.rows)) : 0.f;
-  // exp(z) of a pair, from its exp(z / T) or anew
-  auto second = [&](float2 e, uint32_t w, float2 nu) {
-    if constexpr (EXPS > 2) {
+  // exp(z) of a pair from its exp(z / T)
+  auto squared = [&](float2 e) {
 #pragma unroll
-      for (int i = 2; i < EXPS; ++i) e = __fmul2_rn(e, e);
-      return e;
+    for (int i = 2; i < EXPS; ++i) e = __fmul2_rn(e, e);
+    return e;
+  };
+  // exp(z / T) and exp(z) of word J of a piece
+  auto both = [&](auto j, uint32_t w, float2& e1) {
+    constexpr int J = decltype(j)::value;
+    if constexpr (EXPS == 2) {
+      const float2 nu = cap.template minus_u<J>(w);
+      e1 = C::ex2_2(C::capped2(w, nu, z1));
+      return C::ex2_2(C::capped2(w, nu, cap.zt));
     } else {
-      const float2 sz = Cap<TABLE>::capped2(w, nu, z1);
-      return make_float2(ds_ex2(sz.x), ds_ex2(sz.y));
+      const float2 e = cap.template e<J>(w);
+      e1 = squared(e);
+      return e;
     }
   };
-  __syncthreads();
 
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const DsRow q(p.logits, row, p.ld, p.vocab);
-    const uint16_t* x_row = q.base + q.off;
+  // what a row needs besides its pieces, fetched in two steps
+  int id = -1, target = -1;
+  float lp = 0.f, rest = 0.f;
+  uint4 named = make_uint4(0u, 0u, 0u, 0u);    // the piece of logit `id`
+  uint32_t x_target = 0u, x_end = 0u;          // the target's logit (thread 0), that of this lane at the row's ends (last warp)
+  auto fetch_ids = [&](int64_t row) {
+    id = tid < p.k ? ds_index(p.ids, p.ids_64, row * p.k + tid, p.vocab) : -1;
+    lp = id >= 0 ? p.logp[row * p.k + tid] : 0.f;
+    rest = p.log_rest != nullptr ? p.log_rest[row] : -INFINITY;
+    target = p.targets != nullptr ? ds_index(p.targets, p.targets_64, row, p.vocab) : -1;
+  };
+  auto fetch_logits = [&](const DsRow& q) {
+    if (id >= 0) named = ld_stream_v4(q.pieces() + ((id + q.off) >> 3));
+    if (tid == 0 && target >= 0) x_target = q.base[q.off + target];
+    if (warp == warps - 1 && q.edge(lane) >= 0) x_end = q.base[q.edge(lane)];
+  };
+
+  __syncthreads();                             // (the table; from here on the groups go their own ways)
+  const int64_t step = int64_t(gridDim.x) * p.groups;
+  int64_t row = int64_t(blockIdx.x) * p.groups + index;
+  if (row >= p.rows) return;
+  DsRow q(p.logits, row, p.ld, p.vocab);
+  Pieces in;                                   // (not STAGED)
+  const uint32_t slot0 = uint32_t(__cvta_generic_to_shared(s_row)) + uint32_t(tid) * 16u;
+  if constexpr (STAGED) {
+    uint32_t to = slot0;
+    const uint4* from = q.pieces() + q.first() + tid;
+    for (int i = q.first() + tid; i < q.last(); i += nt, to += uint32_t(nt) * 16u, from += nt) cp_async16(to, from);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  } else {
+    in.fetch(q, tid, nt);
+  }
+  fetch_ids(row);
+  fetch_logits(q);
+  while (row < p.rows) {
     // ---- what the teacher names, a thread each
-    int id = -1;
-    float lp = 0.f, prob = 0.f, x = 0.f;
-    if (tid < p.k) {
-      id = ds_index(p.ids, p.ids_64, row * p.k + tid, p.vocab);
-      if (id >= 0) {
-        lp = p.logp[row * p.k + tid];
-        prob = expf(lp);
-        x = __uint_as_float(uint32_t(x_row[id]) << 16);
-      }
-    }
-    const float rest = p.log_rest != nullptr ? p.log_rest[row] : -INFINITY;
-    const int target = p.targets != nullptr ? ds_index(p.targets, p.targets_64, row, p.vocab) : -1;
+    const int at = id + q.off;
+    const bool present = id >= 0;
     bool again = false;                        // another thread has the same logit
-    if (id >= 0) {
-      const int at = id + q.off;
-      const uint32_t bit = 1u << (at & 31);
-      again = atomicOr(s_map + (at >> 5), bit) & bit;
+    if (present) again = atomicOr(s_map + (at >> 5), 1u << (at & 31)) >> (at & 31) & 1u;
+    const float prob = present ? expf(lp) : 0.f;
+    float x = 0.f, s_here = 0.f, e_here = 0.f, e1_here = 0.f;
+    if (present) {
+      const uint32_t word = at & 4 ? (at & 2 ? named.w : named.z) : (at & 2 ? named.y : named.x);
+      x = __uint_as_float(at & 1 ? word & 0xffff0000u : word << 16);
+      s_here = cap.z_over_t(x);
+      e_here = expf(s_here);
+      e1_here = TWO ? expf(cap.z(x)) : 0.f;
     }
-    s_ids[tid] = id;
-    s_p[tid] = prob;
-    const bool repeats = __syncthreads_or(again);
-    bool first = id >= 0;                      // it is this thread's to count the logit and to write its gradient
+    const float xt_here = __uint_as_float(x_target << 16);             // (thread 0's)
+    const float rest_here = rest, lp_here = lp;
+    const int target_here = target, id_here = id;
+    const bool repeats = group.sync_or(again);
+    bool first = present;                      // it is this thread's to count the logit and to write its gradient
     float prob_here = prob;                    // the teacher's probability for the logit, entries that repeat it added up in order
-    if (repeats && id >= 0) {
+    if (repeats && present) {
       prob_here = 0.f;
       for (int i = 0; i < p.k; ++i)
-        if (s_ids[i] == id) {
+        if (ds_index(p.ids, p.ids_64, row * p.k + i, p.vocab) == id) {
           first &= i >= tid;
-          prob_here += s_p[i];
+          prob_here += expf(p.logp[row * p.k + i]);
         }
     }
-    const float s_here = id >= 0 ? cap.z_over_t(x) : 0.f;
-    const float e_here = id >= 0 ? expf(s_here) : 0.f;
-    const float e1_here = TWO && id >= 0 ? expf(cap.z(x)) : 0.f;
+    const bool target_named = tid == 0 && target >= 0 && (s_map[(target + q.off) >> 5] >> ((target + q.off) & 31) & 1u);
 
     // ---- first pass
     float2 acc = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
     uint32_t top = 0u;
-    const uint4* src = reinterpret_cast<const uint4*>(q.base);
-    uint4 w0 = tid < q.pieces ? ld_stream_v4(src + tid) : make_uint4(0u, 0u, 0u, 0u);
-    uint4 w1 = tid + nt < q.pieces ? ld_stream_v4(src + tid + nt) : make_uint4(0u, 0u, 0u, 0u);
-    for (int i = tid; i < q.pieces; i += nt) {
-      uint4 w = w0;
-      w0 = w1;
-      if (i + 2 * nt < q.pieces) w1 = ld_stream_v4(src + i + 2 * nt);
-      const uint32_t out = q.outside(i), skip = uint32_t(s_named[i]) | out;
-      if (out) clear_outside(w, out);
-      const uint32_t wi[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 nu = cap.minus_u(wi[j], top);
-        const float2 s = Cap<TABLE>::capped2(wi[j], nu, cap.zt);
-        float2 e = make_float2(ds_ex2(s.x), ds_ex2(s.y));
-        if (skip) {
-          if (skip >> (2 * j) & 1u) e.x = 0.f;
-          if (skip >> (2 * j + 1) & 1u) e.y = 0.f;
-        }
-        acc = __fadd2_rn(acc, e);
-        if constexpr (EXPS > 2) {
-          acc1 = __fadd2_rn(acc1, second(e, wi[j], nu));
-        } else if constexpr (EXPS == 2) {
-          float2 e1 = second(e, wi[j], nu);
-          if (skip) {
-            if (skip >> (2 * j) & 1u) e1.x = 0.f;
-            if (skip >> (2 * j + 1) & 1u) e1.y = 0.f;
-          }
-          acc1 = __fadd2_rn(acc1, e1);
-        }
-      }
+    auto add_some = [&](const uint4& w, uint32_t skip) {               // a piece's elements without a bit in `skip`
+      four_words(w, [&](auto j, uint32_t v) {
+        const uint32_t out = skip >> (2 * j) & 3u;
+        v &= (out & 1u ? 0u : 0xffffu) | (out & 2u ? 0u : 0xffff0000u);
+        if (TABLES != 0) top = __vmaxu2(top, v & 0x7fff7fffu);
+        float2 e1;
+        const float2 e = both(j, v, e1);
+        acc = __fadd2_rn(acc, make_float2(out & 1u ? 0.f : e.x, out & 2u ? 0.f : e.y));
+        if (TWO) acc1 = __fadd2_rn(acc1, make_float2(out & 1u ? 0.f : e1.x, out & 2u ? 0.f : e1.y));
+      });
+    };
+    // (the named logits of a piece that is not the row's as a whole leave the others to the lanes below)
+    if (first && at >> 3 >= q.first() && at >> 3 < q.last()) {
+      const uint32_t marks = s_named[at >> 3];
+      if ((marks & ((1u << (at & 7)) - 1u)) == 0u) add_some(named, marks);
     }
-    if (Cap<TABLE>::is_nan(top)) acc.x = acc1.x = __int_as_float(0x7fffffff);
-    float sums[TWO ? 5 : 3] = {acc.x + acc.y, first ? e_here : 0.f, prob};
+    // the two pieces at the row's ends, an element per lane of the last warp
+    const int edge = warp == warps - 1 ? q.edge(lane) : -1;
+    const bool edge_mine = edge >= 0 && !(s_map[edge >> 5] >> (edge & 31) & 1u);
+    const float x_edge = __uint_as_float(x_end << 16);
+    float e_edge = 0.f, e1_edge = 0.f;
+    if (edge_mine) {
+      e_edge = expf(cap.z_over_t(x_edge));
+      e1_edge = TWO ? expf(cap.z(x_edge)) : 0.f;
+      acc.x += e_edge;
+      if (TWO) acc1.x += e1_edge;
+    }
+    const int64_t next = row + step;
+    const DsRow q_next(p.logits, next < p.rows ? next : row, p.ld, p.vocab);
+    if (next < p.rows) fetch_ids(next);
+    auto add = [&](const uint4& w, int i) {
+      const bool skip = s_named[i] != 0;
+      float2 e[4], e1[4];
+      four_words(w, [&](auto j, uint32_t v) { e[j] = both(j, v, e1[j]); });
+      // (no branch: the look-ups do not wait for the mark)
+      const float2 sum = __fadd2_rn(__fadd2_rn(e[0], e[1]), __fadd2_rn(e[2], e[3]));
+      acc = __fadd2_rn(acc, make_float2(skip ? 0.f : sum.x, skip ? 0.f : sum.y));
+      if (TABLE) top = __vmaxu2(top, C::largest(w));                 // (a NaN that is named is one of the row's all the same)
+      if (TWO) {
+        const float2 sum1 = __fadd2_rn(__fadd2_rn(e1[0], e1[1]), __fadd2_rn(e1[2], e1[3]));
+        acc1 = __fadd2_rn(acc1, make_float2(skip ? 0.f : sum1.x, skip ? 0.f : sum1.y));
+      }
+    };
+    if constexpr (STAGED) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      uint32_t slot = slot0;
+#pragma unroll 1
+      for (int i = q.first() + tid; i < q.last(); i += nt, slot += uint32_t(nt) * 16u) add(lds128(slot), i);
+    } else {
+      in.each(q, q.last(), tid, nt, add);
+      in.fetch(GRAD ? q : q_next, tid, nt);
+    }
+    if (next < p.rows) fetch_logits(q_next);
+    if (C::is_nan(top)) acc.x = acc1.x = __int_as_float(0x7fffffff);
+    // (the entries' sums by the warps that have entries)
+    const int entry_warps = (p.k + 31) >> 5;
+    float of_row[TWO ? 2 : 1] = {acc.x + acc.y}, of_entries[TWO ? 3 : 2] = {first ? e_here : 0.f, prob};
     if constexpr (TWO) {
-      sums[3] = acc1.x + acc1.y;
-      sums[4] = first ? e1_here : 0.f;
+      of_row[1] = acc1.x + acc1.y;
+      of_entries[2] = first ? e1_here : 0.f;
     }
-    ds_block_sum(sums, s_red, warps);
-    const float tail = sums[0], kept = sums[1], total = tail + kept, inv = __fdiv_rn(1.0f, total);
-    const float total1 = TWO ? sums[3] + sums[TWO ? 4 : 0] : total;
-    const float p_rest = expf(rest), mass = sums[2] + p_rest;
-
-    // ---- the row's loss
-    float term = 0.f;
-    if (prob > 0.f) {
-      const float share = e_here * inv;
-      term = prob * (lp - (share > 1e-30f ? logf(share) : s_here - logf(total)));
-    }
-    float terms[1] = {term};
-    ds_block_sum(terms, s_loss, warps);
-    if (tid == 0 && p.row_loss != nullptr) {
-      float loss = terms[0];
-      if (p_rest > 0.f) loss += p_rest * (rest - log_share(tail, kept));
-      loss *= w_soft * t * t;
-      if (w_soft == 0.f) loss = 0.f;
-      if (target >= 0 && w_hard != 0.f) {
-        const float xt = __uint_as_float(uint32_t(x_row[target]) << 16);
-        loss += w_hard * (logf(total1) - cap.z(xt));
+    ds_warp_sums(of_row, s_red, warp, true);
+    ds_warp_sums(of_entries, s_red + 2 * (kDsMaxThreads / 32), warp, warp < entry_warps);
+    group.sync();
+    ds_add_warps(of_row, s_red, warps);
+    ds_add_warps(of_entries, s_red + 2 * (kDsMaxThreads / 32), entry_warps);
+    const float tail = of_row[0], kept = of_entries[0], total = tail + kept, inv = __fdiv_rn(1.0f, total);
+    const float total1 = TWO ? of_row[TWO ? 1 : 0] + of_entries[TWO ? 2 : 0] : total;
+    const float p_rest = expf(rest_here), mass = of_entries[1] + p_rest;
+    if (present) s_map[at >> 5] = 0u;          // (last looked at before the sums)
+    // ---- the entries' share of the row's loss
+    if (warp < entry_warps) {
+      float term = 0.f;
+      if (prob > 0.f) {
+        const float share = e_here * inv;
+        term = prob * (lp_here - (share > 1e-30f ? logf(share) : s_here - logf(total)));
       }
-      p.row_loss[row] = loss;
+      term = ds_warp_sum(term);
+      if (lane == 0) s_loss[warp] = term;
     }
 
     // ---- second pass
+    const float soft = w_soft * t;
+    const float a = soft == 0.f ? 0.f : soft * (mass * inv - (p_rest > 0.f && tail > 0.f ? __fdiv_rn(p_rest, tail) : 0.f));
+    const float b = target_here >= 0 && w_hard != 0.f ? w_hard * __fdiv_rn(1.0f, total1) : 0.f;
+    uint16_t* d_base = static_cast<uint16_t*>(p.d) + (q.base - static_cast<const uint16_t*>(p.logits));
     if constexpr (GRAD) {
-      const float soft = w_soft * t;
-      const float a = soft == 0.f ? 0.f : soft * (mass * inv - (p_rest > 0.f && tail > 0.f ? __fdiv_rn(p_rest, tail) : 0.f));
-      const float b = target >= 0 && w_hard != 0.f ? w_hard * __fdiv_rn(1.0f, total1) : 0.f;
-      uint16_t* d_base = static_cast<uint16_t*>(p.d) + (q.base - static_cast<const uint16_t*>(p.logits));
       const float ab = TWO ? a : a + b;
-      const float2 a2 = make_float2(ab, ab), b2 = make_float2(b, b), gs2 = make_float2(-gs, -gs), two = make_float2(2.f, 2.f);
-      w0 = tid < q.pieces ? ld_stream_v4(src + tid) : make_uint4(0u, 0u, 0u, 0u);
-      w1 = tid + nt < q.pieces ? ld_stream_v4(src + tid + nt) : make_uint4(0u, 0u, 0u, 0u);
-      for (int i = tid; i < q.pieces; i += nt) {
-        const uint4 w = w0;
-        w0 = w1;
-        if (i + 2 * nt < q.pieces) w1 = ld_stream_v4(src + i + 2 * nt);
-        const uint32_t wi[4] = {w.x, w.y, w.z, w.w};
+      const float2 a2 = make_float2(ab, ab), b2 = make_float2(b, b), gs2 = make_float2(-gs, -gs);
+      auto body = [&](const uint4& w, int i) {
         uint4 o;
         uint32_t* op = &o.x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 nu = cap.minus_u(wi[j], top);
-          const float2 s = Cap<TABLE>::capped2(wi[j], nu, cap.zt);
-          const float2 e = make_float2(ds_ex2(s.x), ds_ex2(s.y));
-          float2 g = __fmul2_rn(a2, e);
-          if (TWO) g = __ffma2_rn(b2, second(e, wi[j], nu), g);
-          const float2 sech = __fmul2_rn(nu, __fadd2_rn(two, nu));       // (negative, as is gs2)
-          g = __fmul2_rn(g, __fmul2_rn(sech, gs2));
-          op[j] = pack_bf16x2(g.x, g.y);
+        four_words(w, [&](auto j, uint32_t v) {
+          constexpr int J = decltype(j)::value;
+          float2 g;
+          const float2 nu = cap.template minus_u<J>(v), e = C::ex2_2(C::capped2(v, nu, cap.zt));
+          g = __fmul2_rn(a2, e);
+          if constexpr (TWO) {
+            const float2 e1 = EXPS == 2 ? C::ex2_2(C::capped2(v, nu, z1)) : squared(e);
+            g = __ffma2_rn(b2, e1, g);
+          }
+          g = __fmul2_rn(g, __fmul2_rn(C::minus_sech2(nu), gs2));
+          op[J] = pack_bf16x2(g.x, g.y);
+        });
+        *reinterpret_cast<uint4*>(d_base + i * 8) = o;
+      };
+      if constexpr (STAGED) {
+        // a place that has been read takes the next row's piece, of which there may be one more
+        uint32_t slot = slot0;
+        const uint4* from = q_next.pieces() + q_next.first() + tid;
+        int more = next < p.rows ? q_next.last() - q_next.first() - tid : 0;
+#pragma unroll 1
+        for (int i = q.first() + tid; i < q.last(); i += nt, slot += uint32_t(nt) * 16u, from += nt, more -= nt) {
+          const uint4 w = lds128(slot);
+          if (more > 0) cp_async16(slot, from);
+          body(w, i);
         }
-        const uint32_t skip = q.outside(i);
-        if (skip == 0u) {
-          *reinterpret_cast<uint4*>(d_base + i * 8) = o;
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (!(skip >> j & 1u)) d_base[i * 8 + j] = uint16_t(j & 1 ? op[j >> 1] >> 16 : op[j >> 1] & 0xffffu);
-        }
+        if (more > 0) cp_async16(slot, from);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      } else {
+        in.each(q, q.last(), tid, nt, body);
+        in.fetch(q_next, tid, nt);
       }
-      __syncthreads();
-      auto write = [&](int at, float g, float x_at) {
-        reinterpret_cast<__nv_bfloat16*>(d_base)[at + q.off] = __float2bfloat16_rn(g * (cap.sech2(x_at) * gs));
+      if (edge_mine)
+        reinterpret_cast<__nv_bfloat16*>(d_base)[edge] = __float2bfloat16_rn((a * e_edge + b * (TWO ? e1_edge : e_edge)) * (cap.sech2(x_edge) * gs));
+    }
+    group.sync();
+    if constexpr (GRAD) {
+      auto write = [&](int column, float g, float x_at) {
+        reinterpret_cast<__nv_bfloat16*>(d_base)[column + q.off] = __float2bfloat16_rn(g * (cap.sech2(x_at) * gs));
       };
       if (first) {
         float g = (soft == 0.f ? 0.f : soft * (mass * inv * e_here - prob_here)) + b * (TWO ? e1_here : e_here);
-        if (id == target) g -= w_hard;
-        write(id, g, x);
+        if (id_here == target_here) g -= w_hard;
+        write(id_here, g, x);
       }
-      if (tid == 0 && target >= 0 && !(s_map[(target + q.off) >> 5] >> ((target + q.off) & 31) & 1u)) {
-        const float xt = __uint_as_float(uint32_t(x_row[target]) << 16);
-        const float e = expf(cap.z_over_t(xt));
-        write(target, a * e + b * (TWO ? expf(cap.z(xt)) : e) - w_hard, xt);
+      if (tid == 0 && target_here >= 0 && !target_named) {
+        const float e = expf(cap.z_over_t(xt_here));
+        write(target_here, a * e + b * (TWO ? expf(cap.z(xt_here)) : e) - w_hard, xt_here);
       }
     }
-    __syncthreads();                           // (the target's thread has read the bitmap)
-    if (id >= 0) s_map[(id + q.off) >> 5] = 0u;
-    __syncthreads();
+    if (tid == 0 && p.row_loss != nullptr) {
+      float loss = 0.f;
+      for (int i = 0; i * 32 < p.k; ++i) loss += s_loss[i];
+      if (p_rest > 0.f) loss += p_rest * (rest_here - log_share(tail, kept));
+      loss = w_soft == 0.f ? 0.f : loss * (w_soft * t * t);
+      if (target_here >= 0 && w_hard != 0.f) loss += w_hard * (logf(total1) - cap.z(xt_here));
+      p.row_loss[row] = loss;
+    }
+    row = next;
+    q = q_next;
   }
+  if constexpr (STAGED) asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------------------
 // A teacher's top logits.  One thread block per row.  The first pass finds the largest logit of every group (the even and the odd elements
 // of a thread's pieces are a group each).  The k-th largest of the groups' maxima is a lower bound of the k-th largest logit
-// that few others reach: with 1024 groups about 1024 ln(1 / (1 - k / 1024)) logits.  The second pass, over the row as the L2 holds it, collects
-// those and sums exp(z / T) of all others.  Candidates are sorted by counting into bins of two keys, then within their bin.
+// that few others reach: with 1024 groups about 1024 ln(1 / (1 - k / 1024)) logits.  The second pass, over the row as the L2 holds it, sums exp(z / T)
+// over the pieces that have none of those and marks the others, a bit each; they follow in their order, a thread each, so that a warp does
+// not go through a branch for nearly every 32 pieces.  The candidates are then sorted by counting into bins of two keys, and within their bin.
 // Where the bound lets too many through (a row of equal logits, large ones side by side), or a NaN is among them, the k-th largest logit is found by
 // bisection on the row's 16-bit keys, and its equals are taken in the row's order.
 // ---------------------------------------------------------------------------------------
@@ -405,7 +576,7 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t key) { return key >= 0x800
 constexpr int kTopBins = 256;
 
 template <bool TABLE>
-__global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs p) {
+__global__ void __launch_bounds__(kDsMaxThreads / 2, 4) top_logits_kernel(const TopArgs p) {
   grid_trigger();
   grid_wait();
   extern __shared__ __align__(16) uint8_t s_ds[];
@@ -413,34 +584,39 @@ __global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs
   __shared__ uint64_t s_cand[kTopMaxCandidates], s_sorted[kTopMaxCandidates];
   __shared__ __align__(16) int s_hist[kTopBins];
   __shared__ int s_begin[kTopBins], s_count[2][kDsMaxThreads / 32], s_n;
+  uint32_t* s_marks = reinterpret_cast<uint32_t*>(s_ds + cap_bytes(TABLE ? kTabE : 0));      // a bit per piece
+  uint32_t* s_list = reinterpret_cast<uint32_t*>(s_sorted);                                  // the marked ones
   __shared__ uint32_t s_bound;
   const int tid = int(threadIdx.x), nt = int(blockDim.x), warps = nt >> 5, lane = tid & 31, warp = tid >> 5;
-  const Cap<TABLE> cap(p.cap, p.temperature, s_ds);
+  using C = Cap<TABLE ? kTabE : 0>;
+  const C cap(p.cap, p.temperature, s_ds);
   const int k = p.k;
   __syncthreads();
 
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const DsRow q(p.logits, row, p.ld, p.vocab);
-    const uint4* src = reinterpret_cast<const uint4*>(q.base);
+  int64_t row = blockIdx.x;
+  if (row >= p.rows) return;
+  DsRow q(p.logits, row, p.ld, p.vocab);
+  Pieces in;
+  in.fetch(q, tid, nt);
+  for (int64_t next; row < p.rows; row = next) {
+    next = row + gridDim.x;
+    const DsRow q_next(p.logits, next < p.rows ? next : row, p.ld, p.vocab);
+    const uint4* src = q.pieces();
+    const int pieces = (q.end + 7) >> 3;
     // ---- first pass: the groups' maxima (NaN aside), as keys; 0 for a group of none
     uint32_t top[2];
     {
-      uint4 w0 = tid < q.pieces ? ld_stream_v4(src + tid) : make_uint4(0u, 0u, 0u, 0u);
-      uint4 w1 = tid + nt < q.pieces ? ld_stream_v4(src + tid + nt) : make_uint4(0u, 0u, 0u, 0u);
       __nv_bfloat162 m = __halves2bfloat162(__ushort_as_bfloat16(0x7fff), __ushort_as_bfloat16(0x7fff));
-      for (int i = tid; i < q.pieces; i += nt) {
-        uint4 w = w0;
-        w0 = w1;
-        if (i + 2 * nt < q.pieces) w1 = ld_stream_v4(src + i + 2 * nt);
-        const uint32_t out = q.outside(i);
-        uint32_t* wi = &w.x;
-        if (out) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) wi[j] |= (out >> (2 * j) & 1u ? 0x7fffu : 0u) | (out >> (2 * j + 1) & 1u ? 0x7fff0000u : 0u);   // NaN
-        }
-        const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(wi);
+      in.each(q, q.last(), tid, nt, [&](const uint4& w, int) {
+        const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&w);
         m = __hmax2(m, __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
+      });
+      const int edge = warp == warps - 1 ? q.edge(lane) : -1;
+      if (edge >= 0) {
+        const __nv_bfloat16 v = __ushort_as_bfloat16(q.base[edge]);
+        m = __hmax2(m, __halves2bfloat162(v, v));
       }
+      in.fetch(q, tid, nt);                    // the second pass's
       const uint32_t bits = *reinterpret_cast<const uint32_t*>(&m);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -510,56 +686,81 @@ __global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs
         if (count(int(top[0] >= (lo | bit)) + int(top[1] >= (lo | bit))) >= k) lo |= bit;
     }
 
-    // ---- second pass: candidates, and the sum of the others
+    // ---- second pass: the sum over the pieces without a candidate (and wholly of the row), and which ones those are not
     float2 acc = make_float2(0.f, 0.f);
     uint32_t nan = 0u;
-    {
-      const uint32_t bits = lo == 0u ? 0xff80u : top_bits(lo);           // (no bound: -inf)
-      const __nv_bfloat162 bound = __halves2bfloat162(__ushort_as_bfloat16(uint16_t(bits)), __ushort_as_bfloat16(uint16_t(bits)));
-      uint4 w0 = tid < q.pieces ? ld_stream_v4(src + tid) : make_uint4(0u, 0u, 0u, 0u);
-      uint4 w1 = tid + nt < q.pieces ? ld_stream_v4(src + tid + nt) : make_uint4(0u, 0u, 0u, 0u);
-      for (int i = tid; i < q.pieces; i += nt) {
-        uint4 w = w0;
-        w0 = w1;
-        if (i + 2 * nt < q.pieces) w1 = ld_stream_v4(src + i + 2 * nt);
-        const uint32_t out = q.outside(i);
-        if (out) clear_outside(w, out);
-        const uint32_t wi[4] = {w.x, w.y, w.z, w.w};
-        uint32_t skip = out;
-        uint32_t ge[4];
+    const uint32_t lo_bits = lo == 0u ? 0xff80u : top_bits(lo);          // (no bound: -inf)
+    const __nv_bfloat162 bound = __halves2bfloat162(__ushort_as_bfloat16(uint16_t(lo_bits)), __ushort_as_bfloat16(uint16_t(lo_bits)));
+    auto reach = [&](uint32_t w) { return __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w), bound); };
+    // bit b of the marks is piece first + b (whole warps, for the ballot); the pieces at the row's ends are listed without one
+    const int whole = q.last() - q.first(), words = (whole + 31) >> 5;
+    in.each(q, q.first() + words * 32, tid, nt, [&](const uint4& w, int i) {
+        const bool skip = (reach(w.x) | reach(w.y) | reach(w.z) | reach(w.w)) != 0u || i >= q.last();
+        const uint32_t marks = __ballot_sync(0xffffffffu, skip && i < q.last());
+        if (lane == 0) s_marks[(i - q.first()) >> 5] = marks;
+        float2 e[4];
+        four_words(w, [&](auto j, uint32_t v) { e[j] = cap.template e<decltype(j)::value>(v); });
+        const float2 sum = __fadd2_rn(__fadd2_rn(e[0], e[1]), __fadd2_rn(e[2], e[3]));
+        acc = __fadd2_rn(acc, make_float2(skip ? 0.f : sum.x, skip ? 0.f : sum.y));
+        if (TABLE && i < q.last()) nan = __vmaxu2(nan, C::largest(w));
+    });
+    in.fetch(q_next, tid, nt);
+    __syncthreads();
+    // ---- the marked pieces, listed in order
+    int marked = 0;
+    for (int i0 = 0; i0 < words; i0 += nt) {
+      uint32_t m = i0 + tid < words ? s_marks[i0 + tid] : 0u;
+      int at = __popc(m);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ge[j] = __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&wi[j]), bound);
-        if (ge[0] | ge[1] | ge[2] | ge[3]) {
-          uint32_t hit = 0u;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) hit |= (ge[j] & 1u) << (2 * j) | (ge[j] >> 31) << (2 * j + 1);
-          hit &= ~out;
-          skip |= hit;
-          for (; hit != 0u; hit &= hit - 1u) {
-            const int at = __ffs(int(hit)) - 1, n = atomicAdd(&s_n, 1);
-            const uint32_t word = at < 4 ? (at < 2 ? wi[0] : wi[1]) : (at < 6 ? wi[2] : wi[3]);
-            if (n < kTopMaxCandidates)
-              s_cand[n] = uint64_t(top_key(at & 1 ? word >> 16 : word & 0xffffu)) << 32 | uint32_t(~uint32_t(i * 8 + at - q.off));
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 s = Cap<TABLE>::capped2(wi[j], cap.minus_u(wi[j], nan), cap.zt);
-          float2 e = make_float2(ds_ex2(s.x), ds_ex2(s.y));
-          if (skip) {
-            if (skip >> (2 * j) & 1u) e.x = 0.f;
-            if (skip >> (2 * j + 1) & 1u) e.y = 0.f;
-          }
-          acc = __fadd2_rn(acc, e);
-        }
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += x;
       }
+      if (lane == 31) s_count[turn][warp] = at;
+      at += marked - __popc(m);
+      __syncthreads();
+      const int c = lane < warps ? s_count[turn][lane] : 0;
+      at += __reduce_add_sync(0xffffffffu, lane < warp ? c : 0);
+      marked += __reduce_add_sync(0xffffffffu, c);
+      turn ^= 1;
+      for (; m != 0u; m &= m - 1u, ++at)
+        if (at < 2 * kTopMaxCandidates - 2) s_list[at] = uint32_t(q.first() + (i0 + tid) * 32 + __ffs(int(m)) - 1);
     }
-    if (Cap<TABLE>::is_nan(nan)) acc.x = __int_as_float(0x7fffffff);
+    const bool crowded = marked > 2 * kTopMaxCandidates - 2;
+    marked = min(marked, 2 * kTopMaxCandidates - 2);
+    if (q.first()) {
+      if (tid == 0) s_list[marked] = 0u;
+      ++marked;
+    }
+    if (q.last() >= q.first() && (q.end & 7)) {
+      if (tid == 0) s_list[marked] = uint32_t(q.last());
+      ++marked;
+    }
+    __syncthreads();
+    // ---- their candidates, and the sum of the others
+    for (int l = tid; l < marked; l += nt) {
+      const int i = int(s_list[l]);
+      const uint4 w = ld_stream_v4(src + i);
+      const uint32_t outside = q.outside(i);
+      four_words(w, [&](auto j, uint32_t v) {
+        const uint32_t ge = reach(v), out = outside >> (2 * j) & 3u;
+        const uint32_t hit = ((ge & 1u) | (ge >> 31) << 1) & ~out, off = hit | out;
+        for (uint32_t rest = hit; rest != 0u; rest &= rest - 1u) {
+          const int h = __ffs(int(rest)) - 1, n = atomicAdd(&s_n, 1);
+          if (n < kTopMaxCandidates) s_cand[n] = uint64_t(top_key(h ? v >> 16 : v & 0xffffu)) << 32 | uint32_t(~uint32_t(i * 8 + 2 * j + h - q.off));
+        }
+        const uint32_t rest = v & ((off & 1u ? 0u : 0xffffu) | (off & 2u ? 0u : 0xffff0000u));
+        if (TABLE) nan = __vmaxu2(nan, rest & 0x7fff7fffu);
+        const float2 e = cap.template e<decltype(j)::value>(rest);
+        acc = __fadd2_rn(acc, make_float2(off & 1u ? 0.f : e.x, off & 2u ? 0.f : e.y));
+      });
+    }
+    if (C::is_nan(nan)) acc.x = __int_as_float(0x7fffffff);
     float others = acc.x + acc.y;
     const bool odd = __syncthreads_or(isnan(others));
     int n = s_n;
     float extra = 0.f;                         // the sum of candidates that are not kept
-    if (n > kTopMaxCandidates || n < k || odd) {
+    if (crowded || n > kTopMaxCandidates || n < k || odd) {
       // the k-th largest key of the row
       auto keys_of = [&](int i, auto&& f) {
         const uint4 w = ld_stream_v4(src + i);
@@ -571,7 +772,7 @@ __global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs
       uint32_t key = 0u;
       for (uint32_t bit = 0x8000u; bit != 0u; bit >>= 1) {
         int c = 0;
-        for (int i = tid; i < q.pieces; i += nt) keys_of(i, [&](int, uint32_t v) { c += v >= (key | bit); });
+        for (int i = tid; i < pieces; i += nt) keys_of(i, [&](int, uint32_t v) { c += v >= (key | bit); });
         if (count(c) >= k) key |= bit;
       }
       if (tid == 0) s_n = 0;
@@ -579,7 +780,7 @@ __global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs
       // those above it, fewer than k; how many equal it; the sum of those below
       int equal = 0;
       others = 0.f;
-      for (int i = tid; i < q.pieces; i += nt)
+      for (int i = tid; i < pieces; i += nt)
         keys_of(i, [&](int j, uint32_t v) {
           if (v > key) s_cand[atomicAdd(&s_n, 1)] = uint64_t(v) << 32 | uint32_t(~uint32_t(i * 8 + j - q.off));
           else if (v == key) ++equal;
@@ -591,7 +792,7 @@ __global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs
       for (int i0 = 0; have < want; i0 += nt) {
         const int i = i0 + tid;
         uint32_t mine = 0u;
-        if (i < q.pieces) keys_of(i, [&](int j, uint32_t v) { mine |= uint32_t(v == key) << j; });
+        if (i < pieces) keys_of(i, [&](int j, uint32_t v) { mine |= uint32_t(v == key) << j; });
         int before = __popc(mine);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -646,78 +847,93 @@ __global__ void __launch_bounds__(kDsMaxThreads) top_logits_kernel(const TopArgs
       }
     }
     float sums[2] = {others + extra, kept};
-    ds_block_sum(sums, s_red, warps);
+    ds_warp_sums(sums, s_red, warp, true);
+    __syncthreads();
+    ds_add_warps(sums, s_red, warps);
     if (tid < k) {
       p.ids[row * k + tid] = int32_t(~uint32_t(s_cand[tid]));
       p.logp[row * k + tid] = s - logf(sums[0] + sums[1]);
     }
     if (tid == 0) p.log_rest[row] = log_share(sums[0], sums[1]);
     __syncthreads();
+    q = q_next;
   }
 }
 
-// Threads for a row of `pieces` 16-byte pieces, two pieces each up to the most there are, and at least `least`.
-static int ds_threads(int64_t pieces, int least) {
+// Threads for a row of `pieces` 16-byte pieces: two pieces each, at least `least` and at most `most` of them.
+static int ds_threads(int64_t pieces, int least, int most) {
   const int64_t want = std::max<int64_t>((pieces + 63) / 64 * 32, (least + 31) / 32 * 32);
-  return int(std::min<int64_t>(std::max<int64_t>(want, 32), kDsMaxThreads));
+  return int(std::min<int64_t>(std::max<int64_t>(want, 32), most));
 }
-static int64_t ds_map_bytes(int64_t vocab) { return (((vocab + 14) / 8 / 4 + 1) * 4 + 15) / 16 * 16; }
 
 // Whether the logits that a block meets pay for its table.
 static bool ds_table(int64_t rows, int64_t vocab) { return std::max<int64_t>(1, rows / (2 * sm_count())) * vocab >= 16384; }
 
-// Blocks of nt threads that an SM holds of `kern`, whose registers and static shared memory are looked up once per device.
+// Blocks of `threads` that an SM holds of `kern`, whose registers and static shared memory are looked up once per device.
 struct DsKernelInfo {
   std::atomic<int> registers[64];
   std::atomic<int> smem[64];
 };
 template <typename K>
-static int ds_blocks(K kern, DsKernelInfo& info, int most_smem, int smem, int nt, int64_t rows, int* blocks) {
+static int ds_blocks(K kern, DsKernelInfo& info, int64_t smem, int threads, int64_t* per_sm) {
   int dev = 0;
   TG_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return TG_ERR_SHAPE;
   if (info.registers[dev].load(std::memory_order_acquire) == 0) {
     cudaFuncAttributes a;
     TG_CUDA_CHECK(cudaFuncGetAttributes(&a, kern));
-    TG_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem));
+    TG_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kDsSmemMax - int64_t(a.sharedSizeBytes))));
     info.smem[dev].store(int(a.sharedSizeBytes), std::memory_order_relaxed);
     info.registers[dev].store(a.numRegs, std::memory_order_release);
   }
   const int per_warp = (info.registers[dev].load(std::memory_order_acquire) * 32 + 255) / 256 * 256;
-  const int64_t by_registers = 65536 / (int64_t(per_warp) * (nt / 32));
+  const int64_t by_registers = 65536 / (int64_t(per_warp) * (threads / 32));
   const int64_t by_smem = (228 * 1024) / (smem + info.smem[dev].load(std::memory_order_relaxed) + 1024);
-  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>({by_registers, by_smem, 2048 / nt, 32}));
-  *blocks = int(std::min<int64_t>(rows, sm_count() * per_sm));
+  *per_sm = std::max<int64_t>(1, std::min<int64_t>({by_registers, by_smem, 2048 / threads, 32}));
   return TG_OK;
 }
 
-template <int EXPS, bool GRAD, bool TABLE>
-static int launch_distill(const DistillArgs& a, int nt, cudaStream_t st) {
+constexpr int64_t kDsDynamicMax = kDsSmemMax - 2 * 1024;     // (less than 2 KB are static)
+
+template <int EXPS, bool GRAD, bool TABLE, bool STAGED>
+static int launch_distill(DistillArgs a, int nt, cudaStream_t st) {
   static DsKernelInfo info;
-  auto kern = softcap_distill_kernel<EXPS, GRAD, TABLE>;
-  const int table = TABLE ? kCapTableBytes : 0, smem = int(ds_map_bytes(a.vocab)) + table;
-  int blocks;
-  if (int rc = ds_blocks(kern, info, int(ds_map_bytes(kDsMaxVocab)) + table, smem, nt, a.rows, &blocks)) return rc;
-  TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, kern, dim3(unsigned(blocks)), nt, size_t(smem), st, a));
+  auto kern = softcap_distill_kernel<EXPS, GRAD, TABLE, STAGED>;
+  const int64_t table = TABLE ? cap_bytes(distill_table(EXPS, GRAD)) : 0, bytes = ds_map_bytes(a.vocab) + (STAGED ? ds_row_bytes(a.vocab) : 0);
+  // two groups in a block where two blocks do not fit on an SM beside each other
+  a.groups = STAGED && 2 * (table + bytes) > kDsDynamicMax && table + 2 * bytes <= kDsDynamicMax && a.rows > sm_count() ? 2 : 1;
+  a.group_bytes = int(bytes);
+  const int64_t smem = table + a.groups * bytes;
+  int64_t per_sm;
+  if (int rc = ds_blocks(kern, info, smem, nt * a.groups, &per_sm)) return rc;
+  const int blocks = int(std::min<int64_t>((a.rows + a.groups - 1) / a.groups, sm_count() * per_sm));
+  TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, kern, dim3(unsigned(blocks)), nt * a.groups, size_t(smem), st, a));
   return TG_OK;
 }
 template <int EXPS, bool GRAD>
 static int launch_distill(const DistillArgs& a, cudaStream_t st) {
-  const int nt = ds_threads((a.vocab + 14) / 8, a.k);
-  return ds_table(a.rows, a.vocab) ? launch_distill<EXPS, GRAD, true>(a, nt, st) : launch_distill<EXPS, GRAD, false>(a, nt, st);
+  // (the loss alone keeps nothing of a row: more and smaller blocks)
+  const int nt = ds_threads((a.vocab + 14) / 8, a.k, GRAD ? kDsMaxThreads : kDsMaxThreads / 2);
+  const bool table = ds_table(a.rows, a.vocab);
+  if constexpr (GRAD) {
+    if (kCapTableBytes + ds_map_bytes(a.vocab) + ds_row_bytes(a.vocab) <= kDsDynamicMax)
+      return table ? launch_distill<EXPS, true, true, true>(a, nt, st) : launch_distill<EXPS, true, false, true>(a, nt, st);
+  }
+  return table ? launch_distill<EXPS, GRAD, true, false>(a, nt, st) : launch_distill<EXPS, GRAD, false, false>(a, nt, st);
 }
 
 template <bool TABLE>
 static int launch_top(const TopArgs& a, int nt, cudaStream_t st) {
   static DsKernelInfo info;
-  const int smem = TABLE ? kCapTableBytes : 0;
-  int blocks;
-  if (int rc = ds_blocks(top_logits_kernel<TABLE>, info, smem, smem, nt, a.rows, &blocks)) return rc;
+  const int smem = ds_map_bytes(a.vocab) / 8 + 16 + (TABLE ? cap_bytes(kTabE) : 0);
+  int64_t per_sm;
+  if (int rc = ds_blocks(top_logits_kernel<TABLE>, info, smem, nt, &per_sm)) return rc;
+  const int blocks = int(std::min<int64_t>(a.rows, sm_count() * per_sm));
   TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, top_logits_kernel<TABLE>, dim3(unsigned(blocks)), nt, size_t(smem), st, a));
   return TG_OK;
 }
 static int launch_top(const TopArgs& a, cudaStream_t st) {
-  const int nt = ds_threads((a.vocab + 14) / 8, a.k);
+  const int nt = ds_threads((a.vocab + 14) / 8, a.k, kDsMaxThreads / 2);
   return ds_table(a.rows, a.vocab) ? launch_top<true>(a, nt, st) : launch_top<false>(a, nt, st);
 }
 
