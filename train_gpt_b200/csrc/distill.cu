@@ -7,6 +7,7 @@
 // of its first and last piece that belong to other rows are read with them and take no part.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "common.cuh"
@@ -198,7 +199,8 @@ __device__ __forceinline__ float ds_warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// The threads that work on one row: a thread block, or one of two groups of a block that share its table.
+// The threads that work on one row: a thread block, or one of up to eight groups of a block that share its table.
+constexpr int kDsMaxGroups = 8;
 struct Group {
   int index, tid, nt;
   __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, %1;" ::"r"(1 + index), "r"(nt) : "memory"); }
@@ -281,7 +283,7 @@ constexpr int ds_map_bytes(int64_t vocab) { return int(((vocab + 14) / 8 + 15) /
 constexpr int64_t ds_row_bytes(int64_t vocab) { return (vocab + 14) / 8 * 16; }
 
 template <int EXPS, bool GRAD, bool TABLE, bool STAGED>
-__global__ void __launch_bounds__(GRAD ? 2 * kDsMaxThreads : kDsMaxThreads / 2, GRAD ? 1 : 4) softcap_distill_kernel(const DistillArgs p) {
+__global__ void __launch_bounds__(2 * kDsMaxThreads, 1) softcap_distill_kernel(const DistillArgs p) {
   constexpr bool TWO = EXPS > 1;
   constexpr int TABLES = TABLE ? distill_table(EXPS, GRAD) : 0;
   using C = Cap<TABLES>;
@@ -289,7 +291,7 @@ __global__ void __launch_bounds__(GRAD ? 2 * kDsMaxThreads : kDsMaxThreads / 2, 
   grid_wait();
   if (p.only_if_scaled && *p.gscale == 1.0f) return;
   extern __shared__ __align__(16) uint8_t s_ds[];
-  __shared__ float s_reds[2][5 * (kDsMaxThreads / 32)], s_losses[2][kDsMaxThreads / 32];
+  __shared__ float s_reds[kDsMaxGroups][5 * (kDsMaxThreads / 32)], s_losses[kDsMaxGroups][kDsMaxThreads / 32];
   const C cap(p.cap, p.temperature, s_ds);
   const int nt = int(blockDim.x) / p.groups, index = int(threadIdx.x) / nt;
   const Group group = {index, int(threadIdx.x) - index * nt, nt};
@@ -548,13 +550,16 @@ __global__ void __launch_bounds__(GRAD ? 2 * kDsMaxThreads : kDsMaxThreads / 2, 
 }
 
 // ---------------------------------------------------------------------------------------
-// A teacher's top logits.  One thread block per row.  The first pass finds the largest logit of every group (the even and the odd elements
-// of a thread's pieces are a group each).  The k-th largest of the groups' maxima is a lower bound of the k-th largest logit
-// that few others reach: with 1024 groups about 1024 ln(1 / (1 - k / 1024)) logits.  The second pass, over the row as the L2 holds it, sums exp(z / T)
-// over the pieces that have none of those and marks the others, a bit each; they follow in their order, a thread each, so that a warp does
-// not go through a branch for nearly every 32 pieces.  The candidates are then sorted by counting into bins of two keys, and within their bin.
-// Where the bound lets too many through (a row of equal logits, large ones side by side), or a NaN is among them, the k-th largest logit is found by
-// bisection on the row's 16-bit keys, and its equals are taken in the row's order.
+// A teacher's top logits.  One thread block per row.  First a bound that at least k logits reach and few others: the largest logit of every
+// group (each of the eight elements of a thread's pieces is one) is found, and the k-th largest of those taken; with 1024 groups about
+// 1024 ln(1 / (1 - k / 1024)) logits reach it.  Where a row is long enough the groups come from an eighth of it, eight pieces of every
+// 64, and the bound is their `rank`-th largest: k / 8 with four standard deviations and four more, so that one row in some thousand has too
+// few.  (All of 8192 x 50304 read twice: 316 us with 8 logits kept, ... so.)
+// The pass over the row sums exp(z / T) over the pieces without a logit that reaches the bound and marks the others, a bit each; they follow in
+// their order, a thread each, so that a warp does not go through a branch for nearly every 32 pieces.  The candidates are then sorted
+// by counting into bins of a key or a few, and within their bin.
+// Where the bound lets too many or too few through (a row of equal logits, large ones side by side), or a NaN is among them, the k-th largest logit is
+// found by bisection on the row's 16-bit keys, and its equals are taken in the row's order.
 // ---------------------------------------------------------------------------------------
 struct TopArgs {
   const void* logits;
@@ -564,7 +569,10 @@ struct TopArgs {
   float* log_rest;
   int rows, vocab, k;
   int64_t ld;
+  int rank;                                    // k, or the sample's
+  int groups, room;                            // of a block; for candidates
 };
+constexpr int kTopSampleFrom = 16384 + 16, kTopSampleTo = 65536;       // logits of rows that are sampled: at most four pieces a thread
 
 // bf16 bits -> an unsigned key of the same order (-0 is 0; NaN above all)
 __device__ __forceinline__ uint32_t top_key(uint32_t bits) {
@@ -574,84 +582,99 @@ __device__ __forceinline__ uint32_t top_key(uint32_t bits) {
 __device__ __forceinline__ uint32_t top_bits(uint32_t key) { return key >= 0x8000u ? key - 0x8000u : 0x8000u | (0x8000u - key); }
 
 constexpr int kTopBins = 256;
+struct TopShared {                             // of a group, followed by room for the candidates, twice, and a bit per piece
+  int hist[kTopBins], begin[kTopBins];
+  float red[2 * (kDsMaxThreads / 32)];
+  int count[2][kDsMaxThreads / 32], n;
+  uint32_t bound;
+};
+static_assert(offsetof(TopShared, hist) % 16 == 0 && sizeof(TopShared) % 8 == 0, "read in 16-byte pieces");
+constexpr int top_group_bytes(int64_t vocab, int room) { return int((sizeof(TopShared) + room * 16 + ((vocab + 14) / 8 + 31) / 32 * 4 + 15) / 16 * 16); }
 
 template <bool TABLE>
-__global__ void __launch_bounds__(kDsMaxThreads / 2, 4) top_logits_kernel(const TopArgs p) {
+__global__ void __launch_bounds__(2 * kDsMaxThreads, 1) top_logits_kernel(const TopArgs p) {
   grid_trigger();
   grid_wait();
   extern __shared__ __align__(16) uint8_t s_ds[];
-  __shared__ float s_red[2 * (kDsMaxThreads / 32)];
-  __shared__ uint64_t s_cand[kTopMaxCandidates], s_sorted[kTopMaxCandidates];
-  __shared__ __align__(16) int s_hist[kTopBins];
-  __shared__ int s_begin[kTopBins], s_count[2][kDsMaxThreads / 32], s_n;
-  uint32_t* s_marks = reinterpret_cast<uint32_t*>(s_ds + cap_bytes(TABLE ? kTabE : 0));      // a bit per piece
-  uint32_t* s_list = reinterpret_cast<uint32_t*>(s_sorted);                                  // the marked ones
-  __shared__ uint32_t s_bound;
-  const int tid = int(threadIdx.x), nt = int(blockDim.x), warps = nt >> 5, lane = tid & 31, warp = tid >> 5;
+  const int nt = int(blockDim.x) / p.groups, index = int(threadIdx.x) / nt;
+  const Group group = {index, int(threadIdx.x) - index * nt, nt};
+  const int tid = group.tid, warps = nt >> 5, lane = tid & 31, warp = tid >> 5;
+  TopShared& sh = *reinterpret_cast<TopShared*>(s_ds + cap_bytes(TABLE ? kTabE : 0) + index * top_group_bytes(p.vocab, p.room));
+  uint64_t *const s_cand = reinterpret_cast<uint64_t*>(&sh + 1), *const s_sorted = s_cand + p.room;
+  uint32_t* const s_marks = reinterpret_cast<uint32_t*>(s_sorted + p.room);   // a bit per piece
+  uint32_t* const s_list = reinterpret_cast<uint32_t*>(s_sorted);             // the marked ones
   using C = Cap<TABLE ? kTabE : 0>;
   const C cap(p.cap, p.temperature, s_ds);
   const int k = p.k;
-  __syncthreads();
-
-  int64_t row = blockIdx.x;
+  __syncthreads();                             // (the table; from here on the groups go their own ways)
+  const int64_t step = int64_t(gridDim.x) * p.groups;
+  int64_t row = int64_t(blockIdx.x) * p.groups + index;
   if (row >= p.rows) return;
   DsRow q(p.logits, row, p.ld, p.vocab);
   Pieces in;
   in.fetch(q, tid, nt);
+  const bool sampled = p.vocab >= kTopSampleFrom && p.vocab <= kTopSampleTo;
   for (int64_t next; row < p.rows; row = next) {
-    next = row + gridDim.x;
+    next = row + step;
     const DsRow q_next(p.logits, next < p.rows ? next : row, p.ld, p.vocab);
     const uint4* src = q.pieces();
     const int pieces = (q.end + 7) >> 3;
     // ---- first pass: the groups' maxima (NaN aside), as keys; 0 for a group of none
-    uint32_t top[2];
+    uint32_t top[8], most = 0u;
     {
-      __nv_bfloat162 m = __halves2bfloat162(__ushort_as_bfloat16(0x7fff), __ushort_as_bfloat16(0x7fff));
-      in.each(q, q.last(), tid, nt, [&](const uint4& w, int) {
+      const __nv_bfloat162 none = __halves2bfloat162(__ushort_as_bfloat16(0x7fff), __ushort_as_bfloat16(0x7fff));
+      __nv_bfloat162 m[4] = {none, none, none, none};
+      auto look = [&](const uint4& w) {
         const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&w);
-        m = __hmax2(m, __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
-      });
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m[j] = __hmax2(m[j], v[j]);
+      };
+      if (sampled) {
+        const int n = (q.last() - q.first()) / 64 * 8;
+#pragma unroll 4
+        for (int i = tid; i < n; i += nt) look(ld_stream_v4(src + q.first() + (i >> 3) * 64 + (i & 7)));
+      } else {
+        in.each(q, q.last(), tid, nt, [&](const uint4& w, int) { look(w); });
+        in.fetch(q, tid, nt);
+      }
       const int edge = warp == warps - 1 ? q.edge(lane) : -1;
       if (edge >= 0) {
         const __nv_bfloat16 v = __ushort_as_bfloat16(q.base[edge]);
-        m = __hmax2(m, __halves2bfloat162(v, v));
+        m[0] = __hmax2(m[0], __halves2bfloat162(v, __ushort_as_bfloat16(0x7fff)));
       }
-      in.fetch(q, tid, nt);                    // the second pass's
-      const uint32_t bits = *reinterpret_cast<const uint32_t*>(&m);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t b = h ? bits >> 16 : bits & 0xffffu;
+      for (int h = 0; h < 8; ++h) {
+        const uint32_t word = *reinterpret_cast<const uint32_t*>(&m[h >> 1]), b = h & 1 ? word >> 16 : word & 0xffffu;
         top[h] = (b & 0x7fffu) > 0x7f80u ? 0u : top_key(b);
+        most = max(most, top[h]);
       }
     }
     // how many of the block's `n`s there are (the same value in every thread); two buffers, so that one barrier a call does
     int turn = 0;
     auto count = [&](int n) {
       n = __reduce_add_sync(0xffffffffu, n);
-      if (lane == 0) s_count[turn][warp] = n;
-      __syncthreads();
-      const int c = __reduce_add_sync(0xffffffffu, lane < warps ? s_count[turn][lane] : 0);
+      if (lane == 0) sh.count[turn][warp] = n;
+      group.sync();
+      const int c = __reduce_add_sync(0xffffffffu, lane < warps ? sh.count[turn][lane] : 0);
       turn ^= 1;
       return c;
     };
-    // ---- the bound: counts by distance from the largest, two keys a bin
-    uint32_t largest = __reduce_max_sync(0xffffffffu, max(top[0], top[1]));
-    if (lane == 0) s_count[turn][warp] = int(largest);
-    for (int i = tid; i < kTopBins; i += nt) s_hist[i] = 0;
-    __syncthreads();
-    largest = __reduce_max_sync(0xffffffffu, lane < warps ? uint32_t(s_count[turn][lane]) : 0u);
+    // ---- the bound: the rank-th largest of the groups' keys (0: there are not so many), by its upper and then by its lower byte
+    uint32_t largest = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) sh.count[turn][warp] = int(largest);
+    auto zero = [&] {
+      for (int i = tid; i < kTopBins; i += nt) sh.hist[i] = 0;
+    };
+    zero();
+    group.sync();
+    largest = __reduce_max_sync(0xffffffffu, lane < warps ? uint32_t(sh.count[turn][lane]) : 0u);
     turn ^= 1;
-    auto bin = [&](uint32_t key) { return key > largest ? 0u : min((largest - key) >> 1, uint32_t(kTopBins - 1)); };
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (top[h] != 0u) atomicAdd(s_hist + bin(top[h]), 1);
-    __syncthreads();
-    // warp 0: the first bin at which the running count reaches `want` (kTopBins: none), or all bins' beginnings
-    auto scan = [&](int want, bool begins) {
+    // warp 0: the first bin at which the running count reaches `want` and the count before it (kTopBins: none), or all bins' beginnings
+    auto scan = [&](int want, bool begins, int& before_it) {
       int v[kTopBins / 32], sum = 0;
 #pragma unroll
       for (int j = 0; j < kTopBins / 32; j += 4) {
-        const int4 b = reinterpret_cast<const int4*>(s_hist)[(lane * (kTopBins / 32) + j) / 4];
+        const int4 b = reinterpret_cast<const int4*>(sh.hist)[(lane * (kTopBins / 32) + j) / 4];
         v[j] = b.x; v[j + 1] = b.y; v[j + 2] = b.z; v[j + 3] = b.w;
       }
 #pragma unroll
@@ -663,28 +686,54 @@ __global__ void __launch_bounds__(kDsMaxThreads / 2, 4) top_logits_kernel(const 
         if (lane >= o) before += x;
       }
       before -= sum;
-      int found = kTopBins;
+      int found = kTopBins, at_found = 0;
 #pragma unroll
       for (int j = 0; j < kTopBins / 32; ++j) {
-        if (begins) s_begin[lane * (kTopBins / 32) + j] = before;
+        if (begins) sh.begin[lane * (kTopBins / 32) + j] = before;
+        if (before + v[j] >= want && found == kTopBins) {
+          found = lane * (kTopBins / 32) + j;
+          at_found = before;
+        }
         before += v[j];
-        if (before >= want && found == kTopBins) found = lane * (kTopBins / 32) + j;
       }
-      return int(__reduce_min_sync(0xffffffffu, unsigned(found)));
+      const int first = int(__reduce_min_sync(0xffffffffu, unsigned(found)));
+      before_it = int(__reduce_max_sync(0xffffffffu, found == first ? unsigned(at_found) : 0u));
+      return first;
     };
+#pragma unroll
+    for (int h = 0; h < 8; ++h)
+      if (top[h] != 0u) atomicAdd(sh.hist + (255 - (top[h] >> 8)), 1);
+    group.sync();
     if (warp == 0) {
-      const int b = scan(k, false);
-      // (the last bin has everything further down: no bound)
-      if (lane == 0) s_bound = b < kTopBins - 1 && largest > 2u * uint32_t(b) + 1u ? largest - 2u * uint32_t(b) - 1u : 0u;
-      if (lane == 0) s_n = 0;
+      int before = 0;
+      const int b = scan(p.rank, false, before);
+      if (lane == 0) {
+        sh.bound = b == kTopBins ? 0u : uint32_t(255 - b) << 8 | 0x80000000u;
+        sh.n = p.rank - before;                // of the bin's own
+      }
     }
-    __syncthreads();
-    uint32_t lo = s_bound;
-    if (lo == 0u) {
-      // the largest key that at least k of the groups reach (0: none)
-      for (uint32_t bit = 0x8000u; bit != 0u; bit >>= 1)
-        if (count(int(top[0] >= (lo | bit)) + int(top[1] >= (lo | bit))) >= k) lo |= bit;
+    group.sync();
+    uint32_t lo = sh.bound;
+    if (lo != 0u) {
+      const int want = sh.n;
+      zero();
+      group.sync();
+#pragma unroll
+      for (int h = 0; h < 8; ++h)
+        if (top[h] != 0u && (top[h] >> 8) == ((lo >> 8) & 0xffu)) atomicAdd(sh.hist + (255 - (top[h] & 0xffu)), 1);
+      group.sync();
+      if (warp == 0) {
+        int before;
+        const int b = scan(want, false, before);
+        if (lane == 0) sh.bound = (lo & 0xff00u) | uint32_t(255 - b);
+      }
+      group.sync();
+      lo = sh.bound;
     }
+    if (tid == 0) sh.n = 0;
+    // the candidates' bins: of as many keys as make 256 of them enough down to the bound
+    const int shift = max(0, 32 - __clz(int((largest > lo ? largest - lo : 0u) >> 8)));
+    auto bin = [&](uint32_t key) { return key > largest ? 0u : min((largest - key) >> shift, uint32_t(kTopBins - 1)); };
 
     // ---- second pass: the sum over the pieces without a candidate (and wholly of the row), and which ones those are not
     float2 acc = make_float2(0.f, 0.f);
@@ -705,7 +754,7 @@ __global__ void __launch_bounds__(kDsMaxThreads / 2, 4) top_logits_kernel(const 
         if (TABLE && i < q.last()) nan = __vmaxu2(nan, C::largest(w));
     });
     in.fetch(q_next, tid, nt);
-    __syncthreads();
+    group.sync();
     // ---- the marked pieces, listed in order
     int marked = 0;
     for (int i0 = 0; i0 < words; i0 += nt) {
@@ -716,18 +765,18 @@ __global__ void __launch_bounds__(kDsMaxThreads / 2, 4) top_logits_kernel(const 
         const int x = __shfl_up_sync(0xffffffffu, at, o);
         if (lane >= o) at += x;
       }
-      if (lane == 31) s_count[turn][warp] = at;
+      if (lane == 31) sh.count[turn][warp] = at;
       at += marked - __popc(m);
-      __syncthreads();
-      const int c = lane < warps ? s_count[turn][lane] : 0;
+      group.sync();
+      const int c = lane < warps ? sh.count[turn][lane] : 0;
       at += __reduce_add_sync(0xffffffffu, lane < warp ? c : 0);
       marked += __reduce_add_sync(0xffffffffu, c);
       turn ^= 1;
       for (; m != 0u; m &= m - 1u, ++at)
-        if (at < 2 * kTopMaxCandidates - 2) s_list[at] = uint32_t(q.first() + (i0 + tid) * 32 + __ffs(int(m)) - 1);
+        if (at < 2 * p.room - 2) s_list[at] = uint32_t(q.first() + (i0 + tid) * 32 + __ffs(int(m)) - 1);
     }
-    const bool crowded = marked > 2 * kTopMaxCandidates - 2;
-    marked = min(marked, 2 * kTopMaxCandidates - 2);
+    const bool crowded = marked > 2 * p.room - 2;
+    marked = min(marked, 2 * p.room - 2);
     if (q.first()) {
       if (tid == 0) s_list[marked] = 0u;
       ++marked;
@@ -736,7 +785,7 @@ __global__ void __launch_bounds__(kDsMaxThreads / 2, 4) top_logits_kernel(const 
       if (tid == 0) s_list[marked] = uint32_t(q.last());
       ++marked;
     }
-    __syncthreads();
+    group.sync();
     // ---- their candidates, and the sum of the others
     for (int l = tid; l < marked; l += nt) {
       const int i = int(s_list[l]);
@@ -746,8 +795,8 @@ __global__ void __launch_bounds__(kDsMaxThreads / 2, 4) top_logits_kernel(const 
         const uint32_t ge = reach(v), out = outside >> (2 * j) & 3u;
         const uint32_t hit = ((ge & 1u) | (ge >> 31) << 1) & ~out, off = hit | out;
         for (uint32_t rest = hit; rest != 0u; rest &= rest - 1u) {
-          const int h = __ffs(int(rest)) - 1, n = atomicAdd(&s_n, 1);
-          if (n < kTopMaxCandidates) s_cand[n] = uint64_t(top_key(h ? v >> 16 : v & 0xffffu)) << 32 | uint32_t(~uint32_t(i * 8 + 2 * j + h - q.off));
+          const int h = __ffs(int(rest)) - 1, n = atomicAdd(&sh.n, 1);
+          if (n < p.room) s_cand[n] = uint64_t(top_key(h ? v >> 16 : v & 0xffffu)) << 32 | uint32_t(~uint32_t(i * 8 + 2 * j + h - q.off));
         }
         const uint32_t rest = v & ((off & 1u ? 0u : 0xffffu) | (off & 2u ? 0u : 0xffff0000u));
         if (TABLE) nan = __vmaxu2(nan, rest & 0x7fff7fffu);
@@ -757,10 +806,10 @@ __global__ void __launch_bounds__(kDsMaxThreads / 2, 4) top_logits_kernel(const 
     }
     if (C::is_nan(nan)) acc.x = __int_as_float(0x7fffffff);
     float others = acc.x + acc.y;
-    const bool odd = __syncthreads_or(isnan(others));
-    int n = s_n;
+    const bool odd = group.sync_or(isnan(others));
+    int n = sh.n;
     float extra = 0.f;                         // the sum of candidates that are not kept
-    if (crowded || n > kTopMaxCandidates || n < k || odd) {
+    if (crowded || n > p.room || n < k || odd) {
       // the k-th largest key of the row
       auto keys_of = [&](int i, auto&& f) {
         const uint4 w = ld_stream_v4(src + i);
@@ -775,18 +824,18 @@ __global__ void __launch_bounds__(kDsMaxThreads / 2, 4) top_logits_kernel(const 
         for (int i = tid; i < pieces; i += nt) keys_of(i, [&](int, uint32_t v) { c += v >= (key | bit); });
         if (count(c) >= k) key |= bit;
       }
-      if (tid == 0) s_n = 0;
-      __syncthreads();
+      if (tid == 0) sh.n = 0;
+      group.sync();
       // those above it, fewer than k; how many equal it; the sum of those below
       int equal = 0;
       others = 0.f;
       for (int i = tid; i < pieces; i += nt)
         keys_of(i, [&](int j, uint32_t v) {
-          if (v > key) s_cand[atomicAdd(&s_n, 1)] = uint64_t(v) << 32 | uint32_t(~uint32_t(i * 8 + j - q.off));
+          if (v > key) s_cand[atomicAdd(&sh.n, 1)] = uint64_t(v) << 32 | uint32_t(~uint32_t(i * 8 + j - q.off));
           else if (v == key) ++equal;
           else others += expf(cap.z_over_t(__uint_as_float(top_bits(v) << 16)));
         });
-      const int equals = count(equal), above = s_n, want = k - above;
+      const int equals = count(equal), above = sh.n, want = k - above;
       // the first `want` of its equals: block after block of pieces, each thread's in its place by a prefix sum
       int have = 0;
       for (int i0 = 0; have < want; i0 += nt) {
@@ -799,64 +848,123 @@ __global__ void __launch_bounds__(kDsMaxThreads / 2, 4) top_logits_kernel(const 
           const int v = __shfl_up_sync(0xffffffffu, before, o);
           if (lane >= o) before += v;
         }
-        if (lane == 31) s_count[turn][warp] = before;
-        __syncthreads();
+        if (lane == 31) sh.count[turn][warp] = before;
+        group.sync();
         int all = 0, at = have + before - __popc(mine);
         for (int v = 0; v < warps; ++v) {
-          if (v < warp) at += s_count[turn][v];
-          all += s_count[turn][v];
+          if (v < warp) at += sh.count[turn][v];
+          all += sh.count[turn][v];
         }
         turn ^= 1;
         for (; mine != 0u && at < want; mine &= mine - 1u, ++at)
           s_cand[above + at] = uint64_t(key) << 32 | uint32_t(~uint32_t(i * 8 + __ffs(int(mine)) - 1 - q.off));
         have += all;
       }
-      __syncthreads();
+      group.sync();
       if (tid == 0 && equals > want) extra = float(equals - want) * expf(cap.z_over_t(__uint_as_float(top_bits(key) << 16)));
       n = k;
     }
     // ---- each candidate's place; from there on all in the order of places, so that results do not depend on that of the atomics
-    for (int i = tid; i < kTopBins; i += nt) s_hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += nt) atomicAdd(s_hist + bin(uint32_t(s_cand[i] >> 32)), 1);
-    __syncthreads();
-    if (warp == 0) scan(0, true);
-    __syncthreads();
+    for (int i = tid; i < kTopBins; i += nt) sh.hist[i] = 0;
+    group.sync();
+    for (int i = tid; i < n; i += nt) atomicAdd(sh.hist + bin(uint32_t(s_cand[i] >> 32)), 1);
+    group.sync();
+    if (warp == 0) {
+      int unused;
+      scan(0, true, unused);
+    }
+    group.sync();
     for (int i = tid; i < n; i += nt) {
       const uint64_t c = s_cand[i];
-      s_sorted[atomicAdd(s_begin + bin(uint32_t(c >> 32)), 1)] = c;      // (a bin's beginning becomes its end)
+      s_sorted[atomicAdd(sh.begin + bin(uint32_t(c >> 32)), 1)] = c;      // (a bin's beginning becomes its end)
     }
-    __syncthreads();
+    group.sync();
     for (int i = tid; i < n; i += nt) {
       const uint64_t mine = s_sorted[i];
       const uint32_t b = bin(uint32_t(mine >> 32));
-      const int end = s_begin[b], begin = end - s_hist[b];
+      const int end = sh.begin[b], begin = end - sh.hist[b];
       int r = begin;
       for (int j = begin; j < end; ++j) r += s_sorted[j] > mine;
       s_cand[r] = mine;
     }
-    __syncthreads();
-    float kept = 0.f, s = 0.f;
-    for (int r = tid; r < n; r += nt) {
-      const float v = cap.z_over_t(__uint_as_float(top_bits(uint32_t(s_cand[r] >> 32)) << 16));
-      if (r < k) {
-        s = v;
-        kept = expf(v);
-      } else {
-        extra += expf(v);
-      }
-    }
-    float sums[2] = {others + extra, kept};
-    ds_warp_sums(sums, s_red, warp, true);
-    __syncthreads();
-    ds_add_warps(sums, s_red, warps);
-    if (tid < k) {
-      p.ids[row * k + tid] = int32_t(~uint32_t(s_cand[tid]));
-      p.logp[row * k + tid] = s - logf(sums[0] + sums[1]);
+    group.sync();
+    auto z_of = [&](int r) { return cap.z_over_t(__uint_as_float(top_bits(uint32_t(s_cand[r] >> 32)) << 16)); };
+    float sums[2] = {others + extra, 0.f};
+    for (int r = tid; r < n; r += nt) sums[r < k] += expf(z_of(r));
+    ds_warp_sums(sums, sh.red, warp, true);
+    group.sync();
+    ds_add_warps(sums, sh.red, warps);
+    const float lse = logf(sums[0] + sums[1]);
+    for (int r = tid; r < k; r += nt) {
+      p.ids[row * k + r] = int32_t(~uint32_t(s_cand[r]));
+      p.logp[row * k + r] = z_of(r) - lse;
     }
     if (tid == 0) p.log_rest[row] = log_share(sums[0], sums[1]);
-    __syncthreads();
+    group.sync();
     q = q_next;
+  }
+}
+
+// The same for rows of at most PIECES 16-byte pieces a lane: a warp per row, which takes the largest k times.  A logit is a number whose order is that of
+// the answer, its key above its place's complement.
+template <int PIECES>
+__global__ void __launch_bounds__(128) top_logits_short_kernel(const TopArgs p) {
+  grid_trigger();
+  grid_wait();
+  const int lane = threadIdx.x & 31, k = p.k;
+  const Cap<0> cap(p.cap, p.temperature, nullptr);
+  for (int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5); row < p.rows; row += int64_t(gridDim.x) * 4) {
+    const DsRow q(p.logits, row, p.ld, p.vocab);
+    const int pieces = (q.end + 7) >> 3;
+    uint32_t v[PIECES * 8], most = 0u;         // (0: none, or taken)
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c) {
+      const int i = lane + c * 32;
+      const uint4 w = i < pieces ? ld_stream_v4(q.pieces() + i) : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t wi[4] = {w.x, w.y, w.z, w.w}, out = i < pieces ? q.outside(i) : 0xffu;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t key = top_key(j & 1 ? wi[j >> 1] >> 16 : wi[j >> 1] & 0xffffu);
+        v[c * 8 + j] = out >> j & 1u ? 0u : key << 16 | uint32_t(0xffff - (i * 8 + j - q.off));
+        most = max(most, v[c * 8 + j]);
+      }
+    }
+    uint32_t mine[2] = {0u, 0u};               // what this lane's places (lane, 32 + lane) got
+#pragma unroll 1
+    for (int r = 0; r < k; ++r) {
+      const uint32_t best = __reduce_max_sync(0xffffffffu, most);
+      mine[0] = lane == r ? best : mine[0];
+      mine[1] = lane + 32 == r ? best : mine[1];
+      most = 0u;
+#pragma unroll
+      for (int j = 0; j < PIECES * 8; ++j) {   // (every lane looks for it: no branch)
+        v[j] = v[j] == best ? 0u : v[j];
+        most = max(most, v[j]);
+      }
+    }
+    float tail = 0.f, kept = 0.f, s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < PIECES * 8; j += 2) {
+      const uint32_t w = (v[j] ? top_bits(v[j] >> 16) : 0u) | (v[j + 1] ? top_bits(v[j + 1] >> 16) : 0u) << 16;
+      const float2 e = cap.template e<3>(w);
+      tail += (v[j] ? e.x : 0.f) + (v[j + 1] ? e.y : 0.f);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (mine[h]) {
+        s[h] = cap.z_over_t(__uint_as_float(top_bits(mine[h] >> 16) << 16));
+        kept += expf(s[h]);
+      }
+    tail = ds_warp_sum(tail);
+    kept = ds_warp_sum(kept);
+    const float lse = logf(tail + kept);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (mine[h]) {
+        p.ids[row * k + 32 * h + lane] = int32_t(0xffffu - (mine[h] & 0xffffu));
+        p.logp[row * k + 32 * h + lane] = s[h] - lse;
+      }
+    if (lane == 0) p.log_rest[row] = log_share(tail, kept);
   }
 }
 
@@ -893,7 +1001,25 @@ static int ds_blocks(K kern, DsKernelInfo& info, int64_t smem, int threads, int6
   return TG_OK;
 }
 
-constexpr int64_t kDsDynamicMax = kDsSmemMax - 2 * 1024;     // (less than 2 KB are static)
+constexpr int64_t kDsDynamicMax = kDsSmemMax - 4 * 1024;     // (less than 4 KB are static)
+
+// Threads and groups for rows that are not kept.  A row alone has phases in which little is on its way, so several are in work on an SM: eight by 128
+// threads each where that is enough for one (`least`).  Fewer and larger groups cost 1.08 and 1.25 times as much a row and may have the better last round.
+static void ds_groups(int64_t rows, int64_t pieces, int least, int* nt, int* groups) {
+  const int64_t sms = sm_count();
+  double best = 0.0;
+  *groups = 1;
+  for (int g = kDsMaxGroups; g >= 2; g /= 2) {
+    if (2 * kDsMaxThreads / g < least || rows <= sms * (g / 2)) continue;
+    const double cost = double((rows + sms * g - 1) / (sms * g) * g) * (g == 8 ? 1.0 : g == 4 ? 1.08 : 1.25);
+    if (best == 0.0 || cost < best) {
+      best = cost;
+      *groups = g;
+    }
+  }
+  *nt = ds_threads(pieces, least, std::min(kDsMaxThreads, 2 * kDsMaxThreads / *groups));
+  if (*nt < 128) *groups = 1;
+}
 
 template <int EXPS, bool GRAD, bool TABLE, bool STAGED>
 static int launch_distill(DistillArgs a, int nt, cudaStream_t st) {
@@ -901,7 +1027,8 @@ static int launch_distill(DistillArgs a, int nt, cudaStream_t st) {
   auto kern = softcap_distill_kernel<EXPS, GRAD, TABLE, STAGED>;
   const int64_t table = TABLE ? cap_bytes(distill_table(EXPS, GRAD)) : 0, bytes = ds_map_bytes(a.vocab) + (STAGED ? ds_row_bytes(a.vocab) : 0);
   // two groups in a block where two blocks do not fit on an SM beside each other
-  a.groups = STAGED && 2 * (table + bytes) > kDsDynamicMax && table + 2 * bytes <= kDsDynamicMax && a.rows > sm_count() ? 2 : 1;
+  if (STAGED) a.groups = 2 * (table + bytes) > kDsDynamicMax && table + 2 * bytes <= kDsDynamicMax && a.rows > sm_count() ? 2 : 1;
+  while (a.groups > 1 && table + a.groups * bytes > kDsDynamicMax) --a.groups;
   a.group_bytes = int(bytes);
   const int64_t smem = table + a.groups * bytes;
   int64_t per_sm;
@@ -912,28 +1039,51 @@ static int launch_distill(DistillArgs a, int nt, cudaStream_t st) {
 }
 template <int EXPS, bool GRAD>
 static int launch_distill(const DistillArgs& a, cudaStream_t st) {
-  // (the loss alone keeps nothing of a row: more and smaller blocks)
-  const int nt = ds_threads((a.vocab + 14) / 8, a.k, GRAD ? kDsMaxThreads : kDsMaxThreads / 2);
   const bool table = ds_table(a.rows, a.vocab);
+  const int64_t pieces = (a.vocab + 14) / 8;
   if constexpr (GRAD) {
-    if (kCapTableBytes + ds_map_bytes(a.vocab) + ds_row_bytes(a.vocab) <= kDsDynamicMax)
+    if (kCapTableBytes + ds_map_bytes(a.vocab) + ds_row_bytes(a.vocab) <= kDsDynamicMax) {
+      const int nt = ds_threads(pieces, a.k, kDsMaxThreads);
       return table ? launch_distill<EXPS, true, true, true>(a, nt, st) : launch_distill<EXPS, true, false, true>(a, nt, st);
+    }
   }
-  return table ? launch_distill<EXPS, GRAD, true, false>(a, nt, st) : launch_distill<EXPS, GRAD, false, false>(a, nt, st);
+  DistillArgs b = a;
+  int nt;
+  ds_groups(a.rows, pieces, (a.k + 31) / 32 * 32, &nt, &b.groups);
+  return table ? launch_distill<EXPS, GRAD, true, false>(b, nt, st) : launch_distill<EXPS, GRAD, false, false>(b, nt, st);
 }
 
 template <bool TABLE>
-static int launch_top(const TopArgs& a, int nt, cudaStream_t st) {
+static int launch_top(TopArgs a, int nt, cudaStream_t st) {
   static DsKernelInfo info;
-  const int smem = ds_map_bytes(a.vocab) / 8 + 16 + (TABLE ? cap_bytes(kTabE) : 0);
+  const int64_t table = TABLE ? cap_bytes(kTabE) : 0, bytes = top_group_bytes(a.vocab, a.room);
+  while (a.groups > 1 && table + a.groups * bytes > kDsDynamicMax) --a.groups;
+  const int64_t smem = table + a.groups * bytes;
   int64_t per_sm;
-  if (int rc = ds_blocks(top_logits_kernel<TABLE>, info, smem, nt, &per_sm)) return rc;
-  const int blocks = int(std::min<int64_t>(a.rows, sm_count() * per_sm));
-  TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, top_logits_kernel<TABLE>, dim3(unsigned(blocks)), nt, size_t(smem), st, a));
+  if (int rc = ds_blocks(top_logits_kernel<TABLE>, info, smem, nt * a.groups, &per_sm)) return rc;
+  const int blocks = int(std::min<int64_t>((a.rows + a.groups - 1) / a.groups, sm_count() * per_sm));
+  TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, top_logits_kernel<TABLE>, dim3(unsigned(blocks)), nt * a.groups, size_t(smem), st, a));
   return TG_OK;
 }
-static int launch_top(const TopArgs& a, cudaStream_t st) {
-  const int nt = ds_threads((a.vocab + 14) / 8, a.k, kDsMaxThreads / 2);
+template <int PIECES>
+static int launch_top_short(const TopArgs& a, cudaStream_t st) {
+  const int64_t warps = std::min<int64_t>(a.rows, int64_t(sm_count()) * 32);
+  TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, top_logits_short_kernel<PIECES>, dim3(unsigned((warps + 3) / 4)), 128, 0, st, a));
+  return TG_OK;
+}
+static int launch_top(TopArgs a, cudaStream_t st) {
+  const int64_t pieces = (a.vocab + 14) / 8;
+  // (where a warp's turns, k of them, are fewer instructions than the general kernel has for so short a row)
+  if (pieces <= 32 && a.k <= 64) return launch_top_short<1>(a, st);
+  if (pieces <= 64 && a.k <= 48) return launch_top_short<2>(a, st);
+  if (pieces <= 128 && a.k <= 32) return launch_top_short<4>(a, st);
+  int nt;
+  // many short rows: two warps each
+  if (pieces <= 512 && a.rows > 8 * sm_count()) {
+    a.groups = kDsMaxGroups;
+    return launch_top<false>(a, 64, st);
+  }
+  ds_groups(a.rows, pieces, 32, &nt, &a.groups);
   return ds_table(a.rows, a.vocab) ? launch_top<true>(a, nt, st) : launch_top<false>(a, nt, st);
 }
 
@@ -953,7 +1103,9 @@ extern "C" int tg_top_logits(const void* logits, float cap, float temperature, i
   if (rows == 0) return TG_OK;
   if ((reinterpret_cast<uintptr_t>(logits) & 1u) != 0) return TG_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
-  const TopArgs a = {logits, cap, temperature, ids, logp, log_rest, int(rows), int(vocab), k, ld};
+  const bool sampled = vocab >= kTopSampleFrom && vocab <= kTopSampleTo;
+  const int rank = sampled ? int(std::ceil(k / 8.0 + 4.0 * std::sqrt(k / 8.0))) + 4 : k;
+  const TopArgs a = {logits, cap, temperature, ids, logp, log_rest, int(rows), int(vocab), k, ld, rank, 1, k <= 64 ? kTopMaxCandidates / 2 : kTopMaxCandidates};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return launch_top(a, st);
 }
@@ -975,7 +1127,7 @@ extern "C" int tg_softcap_distill(const tg_distill_args* args, void* stream) {
   const float t = soft ? g.temperature : 1.0f;
   const int exps = !(soft && hard) || t == 1.0f ? 1 : t == 2.0f ? 3 : t == 4.0f ? 4 : 2;
   const DistillArgs a = {g.logits, g.ids, g.logp, g.log_rest, hard ? g.targets : nullptr, g.ids_64, g.targets_64, g.cap, t,
-                         g.weight, g.dlogits, g.gscale, g.only_if_scaled, g.row_loss, int(g.rows), int(g.vocab), g.k, g.ld};
+                         g.weight, g.dlogits, g.gscale, g.only_if_scaled, g.row_loss, int(g.rows), int(g.vocab), g.k, g.ld, 1, 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool grad = g.dlogits != nullptr;
   if (exps == 1) return grad ? launch_distill<1, true>(a, st) : launch_distill<1, false>(a, st);
