@@ -233,16 +233,44 @@ struct SandwichBwd {
   int cols;
 };
 
-constexpr int sw_bwd_warps(int) { return 8; }
-constexpr int kSwBwdSlots = 2;
+// Sixteen warps a block, one block per SM.  A warp has at most two pieces of 256 columns of a row (their column sums are 32 registers), a row as many
+// warps as it needs: `wpr`, the rest of the sixteen their own rows.  With the reduction behind it: 32768 x 2048 128 us (6.3 TB/s), 16384 x
+// 1024 37.4, 3001 x 4096 38.9, 8191 x 8184 188, 65536 x 256 39.7, 128 x 128 5.0; with four pieces a warp and eight warps 127, 37.8, 39.4,
+// 204, 50.7 and 4.7.
+constexpr int kSwBwdWarps = 16;
 
-template <int NCHUNK, int WPR, bool FULL>
-__global__ void __launch_bounds__(sw_bwd_warps(WPR) * 32) sandwich_bwd_kernel(const SandwichBwd p) {
-  constexpr int WARPS = sw_bwd_warps(WPR), RPB = WARPS / WPR, SLOTS = kSwBwdSlots, kRowBytes = NCHUNK * 512, kSlotBytes = 4 * kRowBytes;
+// N sums over a row of wpr warps, as row_sums
+template <int N>
+__device__ __forceinline__ void group_sums(float (&v)[N], float (*red)[kSwBwdWarps], int warp, int lane, int wpr, int first, int barrier) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+  if (wpr > 1) {
+    if (lane == 0) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) red[n][warp] = v[n];
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(wpr * 32) : "memory");   // this row's warps only
+    const int at = lane & (kSwBwdWarps - 1);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      v[n] = at < wpr ? red[n][first + at] : 0.f;
+#pragma unroll
+      for (int o = kSwBwdWarps / 2; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+    }
+  }
+}
+
+template <int NCHUNK, int SLOTS, bool FULL>
+__global__ void __launch_bounds__(kSwBwdWarps * 32) sandwich_bwd_kernel(const SandwichBwd p, int wpr) {
+  constexpr int WARPS = kSwBwdWarps, kRowBytes = NCHUNK * 512, kSlotBytes = 4 * kRowBytes;
   __shared__ float s_red3[3][WARPS], s_red1[1][WARPS];
   extern __shared__ float4 s_w[];              // planes of w and pre, then [warps][slots][x' | y | g | gh]
   const int cols = p.cols, pieces = cols / 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col_base = (warp % WPR) * (NCHUNK * 256) + lane * 8;
+  const int rpb = WARPS / wpr, row_of_block = warp / wpr, first = row_of_block * wpr, barrier = 1 + row_of_block;
+  const bool works = row_of_block < rpb;       // (sixteen is not a multiple of every row's warps)
+  const int col_base = (warp - first) * (NCHUNK * 256) + lane * 8;
   float4* s_pre = s_w + 2 * pieces;
   const uint32_t slot0 = uint32_t(__cvta_generic_to_shared(s_w)) + uint32_t(cols) * 8u + uint32_t(warp) * SLOTS * kSlotBytes + uint32_t(lane) * 16u;
   const float inv_d = __fdiv_rn(1.0f, float(cols));
@@ -257,8 +285,8 @@ __global__ void __launch_bounds__(sw_bwd_warps(WPR) * 32) sandwich_bwd_kernel(co
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc_p[c][j] = acc_c[c][j] = splat(0.f);
 
-  const int64_t stride = int64_t(gridDim.x) * RPB;
-  int64_t row = int64_t(blockIdx.x) * RPB + warp / WPR;
+  const int64_t stride = int64_t(gridDim.x) * rpb;
+  int64_t row = works ? int64_t(blockIdx.x) * rpb + row_of_block : p.rows;
   auto prefetch = [&](int64_t r, int slot) {
     if (r < p.rows) {
       const uint32_t dst = slot0 + uint32_t(slot) * kSlotBytes;
@@ -308,7 +336,7 @@ __global__ void __launch_bounds__(sw_bwd_warps(WPR) * 32) sandwich_bwd_kernel(co
         sums[1] += t.x + t.y;
       }
     }
-    row_sums<3, WPR, WARPS>(sums, s_red3, warp, lane);
+    group_sums<3>(sums, s_red3, warp, lane, wpr, first, barrier);
     const float r = __frsqrt_rn(__fmaf_rn(sums[0], inv_d, p.eps)), s = __frsqrt_rn(__fmaf_rn(sums[2], inv_d, p.eps));
     const float nm = -(r * r) * (sums[1] * inv_d);    // d = g + r (a + x' nm)
 
@@ -342,8 +370,8 @@ __global__ void __launch_bounds__(sw_bwd_warps(WPR) * 32) sandwich_bwd_kernel(co
       for (int j = 0; j < 4; ++j) t = __ffma2_rn(__fmul2_rn(d[c][j], m[j]), y[j], t);
       sum4[0] += t.x + t.y;
     }
-    row_sums<1, WPR, WARPS>(sum4, s_red1, warp, lane);
-    if (token && p.dgate_token != nullptr && lane == 0 && warp % WPR == 0) p.dgate_token[row] = __float2bfloat16_rn(s * sum4[0]);
+    group_sums<1>(sum4, s_red1, warp, lane, wpr, first, barrier);
+    if (token && p.dgate_token != nullptr && lane == 0 && warp == first) p.dgate_token[row] = __float2bfloat16_rn(s * sum4[0]);
     const float gsr = gate * s, nm2 = -(s * s) * (sum4[0] * inv_d);
 
     // ---- dy and C
@@ -368,32 +396,29 @@ __global__ void __launch_bounds__(sw_bwd_warps(WPR) * 32) sandwich_bwd_kernel(co
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 
   grid_trigger();          // the reduction's blocks may take the places of this kernel's as they leave
-  // the block's rows added up in order over the (now idle) planes, then published
+  // every warp's column sums over the (now idle) slots, then the block's rows added up in order and published
   __syncthreads();
-  float* s_sum = reinterpret_cast<float*>(s_w);
-  for (int i = threadIdx.x; i < 2 * cols; i += blockDim.x) s_sum[i] = 0.f;
-  __syncthreads();
-  for (int turn = 0; turn < RPB; ++turn) {
-    if (warp / WPR == turn) {
+  float* s_sum = reinterpret_cast<float*>(s_w) + 2 * cols;
+  constexpr int kWarpCols = NCHUNK * 256;
 #pragma unroll
-      for (int c = 0; c < NCHUNK; ++c) {
-        const int col = col_base + c * 256;
-        if (!(FULL || col < cols)) continue;
+  for (int c = 0; c < NCHUNK; ++c) {
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-          float4* dst = reinterpret_cast<float4*>(s_sum + which * cols + col);
-          float4 a = dst[0], b = dst[1];
-          const float2(&v)[4] = which ? acc_c[c] : acc_p[c];
-          a.x += v[0].x; a.y += v[0].y; a.z += v[1].x; a.w += v[1].y;
-          b.x += v[2].x; b.y += v[2].y; b.z += v[3].x; b.w += v[3].y;
-          dst[0] = a; dst[1] = b;
-        }
-      }
+    for (int which = 0; which < 2; ++which) {
+      const float2(&v)[4] = which ? acc_c[c] : acc_p[c];
+      float4* dst = reinterpret_cast<float4*>(s_sum + (warp * 2 + which) * kWarpCols + c * 256 + lane * 8);
+      dst[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+      dst[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
     }
-    __syncthreads();
   }
+  __syncthreads();
   float* out = p.partial + int64_t(blockIdx.x) * 2 * cols;
-  for (int i = threadIdx.x; i < 2 * cols; i += blockDim.x) out[i] = s_sum[i];
+  for (int i = threadIdx.x; i < 2 * cols; i += blockDim.x) {
+    const int which = i >= cols, col = which ? i - cols : i, w = col / kWarpCols;
+    const float* from = s_sum + (w * 2 + which) * kWarpCols + (col - w * kWarpCols);
+    float t = 0.f;
+    for (int r = 0; r < rpb; ++r) t += from[r * wpr * 2 * kWarpCols];
+    out[i] = t;
+  }
 }
 
 // Column sums of the blocks' partial ones, 32 columns a block, warp w those of blocks w, w + 32, ...: an order that the number of blocks
@@ -462,18 +487,25 @@ static int launch_sandwich_fwd(const SandwichFwd& a, cudaStream_t st) {
   return TG_OK;
 }
 
-static int sandwich_bwd_blocks(int64_t rows, const SandwichGeom& g) {
-  const int rpb = sw_bwd_warps(g.wpr) / g.wpr;
+struct SandwichBwdGeom {
+  int nchunk, wpr;
+};
+static SandwichBwdGeom sandwich_bwd_geom(int64_t cols) {
+  const int chunks = int((cols + 255) / 256), nchunk = chunks == 1 ? 1 : 2;
+  return {nchunk, (chunks + nchunk - 1) / nchunk};
+}
+static int sandwich_bwd_blocks(int64_t rows, int64_t cols) {
+  const int rpb = kSwBwdWarps / sandwich_bwd_geom(cols).wpr;
   return int(std::min<int64_t>((rows + rpb - 1) / rpb, sm_count()));
 }
-template <int NC, int WPR, bool FULL>
-static int launch_sandwich_bwd(const SandwichBwd& a, int blocks, cudaStream_t st) {
+template <int NC, int SLOTS, bool FULL>
+static int launch_sandwich_bwd(const SandwichBwd& a, int wpr, int blocks, cudaStream_t st) {
   static std::atomic<bool> done[64];
-  auto kern = sandwich_bwd_kernel<NC, WPR, FULL>;
-  constexpr int warps = sw_bwd_warps(WPR), stage = warps * kSwBwdSlots * NC * 2048, most = WPR * NC * 256 * 8 + stage;
-  static_assert(most + 1024 <= 227 * 1024, "row slots exceed shared memory");
+  auto kern = sandwich_bwd_kernel<NC, SLOTS, FULL>;
+  constexpr int stage = kSwBwdWarps * SLOTS * NC * 2048, most = (SLOTS == 2 ? 8192 : 4096) * 8 + stage;
+  static_assert(most + 512 <= 227 * 1024, "row slots exceed shared memory");
   if (int rc = allow_smem(kern, most, done)) return rc;
-  TG_CUDA_CHECK(launch_early(kern, blocks, warps * 32, a.cols * 8 + stage, st, a));
+  TG_CUDA_CHECK(launch_early(kern, blocks, kSwBwdWarps * 32, a.cols * 8 + stage, st, a, wpr));
   return TG_OK;
 }
 
@@ -500,11 +532,13 @@ static int launch_fwd_case(const SandwichGeom& g, const SandwichFwd& a, cudaStre
   TG_SANDWICH_CASES(TG_CALL)
 #undef TG_CALL
 }
-static int launch_bwd_case(const SandwichGeom& g, const SandwichBwd& a, int blocks, cudaStream_t st) {
+// Rows on their way while one is worked on: two, but one where the vectors leave no room.
+static int launch_bwd_case(const SandwichBwd& a, int blocks, cudaStream_t st) {
+  const SandwichBwdGeom g = sandwich_bwd_geom(a.cols);
   const bool full = a.cols == g.wpr * g.nchunk * 256;
-#define TG_CALL(N, W, F) launch_sandwich_bwd<N, W, F>(a, blocks, st)
-  TG_SANDWICH_CASES(TG_CALL)
-#undef TG_CALL
+  if (g.nchunk == 1) return full ? launch_sandwich_bwd<1, 3, true>(a, g.wpr, blocks, st) : launch_sandwich_bwd<1, 3, false>(a, g.wpr, blocks, st);
+  if (a.cols <= 4096) return full ? launch_sandwich_bwd<2, 3, true>(a, g.wpr, blocks, st) : launch_sandwich_bwd<2, 3, false>(a, g.wpr, blocks, st);
+  return full ? launch_sandwich_bwd<2, 2, true>(a, g.wpr, blocks, st) : launch_sandwich_bwd<2, 2, false>(a, g.wpr, blocks, st);
 }
 
 static bool gate_ok(const void* gate, int kind) {
@@ -537,7 +571,7 @@ extern "C" int tg_sandwich_norm_fwd(const void* x, const void* branch, const voi
 extern "C" int64_t tg_sandwich_norm_bwd_scratch_bytes(int64_t rows, int64_t cols) {
   SandwichGeom g;
   if (rows <= 0 || !sandwich_geom(cols, &g)) return 0;
-  return int64_t(sandwich_bwd_blocks(rows, g)) * 2 * cols * int64_t(sizeof(float));
+  return int64_t(sandwich_bwd_blocks(rows, cols)) * 2 * cols * int64_t(sizeof(float));
 }
 
 extern "C" int tg_sandwich_norm_bwd(const void* x_new, const void* branch, const void* post, const void* pre, const void* gate, int gate_kind,
@@ -559,11 +593,11 @@ extern "C" int tg_sandwich_norm_bwd(const void* x_new, const void* branch, const
   }
   using B = const __nv_bfloat16*;
   using M = __nv_bfloat16*;
-  const int blocks = sandwich_bwd_blocks(rows, g);
+  const int blocks = sandwich_bwd_blocks(rows, cols);
   const SandwichVectors v = {B(post), B(pre), B(gate), gate_kind};
   const SandwichBwd a = {B(x_new), B(branch), v, residual_scale, eps, B(g_new), B(g_h), M(dx), M(dbranch), gate_kind == TG_GATE_TOKEN ? M(dgate) : nullptr,
                          static_cast<float*>(scratch), rows, int(cols)};
-  if (int rc = launch_bwd_case(g, a, blocks, st)) return rc;
+  if (int rc = launch_bwd_case(a, blocks, st)) return rc;
   const SandwichReduce red = {static_cast<const float*>(scratch), v, M(dpost), M(dpre), gate_kind == TG_GATE_CHANNEL ? M(dgate) : nullptr, blocks, int(cols)};
   TG_CUDA_CHECK(launch_if_short(true, sandwich_reduce_kernel, dim3(unsigned((cols + 31) / 32)), 1024, 0, st, red));
   return TG_OK;
