@@ -18,7 +18,7 @@ namespace tg {
 
 constexpr int kDsMaxThreads = 512;                  // of a row
 constexpr int64_t kDsSmemMax = 227 * 1024;
-constexpr int kDsMaxVocab = 1 << 19;
+constexpr int kDsMaxVocab = 1 << 20;
 constexpr int kTopMaxCandidates = 1024;
 constexpr float kDsLog2e = 1.4426950408889634f;
 
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(2 * kDsMaxThreads, 1) softcap_distill_kernel(c
 // group (each of the eight elements of a thread's pieces is one) is found, and the k-th largest of those taken; with 1024 groups about
 // 1024 ln(1 / (1 - k / 1024)) logits reach it.  Where a row is long enough the groups come from an eighth of it, eight pieces of every
 // 64, and the bound is their `rank`-th largest: k / 8 with four standard deviations and four more, so that one row in some thousand has too
-// few.  (All of 8192 x 50304 read twice: 316 us with 8 logits kept, ... so.)
+// few.  (All of a row read twice: 8192 x 50304 with 8 logits 316 us instead of 256, 2048 x 131072 with 64 234 us instead of 168.)
 // The pass over the row sums exp(z / T) over the pieces without a logit that reaches the bound and marks the others, a bit each; they follow in
 // their order, a thread each, so that a warp does not go through a branch for nearly every 32 pieces.  The candidates are then sorted
 // by counting into bins of a key or a few, and within their bin.
@@ -572,7 +572,7 @@ struct TopArgs {
   int rank;                                    // k, or the sample's
   int groups, room;                            // of a block; for candidates
 };
-constexpr int kTopSampleFrom = 16384 + 16, kTopSampleTo = 65536;       // logits of rows that are sampled: at most four pieces a thread
+constexpr int kTopSampleFrom = 16384 + 16;     // logits of a row that is sampled (at least 256 pieces of it)
 
 // bf16 bits -> an unsigned key of the same order (-0 is 0; NaN above all)
 __device__ __forceinline__ uint32_t top_key(uint32_t bits) {
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(2 * kDsMaxThreads, 1) top_logits_kernel(const 
   DsRow q(p.logits, row, p.ld, p.vocab);
   Pieces in;
   in.fetch(q, tid, nt);
-  const bool sampled = p.vocab >= kTopSampleFrom && p.vocab <= kTopSampleTo;
+  const bool sampled = p.vocab >= kTopSampleFrom;
   for (int64_t next; row < p.rows; row = next) {
     next = row + step;
     const DsRow q_next(p.logits, next < p.rows ? next : row, p.ld, p.vocab);
@@ -1103,7 +1103,7 @@ extern "C" int tg_top_logits(const void* logits, float cap, float temperature, i
   if (rows == 0) return TG_OK;
   if ((reinterpret_cast<uintptr_t>(logits) & 1u) != 0) return TG_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
-  const bool sampled = vocab >= kTopSampleFrom && vocab <= kTopSampleTo;
+  const bool sampled = vocab >= kTopSampleFrom;
   const int rank = sampled ? int(std::ceil(k / 8.0 + 4.0 * std::sqrt(k / 8.0))) + 4 : k;
   const TopArgs a = {logits, cap, temperature, ids, logp, log_rest, int(rows), int(vocab), k, ld, rank, 1, k <= 64 ? kTopMaxCandidates / 2 : kTopMaxCandidates};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
