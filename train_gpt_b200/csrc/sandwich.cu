@@ -23,26 +23,29 @@
 
 namespace tg {
 
-// ---- N sums over a row at once; `red` holds N floats per warp of the block.  Two rounds a row with a buffer of their own each: a warp
+constexpr int kSwWarps = 16;                   // of a block
+constexpr int kSwMaxCols = 8192;
+
+// N sums over a row of wpr warps; `red` holds N floats per warp of the block.  Two rounds a row with a buffer of their own each: a warp
 // that writes one of the next row has passed the other's barrier, which every warp of the row reaches after reading the first.
-template <int N, int WPR, int WARPS>
-__device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[WARPS], int warp, int lane) {
+template <int N>
+__device__ __forceinline__ void group_sums(float (&v)[N], float (*red)[kSwWarps], int warp, int lane, int wpr, int first, int barrier) {
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
-  if constexpr (WPR > 1) {
+  if (wpr > 1) {
     if (lane == 0) {
 #pragma unroll
       for (int n = 0; n < N; ++n) red[n][warp] = v[n];
     }
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / WPR), "n"(WPR * 32) : "memory");   // this row's warps only
-    const int g0 = (warp / WPR) * WPR;
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(wpr * 32) : "memory");   // this row's warps only
+    const int at = lane & (kSwWarps - 1);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      v[n] = red[n][g0];
+      v[n] = at < wpr ? red[n][first + at] : 0.f;
 #pragma unroll
-      for (int i = 1; i < WPR; ++i) v[n] += red[n][g0 + i];
+      for (int o = kSwWarps / 2; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
     }
   }
 }
@@ -126,24 +129,31 @@ __device__ __forceinline__ uint4 normed8(const uint4& xw, const float2 (&g)[4], 
   return o;
 }
 
-constexpr int sw_fwd_warps(int wpr) { return wpr == 8 ? 16 : 8; }
+// Sixteen warps a block.  A row of up to 512 columns has a warp, two slots and two blocks per SM (65536 x 256 21.3 us, 32768 x 512 20.6,
+// with one 26.9 and 26.7); up to 1024 a warp, with one block (16384 x 1024 20.0; two: 22.7); up to 2048 four warps with two pieces of 256
+// columns each and three slots (32768 x 2048 83.7 us, 6.4 TB/s; two warps of four pieces 99.5, with two slots 97.4); above, as many warps
+// as have three or four pieces each and two slots (8191 x 8184 90.5 us, 8000 x 3400 39.1; with two pieces 115 and 49, as a block then has half the rows).
+constexpr int sw_fwd_per_sm(int nchunk, int slots) { return nchunk <= 2 && slots == 2 ? 2 : 1; }
 
-template <int NCHUNK, int WPR, bool FULL>
-__global__ void __launch_bounds__(sw_fwd_warps(WPR) * 32) sandwich_fwd_kernel(const SandwichFwd p) {
-  constexpr int WARPS = sw_fwd_warps(WPR), RPB = WARPS / WPR, kRowBytes = NCHUNK * 512, kSlotBytes = 2 * kRowBytes;
+template <int NCHUNK, int SLOTS, bool FULL>
+__global__ void __launch_bounds__(kSwWarps * 32, sw_fwd_per_sm(NCHUNK, SLOTS)) sandwich_fwd_kernel(const SandwichFwd p, int wpr) {
+  constexpr int WARPS = kSwWarps, kRowBytes = NCHUNK * 512, kSlotBytes = 2 * kRowBytes;
   __shared__ float s_red[2][1][WARPS];
-  extern __shared__ float4 s_w[];              // planes of w and pre, then [warps][2][x row | y row]
+  extern __shared__ float4 s_w[];              // planes of w and pre, then [warps][slots][x row | y row]
   const int cols = p.cols, pieces = cols / 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col_base = (warp % WPR) * (NCHUNK * 256) + lane * 8;
+  const int rpb = WARPS / wpr, row_of_block = warp / wpr, first = row_of_block * wpr, barrier = 1 + row_of_block;
+  const bool works = row_of_block < rpb;       // (sixteen is not a multiple of every row's warps)
+  const int col_base = (warp - first) * (NCHUNK * 256) + lane * 8;
+  const bool token = p.v.gate_kind == TG_GATE_TOKEN;
   float4* s_pre = s_w + 2 * pieces;
-  const uint32_t slot0 = uint32_t(__cvta_generic_to_shared(s_w)) + uint32_t(cols) * 8u + uint32_t(warp) * 2u * kSlotBytes + uint32_t(lane) * 16u;
+  const uint32_t slot0 = uint32_t(__cvta_generic_to_shared(s_w)) + uint32_t(cols) * 8u + uint32_t(warp) * SLOTS * kSlotBytes + uint32_t(lane) * 16u;
   grid_trigger();
   grid_wait();
   fill_planes(p.v, s_w, s_pre, pieces);
   __syncthreads();
 
-  const int64_t stride = int64_t(gridDim.x) * RPB;
-  int64_t row = int64_t(blockIdx.x) * RPB + warp / WPR;
+  const int64_t stride = int64_t(gridDim.x) * rpb;
+  int64_t row = works ? int64_t(blockIdx.x) * rpb + row_of_block : p.rows;
   auto prefetch = [&](int64_t r, int slot) {
     if (r < p.rows) {
 #pragma unroll
@@ -157,17 +167,24 @@ __global__ void __launch_bounds__(sw_fwd_warps(WPR) * 32) sandwich_fwd_kernel(co
     }
     asm volatile("cp.async.commit_group;" ::: "memory");   // an empty group keeps the wait count uniform
   };
-  prefetch(row, 0);
-  for (int it = 0; row < p.rows; row += stride, ++it) {
-    const uint32_t base = slot0 + (it & 1) * kSlotBytes;
-    prefetch(row + stride, (it & 1) ^ 1);
-    const float gate = p.v.gate_kind == TG_GATE_TOKEN ? __bfloat162float(p.v.gate[row]) : 1.0f;
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
+#pragma unroll
+  for (int s = 0; s < SLOTS - 1; ++s) prefetch(row + s * stride, s);
+  int slot = 0, slot_in = SLOTS - 1;
+  const uint16_t* gates = reinterpret_cast<const uint16_t*>(p.v.gate);
+  uint32_t next_gate = token && row < p.rows ? gates[row] : 0x3f80u;     // its bits, a row ahead (16000 x 1280 33.4 us, loaded in its turn 41.1)
+  for (; row < p.rows; row += stride) {
+    const uint32_t base = slot0 + uint32_t(slot) * kSlotBytes;
+    prefetch(row + (SLOTS - 1) * stride, slot_in);    // into the slot that the previous row has left
+    const float gate = __uint_as_float(next_gate << 16);
+    if (token && row + stride < p.rows) next_gate = gates[row + stride];
+    asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 1) : "memory");
+    slot_in = slot;
+    if (++slot == SLOTS) slot = 0;
     float part[NCHUNK];
 #pragma unroll
     for (int c = 0; c < NCHUNK; ++c) part[c] = (FULL || col_base + c * 256 < cols) ? sumsq8(lds128(base + kRowBytes + c * 512)) : 0.f;
     float ss[1] = {tree_sum(part)};
-    row_sums<1, WPR, WARPS>(ss, s_red[0], warp, lane);
+    group_sums<1>(ss, s_red[0], warp, lane, wpr, first, barrier);
     const float rg = __frsqrt_rn(__fdiv_rn(ss[0], float(cols)) + p.eps) * gate;
 
     uint4 xo[NCHUNK];
@@ -184,7 +201,7 @@ __global__ void __launch_bounds__(sw_fwd_warps(WPR) * 32) sandwich_fwd_kernel(co
       part[c] = sumsq8(xo[c]);
     }
     ss[0] = tree_sum(part);
-    row_sums<1, WPR, WARPS>(ss, s_red[1], warp, lane);
+    group_sums<1>(ss, s_red[1], warp, lane, wpr, first, barrier);
     const float r = __frsqrt_rn(__fdiv_rn(ss[0], float(cols)) + p.eps);
 
     constexpr int G = pow2_at_least(NCHUNK);
@@ -233,38 +250,14 @@ struct SandwichBwd {
   int cols;
 };
 
-// Sixteen warps a block, one block per SM.  A warp has at most two pieces of 256 columns of a row (their column sums are 32 registers), a row as many
-// warps as it needs: `wpr`, the rest of the sixteen their own rows.  With the reduction behind it: 32768 x 2048 128 us (6.3 TB/s), 16384 x
+// Sixteen warps a block, one block per SM.  A warp has two pieces of 256 columns of a row (their column sums are 32 registers), a row as many
+// warps as it needs: `wpr`, the rest of the sixteen their own rows.  Three pieces where a block then has five thirds of the rows or more
+// (32768 x 768 56.5 us instead of 64.2, 4096 x 2304 27.2 instead of 30.5; 20000 x 1536, eight rows instead of five, 67.5 instead of 63.0).  With the reduction behind it: 32768 x 2048 128 us (6.3 TB/s), 16384 x
 // 1024 37.4, 3001 x 4096 38.9, 8191 x 8184 188, 65536 x 256 39.7, 128 x 128 5.0; with four pieces a warp and eight warps 127, 37.8, 39.4,
 // 204, 50.7 and 4.7.
-constexpr int kSwBwdWarps = 16;
-
-// N sums over a row of wpr warps, as row_sums
-template <int N>
-__device__ __forceinline__ void group_sums(float (&v)[N], float (*red)[kSwBwdWarps], int warp, int lane, int wpr, int first, int barrier) {
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
-  if (wpr > 1) {
-    if (lane == 0) {
-#pragma unroll
-      for (int n = 0; n < N; ++n) red[n][warp] = v[n];
-    }
-    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(wpr * 32) : "memory");   // this row's warps only
-    const int at = lane & (kSwBwdWarps - 1);
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      v[n] = at < wpr ? red[n][first + at] : 0.f;
-#pragma unroll
-      for (int o = kSwBwdWarps / 2; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
-    }
-  }
-}
-
 template <int NCHUNK, int SLOTS, bool FULL>
-__global__ void __launch_bounds__(kSwBwdWarps * 32) sandwich_bwd_kernel(const SandwichBwd p, int wpr) {
-  constexpr int WARPS = kSwBwdWarps, kRowBytes = NCHUNK * 512, kSlotBytes = 4 * kRowBytes;
+__global__ void __launch_bounds__(kSwWarps * 32) sandwich_bwd_kernel(const SandwichBwd p, int wpr) {
+  constexpr int WARPS = kSwWarps, kRowBytes = NCHUNK * 512, kSlotBytes = 4 * kRowBytes;
   __shared__ float s_red3[3][WARPS], s_red1[1][WARPS];
   extern __shared__ float4 s_w[];              // planes of w and pre, then [warps][slots][x' | y | g | gh]
   const int cols = p.cols, pieces = cols / 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -461,82 +454,66 @@ __global__ void __launch_bounds__(1024) sandwich_reduce_kernel(const SandwichRed
 
 // ---- launches ----------------------------------------------------------------------------------------------------
 
-struct SandwichGeom {
-  int nchunk, wpr;
-};
-// 1, 2 or 4 pieces of 256 columns a warp up to 1024 columns, then two, four or eight warps with three or four each.
-static bool sandwich_geom(int64_t cols, SandwichGeom* g) {
-  if (cols <= 0 || cols > 8192) return false;
-  const int chunks = int((cols + 255) / 256);
-  g->wpr = chunks <= 4 ? 1 : chunks <= 8 ? 2 : chunks <= 16 ? 4 : 8;
-  g->nchunk = g->wpr == 1 ? pow2_at_least(chunks) : chunks <= 3 * g->wpr ? 3 : 4;
-  return true;
-}
-
-template <int NC, int WPR, bool FULL>
-static int launch_sandwich_fwd(const SandwichFwd& a, cudaStream_t st) {
+template <int NC, int SLOTS, bool FULL>
+static int launch_sandwich_fwd(const SandwichFwd& a, int wpr, cudaStream_t st) {
   static std::atomic<bool> done[64];
-  auto kern = sandwich_fwd_kernel<NC, WPR, FULL>;
-  constexpr int warps = sw_fwd_warps(WPR), stage = warps * 2 * NC * 1024, most = WPR * NC * 256 * 8 + stage;
-  static_assert(most + 1024 <= 227 * 1024, "row slots exceed shared memory");
+  auto kern = sandwich_fwd_kernel<NC, SLOTS, FULL>;
+  constexpr int stage = kSwWarps * SLOTS * NC * 1024, most = kSwMaxCols * 8 + stage;
+  static_assert(most + 512 <= 227 * 1024, "row slots exceed shared memory");
   if (int rc = allow_smem(kern, most, done)) return rc;
-  const int smem = a.cols * 8 + stage, per_sm = std::max(1, std::min((227 * 1024) / (smem + 1280), 3));
-  const int64_t need = (a.rows + warps / WPR - 1) / (warps / WPR);
-  const int blocks = int(std::min<int64_t>(need, int64_t(sm_count()) * per_sm));
-  TG_CUDA_CHECK(launch_early(kern, blocks, warps * 32, smem, st, a));
+  const int rpb = kSwWarps / wpr;
+  const int blocks = int(std::min<int64_t>((a.rows + rpb - 1) / rpb, int64_t(sm_count()) * sw_fwd_per_sm(NC, SLOTS)));
+  TG_CUDA_CHECK(launch_early(kern, blocks, kSwWarps * 32, a.cols * 8 + stage, st, a, wpr));
   return TG_OK;
 }
+template <int NC, int SLOTS>
+static int launch_fwd_case(const SandwichFwd& a, int chunks, cudaStream_t st) {
+  const int wpr = (chunks + NC - 1) / NC;
+  return a.cols == wpr * NC * 256 ? launch_sandwich_fwd<NC, SLOTS, true>(a, wpr, st) : launch_sandwich_fwd<NC, SLOTS, false>(a, wpr, st);
+}
+static int launch_fwd_case(const SandwichFwd& a, cudaStream_t st) {
+  const int chunks = (a.cols + 255) / 256;
+  if (chunks == 1) return launch_fwd_case<1, 2>(a, chunks, st);
+  if (chunks == 2) return launch_fwd_case<2, 2>(a, chunks, st);
+  if (chunks > 4 && chunks <= 8) return launch_fwd_case<2, 3>(a, chunks, st);
+  // three pieces a warp where a block then has four fifths of the rows that it has with four (8000 x 2816 30.8 us with three, 32.6 with
+  // four; 8000 x 4600, two rows instead of three, 57.0 and 52.3)
+  if (kSwWarps / ((chunks + 2) / 3) * 5 >= kSwWarps / ((chunks + 3) / 4) * 4) return launch_fwd_case<3, 2>(a, chunks, st);
+  return launch_fwd_case<4, 2>(a, chunks, st);
+}
 
+constexpr int kSwThreeMax = 15 * 256;          // (columns whose vectors fit beside the rows of three pieces a warp)
 struct SandwichBwdGeom {
   int nchunk, wpr;
 };
 static SandwichBwdGeom sandwich_bwd_geom(int64_t cols) {
-  const int chunks = int((cols + 255) / 256), nchunk = chunks == 1 ? 1 : 2;
+  const int chunks = int((cols + 255) / 256);
+  const bool three = kSwWarps / ((chunks + 2) / 3) * 3 >= kSwWarps / ((chunks + 1) / 2) * 5 && chunks <= kSwThreeMax / 256;
+  const int nchunk = chunks == 1 ? 1 : three ? 3 : 2;
   return {nchunk, (chunks + nchunk - 1) / nchunk};
 }
 static int sandwich_bwd_blocks(int64_t rows, int64_t cols) {
-  const int rpb = kSwBwdWarps / sandwich_bwd_geom(cols).wpr;
+  const int rpb = kSwWarps / sandwich_bwd_geom(cols).wpr;
   return int(std::min<int64_t>((rows + rpb - 1) / rpb, sm_count()));
 }
 template <int NC, int SLOTS, bool FULL>
 static int launch_sandwich_bwd(const SandwichBwd& a, int wpr, int blocks, cudaStream_t st) {
   static std::atomic<bool> done[64];
   auto kern = sandwich_bwd_kernel<NC, SLOTS, FULL>;
-  constexpr int stage = kSwBwdWarps * SLOTS * NC * 2048, most = (SLOTS == 2 ? 8192 : 4096) * 8 + stage;
+  constexpr int stage = kSwWarps * SLOTS * NC * 2048, most = (NC == 3 ? kSwThreeMax : SLOTS == 2 ? kSwMaxCols : kSwMaxCols / 2) * 8 + stage;
   static_assert(most + 512 <= 227 * 1024, "row slots exceed shared memory");
   if (int rc = allow_smem(kern, most, done)) return rc;
-  TG_CUDA_CHECK(launch_early(kern, blocks, kSwBwdWarps * 32, a.cols * 8 + stage, st, a, wpr));
+  TG_CUDA_CHECK(launch_early(kern, blocks, kSwWarps * 32, a.cols * 8 + stage, st, a, wpr));
   return TG_OK;
 }
 
-#define TG_SANDWICH_CASES(CALL)                                                                    \
-  if (g.wpr == 1) {                                                                                \
-    if (g.nchunk == 1) return full ? CALL(1, 1, true) : CALL(1, 1, false);                         \
-    if (g.nchunk == 2) return full ? CALL(2, 1, true) : CALL(2, 1, false);                         \
-    return full ? CALL(4, 1, true) : CALL(4, 1, false);                                            \
-  }                                                                                                \
-  if (g.wpr == 2) {                                                                                \
-    if (g.nchunk == 3) return full ? CALL(3, 2, true) : CALL(3, 2, false);                         \
-    return full ? CALL(4, 2, true) : CALL(4, 2, false);                                            \
-  }                                                                                                \
-  if (g.wpr == 4) {                                                                                \
-    if (g.nchunk == 3) return full ? CALL(3, 4, true) : CALL(3, 4, false);                         \
-    return full ? CALL(4, 4, true) : CALL(4, 4, false);                                            \
-  }                                                                                                \
-  if (g.nchunk == 3) return full ? CALL(3, 8, true) : CALL(3, 8, false);                           \
-  return full ? CALL(4, 8, true) : CALL(4, 8, false);
 
-static int launch_fwd_case(const SandwichGeom& g, const SandwichFwd& a, cudaStream_t st) {
-  const bool full = a.cols == g.wpr * g.nchunk * 256;
-#define TG_CALL(N, W, F) launch_sandwich_fwd<N, W, F>(a, st)
-  TG_SANDWICH_CASES(TG_CALL)
-#undef TG_CALL
-}
-// Rows on their way while one is worked on: two, but one where the vectors leave no room.
+// Rows on their way while one is worked on: two, but one where the vectors or the pieces leave no room.
 static int launch_bwd_case(const SandwichBwd& a, int blocks, cudaStream_t st) {
   const SandwichBwdGeom g = sandwich_bwd_geom(a.cols);
   const bool full = a.cols == g.wpr * g.nchunk * 256;
   if (g.nchunk == 1) return full ? launch_sandwich_bwd<1, 3, true>(a, g.wpr, blocks, st) : launch_sandwich_bwd<1, 3, false>(a, g.wpr, blocks, st);
+  if (g.nchunk == 3) return full ? launch_sandwich_bwd<3, 2, true>(a, g.wpr, blocks, st) : launch_sandwich_bwd<3, 2, false>(a, g.wpr, blocks, st);
   if (a.cols <= 4096) return full ? launch_sandwich_bwd<2, 3, true>(a, g.wpr, blocks, st) : launch_sandwich_bwd<2, 3, false>(a, g.wpr, blocks, st);
   return full ? launch_sandwich_bwd<2, 2, true>(a, g.wpr, blocks, st) : launch_sandwich_bwd<2, 2, false>(a, g.wpr, blocks, st);
 }
@@ -555,8 +532,7 @@ extern "C" int tg_sandwich_norm_fwd(const void* x, const void* branch, const voi
                                     int64_t cols, void* stream) {
   if (rows < 0 || cols <= 0 || cols % 8 != 0 || !gate_ok(gate, gate_kind) || post == nullptr || pre == nullptr || x_new == nullptr) return TG_ERR_SHAPE;
   if ((q == nullptr) != (scales == nullptr) || (q == nullptr && h == nullptr) || (q != nullptr && cols % kTile != 0)) return TG_ERR_SHAPE;
-  SandwichGeom g;
-  if (!sandwich_geom(cols, &g)) return TG_ERR_TOO_LARGE;
+  if (cols > kSwMaxCols) return TG_ERR_TOO_LARGE;
   if (rows == 0) return TG_OK;
   if (!aligned16(x) || !aligned16(branch) || !aligned16(post) || !aligned16(pre) || !gate_aligned(gate, gate_kind) || !aligned16(x_new) ||
       !aligned16(h) || !aligned16(q))
@@ -565,12 +541,11 @@ extern "C" int tg_sandwich_norm_fwd(const void* x, const void* branch, const voi
   using B = const __nv_bfloat16*;
   const SandwichFwd a = {B(x), B(branch), {B(post), B(pre), B(gate), gate_kind}, residual_scale, eps, static_cast<__nv_bfloat16*>(x_new),
                          static_cast<__nv_bfloat16*>(h), static_cast<uint8_t*>(q), scales, rows, int(cols)};
-  return launch_fwd_case(g, a, static_cast<cudaStream_t>(stream));
+  return launch_fwd_case(a, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int64_t tg_sandwich_norm_bwd_scratch_bytes(int64_t rows, int64_t cols) {
-  SandwichGeom g;
-  if (rows <= 0 || !sandwich_geom(cols, &g)) return 0;
+  if (rows <= 0 || cols <= 0 || cols > kSwMaxCols) return 0;
   return int64_t(sandwich_bwd_blocks(rows, cols)) * 2 * cols * int64_t(sizeof(float));
 }
 
@@ -579,8 +554,7 @@ extern "C" int tg_sandwich_norm_bwd(const void* x_new, const void* branch, const
                                     void* dpre, void* dgate, void* scratch, int64_t rows, int64_t cols, void* stream) {
   if (rows < 0 || cols <= 0 || cols % 8 != 0 || !gate_ok(gate, gate_kind) || post == nullptr || pre == nullptr || dpost == nullptr || dpre == nullptr)
     return TG_ERR_SHAPE;
-  SandwichGeom g;
-  if (!sandwich_geom(cols, &g)) return TG_ERR_TOO_LARGE;
+  if (cols > kSwMaxCols) return TG_ERR_TOO_LARGE;
   if (!aligned16(x_new) || !aligned16(branch) || !aligned16(post) || !aligned16(pre) || !gate_aligned(gate, gate_kind) || !aligned16(g_new) ||
       !aligned16(g_h) || !aligned16(dx) || !aligned16(dbranch) || !aligned16(scratch))
     return TG_ERR_ALIGN;
