@@ -786,18 +786,39 @@ __global__ void __launch_bounds__(2 * kDsMaxThreads, 1) top_logits_kernel(const 
       ++marked;
     }
     group.sync();
-    // ---- their candidates, and the sum of the others
-    for (int l = tid; l < marked; l += nt) {
-      const int i = int(s_list[l]);
-      const uint4 w = ld_stream_v4(src + i);
-      const uint32_t outside = q.outside(i);
+    // ---- their candidates, a warp's with one addition to the count, and the sum of the others
+    auto listed = [&](int l) { return l < marked ? ld_stream_v4(src + s_list[l]) : make_uint4(0u, 0u, 0u, 0u); };
+    uint4 w_next = listed(tid);
+    for (int l0 = warp * 32; l0 < marked; l0 += nt) {
+      const int l = l0 + lane, i = l < marked ? int(s_list[l]) : 0;
+      const uint4 w = w_next;
+      w_next = listed(l + nt);
+      const uint32_t outside = l < marked ? q.outside(i) : 0xffu;
+      uint32_t hit = 0u;
       four_words(w, [&](auto j, uint32_t v) {
-        const uint32_t ge = reach(v), out = outside >> (2 * j) & 3u;
-        const uint32_t hit = ((ge & 1u) | (ge >> 31) << 1) & ~out, off = hit | out;
-        for (uint32_t rest = hit; rest != 0u; rest &= rest - 1u) {
-          const int h = __ffs(int(rest)) - 1, n = atomicAdd(&sh.n, 1);
-          if (n < p.room) s_cand[n] = uint64_t(top_key(h ? v >> 16 : v & 0xffffu)) << 32 | uint32_t(~uint32_t(i * 8 + 2 * j + h - q.off));
-        }
+        const uint32_t ge = reach(v);
+        hit |= ((ge & 1u) | (ge >> 31) << 1) << (2 * decltype(j)::value);
+      });
+      hit &= ~outside;
+      const int hits = __popc(hit);
+      int before = 0, all = 0;
+      for (int t = 1;; ++t) {
+        const uint32_t lanes = __ballot_sync(0xffffffffu, hits >= t);
+        if (lanes == 0u) break;
+        before += __popc(lanes & ((1u << lane) - 1u));
+        all += __popc(lanes);
+      }
+      int at = 0;
+      if (lane == 0 && all > 0) at = atomicAdd(&sh.n, all);
+      at = __shfl_sync(0xffffffffu, at, 0) + before;
+      for (uint32_t rest = hit; rest != 0u; rest &= rest - 1u, ++at) {
+        const int h = __ffs(int(rest)) - 1;
+        const uint32_t v = h & 4 ? (h & 2 ? w.w : w.z) : (h & 2 ? w.y : w.x);
+        if (at < p.room) s_cand[at] = uint64_t(top_key(h & 1 ? v >> 16 : v & 0xffffu)) << 32 | uint32_t(~uint32_t(i * 8 + h - q.off));
+      }
+      const uint32_t off8 = hit | outside;
+      four_words(w, [&](auto j, uint32_t v) {
+        const uint32_t off = off8 >> (2 * decltype(j)::value);
         const uint32_t rest = v & ((off & 1u ? 0u : 0xffffu) | (off & 2u ? 0u : 0xffff0000u));
         if (TABLE) nan = __vmaxu2(nan, rest & 0x7fff7fffu);
         const float2 e = cap.template e<decltype(j)::value>(rest);
