@@ -3,7 +3,8 @@
 Tolerances.  Capped logits over T come from u = 2 / (1 + exp(2 |x| / c)), three approximations of 2^-22 of themselves and a few roundings of
 2^-24, so that z / T is off by at most (c / T) 2^-20 and exp of it by DELTA = (c / T) 2^-20 + 2^-21 of itself.  Sums of such terms are off by as
 much and by the additions' 2^-24 each over the depth of the sum (below 2^8).  A log-probability is off by twice that and by the rounding
-of numbers up to 2 c / T + 17.  A gradient's element is rounded to bf16 once, 2^-8 of it, after errors of 4 DELTA + 2^-16 of its summands."""
+of numbers up to 2 c / T + 17.  A gradient's element is rounded to bf16 once, 2^-8 of it, after errors of 4 DELTA + 2^-16 of its summands; below
+2^-126 bf16's numbers lie 2^-133 apart, so that half of that is lost there whatever the element (at a cap of 64 elements reach 2^-180)."""
 import math
 
 import pytest
@@ -71,6 +72,49 @@ def test_top_logits_of_equal_sorted_and_crowded_rows():
     wide = torch.full((2, 130001), 0.5, device="cuda", dtype=torch.bfloat16)
     wide[1, -1] = 3
     _check_top(wide, 15.0, 100, 1.0)
+
+
+@pytest.mark.parametrize("vocab", [16416, 50257, 140001])
+def test_top_logits_where_a_sample_of_the_row_misleads(vocab):
+    """The bound comes from eight 16-byte pieces of every 64 of a long row: the largest logits all in the others, all in those, or in one of the two
+    in so small a number that the bound lets too few through."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(6, vocab, device="cuda", generator=g)
+    start = torch.arange(6, device="cuda").unsqueeze(1) * vocab                 # (a row's own pieces begin at the next 16-byte boundary)
+    piece = (torch.arange(vocab, device="cuda").unsqueeze(0) - (-start) % 8) // 8
+    seen = (piece >= 0) & (piece % 64 < 8)
+    big = 3 + 3 * torch.rand(6, vocab, device="cuda", generator=g)
+    few = torch.rand(6, vocab, device="cuda", generator=g) < 400 / vocab
+    x = torch.where(torch.stack([~seen[0], seen[1], ~seen[2] & few[2], seen[3] & few[3], few[4], torch.zeros_like(few[5])]), big, x)
+    x[5] = torch.where(seen[5], x[5], -20.0)
+    for k in (1, 33, 64, 65, 256):
+        _check_top(x.to(torch.bfloat16), 15.0, k, 1.0)
+
+
+@pytest.mark.parametrize("rows,vocab,k", [(160, 40001, 16), (320, 33000, 64), (700, 20000, 200), (1200, 5000, 20), (1190, 1500, 100), (1300, 4095, 256), (600, 9001, 8)])
+def test_top_logits_of_more_rows_than_fit(rows, vocab, k):
+    """Several rows at a time on an SM, with one or two groups of threads left without a row in the last round."""
+    _check_top(_logits(rows, vocab, seed=rows), 15.0, k, 1.0)
+
+
+@pytest.mark.parametrize("cap,t", [(64.0, 1.0), (2.0 ** -10, 1.0), (1.0, 1024.0), (2.0, 0.03125), (11.0, 3.0)])
+def test_the_range_of_caps_and_temperatures(cap, t):
+    """Logits in proportion to the cap, so that tanh is far from its ends and at them."""
+    x = (_logits(40, 5003, seed=11).float() * (cap / 15)).to(torch.bfloat16)
+    top = _check_top(x, cap, 40, t)
+    targets = torch.randint(0, 5003, (40,), device="cuda")
+    _check_distill((_logits(40, 5003, seed=12).float() * (cap / 15)).to(torch.bfloat16), top.ids, top.logp, top.log_rest, cap, targets, t, 0.25)
+    if cap <= 64 * t:
+        _check_distill((_logits(170, 20001, seed=13).float() * (cap / 15)).to(torch.bfloat16), *_check_top((_logits(170, 20001, seed=14).float() * (cap / 15)).to(torch.bfloat16), cap, 8, t),
+                       cap, None, t, 1.0)
+
+
+def test_the_largest_vocabulary():
+    vocab = 1 << 20
+    x = _logits(3, vocab, seed=15)
+    top = _check_top(x, 15.0, 100, 2.0)
+    targets = torch.tensor([vocab - 1, 5, vocab], device="cuda")
+    _check_distill(_logits(3, vocab, seed=16), top.ids, top.logp, top.log_rest, 15.0, targets, 2.0, 0.5)
 
 
 def test_top_logits_with_infinities_and_nan():
@@ -150,7 +194,7 @@ def _check_distill(x, ids, logp, rest, cap, targets, t, w, mass=1.0):
     assert float((rows.reshape(-1).double() - row)[fin].abs().max()) <= tol
     if bool(fin.all()):
         assert abs(float(loss.detach()) - float(row.mean())) <= tol
-    bound = 2.0 ** -8 * d.abs() + (4 * _delta(cap, min(t, 1.0)) + 2.0 ** -16) * size
+    bound = 2.0 ** -8 * d.abs() + (4 * _delta(cap, min(t, 1.0)) + 2.0 ** -16) * size + 2.0 ** -133
     off = (got.reshape(-1, vocab).double() - d).abs()
     assert bool((off <= bound).all()), float((off / bound).max())
     with torch.no_grad():
@@ -166,6 +210,14 @@ def test_distillation(rows, vocab, k, cap, t, w, rest):
     targets = torch.randint(0, vocab, (rows,), device="cuda", dtype=torch.int32 if rows % 2 else torch.int64)
     targets[::2] = ids[::2, 0].to(targets.dtype)                             # some of them named by the teacher
     _check_distill(_logits(rows, vocab, seed=7), ids, logp, log_rest, cap, targets if w < 1 else None, t, w)
+
+
+@pytest.mark.parametrize("rows,vocab,k,t,w", [(450, 9001, 130, 1.0, 1.0), (1201, 5000, 8, 2.0, 0.5), (700, 30001, 64, 4.0, 0.5), (330, 130000, 20, 3.0, 0.5), (1190, 300, 100, 1.0, 0.5)])
+def test_distillation_of_more_rows_than_fit(rows, vocab, k, t, w):
+    """Rows beside each other on an SM (two that share a table, up to eight that are not kept), the last round not full."""
+    ids, logp, rest = _teacher(rows, vocab, k, 15.0, t)
+    targets = torch.randint(0, vocab, (rows,), device="cuda") if w < 1 else None
+    _check_distill(_logits(rows, vocab, seed=8), ids, logp, rest, 15.0, targets, t, w)
 
 
 def test_missing_entries_padding_and_what_they_hold():
