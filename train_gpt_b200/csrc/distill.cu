@@ -17,6 +17,10 @@
 namespace tg {
 
 constexpr int kDsMaxThreads = 512;                  // of a row
+// Threads of a block.  Those that keep their rows have the registers of half as many: 8192 x 50304 with 64 logits takes 427 us with 256 threads a
+// row and two pieces of a thread's at a time, 541 with 512 and two pieces, 551 with 512 and one (64 registers spill).  Rows that are not kept
+// come from memory with every read, and need the threads: 4096 x 130000 735 us, with half of them 897.
+constexpr int ds_block_threads(bool staged) { return staged ? kDsMaxThreads : 2 * kDsMaxThreads; }
 constexpr int64_t kDsSmemMax = 227 * 1024;
 constexpr int kDsMaxVocab = 1 << 20;
 constexpr int kTopMaxCandidates = 1024;
@@ -283,7 +287,7 @@ constexpr int ds_map_bytes(int64_t vocab) { return int(((vocab + 14) / 8 + 15) /
 constexpr int64_t ds_row_bytes(int64_t vocab) { return (vocab + 14) / 8 * 16; }
 
 template <int EXPS, bool GRAD, bool TABLE, bool STAGED>
-__global__ void __launch_bounds__(2 * kDsMaxThreads, 1) softcap_distill_kernel(const DistillArgs p) {
+__global__ void __launch_bounds__(ds_block_threads(STAGED), 1) softcap_distill_kernel(const DistillArgs p) {
   constexpr bool TWO = EXPS > 1;
   constexpr int TABLES = TABLE ? distill_table(EXPS, GRAD) : 0;
   using C = Cap<TABLES>;
@@ -440,7 +444,7 @@ __global__ void __launch_bounds__(2 * kDsMaxThreads, 1) softcap_distill_kernel(c
     if constexpr (STAGED) {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       uint32_t slot = slot0;
-#pragma unroll 1
+#pragma unroll 2
       for (int i = q.first() + tid; i < q.last(); i += nt, slot += uint32_t(nt) * 16u) add(lds128(slot), i);
     } else {
       in.each(q, q.last(), tid, nt, add);
@@ -505,7 +509,7 @@ __global__ void __launch_bounds__(2 * kDsMaxThreads, 1) softcap_distill_kernel(c
         uint32_t slot = slot0;
         const uint4* from = q_next.pieces() + q_next.first() + tid;
         int more = next < p.rows ? q_next.last() - q_next.first() - tid : 0;
-#pragma unroll 1
+#pragma unroll 2
         for (int i = q.first() + tid; i < q.last(); i += nt, slot += uint32_t(nt) * 16u, from += nt, more -= nt) {
           const uint4 w = lds128(slot);
           if (more > 0) cp_async16(slot, from);
@@ -1026,19 +1030,19 @@ constexpr int64_t kDsDynamicMax = kDsSmemMax - 4 * 1024;     // (less than 4 KB 
 
 // Threads and groups for rows that are not kept.  A row alone has phases in which little is on its way, so several are in work on an SM: eight by 128
 // threads each where that is enough for one (`least`).  Fewer and larger groups cost 1.08 and 1.25 times as much a row and may have the better last round.
-static void ds_groups(int64_t rows, int64_t pieces, int least, int* nt, int* groups) {
+static void ds_groups(int64_t rows, int64_t pieces, int least, int block, int* nt, int* groups) {
   const int64_t sms = sm_count();
   double best = 0.0;
   *groups = 1;
   for (int g = kDsMaxGroups; g >= 2; g /= 2) {
-    if (2 * kDsMaxThreads / g < least || rows <= sms * (g / 2)) continue;
+    if (block / g < std::max(least, 128) || rows <= sms * (g / 2)) continue;
     const double cost = double((rows + sms * g - 1) / (sms * g) * g) * (g == 8 ? 1.0 : g == 4 ? 1.08 : 1.25);
     if (best == 0.0 || cost < best) {
       best = cost;
       *groups = g;
     }
   }
-  *nt = ds_threads(pieces, least, std::min(kDsMaxThreads, 2 * kDsMaxThreads / *groups));
+  *nt = ds_threads(pieces, least, block / std::max(*groups, 2));
   if (*nt < 128) *groups = 1;
 }
 
@@ -1064,13 +1068,13 @@ static int launch_distill(const DistillArgs& a, cudaStream_t st) {
   const int64_t pieces = (a.vocab + 14) / 8;
   if constexpr (GRAD) {
     if (kCapTableBytes + ds_map_bytes(a.vocab) + ds_row_bytes(a.vocab) <= kDsDynamicMax) {
-      const int nt = ds_threads(pieces, a.k, kDsMaxThreads);
+      const int nt = ds_threads(pieces, a.k, ds_block_threads(true) / 2);
       return table ? launch_distill<EXPS, true, true, true>(a, nt, st) : launch_distill<EXPS, true, false, true>(a, nt, st);
     }
   }
   DistillArgs b = a;
   int nt;
-  ds_groups(a.rows, pieces, (a.k + 31) / 32 * 32, &nt, &b.groups);
+  ds_groups(a.rows, pieces, (a.k + 31) / 32 * 32, ds_block_threads(false), &nt, &b.groups);
   return table ? launch_distill<EXPS, GRAD, true, false>(b, nt, st) : launch_distill<EXPS, GRAD, false, false>(b, nt, st);
 }
 
@@ -1104,7 +1108,7 @@ static int launch_top(TopArgs a, cudaStream_t st) {
     a.groups = kDsMaxGroups;
     return launch_top<false>(a, 64, st);
   }
-  ds_groups(a.rows, pieces, 32, &nt, &a.groups);
+  ds_groups(a.rows, pieces, 32, 2 * kDsMaxThreads, &nt, &a.groups);
   return ds_table(a.rows, a.vocab) ? launch_top<true>(a, nt, st) : launch_top<false>(a, nt, st);
 }
 
