@@ -335,6 +335,48 @@ def test_overwritten_inputs_scale_the_gradient_at_hand():
             (t.ids, t.logp)[which].zero_()
         (got,) = torch.autograd.grad(loss, leaf, torch.tensor(2.0, device="cuda"))
         assert torch.equal(got, 2 * want)
+        # the gradient at hand has gone to the caller, or there is nothing to make another from
+        t = losses.TopLogits(ids.clone(), logp.clone(), rest)
+        loss = losses.capped_distillation(leaf, t, 15.0)
+        torch.autograd.grad(loss, leaf, retain_graph=True)
+        with torch.no_grad():
+            (t.ids, t.logp)[which].zero_()
+        with pytest.raises(RuntimeError, match="overwritten"):
+            torch.autograd.grad(loss, leaf)
+
+
+def test_one_row_for_many():
+    """Expanded logits, whose rows lie on one another, at every axis."""
+    from train_gpt_b200 import losses
+    row = _logits(1, 777, seed=21)
+    ids, logp, rest = _teacher(6, 777, 8, 15.0, 1.0)
+    for x in (row.expand(6, 777), row.view(1, 1, 777).expand(2, 3, 777), _logits(3, 777, seed=22).expand(2, 3, 777), _logits(2, 777, seed=23).view(2, 1, 777).expand(2, 3, 777)):
+        _check_top(x, 15.0, 20, 1.0)
+        lead = x.shape[:-1]
+        t = losses.TopLogits(ids.view(*lead, 8), logp.view(*lead, 8), rest.view(lead))
+        leaf = x.clone().requires_grad_()
+        want = losses.capped_distillation(leaf, t, 15.0)
+        want.backward()
+        base = x.detach().requires_grad_()
+        got = losses.capped_distillation(base, t, 15.0)
+        (d,) = torch.autograd.grad(got, base)
+        assert torch.equal(got.detach(), want.detach()) and torch.equal(d, leaf.grad)
+
+
+def test_a_teacher_that_names_nothing():
+    """No entries: all of its probability is the rest's."""
+    from train_gpt_b200 import losses
+    x = _logits(5, 301, seed=24)
+    ids, logp, rest = torch.zeros(5, 0, dtype=torch.int32, device="cuda"), torch.zeros(5, 0, device="cuda"), torch.zeros(5, device="cuda")
+    leaf = x.clone().requires_grad_()
+    loss = losses.capped_distillation(leaf, losses.TopLogits(ids, logp, rest), 15.0, target_ids=torch.arange(5, device="cuda"), weight=0.5)
+    loss.backward()
+    hard = x.clone().requires_grad_()
+    want = losses.capped_distillation(hard, losses.TopLogits(ids, logp, rest), 15.0, target_ids=torch.arange(5, device="cuda"), weight=0.0)
+    want.backward()
+    # its own rest is all there is, so that only the targets' half is left
+    assert abs(float(loss.detach()) - 0.5 * float(want.detach())) <= _log_tol(15.0, 1.0)
+    assert float((leaf.grad.double() - 0.5 * hard.grad.double()).abs().max()) <= 2.0 ** -8 * 0.5 / 5 + (4 * _delta(15.0, 1.0) + 2.0 ** -16) * 2 / 5
 
 
 def test_second_derivatives_are_an_error():

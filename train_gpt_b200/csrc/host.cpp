@@ -369,14 +369,14 @@ LogitRows logit_rows(const Tensor& logits) {
   r.ld = r.vocab;
   if (r.rows == 0 || logits.is_contiguous()) return r;
   bool lies = logits.stride(-1) == 1;
-  int64_t pitch = 0, next = 0;                 // of the rows; what the next axis outwards has to step by
+  int64_t pitch = -1, next = 0;                // of the rows (-1: there is one); what the next axis outwards has to step by
   for (int64_t i = logits.dim() - 2; i >= 0; --i) {
     if (logits.size(i) == 1) continue;
-    if (pitch == 0) pitch = logits.stride(i);
+    if (pitch < 0) pitch = logits.stride(i);
     else lies = lies && logits.stride(i) == next;
     next = logits.stride(i) * logits.size(i);
   }
-  if (lies && (pitch >= r.vocab || pitch == 0)) r.ld = std::max(pitch, r.vocab);
+  if (lies && (pitch >= r.vocab || pitch < 0)) r.ld = std::max(pitch, r.vocab);
   else r.t = logits.contiguous();
   return r;
 }
@@ -1187,6 +1187,7 @@ struct CappedDistillationBackward : public Node {
       const Tensor g = grads[0].to(at::kFloat).contiguous();
       const c10::cuda::CUDAGuard guard(d.device());
       if (versions_now() != versions) {
+        if (given) throw std::runtime_error("capped_distillation: inputs were overwritten between two backward passes");
         out[0] = (d * g).to(at::kBFloat16);
       } else {
         const bool again = given;
