@@ -63,7 +63,7 @@ struct Cap {
   float zt;            // c log2(e) / T: z / T in powers of two is sign(x) zt (1 - u)
   float c, inv_c, inv_t;
   uint32_t minus_lo2;  // minus the table's first magnitude as bf16 bits, twice
-  uint32_t tab2;       // its address, twice: plus a pair of entries times 4, two 16-bit addresses
+  uint32_t tab2;       // its address, twice: plus a pair of entries times 4, two 16-bit addresses (which a block of a cluster's would exceed)
   __device__ __forceinline__ Cap(float cap, float temperature, void* tables) {
     c = cap;
     inv_c = __fdiv_rn(1.0f, cap);
@@ -251,11 +251,13 @@ __device__ __forceinline__ float log_share(float part, float other) {
 // teacher does not name.  Those it does are marked in a bitmap, a byte per piece, and computed by one thread each; what else is in a piece with a
 // mark is added by the thread of its lowest one, which is the same whatever the order of the marks was.  Second pass: the gradient, from the
 // row as the first has left it in shared memory, after which the threads of the named logits and the target write theirs over it.
-// (Read again instead -- a vocabulary that does not fit is -- a third of it comes from memory, with 444 rows of 100 KB and their gradients in
-// work: 8192 x 50304 with 64 logits 551 us, of which the second pass 330, however little it computes.)  Two rows of 50304 logits
-// fit on an SM only with one table for both, hence the groups.
-// A row has three barriers, and a chain of loads (an id, its logit) at its beginning: its first pieces and the next row's ids and logits are
-// fetched a phase ahead, and the next row as a whole comes as far as the L2 during the second pass.
+// (A vocabulary that does not fit is read again, about a third of it from memory: 4096 x 130000 735 us, 1.9 times the time a logit.)  Two rows of
+// 50304 logits fit on an SM only with one table for both, hence the groups.
+// A row has three barriers, and a chain of loads (an id, its logit) at its beginning: the next row's ids and logits are fetched a phase ahead, and
+// its pieces take the places of this one's as the second pass leaves them.
+// 8192 x 50304 with 64 logits: 427 us (3.9 TB/s), 464 with a target at another temperature.  A row's 28100 cycles are 11800 of the first pass, 14100
+// of the second, 2300 around the barriers; with two rows at once look-ups (3.5 cycles of shared memory for 32) and exponentials (two cycles)
+// each take about 80 % of that.
 // EXPS: 1 where one sum does (one temperature, or one of the two losses), 2 for two exponentials, 3 and 4 where the second is the first one
 // squared once or twice (temperatures 2 and 4).
 // ---------------------------------------------------------------------------------------
@@ -554,7 +556,7 @@ __global__ void __launch_bounds__(ds_block_threads(STAGED), 1) softcap_distill_k
 }
 
 // ---------------------------------------------------------------------------------------
-// A teacher's top logits.  One thread block per row.  First a bound that at least k logits reach and few others: the largest logit of every
+// A teacher's top logits.  A group of threads per row.  First a bound that at least k logits reach and few others: the largest logit of every
 // group (each of the eight elements of a thread's pieces is one) is found, and the k-th largest of those taken; with 1024 groups about
 // 1024 ln(1 / (1 - k / 1024)) logits reach it.  Where a row is long enough the groups come from an eighth of it, eight pieces of every
 // 64, and the bound is their `rank`-th largest: k / 8 with four standard deviations and four more, so that one row in some thousand has too
@@ -564,6 +566,8 @@ __global__ void __launch_bounds__(ds_block_threads(STAGED), 1) softcap_distill_k
 // by counting into bins of a key or a few, and within their bin.
 // Where the bound lets too many or too few through (a row of equal logits, large ones side by side), or a NaN is among them, the k-th largest logit is
 // found by bisection on the row's 16-bit keys, and its equals are taken in the row's order.
+// 8192 x 50304: 252 us with 8 logits kept, 320 with 256 (2.6 TB/s).  Of a row's 90000 cycles, eight rows at once, the pass over it has 47000, the
+// sample and the bound 10000; the rest are the candidates', short steps between barriers.
 // ---------------------------------------------------------------------------------------
 struct TopArgs {
   const void* logits;
@@ -748,14 +752,14 @@ __global__ void __launch_bounds__(2 * kDsMaxThreads, 1) top_logits_kernel(const 
     // bit b of the marks is piece first + b (whole warps, for the ballot); the pieces at the row's ends are listed without one
     const int whole = q.last() - q.first(), words = (whole + 31) >> 5;
     in.each(q, q.first() + words * 32, tid, nt, [&](const uint4& w, int i) {
-        const bool skip = (reach(w.x) | reach(w.y) | reach(w.z) | reach(w.w)) != 0u || i >= q.last();
-        const uint32_t marks = __ballot_sync(0xffffffffu, skip && i < q.last());
-        if (lane == 0) s_marks[(i - q.first()) >> 5] = marks;
-        float2 e[4];
-        four_words(w, [&](auto j, uint32_t v) { e[j] = cap.template e<decltype(j)::value>(v); });
-        const float2 sum = __fadd2_rn(__fadd2_rn(e[0], e[1]), __fadd2_rn(e[2], e[3]));
-        acc = __fadd2_rn(acc, make_float2(skip ? 0.f : sum.x, skip ? 0.f : sum.y));
-        if (TABLE && i < q.last()) nan = __vmaxu2(nan, C::largest(w));
+      const bool skip = (reach(w.x) | reach(w.y) | reach(w.z) | reach(w.w)) != 0u || i >= q.last();
+      const uint32_t marks = __ballot_sync(0xffffffffu, skip && i < q.last());
+      if (lane == 0) s_marks[(i - q.first()) >> 5] = marks;
+      float2 e[4];
+      four_words(w, [&](auto j, uint32_t v) { e[j] = cap.template e<decltype(j)::value>(v); });
+      const float2 sum = __fadd2_rn(__fadd2_rn(e[0], e[1]), __fadd2_rn(e[2], e[3]));
+      acc = __fadd2_rn(acc, make_float2(skip ? 0.f : sum.x, skip ? 0.f : sum.y));
+      if (TABLE && i < q.last()) nan = __vmaxu2(nan, C::largest(w));
     });
     in.fetch(q_next, tid, nt);
     group.sync();
