@@ -91,6 +91,22 @@ def test_top_logits_where_a_sample_of_the_row_misleads(vocab):
         _check_top(x.to(torch.bfloat16), 15.0, k, 1.0)
 
 
+@pytest.mark.parametrize("vocab", [4099, 30000])
+def test_top_logits_on_a_coarse_grid(vocab):
+    """Hundreds of logits equal to the k-th, above and below 0, with and without a NaN."""
+    from train_gpt_b200 import losses
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(5, vocab, device="cuda", generator=g)
+    x = torch.stack([1 + 0.02 * x[0], -1 + 0.02 * x[1], (2 * x[2]).round(), 64 + x[3], -x[4].abs().round()]).to(torch.bfloat16)
+    for k in (1, 7, 64, 256):
+        _check_top(x, 15.0, k, 1.0)
+    x[:, vocab // 2] = float("nan")
+    top = losses.top_logits(x, 15.0, 64)
+    x[:, vocab // 2] = INF
+    ids = ref.top_logits(x.double(), 15.0, 64, 1.0)[0]
+    assert torch.equal(top.ids.long(), ids) and bool(top.logp.isnan().all())
+
+
 @pytest.mark.parametrize("rows,vocab,k", [(160, 40001, 16), (320, 33000, 64), (700, 20000, 200), (1200, 5000, 20), (1190, 1500, 100), (1300, 4095, 256), (600, 9001, 8)])
 def test_top_logits_of_more_rows_than_fit(rows, vocab, k):
     """Several rows at a time on an SM, with one or two groups of threads left without a row in the last round."""

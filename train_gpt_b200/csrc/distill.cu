@@ -565,7 +565,8 @@ __global__ void __launch_bounds__(ds_block_threads(STAGED), 1) softcap_distill_k
 // their order, a thread each, so that a warp does not go through a branch for nearly every 32 pieces.  The candidates are then sorted
 // by counting into bins of a key or a few, and within their bin.
 // Where the bound lets too many or too few through (a row of equal logits, large ones side by side), or a NaN is among them, the k-th largest logit is
-// found by bisection on the row's 16-bit keys, and its equals are taken in the row's order.
+// found by bisection on the row's 16-bit keys, from the bound on, and its equals are taken in the row's order: 1024 x 50304 with 64
+// kept 160 us with all logits equal and 227 with hundreds equal to the 64th (bisection of all keys: 858 and 562), 43 as a rule.
 // 8192 x 50304: 252 us with 8 logits kept, 320 with 256 (2.6 TB/s).  Of a row's 90000 cycles, eight rows at once, the pass over it has 47000, the
 // sample and the bound 10000; the rest are the candidates', short steps between barriers.
 // ---------------------------------------------------------------------------------------
@@ -847,11 +848,20 @@ __global__ void __launch_bounds__(2 * kDsMaxThreads, 1) top_logits_kernel(const 
         for (int j = 0; j < 8; ++j)
           if (!(skip >> j & 1u)) f(j, top_key(j & 1 ? wi[j >> 1] >> 16 : wi[j >> 1] & 0xffffu));
       };
-      uint32_t key = 0u;
-      for (uint32_t bit = 0x8000u; bit != 0u; bit >>= 1) {
+      auto reached = [&](uint32_t v) {
         int c = 0;
-        for (int i = tid; i < pieces; i += nt) keys_of(i, [&](int, uint32_t v) { c += v >= (key | bit); });
-        if (count(c) >= k) key |= bit;
+        for (int i = tid; i < pieces; i += nt) keys_of(i, [&](int, uint32_t u) { c += u >= v; });
+        return count(c) >= k;
+      };
+      // it lies at the bound or little above where that lets enough through (steps of 1, 2, 4, ...), else below
+      const bool enough = crowded || n >= k;
+      uint32_t key = enough ? lo : 0u, step = enough ? 1u : 0x10000u, last = enough || odd ? 0xffffu : lo;
+      for (; key + step <= last && reached(key + step); step *= 2u) key += step;
+      last = min(last, key + step - 1u);
+      while (key < last) {
+        const uint32_t mid = (key + last + 1u) >> 1;
+        if (reached(mid)) key = mid;
+        else last = mid - 1u;
       }
       if (tid == 0) sh.n = 0;
       group.sync();
