@@ -66,12 +66,12 @@ def _check(x, y, post, pre, gate, alpha, g, gh, quantize=False):
 
 @pytest.mark.parametrize("gate", ["none", "channel", "token"])
 @pytest.mark.parametrize("rows,cols", [(1, 8), (3, 128), (129, 256), (33, 264), (700, 1024), (50, 1032), (1000, 2048), (7, 1536), (65, 2304), (300, 4096), (5, 5000),
-                                       (40, 6144), (16, 8192), (600, 8184)])
+                                       (40, 6144), (16, 8192), (600, 8184), (5000, 520), (2500, 768), (1600, 1288), (1300, 2824), (500, 2560), (700, 3464), (333, 4616), (300, 7000)])
 def test_against_the_formulas(rows, cols, gate):
     _check(*_inputs((rows, cols), gate)[:5], 0.9, *_inputs((rows, cols), gate)[5:])
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 128), (200, 384), (1000, 1024), (257, 2048), (16, 8192), (31, 4224)])
+@pytest.mark.parametrize("rows,cols", [(1, 128), (200, 384), (1000, 1024), (257, 2048), (16, 8192), (31, 4224), (2500, 768), (1600, 1280), (1300, 2944), (700, 5120)])
 def test_quantised_form(rows, cols):
     i = _inputs((rows, cols), "channel", seed=3)
     _check(*i[:5], 1.0, *i[5:], quantize=True)
