@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(ds_block_threads(STAGED), 1) softcap_distill_k
 // Where the bound lets too many or too few through (a row of equal logits, large ones side by side), or a NaN is among them, the k-th largest logit is
 // found by bisection on the row's 16-bit keys, from the bound on, and its equals are taken in the row's order: 1024 x 50304 with 64
 // kept 160 us with all logits equal and 227 with hundreds equal to the 64th (bisection of all keys: 858 and 562), 43 as a rule.
-// 8192 x 50304: 252 us with 8 logits kept, 320 with 256 (2.6 TB/s).  Of a row's 90000 cycles, eight rows at once, the pass over it has 47000, the
+// 8192 x 50304: 248 us with 8 logits kept, 314 with 256 (2.6 TB/s).  Of a row's 90000 cycles, eight rows at once, the pass over it has 47000, the
 // sample and the bound 10000; the rest are the candidates', short steps between barriers.
 // ---------------------------------------------------------------------------------------
 struct TopArgs {
@@ -589,6 +589,12 @@ __device__ __forceinline__ uint32_t top_key(uint32_t bits) {
   return bits & 0x8000u ? 0x8000u - (bits & 0x7fffu) : 0x8000u + bits;
 }
 __device__ __forceinline__ uint32_t top_bits(uint32_t key) { return key >= 0x8000u ? key - 0x8000u : 0x8000u | (0x8000u - key); }
+
+// the larger of each of two pairs of bf16, NaN where one of them is
+__device__ __forceinline__ uint32_t top_max_nan(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
 
 constexpr int kTopBins = 256;
 struct TopShared {                             // of a group, followed by room for the candidates, twice, and a bit per piece
@@ -753,14 +759,14 @@ __global__ void __launch_bounds__(2 * kDsMaxThreads, 1) top_logits_kernel(const 
     // bit b of the marks is piece first + b (whole warps, for the ballot); the pieces at the row's ends are listed without one
     const int whole = q.last() - q.first(), words = (whole + 31) >> 5;
     in.each(q, q.first() + words * 32, tid, nt, [&](const uint4& w, int i) {
-      const bool skip = (reach(w.x) | reach(w.y) | reach(w.z) | reach(w.w)) != 0u || i >= q.last();
+      const uint32_t most = top_max_nan(top_max_nan(w.x, w.y), top_max_nan(w.z, w.w));     // (a NaN marks its piece too)
+      const bool skip = __hgeu2_mask(*reinterpret_cast<const __nv_bfloat162*>(&most), bound) != 0u || i >= q.last();
       const uint32_t marks = __ballot_sync(0xffffffffu, skip && i < q.last());
       if (lane == 0) s_marks[(i - q.first()) >> 5] = marks;
       float2 e[4];
       four_words(w, [&](auto j, uint32_t v) { e[j] = cap.template e<decltype(j)::value>(v); });
       const float2 sum = __fadd2_rn(__fadd2_rn(e[0], e[1]), __fadd2_rn(e[2], e[3]));
       acc = __fadd2_rn(acc, make_float2(skip ? 0.f : sum.x, skip ? 0.f : sum.y));
-      if (TABLE && i < q.last()) nan = __vmaxu2(nan, C::largest(w));
     });
     in.fetch(q_next, tid, nt);
     group.sync();
