@@ -285,7 +285,8 @@ int tg_softcap_ce_bwd(const void* tanh_in, const int32_t* targets, const float* 
 int tg_top_logits(const void* logits, float cap, float temperature, int32_t* ids, float* logp, float* log_rest, int64_t rows,
                   int64_t vocab, int64_t ld, int k, void* stream);
 
-/* A student's loss against a teacher's top logits, and its gradient, from one read of the student's logits.  Per row, with
+/* A student's loss against a teacher's top logits, and its gradient, from one read of the student's logits (two with a gradient of
+ * more than about 100000 logits a row).  Per row, with
  * s = z / T, q = softmax(s), q1 = softmax(z), p_j = exp(logp_j), K the named logits and q_R = sum_{i not in K} q_i:
  *   weight T^2 [ sum_j p_j (logp_j - log q[id_j]) + p_R (log_rest - log q_R) ] + (1 - weight) (-log q1[target])
  * Terms whose probability is 0 are 0.  An id outside [0, vocab) is no entry (its logp is not read) and a target outside it no

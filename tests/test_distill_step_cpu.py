@@ -56,3 +56,19 @@ def test_checkpoint_round_trip(tmp_path):
         checkpoint.load_params(plain, tree)
     with pytest.raises(ValueError, match="layer parameters"):
         checkpoint.load_params(b, checkpoint.params_tree(plain))
+
+
+def test_a_living_graph_is_seen():
+    from train_gpt_b200.step import _graph_alive
+    model = GPT(_cfg(), "cpu")
+    ids = torch.randint(0, 256, (2, 16))
+    assert not _graph_alive(model.parameters())
+    loss = model.loss(ids, ids)
+    assert _graph_alive(model.parameters())
+    loss.backward()
+    assert _graph_alive(model.parameters())
+    del loss
+    assert not _graph_alive(model.parameters()) and not _graph_alive(model.parameters())
+    with torch.no_grad():
+        kept = model.loss(ids, ids)
+    assert not _graph_alive(model.parameters()) and kept.isfinite()

@@ -101,3 +101,18 @@ def test_a_step_without_a_teacher_is_unchanged():
     loss, _ = tr.step(ids, targets, teacher=_teacher(cfg).top_logits(ids, 16))
     assert torch.isfinite(loss)
     assert torch.isfinite(tr.step(ids, targets)[0])
+
+
+def test_a_living_loss_refuses_the_capture():
+    from train_gpt_b200.step import Trainer
+    cfg = _cfg(distill_temperature=2.0, distill_weight=0.5)
+    tr = Trainer(cfg, torch.device("cuda", 0), seed=3, graph=True)
+    ids, targets = _batch(cfg, 1)
+    top = _teacher(cfg).top_logits(ids, 16, 2.0)
+    loss = tr.model.distillation_loss(ids, targets, top)
+    with pytest.raises(RuntimeError, match="still alive"):
+        tr.step(ids, targets, teacher=top)
+    want = loss.detach().clone()
+    del loss
+    got, _ = tr.step(ids, targets, teacher=top)
+    assert torch.equal(got, want)

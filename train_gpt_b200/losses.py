@@ -73,6 +73,7 @@ def capped_distillation(logits: torch.Tensor, teacher: TopLogits, cap: float, ta
     and log_rest 0 adds 0 to the sum and has gradient 0, but counts in the mean.  An id named twice is one logit with both
     probabilities.  Differentiable once, with respect to logits.
 
-    As with `capped_cross_entropy`, with gradients on the FORWARD writes the gradient too, from the same read of the logits; logits and
+    As with `capped_cross_entropy`, with gradients on the FORWARD writes the gradient too, from the same read of the logits
+    (from a second one beyond some 100000 logits a row); logits and
     gradient stay allocated until the backward pass or the result's end."""
     return ops._host().capped_distillation(logits, teacher.ids, teacher.logp, teacher.log_rest, cap, target_ids, temperature, weight)
