@@ -251,7 +251,7 @@ __device__ __forceinline__ float log_share(float part, float other) {
 // teacher does not name.  Those it does are marked in a bitmap, a byte per piece, and computed by one thread each; what else is in a piece with a
 // mark is added by the thread of its lowest one, which is the same whatever the order of the marks was.  Second pass: the gradient, from the
 // row as the first has left it in shared memory, after which the threads of the named logits and the target write theirs over it.
-// (A vocabulary that does not fit is read again, about a third of it from memory: 4096 x 130000 735 us, 1.9 times the time a logit.)  Two rows of
+// (A vocabulary that does not fit is read again, about a third of it from memory: 4096 x 130000 735 us, 1.3 times the time a logit.)  Two rows of
 // 50304 logits fit on an SM only with one table for both, hence the groups.
 // A row has three barriers, and a chain of loads (an id, its logit) at its beginning: the next row's ids and logits are fetched a phase ahead, and
 // its pieces take the places of this one's as the second pass leaves them.
