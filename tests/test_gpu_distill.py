@@ -228,7 +228,7 @@ def test_distillation(rows, vocab, k, cap, t, w, rest):
     _check_distill(_logits(rows, vocab, seed=7), ids, logp, log_rest, cap, targets if w < 1 else None, t, w)
 
 
-@pytest.mark.parametrize("rows,vocab,k,t,w", [(450, 9001, 130, 1.0, 1.0), (1201, 5000, 8, 2.0, 0.5), (700, 30001, 64, 4.0, 0.5), (330, 130000, 20, 3.0, 0.5), (1190, 300, 100, 1.0, 0.5)])
+@pytest.mark.parametrize("rows,vocab,k,t,w", [(450, 9001, 130, 1.0, 1.0), (1201, 5000, 8, 2.0, 0.5), (700, 30001, 64, 4.0, 0.5), (330, 130000, 20, 3.0, 0.5), (1190, 300, 100, 1.0, 0.5), (12001, 300, 20, 2.0, 0.5), (5003, 1024, 70, 1.0, 1.0), (9001, 777, 5, 3.0, 0.5)])
 def test_distillation_of_more_rows_than_fit(rows, vocab, k, t, w):
     """Rows beside each other on an SM (two that share a table, up to eight that are not kept), the last round not full."""
     ids, logp, rest = _teacher(rows, vocab, k, 15.0, t)

@@ -1019,7 +1019,8 @@ static int ds_threads(int64_t pieces, int least, int most) {
   return int(std::min<int64_t>(std::max<int64_t>(want, 32), most));
 }
 
-// Whether the logits that a block meets pay for its table.
+// Whether the logits that a block meets pay for its table: 128 rows of 8192 with the gradient 7.7 us with it and 7.6 without, of 16384 8.15 and
+// 8.25, of 32768 11.0 and 12.2; 2000 of 4096 27.3 and 28.9 (evaluated 14.0 and 15.8).
 static bool ds_table(int64_t rows, int64_t vocab) { return std::max<int64_t>(1, rows / (2 * sm_count())) * vocab >= 16384; }
 
 // Blocks of `threads` that an SM holds of `kern`, whose registers and static shared memory are looked up once per device.
@@ -1050,7 +1051,8 @@ constexpr int64_t kDsDynamicMax = kDsSmemMax - 4 * 1024;     // (less than 4 KB 
 
 // Threads and groups for rows that are not kept.  A row alone has phases in which little is on its way, so several are in work on an SM: eight by 128
 // threads each where that is enough for one (`least`).  Fewer and larger groups cost 1.08 and 1.25 times as much a row and may have the better last round.
-static void ds_groups(int64_t rows, int64_t pieces, int least, int block, int* nt, int* groups) {
+// Rows with fewer than `least_group` threads have a block each (128 where there is no table to share: 500 x 500 4.8 us, in groups 6.1).
+static void ds_groups(int64_t rows, int64_t pieces, int least, int block, int least_group, int* nt, int* groups) {
   const int64_t sms = sm_count();
   double best = 0.0;
   *groups = 1;
@@ -1063,7 +1065,7 @@ static void ds_groups(int64_t rows, int64_t pieces, int least, int block, int* n
     }
   }
   *nt = ds_threads(pieces, least, block / std::max(*groups, 2));
-  if (*nt < 128) *groups = 1;
+  if (*nt < least_group) *groups = 1;
 }
 
 template <int EXPS, bool GRAD, bool TABLE, bool STAGED>
@@ -1071,8 +1073,10 @@ static int launch_distill(DistillArgs a, int nt, cudaStream_t st) {
   static DsKernelInfo info;
   auto kern = softcap_distill_kernel<EXPS, GRAD, TABLE, STAGED>;
   const int64_t table = TABLE ? cap_bytes(distill_table(EXPS, GRAD)) : 0, bytes = ds_map_bytes(a.vocab) + (STAGED ? ds_row_bytes(a.vocab) : 0);
-  // two groups in a block where two blocks do not fit on an SM beside each other
-  if (STAGED) a.groups = 2 * (table + bytes) > kDsDynamicMax && table + 2 * bytes <= kDsDynamicMax && a.rows > sm_count() ? 2 : 1;
+  // groups that share a block's table where a row has less than 128 threads (16384 x 1024 88 us, a table each 149; from 128 on 1.03 times the
+  // time) and where two blocks do not fit on an SM beside each other
+  if (STAGED && TABLE && nt < 128) a.groups = int(std::max<int64_t>(1, std::min<int64_t>({kDsMaxGroups, ds_block_threads(true) / nt, a.rows / sm_count()})));
+  else if (STAGED) a.groups = 2 * (table + bytes) > kDsDynamicMax && table + 2 * bytes <= kDsDynamicMax && a.rows > sm_count() ? 2 : 1;
   while (a.groups > 1 && table + a.groups * bytes > kDsDynamicMax) --a.groups;
   a.group_bytes = int(bytes);
   const int64_t smem = table + a.groups * bytes;
@@ -1094,7 +1098,7 @@ static int launch_distill(const DistillArgs& a, cudaStream_t st) {
   }
   DistillArgs b = a;
   int nt;
-  ds_groups(a.rows, pieces, (a.k + 31) / 32 * 32, ds_block_threads(false), &nt, &b.groups);
+  ds_groups(a.rows, pieces, (a.k + 31) / 32 * 32, ds_block_threads(false), table ? 32 : 128, &nt, &b.groups);
   return table ? launch_distill<EXPS, GRAD, true, false>(b, nt, st) : launch_distill<EXPS, GRAD, false, false>(b, nt, st);
 }
 
@@ -1118,17 +1122,18 @@ static int launch_top_short(const TopArgs& a, cudaStream_t st) {
 }
 static int launch_top(TopArgs a, cudaStream_t st) {
   const int64_t pieces = (a.vocab + 14) / 8;
-  // (where a warp's turns, k of them, are fewer instructions than the general kernel has for so short a row)
+  // where a warp's turns, k of them, take no longer than the general kernel's steps: 8192 x 240 with 64 kept 34 us (the latter 44), x 500 with 48 45
+  // (45), x 1000 with 20 41 (41), with 8 26 (39)
   if (pieces <= 32 && a.k <= 64) return launch_top_short<1>(a, st);
   if (pieces <= 64 && a.k <= 48) return launch_top_short<2>(a, st);
-  if (pieces <= 128 && a.k <= 32) return launch_top_short<4>(a, st);
+  if (pieces <= 128 && a.k <= 20) return launch_top_short<4>(a, st);
   int nt;
-  // many short rows: two warps each
-  if (pieces <= 512 && a.rows > 8 * sm_count()) {
+  // many short rows, eight to a block with two warps each: 8192 x 4000 with 64 kept 70 us, four warps 77, with 128 94 and 88; x 2000 53 and 72, 79 and 82
+  if (pieces <= 512 && pieces * a.k <= 48 * 1024 && a.rows > 8 * sm_count()) {
     a.groups = kDsMaxGroups;
     return launch_top<false>(a, 64, st);
   }
-  ds_groups(a.rows, pieces, 32, 2 * kDsMaxThreads, &nt, &a.groups);
+  ds_groups(a.rows, pieces, 32, 2 * kDsMaxThreads, 128, &nt, &a.groups);
   return ds_table(a.rows, a.vocab) ? launch_top<true>(a, nt, st) : launch_top<false>(a, nt, st);
 }
 
