@@ -1151,6 +1151,7 @@ extern "C" int tg_top_logits(const void* logits, float cap, float temperature, i
   if (!ds_cap_fits(cap, temperature)) return TG_ERR_SHAPE;
   if (rows > INT32_MAX || vocab > kDsMaxVocab || k > TG_TOP_LOGITS_MAX) return TG_ERR_TOO_LARGE;
   if (rows == 0) return TG_OK;
+  if (logits == nullptr) return TG_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(logits) & 1u) != 0) return TG_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
   const bool sampled = vocab >= kTopSampleFrom;
@@ -1169,6 +1170,7 @@ extern "C" int tg_softcap_distill(const tg_distill_args* args, void* stream) {
   if (g.dlogits == nullptr && g.row_loss == nullptr) return TG_ERR_SHAPE;
   if (g.rows > INT32_MAX || g.vocab > kDsMaxVocab || g.k > TG_TOP_LOGITS_MAX) return TG_ERR_TOO_LARGE;
   if (g.rows == 0) return TG_OK;
+  if (g.logits == nullptr) return TG_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(g.logits) & 1u) != 0) return TG_ERR_ALIGN;
   if (g.dlogits != nullptr && ((reinterpret_cast<uintptr_t>(g.logits) ^ reinterpret_cast<uintptr_t>(g.dlogits)) & 15u) != 0) return TG_ERR_ALIGN;
   if (int rc = check_arch()) return rc;

@@ -534,6 +534,7 @@ extern "C" int tg_sandwich_norm_fwd(const void* x, const void* branch, const voi
   if ((q == nullptr) != (scales == nullptr) || (q == nullptr && h == nullptr) || (q != nullptr && cols % kTile != 0)) return TG_ERR_SHAPE;
   if (cols > kSwMaxCols) return TG_ERR_TOO_LARGE;
   if (rows == 0) return TG_OK;
+  if (x == nullptr || branch == nullptr) return TG_ERR_SHAPE;
   if (!aligned16(x) || !aligned16(branch) || !aligned16(post) || !aligned16(pre) || !gate_aligned(gate, gate_kind) || !aligned16(x_new) ||
       !aligned16(h) || !aligned16(q))
     return TG_ERR_ALIGN;
@@ -555,6 +556,7 @@ extern "C" int tg_sandwich_norm_bwd(const void* x_new, const void* branch, const
   if (rows < 0 || cols <= 0 || cols % 8 != 0 || !gate_ok(gate, gate_kind) || post == nullptr || pre == nullptr || dpost == nullptr || dpre == nullptr)
     return TG_ERR_SHAPE;
   if (cols > kSwMaxCols) return TG_ERR_TOO_LARGE;
+  if (rows > 0 && (x_new == nullptr || branch == nullptr || dx == nullptr || dbranch == nullptr || scratch == nullptr)) return TG_ERR_SHAPE;
   if (!aligned16(x_new) || !aligned16(branch) || !aligned16(post) || !aligned16(pre) || !gate_aligned(gate, gate_kind) || !aligned16(g_new) ||
       !aligned16(g_h) || !aligned16(dx) || !aligned16(dbranch) || !aligned16(scratch))
     return TG_ERR_ALIGN;
