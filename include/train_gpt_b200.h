@@ -300,8 +300,9 @@ typedef struct tg_distill_args {
   const void* targets;     /* int32 [rows], or int64 with targets_64, or NULL: no such term                        */
   int ids_64, targets_64;
   float cap, temperature, weight;   /* limits of cap and T as in tg_top_logits; 0 <= weight <= 1                   */
-  void* dlogits;           /* bf16 [rows, ld] or NULL: gscale / rows * d(sum of the rows' losses)/dlogits; not the logits'
-                              buffer, and as far from a 16-byte boundary as they are (else TG_ERR_ALIGN)           */
+  void* dlogits;           /* bf16 [rows, ld] or NULL: gscale / rows * d(sum of the rows' losses)/dlogits; no element of
+                              the logits' (else TG_ERR_SHAPE), and as far from a 16-byte boundary as they are
+                              (else TG_ERR_ALIGN)                                                                 */
   const float* gscale;     /* device float or NULL for 1                                                           */
   int only_if_scaled;      /* the launch does nothing where *gscale is 1                                           */
   float* row_loss;         /* [rows] or NULL                                                                       */

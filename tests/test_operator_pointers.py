@@ -1,5 +1,5 @@
-"""Pointers that the C entries of the distillation operators and of the sandwich norm cannot do without:
-refused with a status before any device work."""
+"""Pointers that the C entries of the distillation operators and of the sandwich norm cannot do without, and outputs that would lie on their
+inputs: refused with a status before any device work."""
 import ctypes
 
 import pytest
@@ -33,6 +33,23 @@ def test_distillation_without_logits(lib):
     from train_gpt_b200._lib import TG_ERR_SHAPE, TG_OK
     assert _distill(lib, logits=None) == _distill(lib, logits=None, dlogits=None) == TG_ERR_SHAPE
     assert _distill(lib, logits=None, rows=0) == TG_OK
+
+
+@pytest.mark.parametrize("elements,rows,vocab,ld", [
+    (0, 4, 100, 100),                       # the logits' own buffer
+    (0, 1, 1, 1),
+    (96, 1, 100, 100),                      # the end of the only row
+    (-96, 1, 100, 100),
+    (296, 4, 100, 100),                     # the last row alone
+    (-296, 4, 100, 100),
+    (96, 4, 100, 200),                      # rows with a pitch: the end of each
+    (128, 4, 100, 200),                     # and the beginning of the next one
+    (-128, 4, 100, 200),
+    (720, 4, 100, 216),                     # three rows further, from 72 on
+])
+def test_gradient_over_the_logits(lib, elements, rows, vocab, ld):
+    from train_gpt_b200._lib import TG_ERR_SHAPE
+    assert _distill(lib, dlogits=ADDRESS[0] + 2 * elements, rows=rows, vocab=vocab, ld=ld) == TG_ERR_SHAPE
 
 
 @pytest.mark.parametrize("missing", ["x", "branch"])

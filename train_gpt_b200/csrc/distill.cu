@@ -1137,6 +1137,13 @@ static int launch_top(TopArgs a, cudaStream_t st) {
   return ds_table(a.rows, a.vocab) ? launch_top<true>(a, nt, st) : launch_top<false>(a, nt, st);
 }
 
+// Whether two sets of rows of one pitch have an element in common.  (Rows between each other's, in one buffer of twice the pitch, have none.)
+static bool ds_rows_overlap(const void* a, const void* b, int64_t rows, int64_t vocab, int64_t ld) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  const int64_t apart = int64_t((x < y ? y - x : x - y) / 2), q = apart / ld, m = apart % ld;
+  return (m < vocab && q < rows) || (ld - m < vocab && q + 1 < rows);
+}
+
 static bool ds_cap_fits(float cap, float temperature) {
   return cap >= 0x1p-10f && cap <= 64.0f && temperature > 0.f && temperature <= 1024.0f && cap <= 64.0f * temperature;
 }
@@ -1173,6 +1180,7 @@ extern "C" int tg_softcap_distill(const tg_distill_args* args, void* stream) {
   if (g.logits == nullptr) return TG_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(g.logits) & 1u) != 0) return TG_ERR_ALIGN;
   if (g.dlogits != nullptr && ((reinterpret_cast<uintptr_t>(g.logits) ^ reinterpret_cast<uintptr_t>(g.dlogits)) & 15u) != 0) return TG_ERR_ALIGN;
+  if (g.dlogits != nullptr && ds_rows_overlap(g.logits, g.dlogits, g.rows, g.vocab, g.ld)) return TG_ERR_SHAPE;
   if (int rc = check_arch()) return rc;
   // one sum does where there is one temperature
   const bool soft = g.weight > 0.f, hard = g.weight < 1.f && g.targets != nullptr;
