@@ -212,13 +212,26 @@ ffi::Error SoftcapCeBwd(cudaStream_t s, BF16 tanh_in, S32 targets, F32 lse, F32 
                "tg_softcap_ce_bwd");
 }
 
+// whether each of these buffers has n elements
+template <typename... B>
+bool Have(int64_t n, const B&... b) {
+  return ((static_cast<int64_t>(b.element_count()) == n) && ...);
+}
+ffi::Error Mismatch(const char* what) { return ffi::Error(ffi::ErrorCode::kInvalidArgument, what); }
+
 // ---- the junction of blocks with a norm on both sides (no counterpart) -----------------------------
+
+bool HaveGate(int32_t kind, int64_t rows, int64_t cols, const BF16& gate) {
+  return kind == TG_GATE_NONE || (kind == TG_GATE_CHANNEL && Have(cols, gate)) || (kind == TG_GATE_TOKEN && Have(rows, gate));
+}
 
 // gate_kind: TG_GATE_NONE (pass any bf16 buffer), TG_GATE_CHANNEL (cols,) or TG_GATE_TOKEN (rows,)
 ffi::Error SandwichNormFwd(cudaStream_t s, BF16 x, BF16 branch, BF16 post, BF16 pre, BF16 gate, RBF16 x_new, RBF16 h, int32_t gate_kind,
                            float residual_scale, float eps) {
   int64_t rows, cols;
   RowsCols(x, &rows, &cols);
+  if (!Have(rows * cols, branch, *x_new, *h) || !Have(cols, post, pre) || !HaveGate(gate_kind, rows, cols, gate))
+    return Mismatch("TgSandwichNormFwd: branch, x_new and h must be like x, post and pre (cols,), gate (cols,) or (rows,) as gate_kind says");
   return Check(tg_sandwich_norm_fwd(x.untyped_data(), branch.untyped_data(), post.untyped_data(), pre.untyped_data(), gate.untyped_data(), gate_kind,
                                     residual_scale, eps, x_new->untyped_data(), h->untyped_data(), nullptr, nullptr, rows, cols, s),
                "tg_sandwich_norm_fwd");
@@ -228,6 +241,8 @@ ffi::Error SandwichNormQuantFwd(cudaStream_t s, BF16 x, BF16 branch, BF16 post, 
                                 int32_t gate_kind, float residual_scale, float eps) {
   int64_t rows, cols;
   RowsCols(x, &rows, &cols);
+  if (!Have(rows * cols, branch, *x_new, *h, *q) || !Have(cols, post, pre) || !HaveGate(gate_kind, rows, cols, gate) || !Have(rows * (cols / 128), *scales))
+    return Mismatch("TgSandwichNormQuantFwd: branch, x_new, h and q must be like x, scales (rows, cols / 128), post and pre (cols,), gate (cols,) or (rows,) as gate_kind says");
   return Check(tg_sandwich_norm_fwd(x.untyped_data(), branch.untyped_data(), post.untyped_data(), pre.untyped_data(), gate.untyped_data(), gate_kind,
                                     residual_scale, eps, x_new->untyped_data(), h->untyped_data(), q->untyped_data(), scales->typed_data(), rows,
                                     cols, s),
@@ -239,6 +254,9 @@ ffi::Error SandwichNormBwd(cudaStream_t s, BF16 x_new, BF16 branch, BF16 post, B
                            RBF16 dpost, RBF16 dpre, RBF16 dgate, RU8 scratch, int32_t gate_kind, float residual_scale, float eps) {
   int64_t rows, cols;
   RowsCols(x_new, &rows, &cols);
+  if (!Have(rows * cols, branch, g_new, g_h, *dx, *dbranch) || !Have(cols, post, pre, *dpost, *dpre) || !HaveGate(gate_kind, rows, cols, gate) ||
+      !HaveGate(gate_kind, rows, cols, *dgate))
+    return Mismatch("TgSandwichNormBwd: branch, gradients, dx and dbranch must be like x_new, post, pre and theirs (cols,), gate and dgate (cols,) or (rows,) as gate_kind says");
   if (static_cast<int64_t>(scratch->element_count()) < tg_sandwich_norm_bwd_scratch_bytes(rows, cols))
     return ffi::Error(ffi::ErrorCode::kInvalidArgument, "TgSandwichNormBwd: scratch result smaller than tg_sandwich_norm_bwd_scratch_bytes");
   return Check(tg_sandwich_norm_bwd(x_new.untyped_data(), branch.untyped_data(), post.untyped_data(), pre.untyped_data(), gate.untyped_data(), gate_kind,
@@ -251,12 +269,12 @@ ffi::Error SandwichNormBwd(cudaStream_t s, BF16 x_new, BF16 branch, BF16 post, B
 
 // ids, logp (rows, k), log_rest (rows,)
 ffi::Error TopLogits(cudaStream_t s, BF16 logits, RS32 ids, RF32 logp, RF32 log_rest, float cap, float temperature) {
-  int64_t rows, vocab, k_rows, k;
+  int64_t rows, vocab;
   RowsCols(logits, &rows, &vocab);
   auto d = ids->dimensions();
-  k = d.size() ? d.back() : 0;
-  k_rows = k ? static_cast<int64_t>(ids->element_count()) / k : 0;
-  if (k_rows != rows || k > TG_TOP_LOGITS_MAX) return ffi::Error(ffi::ErrorCode::kInvalidArgument, "TgTopLogits: ids must be (rows, k)");
+  const int64_t k = d.size() ? d.back() : 0;
+  if (k > TG_TOP_LOGITS_MAX || !Have(rows * k, *ids, *logp) || !Have(rows, *log_rest))
+    return Mismatch("TgTopLogits: ids and logp must be (rows, k), log_rest (rows,)");
   return Check(tg_top_logits(logits.untyped_data(), cap, temperature, ids->typed_data(), logp->typed_data(), log_rest->typed_data(), rows, vocab, vocab,
                              static_cast<int>(k), s),
                "tg_top_logits");
@@ -270,9 +288,8 @@ ffi::Error SoftcapDistill(cudaStream_t s, BF16 logits, S32 ids, F32 logp, F32 lo
   RowsCols(logits, &a.rows, &a.vocab);
   auto d = ids.dimensions();
   const int64_t k = d.size() ? d.back() : 0;
-  if (k > TG_TOP_LOGITS_MAX || static_cast<int64_t>(ids.element_count()) != a.rows * k || logp.element_count() != ids.element_count() ||
-      static_cast<int64_t>(log_rest.element_count()) != a.rows || static_cast<int64_t>(targets.element_count()) != a.rows)
-    return ffi::Error(ffi::ErrorCode::kInvalidArgument, "TgSoftcapDistill: ids and logp must be (rows, k), log_rest and targets (rows,)");
+  if (k > TG_TOP_LOGITS_MAX || !Have(a.rows * k, ids, logp) || !Have(a.rows, log_rest, targets, *row_loss) || !Have(a.rows * a.vocab, *dlogits))
+    return Mismatch("TgSoftcapDistill: ids and logp must be (rows, k), log_rest, targets and row_loss (rows,), dlogits like logits");
   a.logits = logits.untyped_data(); a.ids = ids.untyped_data(); a.logp = logp.typed_data(); a.log_rest = log_rest.typed_data();
   a.targets = targets.untyped_data(); a.cap = cap; a.temperature = temperature; a.weight = weight;
   a.dlogits = dlogits->untyped_data(); a.row_loss = row_loss->typed_data();
