@@ -459,6 +459,7 @@ void tgh::register_step(py::module_& m) {
                                              final_norm, unembed, layers, g_embed, g_pos, g_final_norm, g_unembed, g_layers, flat, params, count,
                                              on_bucket, on_attention, on_end);
       }))
+      .def("applies", &StepProgram::applies)
       .def("step", [](StepProgram& p, const Tensor& ids, const Tensor& targets, double lr, double b1, double b2, double eps, double weight_decay,
                       double clip) { return p.applies() ? std::optional(p.step(ids, targets, Hyper{lr, b1, b2, eps, weight_decay, clip})) : std::nullopt; });
   m.def("softcap_ce_fits", [](double cap, int64_t rows, int64_t vocab) { return bool(api.tgh_softcap_ce_fits(float(cap), rows, vocab)); });

@@ -460,8 +460,8 @@ class Trainer:
     through autograd.
     Capture needs two eager warm-up steps; parameters and optimizer
     state are restored after them, so a captured run follows the same trajectory as an eager one.
-    A step that goes through autograd for a teacher or a sandwich norm is not captured while a loss of the same
-    model is alive: the stream of that loss's graph would be drawn into the capture, which ends the process.
+    A step that goes through autograd (other switches, a teacher, a frozen parameter) is not captured while a loss of the
+    same model is alive: the stream of that loss's graph would be drawn into the capture, which ends the process.
     """
 
     def __init__(self, cfg: StepConfig, device, world_size: int = 1, seed: int = 0, graph: bool = False,
@@ -565,7 +565,8 @@ class Trainer:
         return [t for st in self.opt.state.values() for t in st.values() if torch.is_tensor(t)]
 
     def _capture(self, ids, targets, teacher=None):
-        if (teacher is not None or self.cfg.block_norm == "sandwich") and _graph_alive(self.model.parameters()):
+        by_program = teacher is None and self._program is not None and self._program.applies()
+        if not by_program and _graph_alive(self.model.parameters()):
             raise RuntimeError("a loss of this model is still alive: delete it before the first step, which is captured")
         self._ids, self._tgt = ids.clone(), targets.clone()
         self._teacher = None if teacher is None else losses.TopLogits(*(None if t is None else t.clone() for t in teacher))
