@@ -9,7 +9,9 @@
 The loss alone (no gradient) has its own table, of exponentials, and keeps no row.  Temperatures choose how the second exponential is had: 1 none, 2
 and 4 the first one squared once and twice, 3 its own.
 
-Tolerances are those of test_gpu_distill."""
+Tolerances are those of test_gpu_distill.  A saturated logit's derivative of the cap is taken in 64 bits as 4 e / (1 + e)^2, e = exp(-2 |x| / c), which
+1 - tanh^2 loses; in the kernels u = 2 / (1 + exp(2 |x| / c)) has an exponent of up to 88 rounded three times, 3 * 88 * 2^-24 of u, which
+(4 DELTA + 2^-16) holds, and what is below 2^-126 may be 0: 2^-125 of the summands (u (2 - u) is at most twice that)."""
 import math
 
 import pytest
@@ -68,6 +70,58 @@ def test_a_nan_anywhere_in_a_row(rows, vocab, t, w):
     for g, v in zip(got, want):
         assert g[hit].isnan().all(), [r for r in at if not g[r].isnan().all()]
         assert torch.equal(g[~hit], v[~hit])
+
+
+def _exact(x, ids, logp, rest, cap, targets, t, w):
+    """(the rows' losses, the gradient of their mean, the size of its summands), the cap's derivative as it is where it is far below 2^-53."""
+    x = x.double()
+    z = ref.capped(x, cap).requires_grad_()
+    vocab = x.shape[1]
+    logq = torch.log_softmax(z / t, -1)
+    ids = ids.long()
+    p = logp.double().exp()
+    row = w * t * t * (p * (logp.double() - logq.gather(1, ids))).sum(-1)
+    named = torch.zeros_like(x, dtype=torch.bool).scatter_(1, ids, True)
+    r = rest.double()
+    row = row + w * t * t * r.exp() * (r - logq.masked_fill(named, -INF).logsumexp(-1))
+    if targets is not None:
+        row = row - (1 - w) * torch.log_softmax(z, -1).gather(1, targets.unsqueeze(-1)).squeeze(-1)
+    (dz,) = torch.autograd.grad(row.mean(), z)
+    e = torch.exp(-2 * x.abs() / cap)
+    sech2 = 4 * e / (1 + e) ** 2
+    # the summands without their signs and without the cap's derivative
+    q, q1 = torch.softmax(z.detach() / t, -1), torch.softmax(z.detach(), -1)
+    tail = torch.where(named, 0.0, q).sum(-1, keepdim=True)
+    size = w * t * (q * (p.sum(-1, keepdim=True) + r.exp().unsqueeze(-1) * (1 + torch.where(named, 0.0, 1 / tail))) + torch.zeros_like(x).scatter_add_(1, ids, p))
+    if targets is not None:
+        size = size + (1 - w) * (q1 + torch.zeros_like(x).scatter_(1, targets.unsqueeze(-1), 1.0))
+    return row.detach(), dz * sech2, size / x.shape[0], sech2
+
+
+@pytest.mark.parametrize("cap", [15.0, 8.0, 0.75])
+@pytest.mark.parametrize("rows,vocab", [FORMS[f] for f in ("plain", "one", "two", "unkept")], ids=("plain", "one", "two", "unkept"))
+@pytest.mark.parametrize("t,w", [(1.0, 1.0), (2.0, 0.5), (3.0, 0.5)])
+def test_saturated_logits(rows, vocab, cap, t, w):
+    """From where tanh is near 1 to far beyond it, both signs, in every element of a piece, on named logits and at the row's ends."""
+    x = _logits(rows, vocab, seed=32).float() * (cap / 15)
+    far = [cap * v for v in (4.0, 8.0, 11.0, 15.9, 16.1, 17.0, 18.0, 20.0, 25.0, 31.0, 33.0, 40.0, 44.0, 46.0, 63.0, 65.0, 130.0, 1e6)] + [3e38, INF]
+    ids, logp, rest = _teacher(rows, vocab, 9, 15.0, t)
+    targets = _targets(rows, vocab, w)
+    r = torch.arange(rows, device="cuda")
+    v = torch.tensor(far, device="cuda")[r % len(far)].unsqueeze(1)
+    u = torch.tensor(far, device="cuda")[(r + 10) % len(far)].unsqueeze(1)
+    x[:, 200:217], x[:, 300:317] = v, -u
+    x[:, :1], x[:, vocab - 1:] = u, -v
+    x.scatter_(1, ids[:, 2:3].long(), -v)
+    x = x.to(torch.bfloat16)
+    row, want, size, sech2 = _exact(x, ids, logp, rest, cap, targets, t, w)
+    got_rows, got, alone = _both(x, (ids, logp, rest), t, w, targets, cap)
+    delta = _delta(max(cap, 15.0), min(t, 1.0))
+    bound = 2.0 ** -8 * want.abs() + (4 * delta + 2.0 ** -16) * size * sech2 + 2.0 ** -125 * size + 2.0 ** -133
+    over = (got.double() - want).abs() / bound
+    assert bool((over <= 1).all()), (float(over.max()), divmod(int(over.argmax()), vocab))
+    tol = w * t * t * (_log_tol(cap, t) + 2.0 ** -18) + (1 - w) * _log_tol(cap, 1.0)
+    assert float((got_rows.double() - row).abs().max()) <= tol and float((alone.double() - row).abs().max()) <= tol
 
 
 @forms

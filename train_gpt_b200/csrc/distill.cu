@@ -47,15 +47,15 @@ __device__ __forceinline__ float ds_lds(uint32_t addr) {
 //
 // Three approximations of the special function unit a logit (two exponentials and a reciprocal), 16 of them a clock and SM, are six clocks for 32
 // logits.  x is a bf16 value, though, and everything here a function of it: between 2^-22 c, below which z is as good as +-2^-22 c,
-// and 16 c, from where on tanh is 1, it has 27 binades of 128 values.  A table over those (of -u by the magnitude, 14 KB, or of E = exp(z / T)
+// and 16 c, from where on tanh is 1, it has 27 binades of 128 values.  A table over those (of -u by the magnitude, or of E = exp(z / T)
 // by magnitude and sign, twice that) makes it a look-up, 3.5 clocks of shared memory for 32 random entries, and fewer instructions.
+// u goes on falling where tanh is 1, and sech^2 with it: the table of -u has two binades more (14.5 KB), up to where exp(2 |x| / c) overflows and u is 0.
 // A quarter of the logits (the last word of four) goes the other way, so that both units work.
 enum { kTabU = 1, kTabE = 2 };
-constexpr int kCapBinadesBelow = 22, kCapBinades = 27;
-constexpr int kCapEntries = kCapBinades * 128 + 1;
-constexpr int kCapTableBytes = (kCapEntries * 4 + 15) / 16 * 16;
+constexpr int kCapBinadesBelow = 22;
+constexpr int cap_entries(int table) { return (table & kTabU ? 29 : 27) * 128 + 1; }
 constexpr int kCapSign = 4096;                                             // entries from the positive logits' to the negative ones'
-constexpr int cap_bytes(int table) { return table == 0 ? 0 : table == kTabU ? kCapTableBytes : kCapSign * 4 + kCapTableBytes; }
+constexpr int cap_bytes(int table) { return table == 0 ? 0 : ((table == kTabE ? kCapSign : 0) * 4 + cap_entries(table) * 4 + 15) / 16 * 16; }
 
 template <int TABLES>
 struct Cap {
@@ -74,7 +74,7 @@ struct Cap {
       const uint32_t c_pow = (__float_as_uint(cap) >> 16) & 0x7f80u;     // 2^floor(log2 c)
       const uint32_t lo = c_pow - (kCapBinadesBelow << 7);
       float* t = static_cast<float*>(tables);
-      for (int i = threadIdx.x; i < kCapEntries; i += blockDim.x) {
+      for (int i = threadIdx.x; i < cap_entries(TABLES); i += blockDim.x) {
         const float nu = __fdiv_rn(-2.0f, 1.0f + expf(2.0f * (__uint_as_float((lo + uint32_t(i)) << 16) * inv_c)));
         if (TABLES & kTabU) t[i] = nu;
         if (TABLES & kTabE) {
@@ -89,7 +89,7 @@ struct Cap {
   }
   // two entries by magnitude, or by magnitude and sign
   __device__ __forceinline__ float2 look_up(uint32_t w, bool by_sign) const {
-    uint32_t at = __viaddmin_s16x2_relu(w & 0x7fff7fffu, minus_lo2, uint32_t(kCapEntries - 1) * 0x10001u);   // max(min(mag - lo, last), 0)
+    uint32_t at = __viaddmin_s16x2_relu(w & 0x7fff7fffu, minus_lo2, uint32_t(cap_entries(TABLES) - 1) * 0x10001u);   // max(min(mag - lo, last), 0)
     if (by_sign) at |= (w >> 3) & 0x10001000u;
     at = at * 4u + tab2;
     return make_float2(ds_lds(at & 0xffffu), ds_lds(at >> 16));
@@ -297,6 +297,7 @@ __global__ void __launch_bounds__(ds_block_threads(STAGED), 1) softcap_distill_k
   grid_wait();
   if (p.only_if_scaled && *p.gscale == 1.0f) return;
   extern __shared__ __align__(16) uint8_t s_ds[];
+  static_assert(kDsMaxGroups * 6 * (kDsMaxThreads / 32) * sizeof(float) <= 3 * 1024, "static shared memory beyond kDsStatic");
   __shared__ float s_reds[kDsMaxGroups][5 * (kDsMaxThreads / 32)], s_losses[kDsMaxGroups][kDsMaxThreads / 32];
   const C cap(p.cap, p.temperature, s_ds);
   const int nt = int(blockDim.x) / p.groups, index = int(threadIdx.x) / nt;
@@ -1047,7 +1048,10 @@ static int ds_blocks(K kern, DsKernelInfo& info, int64_t smem, int threads, int6
   return TG_OK;
 }
 
-constexpr int64_t kDsDynamicMax = kDsSmemMax - 4 * 1024;     // (less than 4 KB are static)
+constexpr int64_t kDsStatic = 3 * 1024;                       // (the loss's; the selection has none)
+constexpr int64_t kDsDynamicMax = kDsSmemMax - kDsStatic;
+// Whether two blocks of `smem` dynamic bytes do not fit on an SM (1 KB of each is the system's).
+constexpr bool ds_alone(int64_t smem) { return 2 * (smem + kDsStatic + 1024) > 228 * 1024; }
 
 // Threads and groups for rows that are not kept.  A row alone has phases in which little is on its way, so several are in work on an SM: eight by 128
 // threads each where that is enough for one (`least`).  Fewer and larger groups cost 1.08 and 1.25 times as much a row and may have the better last round.
@@ -1076,7 +1080,7 @@ static int launch_distill(DistillArgs a, int nt, cudaStream_t st) {
   // groups that share a block's table where a row has less than 128 threads (16384 x 1024 88 us, a table each 149; from 128 on 1.03 times the
   // time) and where two blocks do not fit on an SM beside each other
   if (STAGED && TABLE && nt < 128) a.groups = int(std::max<int64_t>(1, std::min<int64_t>({kDsMaxGroups, ds_block_threads(true) / nt, a.rows / sm_count()})));
-  else if (STAGED) a.groups = 2 * (table + bytes) > kDsDynamicMax && table + 2 * bytes <= kDsDynamicMax && a.rows > sm_count() ? 2 : 1;
+  else if (STAGED) a.groups = ds_alone(table + bytes) && table + 2 * bytes <= kDsDynamicMax && a.rows > sm_count() ? 2 : 1;
   while (a.groups > 1 && table + a.groups * bytes > kDsDynamicMax) --a.groups;
   a.group_bytes = int(bytes);
   const int64_t smem = table + a.groups * bytes;
@@ -1091,7 +1095,7 @@ static int launch_distill(const DistillArgs& a, cudaStream_t st) {
   const bool table = ds_table(a.rows, a.vocab);
   const int64_t pieces = (a.vocab + 14) / 8;
   if constexpr (GRAD) {
-    if (kCapTableBytes + ds_map_bytes(a.vocab) + ds_row_bytes(a.vocab) <= kDsDynamicMax) {
+    if (cap_bytes(kTabU) + ds_map_bytes(a.vocab) + ds_row_bytes(a.vocab) <= kDsDynamicMax) {
       const int nt = ds_threads(pieces, a.k, ds_block_threads(true) / 2);
       return table ? launch_distill<EXPS, true, true, true>(a, nt, st) : launch_distill<EXPS, true, false, true>(a, nt, st);
     }
