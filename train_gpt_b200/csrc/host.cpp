@@ -1201,8 +1201,16 @@ struct CappedDistillationBackward : public Node {
   }
 };
 
+// A forward-mode derivative would be dropped without a word: no operator here has one.
+void no_tangent(std::initializer_list<const Tensor*> inputs, const char* what) {
+  for (const Tensor* t : inputs)
+    if (t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error(cat(what, " has no forward-mode derivative"));
+}
+
 Tensor capped_distillation(const Tensor& logits, const Tensor& ids, const Tensor& logp, const std::optional<Tensor>& log_rest, double cap,
                            const std::optional<Tensor>& targets, double temperature, double weight) {
+  no_tangent({&logits, &logp}, "capped_distillation");
+  if (log_rest) no_tangent({&*log_rest}, "capped_distillation");
   Distill a = distill_args(logits, ids, logp, log_rest, cap, targets, temperature, weight);
   const bool track = at::GradMode::is_enabled() && logits.requires_grad();
   const c10::cuda::CUDAGuard guard(logits.device());
@@ -1259,6 +1267,8 @@ Sandwich sandwich_norm(const Tensor& x, const Tensor& branch, const Tensor& post
                        double residual_scale, bool want_q) {
   bool track = x.requires_grad() || branch.requires_grad() || post.requires_grad() || pre.requires_grad() || (gate && gate->requires_grad());
   track = track && at::GradMode::is_enabled();
+  no_tangent({&x, &branch, &post, &pre}, "sandwich_norm");
+  if (gate) no_tangent({&*gate}, "sandwich_norm");
   Sandwich o;
   {
     at::AutoDispatchBelowADInplaceOrView below;

@@ -55,7 +55,7 @@ def sandwich_norm(x, branch, post_scale, scale, eps: float, gate=None, residual_
     per channel, or (..., 1) bf16 for one per token; residual_scale and eps are static.
 
     Returns (x_new, h), or with quantize=True (D a multiple of 128) (x_new, h, q, scales), q and scales the 1x128 e4m3 form
-    of h that `fp8.block_scaled_matmul` takes as `a_quantized`; they carry no gradient, h does.  Differentiable once, in x,
+    of h that `fp8.block_scaled_matmul` takes as `a_quantized`; they carry no gradient, h does.  Differentiable once, in reverse mode, in x,
     branch, both scales and the gate; the backward pass keeps x_new and branch and computes the factors again.  32768 x 2048
     forward and backward is one kernel each way and a small one for the scales' gradients."""
     return ops._host().sandwich_norm(x, branch, post_scale, scale, eps, gate, residual_scale, quantize)

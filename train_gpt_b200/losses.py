@@ -71,7 +71,7 @@ def capped_distillation(logits: torch.Tensor, teacher: TopLogits, cap: float, ta
     logits (..., vocab) bf16 as top_logits takes them; teacher.ids (..., k) with k <= 256; target_ids (...) int32 or int64.
     Ids and targets outside the vocabulary take no part (their logp is not read): a padded token with ids of -1, a target of -1
     and log_rest 0 adds 0 to the sum and has gradient 0, but counts in the mean.  An id named twice is one logit with both
-    probabilities.  Differentiable once, with respect to logits.
+    probabilities.  Differentiable once, in reverse mode, with respect to logits.
 
     As with `capped_cross_entropy`, with gradients on the FORWARD writes the gradient too, from the same read of the logits
     (from a second one beyond some 100000 logits a row); logits and
