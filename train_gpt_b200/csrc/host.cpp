@@ -1218,6 +1218,9 @@ Tensor capped_distillation(const Tensor& logits, const Tensor& ids, const Tensor
   {
     at::AutoDispatchBelowADInplaceOrView below;
     if (track && (reinterpret_cast<uintptr_t>(ptr(a.x.t)) & 15u)) a.x = logit_rows(a.x.t.clone(at::MemoryFormat::Contiguous));
+    if (track)                               // what inference mode made counts no changes: its values are kept
+      for (Tensor* t : {&a.x.t, &a.ids, &a.logp, &a.log_rest, &a.targets})
+        if (t->defined() && t->is_inference()) *t = t->clone();
     if (track) d = a.gradient(logits.sizes());
     const Tensor row_loss = empty({a.x.rows}, at::kFloat, logits);
     if (a.x.rows > 0) {

@@ -75,5 +75,7 @@ def capped_distillation(logits: torch.Tensor, teacher: TopLogits, cap: float, ta
 
     As with `capped_cross_entropy`, with gradients on the FORWARD writes the gradient too, from the same read of the logits
     (from a second one beyond some 100000 logits a row); logits and
-    gradient stay allocated until the backward pass or the result's end."""
+    gradient stay allocated until the backward pass or the result's end.  An upstream gradient other than 1 makes the gradient again from
+    the inputs, or scales the one at hand where they were overwritten in between; tensors made under `torch.inference_mode()`, which count
+    no changes, are copied."""
     return ops._host().capped_distillation(logits, teacher.ids, teacher.logp, teacher.log_rest, cap, target_ids, temperature, weight)
