@@ -1086,7 +1086,7 @@ static int launch_distill(DistillArgs a, int nt, cudaStream_t st) {
   const int64_t smem = table + a.groups * bytes;
   int64_t per_sm;
   if (int rc = ds_blocks(kern, info, smem, nt * a.groups, &per_sm)) return rc;
-  const int blocks = int(std::min<int64_t>((a.rows + a.groups - 1) / a.groups, sm_count() * per_sm));
+  const int blocks = int(std::min<int64_t>((int64_t(a.rows) + a.groups - 1) / a.groups, sm_count() * per_sm));
   TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, kern, dim3(unsigned(blocks)), nt * a.groups, size_t(smem), st, a));
   return TG_OK;
 }
@@ -1114,7 +1114,7 @@ static int launch_top(TopArgs a, int nt, cudaStream_t st) {
   const int64_t smem = table + a.groups * bytes;
   int64_t per_sm;
   if (int rc = ds_blocks(top_logits_kernel<TABLE>, info, smem, nt * a.groups, &per_sm)) return rc;
-  const int blocks = int(std::min<int64_t>((a.rows + a.groups - 1) / a.groups, sm_count() * per_sm));
+  const int blocks = int(std::min<int64_t>((int64_t(a.rows) + a.groups - 1) / a.groups, sm_count() * per_sm));
   TG_CUDA_CHECK(launch_if_short(int64_t(a.rows) * a.vocab <= 1 << 20, top_logits_kernel<TABLE>, dim3(unsigned(blocks)), nt * a.groups, size_t(smem), st, a));
   return TG_OK;
 }
