@@ -255,7 +255,7 @@ __device__ __forceinline__ float log_share(float part, float other) {
 // 50304 logits fit on an SM only with one table for both, hence the groups.
 // A row has three barriers, and a chain of loads (an id, its logit) at its beginning: the next row's ids and logits are fetched a phase ahead, and
 // its pieces take the places of this one's as the second pass leaves them.
-// 8192 x 50304 with 64 logits: 427 us (3.9 TB/s), 464 with a target at another temperature.  A row's 28100 cycles are 11800 of the first pass, 14100
+// 8192 x 50304 with 64 logits: 427 us (3.9 TB/s); with a target 448 at T = 1, 465 at 2 and 4 (below), 603 at any other.  A row's 28100 cycles are 11800 of the first pass, 14100
 // of the second, 2300 around the barriers; with two rows at once look-ups (3.5 cycles of shared memory for 32) keep that pipe busy for 68 %,
 // exponentials theirs for 59 %, and instructions are issued in 62 % of the cycles.
 // EXPS: 1 where one sum does (one temperature, or one of the two losses), 2 for two exponentials, 3 and 4 where the second is the first one
@@ -1078,7 +1078,8 @@ static int launch_distill(DistillArgs a, int nt, cudaStream_t st) {
   auto kern = softcap_distill_kernel<EXPS, GRAD, TABLE, STAGED>;
   const int64_t table = TABLE ? cap_bytes(distill_table(EXPS, GRAD)) : 0, bytes = ds_map_bytes(a.vocab) + (STAGED ? ds_row_bytes(a.vocab) : 0);
   // groups that share a block's table where a row has less than 128 threads (16384 x 1024 88 us, a table each 149; from 128 on 1.03 times the
-  // time) and where two blocks do not fit on an SM beside each other
+  // time) and where two blocks do not fit on an SM beside each other (from 46002 logits on).  Beyond 50457 a row is alone on its SM, with its 256
+  // threads (up to 100937, which still are kept): 1.04 ps a logit at 8192 x 50304, 1.25 at 4096 x 65536 (336 us), 1.15 at 4096 x 100277 (474)
   if (STAGED && TABLE && nt < 128) a.groups = int(std::max<int64_t>(1, std::min<int64_t>({kDsMaxGroups, ds_block_threads(true) / nt, a.rows / sm_count()})));
   else if (STAGED) a.groups = ds_alone(table + bytes) && table + 2 * bytes <= kDsDynamicMax && a.rows > sm_count() ? 2 : 1;
   while (a.groups > 1 && table + a.groups * bytes > kDsDynamicMax) --a.groups;
@@ -1186,7 +1187,8 @@ extern "C" int tg_softcap_distill(const tg_distill_args* args, void* stream) {
   if (g.dlogits != nullptr && ((reinterpret_cast<uintptr_t>(g.logits) ^ reinterpret_cast<uintptr_t>(g.dlogits)) & 15u) != 0) return TG_ERR_ALIGN;
   if (g.dlogits != nullptr && ds_rows_overlap(g.logits, g.dlogits, g.rows, g.vocab, g.ld)) return TG_ERR_SHAPE;
   if (int rc = check_arch()) return rc;
-  // one sum does where there is one temperature
+  // One sum does where there is one temperature.  exp(z) is exp(z / T) squared at the two temperatures that are powers of two above 1 and in use, for a
+  // product or two; at any other it is an exponential of its own, the other pipe that is short (8192 x 50257 465 and 603 us, the loss alone 197 and 289)
   const bool soft = g.weight > 0.f, hard = g.weight < 1.f && g.targets != nullptr;
   const float t = soft ? g.temperature : 1.0f;
   const int exps = !(soft && hard) || t == 1.0f ? 1 : t == 2.0f ? 3 : t == 4.0f ? 4 : 2;

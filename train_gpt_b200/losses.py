@@ -51,9 +51,9 @@ def top_logits(logits: torch.Tensor, cap: float, k: int, temperature: float = 1.
 
     logits: (..., vocab) bf16, uncapped as `capped_cross_entropy` takes them; rows may have a pitch (a slice of a padded
     vocabulary).  1 <= k <= 256, vocab <= 2**20, 2**-10 <= cap <= 64, 0 < temperature <= 1024, cap / temperature <= 64.
-    Nothing is differentiated.  A row is read once and, for a first bound, an eighth of it (all of it below 16416 logits); the result does
-    not depend on scheduling.  A row with hundreds of logits equal to the k-th, or with a NaN, is read some
-    five to twenty times."""
+    Nothing is differentiated.  A row is read once and, for a first bound, an eighth of it (all of it below 16400 logits; rows of up to
+    249, 505 and 1017 logits with at most 64, 48 and 20 kept are read once); the result does not depend on scheduling.  A row with hundreds of
+    logits equal to the k-th, or with a NaN, is read some five to twenty times."""
     return TopLogits(*ops._host().top_logits(logits, cap, k, temperature))
 
 
