@@ -243,6 +243,89 @@ int tg_sandwich_norm_bwd(const void* x_new, const void* branch, const void* post
                          float residual_scale, float eps, const void* g_new, const void* g_h, void* dx, void* dbranch, void* dpost,
                          void* dpre, void* dgate, void* scratch, int64_t rows, int64_t cols, void* stream);
 
+/* ---- a block with rotary positions, a gated feed-forward, dropout ------------------- */
+
+/* No counterpart in the reference.  The norm of every head of queries and keys and the rotation by position, one pass over both:
+ *   y = R(t) (x * rsqrt(mean(x^2) + eps) * scale), in float32 with one rounding; without scales y = R(t) x
+ * R(t) turns the pair of elements (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where interleaved, by the angle t * theta^(-2 i / rotary_dim);
+ * elements from rotary_dim on are not rotated.
+ *   q, k      bf16 [batch, tokens, heads or kv_heads, dim], unit stride along dim, the other strides (batch, token, head) given in
+ *             elements, multiples of 8; 16-byte aligned
+ *   q_out, k_out  bf16, contiguous; they overlap no input
+ *   q_scale, k_scale  bf16 [dim], both or neither (then there is no norm)
+ *   positions int32 (or int64 if positions_64) with a stride per batch and per token, or NULL: a token's place in its sequence.  The angle is
+ *             exact to float32's rounding for |t| < 2^31
+ *   dim, rotary_dim multiples of 16, 16 <= dim <= 512, 0 <= rotary_dim <= dim; batch * tokens < 2^31
+ * Backward, from the gradients g_q, g_k of the outputs (strides as above): q_out and k_out receive the gradients of q and k, dq_scale and
+ * dk_scale bf16 [dim] those of the scales.  Without scales q and k are not read.
+ *   scratch   tg_qk_norm_rope_bwd_scratch_bytes(args) bytes, 16-byte aligned, contents undefined on entry and exit
+ * Deterministic (no atomics). */
+typedef struct tg_qk_args {
+  const void *q, *k;
+  int64_t q_stride[3], k_stride[3];
+  void *q_out, *k_out;
+  const void *q_scale, *k_scale;
+  const void* positions;
+  int positions_64;
+  int64_t positions_stride[2];
+  int64_t batch, tokens;
+  int heads, kv_heads, dim, rotary_dim, interleaved;
+  float eps;
+  double theta;
+  const void *g_q, *g_k;
+  int64_t g_q_stride[3], g_k_stride[3];
+  void *dq_scale, *dk_scale;
+  void* scratch;
+} tg_qk_args;
+int tg_qk_norm_rope_fwd(const tg_qk_args* args, void* stream);
+int64_t tg_qk_norm_rope_bwd_scratch_bytes(const tg_qk_args* args);
+int tg_qk_norm_rope_bwd(const tg_qk_args* args, void* stream);
+
+/* No counterpart in the reference.  h = act(x w_gate) * (x w_up) in bf16 with float32 accumulation and one rounding: both projections, the
+ * activation and the product in one kernel.
+ *   x         bf16 [rows, cols], row pitch ldx;  w_gate, w_up  bf16 [cols, inner], row pitches ld_gate, ld_up;  h bf16 [rows, inner]
+ *             cols, inner and the pitches multiples of 8, pointers 16-byte aligned, sizes up to 2^30
+ *   saved_gate, saved_up, saved_exponents   what the backward pass needs, all or none: [rows, inner] of 16 bits each and
+ *             tg_gated_linear_exponent_bytes(rows, inner) bytes; 16-byte aligned
+ *   status    a device word as in tg_gemm_args, or NULL
+ * Backward, from the gradient g bf16 [rows, inner] of h and what was saved: dx bf16 [rows, cols] (or NULL), dw_gate and dw_up bf16 [cols, inner]
+ * (both or neither).  The gradients at the two projections are rounded to bf16 once before the products.
+ *   scratch   tg_gated_linear_bwd_scratch_bytes(rows, inner) bytes, 16-byte aligned, contents undefined on entry and exit
+ * Deterministic. */
+#define TG_GATED_SILU 0
+#define TG_GATED_GELU 1
+#define TG_GATED_RELU 2
+typedef struct tg_gated_args {
+  const void* x;
+  int64_t ldx;
+  const void* w_gate;
+  int64_t ld_gate;
+  const void* w_up;
+  int64_t ld_up;
+  int act;
+  void* h;
+  void *saved_gate, *saved_up;
+  uint8_t* saved_exponents;
+  const void* g;
+  void *dx, *dw_gate, *dw_up;
+  void* scratch;
+  int64_t rows, cols, inner;
+  uint32_t* status;
+} tg_gated_args;
+int64_t tg_gated_linear_exponent_bytes(int64_t rows, int64_t inner);
+int tg_gated_linear_fwd(const tg_gated_args* args, void* stream);
+int64_t tg_gated_linear_bwd_scratch_bytes(int64_t rows, int64_t inner);
+int tg_gated_linear_bwd(const tg_gated_args* args, void* stream);
+
+/* No counterpart in the reference.  y = bf16(residual + keep * x * 65536 / (65536 - t)) with t = p * 65536 rounded to an integer (ties to even)
+ * and keep true where 16 random bits are at least t.  The bits of elements 8 i .. 8 i + 7 are the words of Philox4x32-10 with the counter
+ * (low word of i, high word of i, site, 0) and the key (low word, high word) of *seed, the low half of each word first.  A dropped
+ * element counts as 0 whatever it is.  The backward pass is the same call on the gradient, without a residual.
+ *   x, y      bf16 [n]; residual bf16 [n] or NULL; 16-byte aligned; y may be the buffer of x or of residual
+ *   seed      device int64, 8-byte aligned
+ *   p         0 <= p <= 1; 0 keeps everything, 1 nothing */
+int tg_dropout(const void* x, const void* residual, double p, const int64_t* seed, uint32_t site, void* y, int64_t n, void* stream);
+
 /* ---- capped-logit cross-entropy --------------------------------------------------- */
 
 /* train-gpt model.py:97 (`cap * tanh(logits / cap)`, bf16, every op rounding) followed by

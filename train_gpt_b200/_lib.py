@@ -17,6 +17,7 @@ TG_OK, TG_ERR_SHAPE, TG_ERR_ALIGN, TG_ERR_ARCH, TG_ERR_CUDA, TG_ERR_TOO_LARGE = 
 TG_NORM_FUSED, TG_NORM_PURE = 0, 1
 TG_MAJOR_K, TG_MAJOR_MN = 0, 1
 TG_OUT_BF16, TG_OUT_F32 = 0, 1
+TG_GATED = {"silu": 0, "gelu": 1, "relu": 2}
 TG_ACT = {"relu2": 1, "gelu": 2, "relu2_bwd": 3, "gelu_bwd": 4}
 
 _p, _i64, _f, _i = C.c_void_p, C.c_int64, C.c_float, C.c_int
@@ -40,6 +41,25 @@ class DistillArgs(C.Structure):
         ("logits", _p), ("ids", _p), ("logp", _p), ("log_rest", _p), ("targets", _p), ("ids_64", _i), ("targets_64", _i),
         ("cap", _f), ("temperature", _f), ("weight", _f), ("dlogits", _p), ("gscale", _p), ("only_if_scaled", _i), ("row_loss", _p),
         ("rows", _i64), ("vocab", _i64), ("ld", _i64), ("k", _i),
+    ]
+
+
+class QkArgs(C.Structure):
+    """struct tg_qk_args"""
+    _fields_ = [
+        ("q", _p), ("k", _p), ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("q_out", _p), ("k_out", _p), ("q_scale", _p), ("k_scale", _p),
+        ("positions", _p), ("positions_64", _i), ("positions_stride", _i64 * 2), ("batch", _i64), ("tokens", _i64),
+        ("heads", _i), ("kv_heads", _i), ("dim", _i), ("rotary_dim", _i), ("interleaved", _i), ("eps", _f), ("theta", C.c_double),
+        ("g_q", _p), ("g_k", _p), ("g_q_stride", _i64 * 3), ("g_k_stride", _i64 * 3), ("dq_scale", _p), ("dk_scale", _p), ("scratch", _p),
+    ]
+
+
+class GatedArgs(C.Structure):
+    """struct tg_gated_args"""
+    _fields_ = [
+        ("x", _p), ("ldx", _i64), ("w_gate", _p), ("ld_gate", _i64), ("w_up", _p), ("ld_up", _i64), ("act", _i), ("h", _p),
+        ("saved_gate", _p), ("saved_up", _p), ("saved_exponents", _p), ("g", _p), ("dx", _p), ("dw_gate", _p), ("dw_up", _p), ("scratch", _p),
+        ("rows", _i64), ("cols", _i64), ("inner", _i64), ("status", _p),
     ]
 
 
@@ -67,6 +87,14 @@ SYMBOLS = {
     "tg_sandwich_norm_fwd": (_i, [_p, _p, _p, _p, _p, _i, _f, _f, _p, _p, _p, _p, _i64, _i64, _p]),
     "tg_sandwich_norm_bwd_scratch_bytes": (_i64, [_i64, _i64]),
     "tg_sandwich_norm_bwd": (_i, [_p, _p, _p, _p, _p, _i, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _p]),
+    "tg_qk_norm_rope_fwd": (_i, [C.POINTER(QkArgs), _p]),
+    "tg_qk_norm_rope_bwd_scratch_bytes": (_i64, [C.POINTER(QkArgs)]),
+    "tg_qk_norm_rope_bwd": (_i, [C.POINTER(QkArgs), _p]),
+    "tg_gated_linear_exponent_bytes": (_i64, [_i64, _i64]),
+    "tg_gated_linear_fwd": (_i, [C.POINTER(GatedArgs), _p]),
+    "tg_gated_linear_bwd_scratch_bytes": (_i64, [_i64, _i64]),
+    "tg_gated_linear_bwd": (_i, [C.POINTER(GatedArgs), _p]),
+    "tg_dropout": (_i, [_p, _p, C.c_double, _p, C.c_uint32, _p, _i64, _p]),
     "tg_softcap_ce_fwd": (_i, [_p, _p, _f, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "tg_softcap_ce_bwd": (_i, [_p, _p, _p, _p, _f, _p, _i64, _i64, _i64, _i64, _p]),
     "tg_top_logits": (_i, [_p, _f, _f, _p, _p, _p, _i64, _i64, _i64, _i, _p]),

@@ -19,7 +19,8 @@ INCLUDE = os.path.join(os.path.dirname(PKG_DIR), "include")
 LIB_PATH = os.path.join(PKG_DIR, "libtrain_gpt_b200.so")
 HOST_PATH = os.path.join(PKG_DIR, "_host.so")
 
-SOURCES = ["runtime.cu", "quantize.cu", "rmsnorm.cu", "sandwich.cu", "gemm_fp8.cu", "gemm_ring.cu", "gemm_skinny.cu", "selftest.cu", "loss.cu", "distill.cu", "optim.cu"]
+SOURCES = ["runtime.cu", "quantize.cu", "rmsnorm.cu", "sandwich.cu", "gemm_fp8.cu", "gemm_ring.cu", "gemm_skinny.cu", "selftest.cu", "loss.cu", "distill.cu", "optim.cu",
+           "qk_rope.cu", "gated.cu", "dropout.cu"]
 
 HOST_SOURCES = ["host.cpp", "step.cpp"]
 

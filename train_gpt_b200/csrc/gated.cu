@@ -1,0 +1,687 @@
+// The gated feed-forward's first half in bf16,
+//
+//     h = act(x Wg) * (x Wu)            x [M, D], Wg and Wu [D, F]; act silu, gelu (by erf) or relu
+//
+// as one kernel: both projections, the activation and the product.  Backward, for the gradient g of h, with G = x Wg and U = x Wu:
+//
+//     dG = g U act'(G),  dU = g act(G),    dx = dG Wg^T + dU Wu^T,    dWg = x^T dG,  dWu = x^T dU
+//
+// one pass for dG and dU and one launch for the three products.  Products are bf16 tcgen05.mma on pairs of SMs (cta_group::2) with float32
+// accumulators in tensor memory; no operand is transposed in memory, the descriptors carry the major-ness.  A cluster of two CTAs has a
+// tile of 256 rows and 256 accumulator columns: CTA r owns rows 128 r.. of it and loads them of A, and half of the 256 rows of B.
+//   forward   A = x, B: the first CTA loads 128 columns of Wg, the second the same of Wu.  Accumulator columns 0-127 are then G and 128-255
+//             are U of the same 128 columns of h, and a thread of the epilogue finds both of an element in its own tensor-memory lane.
+//   dx        A = dG and then dU, B = Wg and then Wu: one contraction of 2 F, so the sum of the two products is made in the accumulator.
+//   dW        A = x^T, B = dG for the first half of the column tiles and dU for the second.
+// dx and dW do not depend on one another: one launch, the problem with the longer items first, pairs that its last round leaves idle
+// begin with the other one.
+//
+// What the forward pass keeps for the backward one is G and U in 16 bits.  bf16 there would cost dx and dW half as much precision again as
+// the rounding of dG and dU (which the tensor cores need) does: fp16 has three more bits, and a power of two per 64 columns of a row
+// (a byte each, 0 but where one of them is beyond 65504) gives it bf16's range.
+//
+// Warp roles of a CTA (320 threads): 0-7 epilogue (warp w reads TMEM lanes 32 (w % 4).., half w / 4 of the columns), 8 TMA producer,
+// 9 MMA issuer (in the first CTA).  Two accumulators take turns, so a tile's epilogue runs beside the next tile's products; results leave
+// through swizzled staging rows and bulk tensor stores, which also clip ragged edges.  Ragged operands arrive as zeros.
+//
+// Every wait on an mbarrier is bounded, as in gemm_fp8.cu (the same codes).
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "cluster.cuh"
+#include "common.cuh"
+#include "gemm_tiles.cuh"
+#include "host_api.h"
+#include "mbarrier.cuh"
+#include "norm.cuh"
+#include "umma.cuh"
+
+namespace tg {
+
+// ---- activations ---------------------------------------------------------------------------------------------------
+
+// Phi(-a) = exp(-a^2 / 2) t R(t) with t = 1 / (1 + 0.3 a): erfc scaled by its exponential is smooth in t, and R is a polynomial fitted to it for
+// a in [0, 14.5] by least squares of the relative error at Chebyshev points, reweighted towards the largest (1.6e-7; 4e-7 in float32).
+// Relative, unlike the quantiser's: a product with U may have any size.
+__device__ __forceinline__ float gated_phi(float g, float e) {      // e = exp(-g^2 / 2)
+  const float t = __fdividef(1.f, fmaf(0.3f, fabsf(g), 1.f));
+  float r = 0.03542373329401016f;
+  r = fmaf(r, t, -0.156158447265625f);
+  r = fmaf(r, t, 0.20455677807331085f);
+  r = fmaf(r, t, -0.05203401297330856f);
+  r = fmaf(r, t, 0.12769177556037903f);
+  r = fmaf(r, t, 0.10017594695091248f);
+  r = fmaf(r, t, 0.12071213871240616f);
+  r = fmaf(r, t, 0.11963200569152832f);
+  const float tail = e * t * r;
+  return g > 0.f ? 1.f - tail : tail;
+}
+template <int ACT>
+__device__ __forceinline__ float gated_act(float g) {
+  if constexpr (ACT == TG_GATED_SILU) return __fdividef(g, 1.f + __expf(-g));
+  if constexpr (ACT == TG_GATED_GELU) return g * gated_phi(g, __expf(-0.5f * g * g));
+  return g > 0.f || g != g ? g : 0.f;
+}
+// act(g) and its derivative
+template <int ACT>
+__device__ __forceinline__ float2 gated_act_slope(float g) {
+  if constexpr (ACT == TG_GATED_SILU) {
+    const float s = __fdividef(1.f, 1.f + __expf(-g)), a = g * s;
+    return make_float2(a, s * (1.f + g * (1.f - s)));
+  }
+  if constexpr (ACT == TG_GATED_GELU) {
+    const float e = __expf(-0.5f * g * g), phi = gated_phi(g, e);
+    return make_float2(g * phi, fmaf(0.3989422804014327f * g, e, phi));
+  }
+  return make_float2(g > 0.f || g != g ? g : 0.f, g > 0.f ? 1.f : 0.f);
+}
+
+// ---- the products --------------------------------------------------------------------------------------------------
+
+constexpr int kGbK = 64;                        // contraction of a stage: 128 bytes of bf16
+constexpr int kGbBox = 64 * 128;                // bytes of an operand box: 64 rows of 128 bytes
+constexpr int kGbStage = 4 * kGbBox;            // a CTA's: two boxes of A, two of B
+constexpr int kGbWarps = 8, kGbThreads = 32 * (kGbWarps + 2);
+constexpr int kGbOutBox = 32 * 128;             // bytes of an output box: 32 rows of 64 columns
+constexpr int kGbBand = 8;                      // 256-row tiles per band of the tile numbering
+enum { kGbForward = 0, kGbData = 1, kGbWeights = 2 };
+
+// A problem of either kernel.  Operand maps have boxes of 64 x 64, output maps of 64 columns x 32 rows.
+struct GatedProblem {
+  CUtensorMap a[2], b[2], d[2];
+  int kind, tiles_m, tiles_n, blocks;           // blocks: stages of the contraction of a tile
+  int half;                                     // kGbData: its first stage that reads the second operands; kGbWeights: column tiles of dWg
+};
+struct GatedSaved {
+  CUtensorMap gate, up;
+  uint8_t* exponents;
+  int64_t rows;
+  int chunks;                                   // of 64 columns
+};
+
+__device__ __forceinline__ void gated_tile(const GatedProblem& p, int item, int& tm, int& tn) {
+  const int per_band = kGbBand * p.tiles_n, b = item / per_band, w = item - b * per_band, rows = min(kGbBand, p.tiles_m - b * kGbBand);
+  tn = w / rows;
+  tm = b * kGbBand + (w - tn * rows);
+}
+
+__device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(y)
+               : "memory");
+}
+// As make_smem_desc: 128-byte swizzle, 8-row groups 1024 bytes apart.  MN-major operands lie in chunks of 64 rows or columns, a box each.
+__device__ __forceinline__ uint64_t gated_desc(uint32_t saddr) {
+  return uint64_t((saddr >> 4) & 0x3FFFu) | uint64_t(kGbBox >> 4) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_magnitude(uint32_t m, uint32_t bits) { return max(m, bits & 0x7fffffffu); }
+
+// Sixteen bytes of this lane's staging row: chunk c of its 128 bytes, swizzled
+__device__ __forceinline__ void stage16(uint32_t row, int lane, int c, uint4 v) { sts128(row + (uint32_t(c ^ (lane & 7)) << 4), v); }
+
+template <int BUFS, bool SAVE>
+struct GatedCfg {
+  static constexpr int bufs = BUFS;             // output boxes of a warp
+  static constexpr int out_bytes = kGbWarps * BUFS * kGbOutBox;
+  static constexpr int stages_fit = (kSmemLimit - 1024 - out_bytes) / kGbStage;
+  static constexpr int stages = stages_fit > 6 ? 6 : stages_fit;
+  static constexpr int smem_bytes = stages * kGbStage + out_bytes;
+  static_assert(stages >= 4 && smem_bytes + 1024 <= kSmemLimit, "shared-memory plan");
+};
+
+// f16 of 64 accumulator values, scaled down by the power of two that keeps the largest (finite) one in range; returns its exponent
+__device__ __forceinline__ uint32_t save_row(const uint32_t (&v0)[32], const uint32_t (&v1)[32], uint32_t row, int lane) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) m = max_magnitude(max_magnitude(m, v0[j]), v1[j]);
+  uint32_t e = 0u;
+  float scale = 1.f;
+  if (m >= 0x477fe000u) {                       // 65504: the exponent that puts the largest below 2^15 (infinities and NaN: as 2^128)
+    e = min(m >> 23, 255u) - 127u - 14u;
+    scale = __uint_as_float((127u - e) << 23);
+  }
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = 8 * c + 2 * j;
+      const float lo = __uint_as_float(at < 32 ? v0[at & 31] : v1[at & 31]), hi = __uint_as_float(at < 32 ? v0[(at + 1) & 31] : v1[(at + 1) & 31]);
+      o[j] = pack_f16x2(lo * scale, hi * scale);
+    }
+    stage16(row, lane, c, make_uint4(o[0], o[1], o[2], o[3]));
+  }
+  return e;
+}
+
+// `one` and, where two is set, `two` with the walk that walk_second gives.
+template <int KIND, int ACT, bool SAVE, typename C>
+__device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedProblem& two, bool both, int rounds, const GatedSaved& saved, unsigned* status) {
+  constexpr int kStages = C::stages;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(16) uint64_t ctl_bars[2 * kStages + 5];
+  __shared__ uint32_t ctl_tmem_ptr;
+  __shared__ int ctl_abort;
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t full0 = smem_u32(ctl_bars), empty0 = full0 + 8u * kStages, tfull0 = empty0 + 8u * kStages, tempty0 = tfull0 + 16u, drain_bar = tempty0 + 16u;
+  volatile uint32_t* tmem_ptr_smem = &ctl_tmem_ptr;
+  volatile int* abort_flag = &ctl_abort;
+  if ((sbase & 1023u) != 0) {   // the swizzled layouts need this alignment (both CTAs have the same layout)
+    if (threadIdx.x == 0 && status != nullptr) atomicCAS(status, 0u, 6u);
+    return;
+  }
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int unit = int(blockIdx.x) / 2, units = int(gridDim.x) / 2;
+  const int n1 = one.tiles_m * one.tiles_n;
+  const Walk walk1 = walk_alone(unit, units, n1);
+  const Walk walk2 = both ? walk_second(unit, units, n1, two.tiles_m * two.tiles_n, rounds) : Walk{0, 0, 0, 1, 0};
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full0 + 8u * s, 1);             // (the first CTA's counts the bytes of both)
+      mbar_init(empty0 + 8u * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull0 + 8u * b, 1);
+      mbar_init(tempty0 + 8u * b, 2 * kGbWarps);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kGbWarps + 1) tmem_take_pair(smem_u32(&ctl_tmem_ptr));
+  tc_fence_before();
+  cluster_sync();                               // both CTAs' barriers exist before either signals across, both have their tensor memory
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_ptr_smem;
+  grid_trigger();
+  grid_wait();
+
+  if (warp == kGbWarps) {
+    // ------------------------------ TMA producer -------------------------------------
+    uint32_t s = 0, ph = 1;
+    bool ok = true;
+    const uint32_t full_leader = map_rank(full0, 0u);
+    auto produce = [&](const GatedProblem& p, const Walk& w) {
+      for (int item = w.first; ok && item < w.n; item = w.next(item)) {
+        int tm, tn;
+        gated_tile(p, item, tm, tn);
+        const int m0 = (2 * tm + int(rank)) * 128;
+        for (int kb = 0; kb < p.blocks; ++kb) {
+          ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, ph, abort_flag, status, 1u));
+          if (!ok) break;
+          if (elect_one()) {
+            const uint32_t dst = sbase + s * kGbStage, fb = full_leader + 8u * s;
+            // The first CTA announces the bytes of both.  The second's may land before that: its barrier phase is the same one,
+            // since the stage was free in both CTAs only after the phase before had completed.
+            if (rank == 0) mbar_expect_tx(full0 + 8u * s, 2 * kGbStage);
+            if constexpr (KIND == kGbForward) {
+              const int k0 = kb * kGbK, n0 = tn * 128;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                tma_load_2d_pair(dst + i * kGbBox, &p.a[0], fb, k0, m0 + 64 * i);
+                tma_load_2d_pair(dst + (2 + i) * kGbBox, &p.b[rank], fb, n0 + 64 * i, k0);
+              }
+            } else if (p.kind == kGbData) {
+              const int sel = kb >= p.half, k0 = (kb - (sel ? p.half : 0)) * kGbK, n0 = tn * 256 + int(rank) * 128;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                tma_load_2d_pair(dst + i * kGbBox, &p.a[sel], fb, k0, m0 + 64 * i);
+                tma_load_2d_pair(dst + (2 + i) * kGbBox, &p.b[sel], fb, k0, n0 + 64 * i);
+              }
+            } else {
+              const int sel = tn >= p.half, k0 = kb * kGbK, n0 = (tn - (sel ? p.half : 0)) * 256 + int(rank) * 128;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                tma_load_2d_pair(dst + i * kGbBox, &p.a[0], fb, m0 + 64 * i, k0);
+                tma_load_2d_pair(dst + (2 + i) * kGbBox, &p.b[sel], fb, n0 + 64 * i, k0);
+              }
+            }
+          }
+          __syncwarp();
+          if (++s == kStages) { s = 0; ph ^= 1u; }
+        }
+      }
+    };
+    produce(one, walk1);
+    if (KIND != kGbForward && both) produce(two, walk2);
+  } else if (warp == kGbWarps + 1) {
+    // ------------------------------ MMA issuer (first CTA) ----------------------------
+    if (rank == 0) {
+      const uint64_t desc_a0 = gated_desc(sbase), desc_b0 = gated_desc(sbase + 2 * kGbBox);
+      const uint32_t desc_hi = uint32_t(desc_a0 >> 32), a_lo0 = uint32_t(desc_a0), b_lo0 = uint32_t(desc_b0);
+      bool ok = true;
+      uint32_t s = 0, sph = 0, buf = 0, bph = 1;
+      auto issue = [&](const GatedProblem& p, const Walk& w) {
+        const int kind = KIND == kGbForward ? kGbForward : p.kind;
+        const uint32_t a_mn = kind == kGbWeights, b_mn = kind != kGbData;
+        // D f32 (bit 4), A and B bf16 (7, 10), major bits 15/16, N>>3 at 17, M>>4 at 24
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (a_mn << 15) | (b_mn << 16) | (uint32_t(256 >> 3) << 17) | (uint32_t(256 >> 4) << 24);
+        // descriptor step per 16 of the contraction: 32 bytes along a K-major row, 16 rows of 128 bytes otherwise
+        const uint32_t a_step = a_mn ? 128u : 2u, b_step = b_mn ? 128u : 2u;
+        for (int item = w.first; ok && item < w.n; item = w.next(item)) {
+          for (int kb = 0; kb < p.blocks; ++kb) {
+            ok = __all_sync(0xffffffffu, (kb > 0 || mbar_wait(tempty0 + 8u * buf, bph, abort_flag, status, 2u)) &&
+                                             mbar_wait(full0 + 8u * s, sph, abort_flag, status, 3u));
+            if (!ok) break;
+            __syncwarp();
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t soff = s * uint32_t(kGbStage >> 4);
+#pragma unroll
+              for (int k = 0; k < kGbK / 16; ++k)
+                umma_bf16_pair(tmem_base + buf * 256u, (uint64_t(desc_hi) << 32) | (a_lo0 + soff + k * a_step),
+                               (uint64_t(desc_hi) << 32) | (b_lo0 + soff + k * b_step), idesc, kb > 0 || k > 0 ? 1u : 0u);
+              umma_commit_both(empty0 + 8u * s);
+              if (kb + 1 == p.blocks) umma_commit_both(tfull0 + 8u * buf);
+            }
+            __syncwarp();
+            if (++s == kStages) { s = 0; sph ^= 1u; }
+          }
+          if ((buf ^= 1u) == 0u) bph ^= 1u;
+        }
+      };
+      issue(one, walk1);
+      if (KIND != kGbForward && both) issue(two, walk2);
+      // nothing issued here may still be running when tensor memory is freed
+      if (elect_one()) {
+        umma_commit_here(drain_bar);
+        mbar_wait(drain_bar, 0u, abort_flag, status, 4u);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------ epilogue ------------------------------------------
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lanes = tmem_base + (uint32_t(quarter * 32) << 16);
+    const uint32_t out = sbase + kStages * kGbStage + uint32_t(warp) * (C::bufs * kGbOutBox), row = out + uint32_t(lane) * 128u;
+    const uint32_t tempty_leader = map_rank(tempty0, 0u), is_lane0 = lane == 0;
+    uint32_t buf = 0, bph = 0;
+    bool ok = true;
+    auto release = [&]() {
+      tc_fence_before();
+      __syncwarp();
+      mbar_arrive_cluster_if(tempty_leader + 8u * buf, is_lane0);
+    };
+    auto rows_free = [&]() {            // the stores before have read their staging rows
+      if (is_lane0) tma_store_wait_read();
+      __syncwarp();
+    };
+    auto staged = [&]() {               // generic writes -> visible to the copy engine
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    };
+    auto finish = [&](const GatedProblem& p, const Walk& w) {
+      for (int item = w.first; item < w.n; item = w.next(item)) {
+        int tm, tn;
+        gated_tile(p, item, tm, tn);
+        const int m0 = (2 * tm + int(rank)) * 128 + quarter * 32;
+        ok = __all_sync(0xffffffffu, mbar_wait(tfull0 + 8u * buf, bph, abort_flag, status, 5u));
+        if (!ok) break;
+        __syncwarp();
+        tc_fence_after();
+        if constexpr (KIND == kGbForward) {
+          const uint32_t at = lanes + buf * 256u + uint32_t(half) * 64u;
+          uint32_t g0[32], g1[32], u0[32], u1[32];
+          tmem_ld32(at, g0);
+          tmem_ld32(at + 32u, g1);
+          tmem_ld32(at + 128u, u0);
+          tmem_ld32(at + 160u, u1);
+          tmem_wait_ld(g0);
+          tmem_wait_ld(g1);
+          tmem_wait_ld(u0);
+          tmem_wait_ld(u1);
+          release();
+          rows_free();
+          const int n0 = tn * 128 + half * 64;
+          if constexpr (SAVE) {
+            const uint32_t eg = save_row(g0, g1, row + kGbOutBox, lane), eu = save_row(u0, u1, row + 2 * kGbOutBox, lane);
+            if (m0 + lane < saved.rows && n0 / 64 < saved.chunks)
+              reinterpret_cast<uint16_t*>(saved.exponents)[int64_t(n0 / 64) * saved.rows + m0 + lane] = uint16_t(eg | eu << 8);
+          }
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int i = 8 * (c & 3) + 2 * j;
+              const uint32_t(&g)[32] = c < 4 ? g0 : g1;
+              const uint32_t(&u)[32] = c < 4 ? u0 : u1;
+              o[j] = pack_bf16x2(gated_act<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]),
+                                 gated_act<ACT>(__uint_as_float(g[i + 1])) * __uint_as_float(u[i + 1]));
+            }
+            stage16(row, lane, c, make_uint4(o[0], o[1], o[2], o[3]));
+          }
+          staged();
+          if (is_lane0) {
+            tma_store_2d(&p.d[0], out, n0, m0);
+            if constexpr (SAVE) {
+              tma_store_2d(&saved.gate, out + kGbOutBox, n0, m0);
+              tma_store_2d(&saved.up, out + 2 * kGbOutBox, n0, m0);
+            }
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          __syncwarp();
+        } else {
+          const int sel = p.kind == kGbWeights && tn >= p.half, n0 = (tn - (sel ? p.half : 0)) * 256 + half * 128;
+          const uint32_t at = lanes + buf * 256u + uint32_t(half) * 128u;
+          rows_free();
+#pragma unroll
+          for (int box = 0; box < 2; ++box) {
+            uint32_t v0[32], v1[32];
+            tmem_ld32(at + 64u * box, v0);
+            tmem_ld32(at + 64u * box + 32u, v1);
+            tmem_wait_ld(v0);
+            tmem_wait_ld(v1);
+            if (box == 1) release();
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int i = 8 * (c & 3) + 2 * j;
+                const uint32_t(&v)[32] = c < 4 ? v0 : v1;
+                o[j] = pack_bf16x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+              }
+              stage16(row + box * kGbOutBox, lane, c, make_uint4(o[0], o[1], o[2], o[3]));
+            }
+          }
+          staged();
+          if (is_lane0) {
+#pragma unroll
+            for (int box = 0; box < 2; ++box) tma_store_2d(&p.d[sel], out + box * kGbOutBox, n0 + 64 * box, m0);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          __syncwarp();
+        }
+        if ((buf ^= 1u) == 0u) bph ^= 1u;
+      }
+    };
+    finish(one, walk1);
+    if (KIND != kGbForward && both && ok) finish(two, walk2);
+    // the last bulk stores must have read their staging rows before the CTA's shared memory goes away
+    if (is_lane0) tma_store_wait_read();
+    __syncwarp();
+  }
+
+  // ------------------------------ teardown ----------------------------------------------
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();              // the partner no longer reads this CTA's shared memory or signals its barriers
+  if (warp == kGbWarps + 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_give_pair(tmem_base);
+  }
+}
+
+template <int ACT, bool SAVE>
+__global__ void __launch_bounds__(kGbThreads, 1) gated_fwd_kernel(const __grid_constant__ GatedProblem p, const __grid_constant__ GatedSaved saved, unsigned* status) {
+  gated_body<kGbForward, ACT, SAVE, GatedCfg<SAVE ? 3 : 1, SAVE>>(p, p, false, 0, saved, status);
+}
+__global__ void __launch_bounds__(kGbThreads, 1)
+gated_bwd_kernel(const __grid_constant__ GatedProblem one, const __grid_constant__ GatedProblem two, int both, int rounds, unsigned* status) {
+  gated_body<kGbData, 0, false, GatedCfg<2, false>>(one, two, both != 0, rounds, GatedSaved{}, status);
+}
+
+// ---- dG and dU -----------------------------------------------------------------------------------------------------
+
+struct GatedSlopes {
+  const __nv_bfloat16* g;
+  const __half *gate, *up;
+  const uint16_t* exponents;
+  __nv_bfloat16 *dgate, *dup;
+  int64_t rows;
+  int inner, chunks;
+};
+constexpr int kGsThreads = 256, kGsRows = kGsThreads / 8, kGsUnroll = 2;
+
+// A block takes 64 columns of 32 rows at a time, eight lanes a row: a row's 128 bytes of each tensor are one request, and its
+// exponents one of a few in the same sector.
+template <int ACT>
+__global__ void __launch_bounds__(kGsThreads) gated_slopes_kernel(const GatedSlopes p) {
+  grid_trigger();
+  grid_wait();
+  const int lane8 = threadIdx.x & 7, r0 = threadIdx.x >> 3;
+  const int64_t groups = (p.rows + kGsRows * kGsUnroll - 1) / (kGsRows * kGsUnroll), items = groups * p.chunks;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t group = item / p.chunks;
+    const int chunk = int(item - group * p.chunks), col = chunk * 64 + lane8 * 8;
+    uint4 g[kGsUnroll], a[kGsUnroll], u[kGsUnroll];
+    uint32_t e[kGsUnroll];
+    int64_t row[kGsUnroll];
+#pragma unroll
+    for (int k = 0; k < kGsUnroll; ++k) {
+      row[k] = (group * kGsUnroll + k) * kGsRows + r0;
+      if (col >= p.inner || row[k] >= p.rows) row[k] = -1;
+      if (row[k] < 0) continue;
+      const int64_t at = row[k] * p.inner + col;
+      g[k] = ld_stream_v4(p.g + at);
+      a[k] = ld_stream_v4(p.gate + at);
+      u[k] = ld_stream_v4(p.up + at);
+      e[k] = p.exponents[int64_t(chunk) * p.rows + row[k]];
+    }
+#pragma unroll
+    for (int k = 0; k < kGsUnroll; ++k) {
+      if (row[k] < 0) continue;
+      const float sa = __uint_as_float((127u + (e[k] & 255u)) << 23), su = __uint_as_float((127u + (e[k] >> 8)) << 23);
+      uint32_t og[4], ou[4];
+      const uint32_t *gw = &g[k].x, *aw = &a[k].x, *uw = &u[k].x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 gv = bf16x2_unpack(gw[j]);
+        const float2 av = __half22float2(*reinterpret_cast<const __half2*>(&aw[j])), uv = __half22float2(*reinterpret_cast<const __half2*>(&uw[j]));
+        const float2 s0 = gated_act_slope<ACT>(av.x * sa), s1 = gated_act_slope<ACT>(av.y * sa);
+        og[j] = pack_bf16x2(gv.x * (uv.x * su) * s0.y, gv.y * (uv.y * su) * s1.y);
+        ou[j] = pack_bf16x2(gv.x * s0.x, gv.y * s1.x);
+      }
+      const int64_t at = row[k] * p.inner + col;
+      *reinterpret_cast<uint4*>(p.dgate + at) = make_uint4(og[0], og[1], og[2], og[3]);
+      *reinterpret_cast<uint4*>(p.dup + at) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+    }
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+
+// [rows][cols] of 16-bit elements, row pitch ld: boxes of 64 columns (128 bytes, swizzled) and box_rows rows
+static int gated_map(CUtensorMap* m, const void* base, bool f16, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  return make_tmap(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, cols, rows, ld * 2, 128, box_rows);
+}
+
+// A launch on pairs: the kernel's shared memory is set, and the pairs that fit at a time are counted, once per device.
+template <typename K, typename... A>
+static int launch_gated(K kern, int smem, std::atomic<int>* units_of, int64_t items, bool early, cudaStream_t st, int& units, A... args) {
+  int dev = 0;
+  TG_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return TG_ERR_SHAPE;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = 2;
+  attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kGbThreads);
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.attrs = attrs;
+  cfg.numAttrs = 1;
+  cfg.stream = st;
+  int fit = units_of[dev].load(std::memory_order_acquire);
+  if (fit == 0) {
+    TG_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cfg.gridDim = dim3(unsigned(sm_count() & ~1));
+    TG_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&fit, kern, &cfg));
+    if (fit < 1) return record_cuda_error(cudaErrorLaunchOutOfResources, "no CTA pair fits on this device");
+    units_of[dev].store(fit, std::memory_order_release);
+  }
+  units = int(std::min<int64_t>(std::max(1, std::min(fit, gemm_pairs())), items));
+  if constexpr (sizeof...(A) > 0) {
+    cfg.gridDim = dim3(unsigned(2 * units));
+    cfg.numAttrs = early ? 2 : 1;
+    TG_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, args...));
+  }
+  return TG_OK;
+}
+
+static int gated_check(const tg_gated_args* a) {
+  if (a == nullptr || a->rows < 0 || a->cols < 8 || a->inner < 8 || a->cols % 8 != 0 || a->inner % 8 != 0) return TG_ERR_SHAPE;
+  if (a->act != TG_GATED_SILU && a->act != TG_GATED_GELU && a->act != TG_GATED_RELU) return TG_ERR_SHAPE;
+  if (a->ldx < a->cols || a->ld_gate < a->inner || a->ld_up < a->inner) return TG_ERR_SHAPE;
+  const int64_t most = int64_t(1) << 30;
+  if (a->rows > most || a->cols > most || a->inner > most) return TG_ERR_TOO_LARGE;
+  auto tiles = [](int64_t n, int64_t t) { return (n + t - 1) / t; };
+  if (tiles(a->rows, 256) * tiles(a->inner, 128) > INT32_MAX / 2 || tiles(a->rows, 256) * tiles(a->cols, 256) > INT32_MAX / 2 ||
+      2 * tiles(a->cols, 256) * tiles(a->inner, 256) > INT32_MAX / 2)
+    return TG_ERR_TOO_LARGE;
+  return TG_OK;
+}
+static bool gated_aligned(const tg_gated_args* a) {
+  return aligned16(a->x) && aligned16(a->w_gate) && aligned16(a->w_up) && a->ldx % 8 == 0 && a->ld_gate % 8 == 0 && a->ld_up % 8 == 0;
+}
+static int64_t gated_chunks(int64_t inner) { return (inner + 63) / 64; }
+
+template <int ACT, bool SAVE>
+static int run_gated_fwd(const GatedProblem& p, const GatedSaved& s, unsigned* status, cudaStream_t st) {
+  static std::atomic<int> units_of[64];
+  const int64_t items = int64_t(p.tiles_m) * p.tiles_n;
+  int units = 0;
+  return launch_gated(gated_fwd_kernel<ACT, SAVE>, GatedCfg<SAVE ? 3 : 1, SAVE>::smem_bytes, units_of, items, items <= 4 * gemm_pairs() && p.blocks <= 64, st,
+                      units, p, s, status);
+}
+template <bool SAVE>
+static int run_gated_fwd(int act, const GatedProblem& p, const GatedSaved& s, unsigned* status, cudaStream_t st) {
+  if (act == TG_GATED_SILU) return run_gated_fwd<TG_GATED_SILU, SAVE>(p, s, status, st);
+  if (act == TG_GATED_GELU) return run_gated_fwd<TG_GATED_GELU, SAVE>(p, s, status, st);
+  return run_gated_fwd<TG_GATED_RELU, SAVE>(p, s, status, st);
+}
+
+}  // namespace tg
+
+using namespace tg;
+
+extern "C" int64_t tg_gated_linear_exponent_bytes(int64_t rows, int64_t inner) {
+  return rows <= 0 || inner <= 0 ? 0 : 2 * rows * gated_chunks(inner);
+}
+
+extern "C" int tg_gated_linear_fwd(const tg_gated_args* a, void* stream) {
+  if (int rc = gated_check(a)) return rc;
+  const bool save = a->saved_gate != nullptr;
+  if (save != (a->saved_up != nullptr) || save != (a->saved_exponents != nullptr)) return TG_ERR_SHAPE;
+  if (a->rows == 0) return TG_OK;
+  if (a->x == nullptr || a->w_gate == nullptr || a->w_up == nullptr || a->h == nullptr) return TG_ERR_SHAPE;
+  if (!gated_aligned(a) || !aligned16(a->h) || !aligned16(a->saved_gate) || !aligned16(a->saved_up) || !aligned16(a->saved_exponents)) return TG_ERR_ALIGN;
+  if (int rc = check_arch()) return rc;
+  const int64_t M = a->rows, D = a->cols, F = a->inner;
+  GatedProblem p = {};
+  GatedSaved s = {};
+  if (int rc = gated_map(&p.a[0], a->x, false, M, D, a->ldx, 64)) return rc;
+  if (int rc = gated_map(&p.b[0], a->w_gate, false, D, F, a->ld_gate, 64)) return rc;
+  if (int rc = gated_map(&p.b[1], a->w_up, false, D, F, a->ld_up, 64)) return rc;
+  if (int rc = gated_map(&p.d[0], a->h, false, M, F, F, 32)) return rc;
+  if (save) {
+    if (int rc = gated_map(&s.gate, a->saved_gate, true, M, F, F, 32)) return rc;
+    if (int rc = gated_map(&s.up, a->saved_up, true, M, F, F, 32)) return rc;
+    s.exponents = a->saved_exponents;
+    s.rows = M;
+    s.chunks = int(gated_chunks(F));
+  }
+  p.kind = kGbForward;
+  p.tiles_m = int((M + 255) / 256);
+  p.tiles_n = int((F + 127) / 128);
+  p.blocks = int((D + kGbK - 1) / kGbK);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return save ? run_gated_fwd<true>(a->act, p, s, a->status, st) : run_gated_fwd<false>(a->act, p, s, a->status, st);
+}
+
+extern "C" int64_t tg_gated_linear_bwd_scratch_bytes(int64_t rows, int64_t inner) {
+  return rows <= 0 || inner <= 0 ? 0 : 2 * ((rows * inner * 2 + 255) / 256 * 256);
+}
+
+extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
+  if (int rc = gated_check(a)) return rc;
+  if ((a->dw_gate == nullptr) != (a->dw_up == nullptr)) return TG_ERR_SHAPE;
+  const int64_t M = a->rows, D = a->cols, F = a->inner;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (M == 0) {
+    if (int rc = check_arch()) return rc;
+    for (void* v : {a->dw_gate, a->dw_up})
+      if (v != nullptr) TG_CUDA_CHECK(cudaMemsetAsync(v, 0, size_t(D) * F * 2, st));
+    return TG_OK;
+  }
+  const bool dx = a->dx != nullptr, dw = a->dw_gate != nullptr;
+  if (a->g == nullptr || a->saved_gate == nullptr || a->saved_up == nullptr || a->saved_exponents == nullptr || a->scratch == nullptr ||
+      (dx && (a->w_gate == nullptr || a->w_up == nullptr)) || (dw && a->x == nullptr))
+    return TG_ERR_SHAPE;
+  if (!gated_aligned(a) || !aligned16(a->g) || !aligned16(a->saved_gate) || !aligned16(a->saved_up) || !aligned16(a->saved_exponents) || !aligned16(a->dx) ||
+      !aligned16(a->dw_gate) || !aligned16(a->dw_up) || !aligned16(a->scratch))
+    return TG_ERR_ALIGN;
+  if (int rc = check_arch()) return rc;
+  if (!dx && !dw) return TG_OK;
+  GatedSlopes s = {};
+  s.g = static_cast<const __nv_bfloat16*>(a->g);
+  s.gate = static_cast<const __half*>(a->saved_gate);
+  s.up = static_cast<const __half*>(a->saved_up);
+  s.exponents = reinterpret_cast<const uint16_t*>(a->saved_exponents);
+  s.dgate = static_cast<__nv_bfloat16*>(a->scratch);
+  s.dup = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(a->scratch) + tg_gated_linear_bwd_scratch_bytes(M, F) / 2);
+  s.rows = M;
+  s.inner = int(F);
+  s.chunks = int(gated_chunks(F));
+  const int64_t items = (M + kGsRows * kGsUnroll - 1) / (kGsRows * kGsUnroll) * s.chunks;
+  auto kern = a->act == TG_GATED_SILU ? gated_slopes_kernel<TG_GATED_SILU> : a->act == TG_GATED_GELU ? gated_slopes_kernel<TG_GATED_GELU> : gated_slopes_kernel<TG_GATED_RELU>;
+  TG_CUDA_CHECK(launch_if_short(items <= 8 * sm_count(), kern, dim3(unsigned(std::min<int64_t>(items, int64_t(sm_count()) * 6))), kGsThreads, 0, st, s));
+
+  GatedProblem data = {}, weights = {};
+  if (dx) {
+    for (int i = 0; i < 2; ++i) {
+      if (int rc = gated_map(&data.a[i], i ? s.dup : s.dgate, false, M, F, F, 64)) return rc;
+      if (int rc = gated_map(&data.b[i], i ? a->w_up : a->w_gate, false, D, F, i ? a->ld_up : a->ld_gate, 64)) return rc;
+    }
+    if (int rc = gated_map(&data.d[0], a->dx, false, M, D, D, 32)) return rc;
+    data.kind = kGbData;
+    data.tiles_m = int((M + 255) / 256);
+    data.tiles_n = int((D + 255) / 256);
+    data.half = int((F + kGbK - 1) / kGbK);
+    data.blocks = 2 * data.half;
+  }
+  if (dw) {
+    if (int rc = gated_map(&weights.a[0], a->x, false, M, D, a->ldx, 64)) return rc;
+    for (int i = 0; i < 2; ++i) {
+      if (int rc = gated_map(&weights.b[i], i ? s.dup : s.dgate, false, M, F, F, 64)) return rc;
+      if (int rc = gated_map(&weights.d[i], i ? a->dw_up : a->dw_gate, false, D, F, F, 32)) return rc;
+    }
+    weights.kind = kGbWeights;
+    weights.tiles_m = int((D + 255) / 256);
+    weights.half = int((F + 255) / 256);
+    weights.tiles_n = 2 * weights.half;
+    weights.blocks = int((M + kGbK - 1) / kGbK);
+  }
+  const bool both = dx && dw, data_first = dx && (!dw || data.blocks >= weights.blocks);
+  const GatedProblem &one = data_first ? data : weights, &two = data_first ? weights : data;
+  const int64_t n1 = int64_t(one.tiles_m) * one.tiles_n, n2 = both ? int64_t(two.tiles_m) * two.tiles_n : 0;
+  static std::atomic<int> units_of[64];
+  using C = GatedCfg<2, false>;
+  int units = 0, rounds = 0;
+  if (int rc = launch_gated(gated_bwd_kernel, C::smem_bytes, units_of, n1 + n2, false, st, units)) return rc;
+  if (both) two_problems_us(n1, double(one.blocks) + 3.0, n2, double(two.blocks) + 3.0, units, rounds);
+  const bool early = n1 + n2 <= 4 * units && one.blocks <= 64;
+  return launch_gated(gated_bwd_kernel, C::smem_bytes, units_of, n1 + n2, early, st, units, one, two, int(both), rounds, reinterpret_cast<unsigned*>(a->status));
+}

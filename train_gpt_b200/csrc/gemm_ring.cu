@@ -46,6 +46,7 @@
 
 #include <algorithm>
 
+#include "cluster.cuh"
 #include "common.cuh"
 #include "gemm_tiles.cuh"
 #include "host_api.h"
@@ -54,34 +55,8 @@
 
 namespace tg {
 
-// ---- cluster forms of the PTX wrappers ---------------------------------------------------
+// ---- one SM or a pair ------------------------------------------------------------------------
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// the same shared-memory offset in CTA `rank` of the cluster
-__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_arrive_cluster_if(uint32_t bar, uint32_t pred) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}"
-               ::"r"(bar), "r"(pred) : "memory");
-}
-// a load into this CTA's shared memory whose bytes are counted by a barrier of either CTA of the pair
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
-      : "memory");
-}
 __device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -89,14 +64,6 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, u
       "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
-}
-// arrives on the barrier at this offset in both CTAs once the MMAs issued before are done
-__device__ __forceinline__ void umma_commit_both(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-               ::"r"(bar), "h"(uint16_t(3)) : "memory");
-}
-__device__ __forceinline__ void umma_commit_here(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 template <int CG>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
@@ -170,21 +137,6 @@ struct RingProblem {
   CUtensorMap a, b, d;
   GemmParams p;
 };
-
-// The items of a problem that one unit (a CTA or a pair) works on: from `first` on in steps of `early_step` below early_end and of `step`
-// from there on, while they are below n.
-struct Walk {
-  int first, early_step, early_end, step, n;
-  __device__ __forceinline__ int next(int item) const { return item + (item < early_end ? early_step : step); }
-};
-__device__ __forceinline__ Walk walk_alone(int unit, int units, int n) { return Walk{unit, 0, 0, units, n}; }
-// Two problems on the same units: the first one's items go round, and the units that its last round leaves idle take `rounds` rounds of the
-// second one's meanwhile, before all take it up, the idle ones first.
-__device__ __forceinline__ Walk walk_second(int unit, int units, int n1, int n2, int rounds) {
-  const int busy = n1 % units, idle = units - busy, early_end = rounds * idle;
-  if (busy == 0) return walk_alone(unit, units, n2);
-  return Walk{unit >= busy ? unit - busy : early_end + idle + unit, idle, early_end, units, n2};
-}
 
 // C and D: the plans of the two problems (TWO) or C twice.
 template <int CG, typename C, typename D, bool TWO, typename START>

@@ -348,6 +348,289 @@ std::array<Tensor, 5> sandwich_norm_bwd(const Tensor& x_new_, const Tensor& bran
   return out;
 }
 
+// ---- rotary positions, the gated feed-forward, dropout --------------------------------------------------------------
+
+// Heads as the kernels read them: [batch, tokens, heads, dim] with unit stride along dim and the others' strides multiples of 16 bytes; as they
+// lie where they are that, copied otherwise.
+struct Heads {
+  Tensor t;
+  int64_t batch = 1, tokens = 1, heads = 0, dim = 0, stride[3] = {0, 0, 0};
+};
+Heads heads_of(const Tensor& t_, const char* name) {
+  if (!t_.is_cuda()) throw std::runtime_error(cat(name, " must be a CUDA tensor (there is no CPU path)"));
+  if (t_.scalar_type() != at::kBFloat16) throw py::type_error(cat(name, " must be torch.bfloat16, got ", dtype_name(t_.scalar_type())));
+  Heads h;
+  Tensor t = t_;
+  const int64_t n = t.dim();
+  if (n > 4) t = t.flatten(0, n - 4);
+  auto lies = [](const Tensor& v) {
+    if (v.size(-1) > 1 && v.stride(-1) != 1) return false;
+    for (int64_t i = 0; i + 1 < v.dim(); ++i)
+      if (v.size(i) > 1 && v.stride(i) % 8 != 0) return false;
+    return (reinterpret_cast<uintptr_t>(v.data_ptr()) & 15u) == 0;
+  };
+  if (t.numel() > 0 && !lies(t)) t = t.clone(at::MemoryFormat::Contiguous);
+  const int64_t d = t.dim();
+  h.dim = t.size(d - 1);
+  h.heads = t.size(d - 2);
+  auto stride = [&](int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; };
+  h.stride[2] = stride(d - 2);
+  if (d > 2) {
+    h.tokens = t.size(d - 3);
+    h.stride[1] = stride(d - 3);
+  }
+  if (d > 3) {
+    h.batch = t.size(d - 4);
+    h.stride[0] = stride(d - 4);
+  }
+  h.t = t;
+  return h;
+}
+
+// What both directions of the rotation are called with.
+struct Rope {
+  Tensor q_scale, k_scale, positions;          // positions: expanded to [batch, tokens], or undefined
+  double eps = 0, theta = 10000;
+  int64_t rotary = 0;
+  bool interleaved = false;
+};
+void need_rope(const Tensor& q, const Tensor& k, const std::optional<Tensor>& q_scale, const std::optional<Tensor>& k_scale, double theta, int64_t rotary) {
+  if (q.dim() < 2 || q.dim() != k.dim()) throw py::value_error(cat("q ", q.sizes(), " and k ", k.sizes(), " must be (..., heads, dim)"));
+  const int64_t n = q.dim(), d = q.size(-1);
+  if (q.sizes().slice(0, n - 2) != k.sizes().slice(0, n - 2) || d != k.size(-1)) throw py::value_error(cat("q ", q.sizes(), " and k ", k.sizes(), " do not match"));
+  if (d % 16 || d == 0 || d > 512) throw py::value_error(cat("dim=", d, " must be a multiple of 16 and at most 512"));
+  if (rotary % 16 || rotary < 0 || rotary > d) throw py::value_error(cat("rotary_dim=", rotary, " must be a multiple of 16 between 0 and dim=", d));
+  if (q.size(-2) == 0 || k.size(-2) == 0) throw py::value_error("q and k must have heads");
+  if (!(theta > 0 && theta <= 1e30)) throw py::value_error(cat("theta=", theta, " must be positive"));
+  if (q_scale.has_value() != k_scale.has_value()) throw py::value_error("q_scale and k_scale: both or neither");
+  if (q_scale) {
+    need_gamma(*q_scale, d);
+    need_gamma(*k_scale, d);
+  }
+}
+Rope rope_of(const Tensor& q, const std::optional<Tensor>& q_scale, const std::optional<Tensor>& k_scale, double eps, const std::optional<Tensor>& positions,
+             double theta, int64_t rotary, bool interleaved) {
+  Rope r;
+  r.eps = eps;
+  r.theta = theta;
+  r.rotary = rotary;
+  r.interleaved = interleaved;
+  if (q_scale) {
+    need_device(*q_scale, q, "q_scale");
+    need_device(*k_scale, q, "k_scale");
+    r.q_scale = need16(*q_scale, at::kBFloat16, "q_scale");
+    r.k_scale = need16(*k_scale, at::kBFloat16, "k_scale");
+  }
+  if (positions) {
+    const auto lead = q.sizes().slice(0, q.dim() - 2);
+    if (positions->scalar_type() != at::kInt && positions->scalar_type() != at::kLong)
+      throw py::type_error(cat("positions must be torch.int32 or torch.int64, got ", dtype_name(positions->scalar_type())));
+    bool fits = positions->dim() <= int64_t(lead.size());
+    for (int64_t i = 1; fits && i <= positions->dim(); ++i) fits = positions->size(-i) == 1 || positions->size(-i) == lead[lead.size() - i];
+    if (!fits) throw py::value_error(cat("positions ", positions->sizes(), " cannot be expanded to the tokens' ", lead));
+    need_device(*positions, q, "positions");
+    Tensor at = positions->expand(lead);
+    if (at.dim() > 2) at = at.flatten(0, -2);
+    r.positions = at;
+  }
+  return r;
+}
+void fill_rope(tg_qk_args& a, const Rope& r) {
+  a.q_scale = ptr(r.q_scale);
+  a.k_scale = ptr(r.k_scale);
+  if (r.positions.defined()) {
+    const Tensor& t = r.positions;
+    a.positions = ptr(t);
+    a.positions_64 = t.scalar_type() == at::kLong;
+    if (t.dim() > 0) a.positions_stride[1] = t.stride(-1);
+    if (t.dim() > 1) a.positions_stride[0] = t.stride(-2);
+  }
+  a.eps = float(r.eps);
+  a.theta = r.theta;
+  a.rotary_dim = int(r.rotary);
+  a.interleaved = r.interleaved;
+}
+// sizes and one side's addresses and strides of a call
+void fill_heads(tg_qk_args& a, const Heads& q, const Heads& k) {
+  constexpr int64_t most = int64_t(1) << 30;
+  if (q.heads > most || k.heads > most) throw py::value_error("too many heads");
+  a.batch = q.batch;
+  a.tokens = q.tokens;
+  a.heads = int(q.heads);
+  a.kv_heads = int(k.heads);
+  a.dim = int(q.dim);
+}
+
+Pair qk_norm_rope_fwd(const Tensor& q_, const Tensor& k_, const std::optional<Tensor>& q_scale, const std::optional<Tensor>& k_scale, double eps,
+                      const std::optional<Tensor>& positions, double theta, int64_t rotary, bool interleaved) {
+  if (rotary < 0 && q_.dim() > 0) rotary = q_.size(-1);
+  need_rope(q_, k_, q_scale, k_scale, theta, rotary);
+  const Heads q = heads_of(q_, "q"), k = heads_of(k_, "k");
+  need_device(k_, q_, "k");
+  const Rope r = rope_of(q_, q_scale, k_scale, eps, positions, theta, rotary, interleaved);
+  const c10::cuda::CUDAGuard guard(q_.device());
+  Pair out = {empty(q_.sizes(), at::kBFloat16, q_), empty(k_.sizes(), at::kBFloat16, k_)};
+  tg_qk_args a = {};
+  fill_heads(a, q, k);
+  fill_rope(a, r);
+  a.q = ptr(q.t);
+  a.k = ptr(k.t);
+  std::copy_n(q.stride, 3, a.q_stride);
+  std::copy_n(k.stride, 3, a.k_stride);
+  a.q_out = ptr(out.first);
+  a.k_out = ptr(out.second);
+  check(api.tg_qk_norm_rope_fwd(&a, cur_stream()), "tg_qk_norm_rope_fwd");
+  return out;
+}
+
+// dq, dk, dq_scale, dk_scale (undefined without scales); q and k are not read then, and may be undefined
+std::array<Tensor, 4> qk_norm_rope_bwd(const Tensor& q_, const Tensor& k_, const Tensor& g_q, const Tensor& g_k, const std::optional<Tensor>& q_scale,
+                                       const std::optional<Tensor>& k_scale, double eps, const std::optional<Tensor>& positions, double theta, int64_t rotary,
+                                       bool interleaved) {
+  if (rotary < 0 && g_q.dim() > 0) rotary = g_q.size(-1);
+  need_rope(g_q, g_k, q_scale, k_scale, theta, rotary);
+  const Heads gq = heads_of(g_q, "g_q"), gk = heads_of(g_k, "g_k");
+  need_device(g_k, g_q, "g_k");
+  const Rope r = rope_of(g_q, q_scale, k_scale, eps, positions, theta, rotary, interleaved);
+  const c10::cuda::CUDAGuard guard(g_q.device());
+  std::array<Tensor, 4> out = {empty(g_q.sizes(), at::kBFloat16, g_q), empty(g_k.sizes(), at::kBFloat16, g_k), Tensor(), Tensor()};
+  tg_qk_args a = {};
+  fill_heads(a, gq, gk);
+  fill_rope(a, r);
+  Heads q, k;
+  Tensor scratch;
+  if (q_scale) {
+    if (!q_.defined() || !k_.defined() || q_.sizes() != g_q.sizes() || k_.sizes() != g_k.sizes()) throw py::value_error("gradients must have the shapes of q and k");
+    q = heads_of(q_, "q");
+    k = heads_of(k_, "k");
+    need_device(q_, g_q, "q");
+    need_device(k_, g_q, "k");
+    a.q = ptr(q.t);
+    a.k = ptr(k.t);
+    std::copy_n(q.stride, 3, a.q_stride);
+    std::copy_n(k.stride, 3, a.k_stride);
+    for (int i : {2, 3}) out[i] = empty({gq.dim}, at::kBFloat16, g_q);
+    a.dq_scale = ptr(out[2]);
+    a.dk_scale = ptr(out[3]);
+    scratch = empty({std::max<int64_t>(api.tg_qk_norm_rope_bwd_scratch_bytes(&a), 16)}, at::kByte, g_q);
+    a.scratch = ptr(scratch);
+  }
+  a.g_q = ptr(gq.t);
+  a.g_k = ptr(gk.t);
+  std::copy_n(gq.stride, 3, a.g_q_stride);
+  std::copy_n(gk.stride, 3, a.g_k_stride);
+  a.q_out = ptr(out[0]);
+  a.k_out = ptr(out[1]);
+  check(api.tg_qk_norm_rope_bwd(&a, cur_stream()), "tg_qk_norm_rope_bwd");
+  return out;
+}
+
+// The gated projections: their operands as the kernels read them.
+struct Gated {
+  Tensor x, gate, up;                          // x [rows, cols]; any pitch
+  int act = 0;
+  int64_t rows = 0, cols = 0, inner = 0;
+};
+Gated gated_of(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, int act) {
+  if (x.dim() == 0) throw py::value_error("x must have at least one dimension");
+  if (w_gate.dim() != 2 || w_gate.sizes() != w_up.sizes()) throw py::value_error(cat("w_gate ", w_gate.sizes(), " and w_up ", w_up.sizes(), " must be matrices of one shape"));
+  Gated g;
+  g.act = act;
+  g.cols = x.size(-1);
+  g.inner = w_gate.size(1);
+  if (g.cols != w_gate.size(0)) throw py::value_error(cat("contracted-dim mismatch: x D=", g.cols, ", weights D=", w_gate.size(0)));
+  if (g.cols % 8 || g.inner % 8 || g.cols == 0 || g.inner == 0) throw py::value_error(cat("D=", g.cols, " and F=", g.inner, " must be multiples of 8"));
+  g.rows = x.numel() / g.cols;
+  const std::pair<const Tensor*, const char*> all[] = {{&x, "x"}, {&w_gate, "w_gate"}, {&w_up, "w_up"}};
+  for (const auto& [t, n] : all) {
+    if (!t->is_cuda()) throw std::runtime_error(cat(n, " must be a CUDA tensor (there is no CPU path)"));
+    if (t->scalar_type() != at::kBFloat16) throw py::type_error(cat(n, " must be torch.bfloat16, got ", dtype_name(t->scalar_type())));
+    need_device(*t, x, n);
+  }
+  auto aligned = [](const Tensor& t) {
+    const Tensor r = readable(t, false);
+    return (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15u) == 0 ? r : r.clone(at::MemoryFormat::Contiguous);
+  };
+  g.x = aligned(as_rows(x, g.rows, g.cols));
+  g.gate = aligned(w_gate);
+  g.up = aligned(w_up);
+  return g;
+}
+tg_gated_args gated_args(const Gated& g) {
+  tg_gated_args a = {};
+  a.x = ptr(g.x);
+  a.ldx = pitch(g.x);
+  a.w_gate = ptr(g.gate);
+  a.ld_gate = pitch(g.gate);
+  a.w_up = ptr(g.up);
+  a.ld_up = pitch(g.up);
+  a.act = g.act;
+  a.rows = g.rows;
+  a.cols = g.cols;
+  a.inner = g.inner;
+  a.status = status_of(g.x);
+  return a;
+}
+// What the forward pass keeps: both projections in 16 bits and their exponents
+struct GatedKept {
+  Tensor gate, up, exponents;
+};
+Tensor gated_linear_fwd(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, int act, GatedKept* kept) {
+  const Gated g = gated_of(x, w_gate, w_up, act);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor h = empty(with_last(x, g.inner), at::kBFloat16, x);
+  tg_gated_args a = gated_args(g);
+  a.h = ptr(h);
+  if (kept != nullptr) {
+    for (Tensor* t : {&kept->gate, &kept->up}) *t = empty({g.rows, g.inner}, at::kHalf, x);
+    kept->exponents = empty({std::max<int64_t>(api.tg_gated_linear_exponent_bytes(g.rows, g.inner), 16)}, at::kByte, x);
+    a.saved_gate = ptr(kept->gate);
+    a.saved_up = ptr(kept->up);
+    a.saved_exponents = static_cast<uint8_t*>(ptr(kept->exponents));
+  }
+  if (g.rows > 0) check(api.tg_gated_linear_fwd(&a, cur_stream()), "tg_gated_linear_fwd");
+  return h;
+}
+// dx, dw_gate, dw_up
+std::array<Tensor, 3> gated_linear_bwd(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, int act, const GatedKept& kept, const Tensor& grad, bool want_dx,
+                                       bool want_dw) {
+  const Gated g = gated_of(x, w_gate, w_up, act);
+  if (grad.sizes() != at::IntArrayRef(with_last(x, g.inner))) throw py::value_error("the gradient must have the output's shape");
+  need_device(grad, x, "g");
+  const Tensor gr = need16(grad, at::kBFloat16, "g");
+  const c10::cuda::CUDAGuard guard(x.device());
+  std::array<Tensor, 3> out;
+  if (want_dx) out[0] = empty(x.sizes(), at::kBFloat16, x);
+  if (want_dw)
+    for (int i : {1, 2}) out[i] = empty({g.cols, g.inner}, at::kBFloat16, x);
+  const Tensor scratch = empty({std::max<int64_t>(api.tg_gated_linear_bwd_scratch_bytes(g.rows, g.inner), 16)}, at::kByte, x);
+  tg_gated_args a = gated_args(g);
+  a.saved_gate = ptr(kept.gate);
+  a.saved_up = ptr(kept.up);
+  a.saved_exponents = static_cast<uint8_t*>(ptr(kept.exponents));
+  a.g = ptr(gr);
+  a.dx = ptr(out[0]);
+  a.dw_gate = ptr(out[1]);
+  a.dw_up = ptr(out[2]);
+  a.scratch = ptr(scratch);
+  check(api.tg_gated_linear_bwd(&a, cur_stream()), "tg_gated_linear_bwd");
+  return out;
+}
+
+Tensor dropout_fwd(const Tensor& x_, double p, const Tensor& seed, int64_t site, const std::optional<Tensor>& residual_) {
+  if (!(p >= 0 && p <= 1)) throw py::value_error(cat("p=", p, " must be between 0 and 1"));
+  if (site < 0 || site >= int64_t(1) << 32) throw py::value_error(cat("site=", site, " must be between 0 and 2^32 - 1"));
+  if (residual_ && residual_->sizes() != x_.sizes()) throw py::value_error(cat("x shape ", x_.sizes(), " != residual shape ", residual_->sizes()));
+  if (seed.numel() != 1) throw py::value_error(cat("seed must be one number, got shape ", seed.sizes()));
+  const Tensor x = need16(x_, at::kBFloat16, "x"), s = need(seed, at::kLong, "seed"), residual = residual_ ? need16(*residual_, at::kBFloat16, "residual") : Tensor();
+  need_device(s, x, "seed");
+  if (residual_) need_device(residual, x, "residual");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor y = empty_as(x);
+  check(api.tg_dropout(ptr(x), ptr(residual), p, static_cast<const int64_t*>(ptr(s)), uint32_t(site), ptr(y), x.numel(), cur_stream()), "tg_dropout");
+  return y;
+}
+
 // ---- loss ---------------------------------------------------------------------------------------------------------
 
 // Logits as rows of one pitch: as they lie where the last axis has unit stride and the others collapse, copied otherwise.
@@ -1293,6 +1576,156 @@ Sandwich sandwich_norm(const Tensor& x, const Tensor& branch, const Tensor& post
   return o;
 }
 
+struct QkNormRopeBackward : public Node {
+  SavedVariable q, k, q_scale, k_scale, positions;
+  std::vector<int64_t> q_shape, k_shape;
+  bool norm = false, placed = false, released = false;
+  double eps = 0, theta = 0;
+  int64_t rotary = 0;
+  bool interleaved = false;
+  std::string name() const override { return "QkNormRopeBackward"; }
+  void release_variables() override {
+    for (SavedVariable* v : {&q, &k, &q_scale, &k_scale, &positions}) v->reset_data();
+    released = true;
+  }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(4);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    if (released) backward_twice();
+    const std::optional<Tensor> a = norm ? std::optional<Tensor>(q_scale.unpack()) : std::nullopt, b = norm ? std::optional<Tensor>(k_scale.unpack()) : std::nullopt;
+    const std::optional<Tensor> at = placed ? std::optional<Tensor>(positions.unpack()) : std::nullopt;
+    const Tensor x = norm ? q.unpack() : Tensor(), y = norm ? k.unpack() : Tensor();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor& any = grads[0].defined() ? grads[0] : grads[1];
+      const c10::cuda::CUDAGuard guard(any.device());
+      auto grad = [&](const Tensor& g, const std::vector<int64_t>& shape) { return g.defined() ? to(g, at::kBFloat16) : at::zeros(shape, any.options().dtype(at::kBFloat16)); };
+      auto d = qk_norm_rope_bwd(x, y, grad(grads[0], q_shape), grad(grads[1], k_shape), a, b, eps, at, theta, rotary, interleaved);
+      for (size_t i = 0; i < 4; ++i) out[i] = std::move(d[i]);
+    }
+    return once_differentiable(std::move(out), *this, "qk_norm_rope");
+  }
+};
+
+Pair qk_norm_rope(const Tensor& q, const Tensor& k, const std::optional<Tensor>& q_scale, const std::optional<Tensor>& k_scale, double eps,
+                  const std::optional<Tensor>& positions, double theta, int64_t rotary, bool interleaved) {
+  bool track = q.requires_grad() || k.requires_grad() || (q_scale && q_scale->requires_grad()) || (k_scale && k_scale->requires_grad());
+  track = track && at::GradMode::is_enabled();
+  no_tangent({&q, &k}, "qk_norm_rope");
+  if (q_scale) no_tangent({&*q_scale}, "qk_norm_rope");
+  if (k_scale) no_tangent({&*k_scale}, "qk_norm_rope");
+  Pair o;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    o = qk_norm_rope_fwd(q, k, q_scale, k_scale, eps, positions, theta, rotary, interleaved);
+  }
+  if (!track) return o;
+  std::shared_ptr<QkNormRopeBackward> node(new QkNormRopeBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(q, k, q_scale ? *q_scale : Tensor(), k_scale ? *k_scale : Tensor()));
+  node->norm = q_scale.has_value();
+  if (node->norm) {
+    node->q = SavedVariable(q, false);
+    node->k = SavedVariable(k, false);
+    node->q_scale = SavedVariable(*q_scale, false);
+    node->k_scale = SavedVariable(*k_scale, false);
+  }
+  node->placed = positions.has_value();
+  if (positions) node->positions = SavedVariable(*positions, false);
+  node->q_shape.assign(q.sizes().begin(), q.sizes().end());
+  node->k_shape.assign(k.sizes().begin(), k.sizes().end());
+  node->eps = eps;
+  node->theta = theta;
+  node->rotary = rotary < 0 ? q.size(-1) : rotary;
+  node->interleaved = interleaved;
+  torch::autograd::set_history(o.first, node);
+  torch::autograd::set_history(o.second, node);
+  return o;
+}
+
+struct GatedLinearBackward : public Node {
+  SavedVariable x, w_gate, w_up;
+  GatedKept kept;
+  int act = 0;
+  std::string name() const override { return "GatedLinearBackward"; }
+  void release_variables() override {
+    for (SavedVariable* v : {&x, &w_gate, &w_up}) v->reset_data();
+    kept = GatedKept();
+  }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(3);
+    if (!grads[0].defined()) return out;
+    if (!kept.gate.defined()) backward_twice();
+    const Tensor a = x.unpack(), b = w_gate.unpack(), c = w_up.unpack();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto d = gated_linear_bwd(a, b, c, act, kept, to(grads[0], at::kBFloat16), task_should_compute_output(0),
+                                task_should_compute_output(1) || task_should_compute_output(2));
+      for (size_t i = 0; i < 3; ++i) out[i] = std::move(d[i]);
+    }
+    return once_differentiable(std::move(out), *this, "gated_linear");
+  }
+};
+
+Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, int act) {
+  const bool track = at::GradMode::is_enabled() && (x.requires_grad() || w_gate.requires_grad() || w_up.requires_grad());
+  no_tangent({&x, &w_gate, &w_up}, "gated_linear");
+  GatedKept kept;
+  Tensor h;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    h = gated_linear_fwd(x, w_gate, w_up, act, track ? &kept : nullptr);
+  }
+  if (!track) return h;
+  std::shared_ptr<GatedLinearBackward> node(new GatedLinearBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(x, w_gate, w_up));
+  node->x = SavedVariable(x, false);
+  node->w_gate = SavedVariable(w_gate, false);
+  node->w_up = SavedVariable(w_up, false);
+  node->kept = std::move(kept);
+  node->act = act;
+  torch::autograd::set_history(h, node);
+  return h;
+}
+
+struct DropoutBackward : public Node {
+  SavedVariable seed;
+  double p = 0;
+  int64_t site = 0;
+  std::string name() const override { return "DropoutBackward"; }
+  void release_variables() override { seed.reset_data(); }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(2);
+    if (!grads[0].defined()) return out;
+    const Tensor s = seed.unpack();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      if (task_should_compute_output(0)) out[0] = dropout_fwd(to(grads[0], at::kBFloat16), p, s, site, std::nullopt);
+    }
+    out = once_differentiable(std::move(out), *this, "dropout");
+    out[1] = grads[0];
+    return out;
+  }
+};
+
+Tensor dropout(const Tensor& x, double p, const Tensor& seed, int64_t site, const std::optional<Tensor>& residual) {
+  const bool track = at::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad()));
+  no_tangent({&x}, "dropout");
+  if (residual) no_tangent({&*residual}, "dropout");
+  Tensor y;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    y = dropout_fwd(x, p, seed, site, residual);
+  }
+  if (!track) return y;
+  std::shared_ptr<DropoutBackward> node(new DropoutBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(x, residual ? *residual : Tensor()));
+  node->seed = SavedVariable(seed, false);
+  node->p = p;
+  node->site = site;
+  torch::autograd::set_history(y, node);
+  return y;
+}
+
 // ---- bindings -------------------------------------------------------------------------------------------------------
 
 Tensor or_none(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
@@ -1335,6 +1768,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     const auto d = sandwich_norm_bwd(x_new, branch, post, pre, eps, or_none(g_new), or_none(g_h), gate, residual_scale);
     return py::make_tuple(d[0], d[1], d[2], d[3], d[4]);
   });
+  m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd);
+  m.def("qk_norm_rope_bwd", [](const std::optional<Tensor>& q, const std::optional<Tensor>& k, const Tensor& g_q, const Tensor& g_k, const std::optional<Tensor>& q_scale,
+                               const std::optional<Tensor>& k_scale, double eps, const std::optional<Tensor>& positions, double theta, int64_t rotary,
+                               bool interleaved) {
+    const auto d = qk_norm_rope_bwd(or_none(q), or_none(k), g_q, g_k, q_scale, k_scale, eps, positions, theta, rotary, interleaved);
+    return py::make_tuple(d[0], d[1], d[2], d[3]);
+  });
+  m.def("qk_norm_rope", &qk_norm_rope);
+  m.def("gated_linear", &gated_linear);
+  m.def("dropout", &dropout);
   m.def("top_logits", &top_logits);
   m.def("softcap_distill", &softcap_distill);
   m.def("sandwich_norm", [](const Tensor& x, const Tensor& branch, const Tensor& post, const Tensor& pre, double eps, const std::optional<Tensor>& gate,

@@ -35,6 +35,8 @@ constexpr auto kF8 = at::kFloat8_e4m3fn;
   X(tg_act_quantize_rowcol) X(tg_quantize_block128) X(tg_rmsnorm_fwd) X(tg_rmsnorm_quant_fwd)                       \
   X(tg_add_rmsnorm_quant_fwd) X(tg_rmsnorm_bwd_scratch_bytes) X(tg_rmsnorm_bwd) X(tg_rmsnorm_bwd_add) X(tgh_rmsnorm_bwd_parts) X(tgh_dgamma_reduce) \
   X(tg_sandwich_norm_fwd) X(tg_sandwich_norm_bwd_scratch_bytes) X(tg_sandwich_norm_bwd) X(tg_top_logits) X(tg_softcap_distill) \
+  X(tg_qk_norm_rope_fwd) X(tg_qk_norm_rope_bwd_scratch_bytes) X(tg_qk_norm_rope_bwd) X(tg_gated_linear_exponent_bytes) X(tg_gated_linear_fwd) \
+  X(tg_gated_linear_bwd_scratch_bytes) X(tg_gated_linear_bwd) X(tg_dropout) \
   X(tg_softcap_ce_fwd) X(tg_softcap_ce_bwd) X(tg_sumsq_scratch_bytes) X(tg_sumsq_bf16) X(tg_adamw_bf16)             \
   X(tg_gemm_workspace_bytes) X(tg_gemm_fp8_blockscaled) X(tgh_gemm_two) X(tgh_quantize_jobs) X(tgh_softcap_ce_fits) X(tgh_softcap_ce) X(tgh_mean) \
   X(tgh_global_norm_scratch_bytes) X(tgh_global_norm) X(tgh_adamw) X(tgh_embed) X(tgh_embed_bwd_cleared)

@@ -128,6 +128,28 @@ def sandwich_norm_bwd(x_new, branch, post_scale, scale, eps: float, g_new=None, 
     return _host().sandwich_norm_bwd(x_new, branch, post_scale, scale, eps, g_new, g_h, gate, residual_scale)
 
 
+# ---- rotary positions ---------------------------------------------------------------------
+
+def rotary_dim_of(rotary_dim: int) -> int:
+    """(the native calls take a negative number for "all of a head")"""
+    if rotary_dim < 0:
+        raise ValueError(f"rotary_dim={rotary_dim} must be a multiple of 16 between 0 and dim")
+    return rotary_dim
+
+
+def qk_norm_rope_fwd(q, k, q_scale, k_scale, eps: float, positions=None, theta: float = 10000.0, rotary_dim: int | None = None,
+                     interleaved: bool = False):
+    """kernels.qk_norm_rope without autograd: (q', k')."""
+    return _host().qk_norm_rope_fwd(q, k, q_scale, k_scale, eps, positions, theta, -1 if rotary_dim is None else rotary_dim_of(rotary_dim), interleaved)
+
+
+def qk_norm_rope_bwd(q, k, g_q, g_k, q_scale, k_scale, eps: float, positions=None, theta: float = 10000.0, rotary_dim: int | None = None,
+                     interleaved: bool = False):
+    """From the gradients of q' and k' and the saved q and k (None without scales): (dq, dk, dq_scale or None, dk_scale or None), all bf16."""
+    return _host().qk_norm_rope_bwd(q, k, g_q, g_k, q_scale, k_scale, eps, positions, theta, -1 if rotary_dim is None else rotary_dim_of(rotary_dim),
+                                    interleaved)
+
+
 # ---- capped-logit cross-entropy -----------------------------------------------------------
 
 def softcap_ce_fwd(logits, targets, cap: float, want_tanh: bool = True):

@@ -39,6 +39,7 @@ FFI_TARGETS = (
     "TgActQuantizeRowcol", "TgActQuantizeRowcolBwd",
     "TgRmsnormFwd", "TgRmsnormQuantFwd", "TgAddRmsnormQuantFwd", "TgRmsnormBwd", "TgRmsnormBwdAdd", "TgRmsnormBwdStatic",
     "TgSandwichNormFwd", "TgSandwichNormQuantFwd", "TgSandwichNormBwd", "TgTopLogits", "TgSoftcapDistill",
+    "TgQkNormRopeFwd", "TgQkNormRopeBwd", "TgGatedLinearFwd", "TgGatedLinearBwd", "TgDropout", "TgDropoutAdd",
     "TgSoftcapCeFwd", "TgSoftcapCeBwd", "TgSumsqBf16", "TgAdamwBf16",
     "TgGemmFwd", "TgGemmDgrad", "TgGemmWgrad",
 )

@@ -297,6 +297,108 @@ ffi::Error SoftcapDistill(cudaStream_t s, BF16 logits, S32 ids, F32 logp, F32 lo
   return Check(tg_softcap_distill(&a, s), "tg_softcap_distill");
 }
 
+// ---- rotary positions, the gated feed-forward, dropout (no counterpart) -----------------------------
+
+// q (batch, tokens, heads, dim), k (batch, tokens, kv_heads, dim), contiguous; positions (batch, tokens)
+bool QkArgs(const BF16& q, const BF16& k, const BF16& q_scale, const BF16& k_scale, const S32& positions, bool norm, tg_qk_args* a) {
+  auto d = q.dimensions();
+  auto e = k.dimensions();
+  if (d.size() != 4 || e.size() != 4 || d[0] != e[0] || d[1] != e[1] || d[3] != e[3]) return false;
+  if (!Have(d[0] * d[1], positions) || (norm && !Have(d[3], q_scale, k_scale))) return false;
+  for (int64_t n : {d[2], e[2], d[3]})
+    if (n > 65536) return false;
+  a->batch = d[0]; a->tokens = d[1]; a->heads = static_cast<int>(d[2]); a->kv_heads = static_cast<int>(e[2]); a->dim = static_cast<int>(d[3]);
+  int64_t* strides[4] = {a->q_stride, a->g_q_stride, a->k_stride, a->g_k_stride};
+  for (int i = 0; i < 4; ++i) {
+    const int64_t heads = i < 2 ? d[2] : e[2];
+    strides[i][0] = d[1] * heads * d[3]; strides[i][1] = heads * d[3]; strides[i][2] = d[3];
+  }
+  a->q = q.untyped_data(); a->k = k.untyped_data();
+  if (norm) { a->q_scale = q_scale.untyped_data(); a->k_scale = k_scale.untyped_data(); }
+  a->positions = positions.untyped_data(); a->positions_stride[0] = d[1]; a->positions_stride[1] = 1;
+  return true;
+}
+
+// norm 0: the rotation alone (pass any bf16 buffers for the scales)
+ffi::Error QkNormRopeFwd(cudaStream_t s, BF16 q, BF16 k, BF16 q_scale, BF16 k_scale, S32 positions, RBF16 q_out, RBF16 k_out, int32_t norm, float eps,
+                         double theta, int32_t rotary_dim, int32_t interleaved) {
+  tg_qk_args a = {};
+  if (!QkArgs(q, k, q_scale, k_scale, positions, norm != 0, &a) || !Have(static_cast<int64_t>(q.element_count()), *q_out) ||
+      !Have(static_cast<int64_t>(k.element_count()), *k_out))
+    return Mismatch("TgQkNormRopeFwd: q and k must be (batch, tokens, heads, dim) of one batch, tokens and dim, the results like them, scales (dim,), positions (batch, tokens)");
+  a.eps = eps; a.theta = theta; a.rotary_dim = rotary_dim; a.interleaved = interleaved;
+  a.q_out = q_out->untyped_data(); a.k_out = k_out->untyped_data();
+  return Check(tg_qk_norm_rope_fwd(&a, s), "tg_qk_norm_rope_fwd");
+}
+
+// scratch: tg_qk_norm_rope_bwd_scratch_bytes bytes that XLA plans; dq_scale and dk_scale are left alone with norm 0
+ffi::Error QkNormRopeBwd(cudaStream_t s, BF16 q, BF16 k, BF16 q_scale, BF16 k_scale, S32 positions, BF16 g_q, BF16 g_k, RBF16 dq, RBF16 dk, RBF16 dq_scale,
+                         RBF16 dk_scale, RU8 scratch, int32_t norm, float eps, double theta, int32_t rotary_dim, int32_t interleaved) {
+  tg_qk_args a = {};
+  if (!QkArgs(q, k, q_scale, k_scale, positions, norm != 0, &a) || !Have(static_cast<int64_t>(q.element_count()), g_q, *dq) ||
+      !Have(static_cast<int64_t>(k.element_count()), g_k, *dk) || (norm != 0 && !Have(a.dim, *dq_scale, *dk_scale)))
+    return Mismatch("TgQkNormRopeBwd: gradients and results must be like q and k, scales and their gradients (dim,), positions (batch, tokens)");
+  a.eps = eps; a.theta = theta; a.rotary_dim = rotary_dim; a.interleaved = interleaved;
+  if (static_cast<int64_t>(scratch->element_count()) < tg_qk_norm_rope_bwd_scratch_bytes(&a))
+    return Mismatch("TgQkNormRopeBwd: scratch result smaller than tg_qk_norm_rope_bwd_scratch_bytes");
+  a.g_q = g_q.untyped_data(); a.g_k = g_k.untyped_data();
+  a.q_out = dq->untyped_data(); a.k_out = dk->untyped_data();
+  a.dq_scale = dq_scale->untyped_data(); a.dk_scale = dk_scale->untyped_data(); a.scratch = scratch->untyped_data();
+  return Check(tg_qk_norm_rope_bwd(&a, s), "tg_qk_norm_rope_bwd");
+}
+
+// what both directions of the gated feed-forward are called with; `inner` values per row in h or its gradient
+bool GatedArgs(cudaStream_t s, const BF16& x, const BF16& w_gate, const BF16& w_up, int64_t outer, RU32& status, tg_gated_args* a) {
+  RowsCols(x, &a->rows, &a->cols);
+  auto d = w_gate.dimensions();
+  if (d.size() != 2 || d[0] != a->cols || !Have(d[0] * d[1], w_up) || outer != a->rows * d[1] || !Have(1, *status)) return false;
+  a->inner = d[1];
+  a->ldx = a->cols; a->ld_gate = a->ld_up = a->inner;
+  a->x = x.untyped_data(); a->w_gate = w_gate.untyped_data(); a->w_up = w_up.untyped_data();
+  a->status = status->typed_data();
+  return cudaMemsetAsync(a->status, 0, sizeof(uint32_t), s) == cudaSuccess;
+}
+
+// saved_gate, saved_up: 2 rows inner bytes each, exponents tg_gated_linear_exponent_bytes (a custom_vjp's residuals); status (1,)
+ffi::Error GatedLinearFwd(cudaStream_t s, BF16 x, BF16 w_gate, BF16 w_up, RBF16 h, RU8 saved_gate, RU8 saved_up, RU8 exponents, RU32 status, int32_t act) {
+  tg_gated_args a = {};
+  if (!GatedArgs(s, x, w_gate, w_up, static_cast<int64_t>(h->element_count()), status, &a) || !Have(2 * a.rows * a.inner, *saved_gate, *saved_up) ||
+      static_cast<int64_t>(exponents->element_count()) < tg_gated_linear_exponent_bytes(a.rows, a.inner))
+    return Mismatch("TgGatedLinearFwd: weights must be (cols, inner), h (rows, inner), saved results 2 rows inner bytes, exponents tg_gated_linear_exponent_bytes, status (1,)");
+  a.act = act; a.h = h->untyped_data();
+  a.saved_gate = saved_gate->untyped_data(); a.saved_up = saved_up->untyped_data(); a.saved_exponents = exponents->typed_data();
+  return Check(tg_gated_linear_fwd(&a, s), "tg_gated_linear_fwd");
+}
+
+ffi::Error GatedLinearBwd(cudaStream_t s, BF16 x, BF16 w_gate, BF16 w_up, U8 saved_gate, U8 saved_up, U8 exponents, BF16 g, RBF16 dx, RBF16 dw_gate,
+                          RBF16 dw_up, RU8 scratch, RU32 status, int32_t act) {
+  tg_gated_args a = {};
+  if (!GatedArgs(s, x, w_gate, w_up, static_cast<int64_t>(g.element_count()), status, &a) || !Have(2 * a.rows * a.inner, saved_gate, saved_up) ||
+      !Have(a.rows * a.cols, *dx) || !Have(a.cols * a.inner, *dw_gate, *dw_up) ||
+      static_cast<int64_t>(exponents.element_count()) < tg_gated_linear_exponent_bytes(a.rows, a.inner) ||
+      static_cast<int64_t>(scratch->element_count()) < tg_gated_linear_bwd_scratch_bytes(a.rows, a.inner))
+    return Mismatch("TgGatedLinearBwd: g must be (rows, inner), results like x and the weights, saved buffers as TgGatedLinearFwd's, scratch tg_gated_linear_bwd_scratch_bytes");
+  a.act = act; a.g = g.untyped_data();
+  a.saved_gate = saved_gate.untyped_data(); a.saved_up = saved_up.untyped_data(); a.saved_exponents = exponents.typed_data();
+  a.dx = dx->untyped_data(); a.dw_gate = dw_gate->untyped_data(); a.dw_up = dw_up->untyped_data(); a.scratch = scratch->untyped_data();
+  return Check(tg_gated_linear_bwd(&a, s), "tg_gated_linear_bwd");
+}
+
+// seed: two words, low and high (a JAX PRNG key is that); site: site bits of the attribute.  TgDropout without a residual is its own backward rule.
+ffi::Error Dropout(cudaStream_t s, BF16 x, U32 seed, RBF16 y, double p, int32_t site) {
+  const int64_t n = static_cast<int64_t>(x.element_count());
+  if (!Have(2, seed) || !Have(n, *y)) return Mismatch("TgDropout: seed must be two words, y like x");
+  return Check(tg_dropout(x.untyped_data(), nullptr, p, static_cast<const int64_t*>(seed.untyped_data()), static_cast<uint32_t>(site), y->untyped_data(), n, s),
+               "tg_dropout");
+}
+ffi::Error DropoutAdd(cudaStream_t s, BF16 x, BF16 residual, U32 seed, RBF16 y, double p, int32_t site) {
+  const int64_t n = static_cast<int64_t>(x.element_count());
+  if (!Have(2, seed) || !Have(n, residual, *y)) return Mismatch("TgDropoutAdd: seed must be two words, residual and y like x");
+  return Check(tg_dropout(x.untyped_data(), residual.untyped_data(), p, static_cast<const int64_t*>(seed.untyped_data()), static_cast<uint32_t>(site),
+                          y->untyped_data(), n, s),
+               "tg_dropout");
+}
+
 // ---- optimiser (train.py:114-123, 132-134) --------------------------------------------------------
 
 ffi::Error SumsqBf16(cudaStream_t s, BF16 x, RF32 out, RU8 scratch) {
@@ -449,3 +551,20 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(TgTopLogits, TopLogits,
 XLA_FFI_DEFINE_HANDLER_SYMBOL(TgSoftcapDistill, SoftcapDistill,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Arg<S32>().Arg<F32>().Arg<F32>().Arg<S32>().Ret<F32>().Ret<BF16>()
                                   .Attr<float>("cap").Attr<float>("temperature").Attr<float>("weight"));
+#define TG_QK_ATTRS Attr<int32_t>("norm").Attr<float>("eps").Attr<double>("theta").Attr<int32_t>("rotary_dim").Attr<int32_t>("interleaved")
+
+XLA_FFI_DEFINE_HANDLER_SYMBOL(TgQkNormRopeFwd, QkNormRopeFwd,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<S32>().Ret<BF16>().Ret<BF16>().TG_QK_ATTRS);
+XLA_FFI_DEFINE_HANDLER_SYMBOL(TgQkNormRopeBwd, QkNormRopeBwd,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<S32>().Arg<BF16>().Arg<BF16>()
+                                  .Ret<BF16>().Ret<BF16>().Ret<BF16>().Ret<BF16>().Ret<U8>().TG_QK_ATTRS);
+XLA_FFI_DEFINE_HANDLER_SYMBOL(TgGatedLinearFwd, GatedLinearFwd,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Ret<BF16>().Ret<U8>().Ret<U8>().Ret<U8>().Ret<U32>()
+                                  .Attr<int32_t>("act"));
+XLA_FFI_DEFINE_HANDLER_SYMBOL(TgGatedLinearBwd, GatedLinearBwd,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Arg<BF16>().Arg<BF16>().Arg<U8>().Arg<U8>().Arg<U8>().Arg<BF16>()
+                                  .Ret<BF16>().Ret<BF16>().Ret<BF16>().Ret<U8>().Ret<U32>().Attr<int32_t>("act"));
+XLA_FFI_DEFINE_HANDLER_SYMBOL(TgDropout, Dropout,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Arg<U32>().Ret<BF16>().Attr<double>("p").Attr<int32_t>("site"));
+XLA_FFI_DEFINE_HANDLER_SYMBOL(TgDropoutAdd, DropoutAdd,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<BF16>().Arg<BF16>().Arg<U32>().Ret<BF16>().Attr<double>("p").Attr<int32_t>("site"));
