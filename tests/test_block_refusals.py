@@ -194,10 +194,14 @@ def test_the_pairs_kernel_keeps_the_gemms_rules():
     """As test_tensor_memory_source and test_warp_order_source for the other GEMMs: dependents start after the allocation, nothing is read
     before the wait for the kernel before, an arrival for a whole warp follows its __syncwarp."""
     text = re.sub(r"//[^\n]*", "", open(os.path.join(ROOT, "train_gpt_b200", "csrc", "gated.cu")).read())
-    body = text[text.index("void gated_body("):text.index("gated_fwd_kernel(")]
-    taken, met, trigger, wait = (body.index(s) for s in ("tmem_take_pair(", "cluster_sync();", "grid_trigger();", "grid_wait();"))
-    assert taken < met < trigger < wait < min(body.index(s) for s in ("tma_load", "tma_store", "exponents"))
-    assert body.count("grid_trigger();") == body.count("grid_wait();") == 1
-    for m in re.finditer(r"\bmbar_arrive(?:_cluster)?_if\(", body):
-        marks = re.findall(r"__syncwarp\(\);|__all_sync\(|\bmbar_wait\(|\btmem_wait_ld\w*\(", body[:m.start()])
+    pairs, few = text[text.index("void gated_body("):text.index("gated_fwd_kernel(")], text[text.index("gated_few_kernel(const"):text.index("struct GatedSlopes")]
+    for body, take, meet, touch in ((pairs, "tmem_take_pair(", "cluster_sync();", ("tma_load", "tma_store", "exponents")), (few, "tmem_take(", "__syncthreads();", ("tma_load", "p.h"))):
+        taken = body.index(take)
+        met, trigger, wait = (body.index(s, taken) for s in (meet, "grid_trigger();", "grid_wait();"))
+        assert taken < met < trigger < wait < min(body.index(s) for s in touch)
+        assert body.count("grid_trigger();") == body.count("grid_wait();") == 1
+    arrivals = list(re.finditer(r"\bmbar_arrive(?:_cluster)?_if\(", pairs))
+    assert arrivals and "mbar_arrive" not in few
+    for m in arrivals:
+        marks = re.findall(r"__syncwarp\(\);|__all_sync\(|\bmbar_wait\(|\btmem_wait_ld\w*\(", pairs[:m.start()])
         assert marks[-1] == "__syncwarp();"

@@ -33,8 +33,8 @@ def _check(x, wg, wu, g, act="silu"):
     grads = torch.autograd.grad(h, leaves, g)
     for got, want, name in zip(grads, ref.gated_bwd(*d[:3], act, d[3]), ("dx", "dw_gate", "dw_up")):
         _near(got, want, name)
-    with torch.no_grad():
-        assert torch.equal(kernels.gated_linear(*leaves, act), h)
+    with torch.no_grad():                       # (up to 128 tokens another kernel, which may add up in another order)
+        _near(kernels.gated_linear(*leaves, act), ref.gated(*d[:3], act), "h alone")
     ops.check_status()
     return h, grads
 
@@ -87,6 +87,10 @@ def test_leading_axes_strides_and_alignment():
         h3 = kernels.gated_linear(*again)
         assert torch.equal(h3, h)
         assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(h3, again, gr), (dx, dg, du)))
+    with torch.no_grad():
+        want = kernels.gated_linear(x, wg, wu)
+        for a, b, c in ((wide[:, 8:72], both[:, :72], both[:, 72:]), (shifted, wg.T.contiguous().T, wu)):
+            assert torch.equal(kernels.gated_linear(a, b, c), want)
     row = x[:1].expand(60, 64)
     assert torch.equal(kernels.gated_linear(row, wg, wu)[7:8], kernels.gated_linear(row, wg, wu)[:1])
 
@@ -145,6 +149,38 @@ def test_projections_beyond_fp16(act):
     off = (ref.BF * (grad * U * da).abs() + grad.abs() * (bend * (U.abs() + eu) + 1.2 * eu)) @ gd.abs().T + (ref.BF * (grad * a).abs() + grad.abs() * (1.2 * eg + 2.0 ** -20 * G.abs())) @ ud.abs().T
     off = 1.01 * (off + ref.BF * want.abs()) + 400 * ref.F32 * ((grad * U * da).abs() @ gd.abs().T + (grad * a).abs() @ ud.abs().T)
     assert ((dx.double() - want).abs() <= off).all()
+
+
+@pytest.mark.parametrize("m", [1, 5, 64, 65, 128])
+@pytest.mark.parametrize("k,f", [(64, 64), (512, 64), (1000, 8), (1024, 512), (2048, 1096), (264, 18960), (72, 40000)])
+def test_few_tokens_alone(m, k, f):
+    """Without a gradient: one to eight ranges of the contraction, tiles beyond one round of the SMs."""
+    x, wg, wu, _ = _make(m, k, f)
+    d = [t.double() for t in (x, wg, wu)]
+    for act in ("silu", "gelu", "relu"):
+        with torch.no_grad():
+            h = kernels.gated_linear(x, wg, wu, act)
+            _near(h, ref.gated(*d, act), act)
+            assert torch.equal(kernels.gated_linear(x, wg, wu, act), h)
+    ops.check_status()
+
+
+def test_few_tokens_in_graphs():
+    x, wg, wu, _ = _make(7, 512, 264)
+    with torch.no_grad():
+        graphs = []
+        kernels.gated_linear(x, wg, wu)
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                outs = [kernels.gated_linear(x, wg, wu, a) for a in ("silu", "gelu", "relu") * 3]
+            graphs.append((g, outs))
+        x.mul_(0.5)
+        want = [kernels.gated_linear(x, wg, wu, a) for a in ("silu", "gelu", "relu") * 3]
+        for g, outs in graphs:
+            g.replay()
+        assert all(torch.equal(a, b) for _, outs in graphs for a, b in zip(outs, want))
+    ops.check_status()
 
 
 def test_large_negative_gates_and_infinities():

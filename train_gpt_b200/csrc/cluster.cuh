@@ -45,6 +45,11 @@ __device__ __forceinline__ void tmem_take_pair(uint32_t dst_smem) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(uint32_t(kTmemCols)) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 }
+// the same for one CTA, which may share its SM with others that take columns
+__device__ __forceinline__ void tmem_take(uint32_t dst_smem, uint32_t cols) {
+  tmem_alloc(dst_smem, cols);
+  tmem_relinquish();
+}
 __device__ __forceinline__ void tmem_give_pair(uint32_t addr) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(uint32_t(kTmemCols)) : "memory");
 }

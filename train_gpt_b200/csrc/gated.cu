@@ -135,7 +135,7 @@ __device__ __forceinline__ uint32_t max_magnitude(uint32_t m, uint32_t bits) { r
 // Sixteen bytes of this lane's staging row: chunk c of its 128 bytes, swizzled
 __device__ __forceinline__ void stage16(uint32_t row, int lane, int c, uint4 v) { sts128(row + (uint32_t(c ^ (lane & 7)) << 4), v); }
 
-template <int BUFS, bool SAVE>
+template <int BUFS>
 struct GatedCfg {
   static constexpr int bufs = BUFS;             // output boxes of a warp
   static constexpr int out_bytes = kGbWarps * BUFS * kGbOutBox;
@@ -352,7 +352,20 @@ __device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedP
           rows_free();
           const int n0 = tn * 128 + half * 64;
           if constexpr (SAVE) {
-            const uint32_t eg = save_row(g0, g1, row + kGbOutBox, lane), eu = save_row(u0, u1, row + 2 * kGbOutBox, lane);
+            // one staging box for the gate's, the up-projection's and the result's rows in turn: with three, four stages were left for the operands
+            // (32768 x 1024 -> 4096 with its backward pass 1352 us, 1332 so)
+            auto send = [&](const CUtensorMap* map) {
+              staged();
+              if (is_lane0) {
+                tma_store_2d(map, out, n0, m0);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+              }
+              rows_free();
+            };
+            const uint32_t eg = save_row(g0, g1, row, lane);
+            send(&saved.gate);
+            const uint32_t eu = save_row(u0, u1, row, lane);
+            send(&saved.up);
             if (m0 + lane < saved.rows && n0 / 64 < saved.chunks)
               reinterpret_cast<uint16_t*>(saved.exponents)[int64_t(n0 / 64) * saved.rows + m0 + lane] = uint16_t(eg | eu << 8);
           }
@@ -372,10 +385,6 @@ __device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedP
           staged();
           if (is_lane0) {
             tma_store_2d(&p.d[0], out, n0, m0);
-            if constexpr (SAVE) {
-              tma_store_2d(&saved.gate, out + kGbOutBox, n0, m0);
-              tma_store_2d(&saved.up, out + 2 * kGbOutBox, n0, m0);
-            }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
           __syncwarp();
@@ -434,11 +443,200 @@ __device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedP
 
 template <int ACT, bool SAVE>
 __global__ void __launch_bounds__(kGbThreads, 1) gated_fwd_kernel(const __grid_constant__ GatedProblem p, const __grid_constant__ GatedSaved saved, unsigned* status) {
-  gated_body<kGbForward, ACT, SAVE, GatedCfg<SAVE ? 3 : 1, SAVE>>(p, p, false, 0, saved, status);
+  gated_body<kGbForward, ACT, SAVE, GatedCfg<1>>(p, p, false, 0, saved, status);
 }
 __global__ void __launch_bounds__(kGbThreads, 1)
 gated_bwd_kernel(const __grid_constant__ GatedProblem one, const __grid_constant__ GatedProblem two, int both, int rounds, unsigned* status) {
-  gated_body<kGbData, 0, false, GatedCfg<2, false>>(one, two, both != 0, rounds, GatedSaved{}, status);
+  gated_body<kGbData, 0, false, GatedCfg<2>>(one, two, both != 0, rounds, GatedSaved{}, status);
+}
+
+// ---- few tokens ----------------------------------------------------------------------------------------------------
+
+// Up to 128 tokens without anything kept: bound by the pass over the weights, so the tiles are made for that.  A block has 64 columns of h (128
+// of the accumulator: the gate's, then the up-projection's) and one row tile, two blocks run on an SM, and where there are fewer tiles than
+// places for them the contraction is cut into up to eight ranges, a cluster's blocks one each: their partial sums meet in shared memory,
+// in the order of the ranges.  (All places busy at once is what counts: 1 x 4096 -> 11008 has 86 tiles of 128 columns for 74 pairs, 55 us there.)
+// Warps 0-3 epilogue, 4 TMA producer, 5 MMA issuer.
+constexpr int kGfRows = 128, kGfThreads = 192, kGfCols = 64, kGfPitch = 2 * kGfCols + 4;      // pitch of a row of partial sums, floats
+template <int BOXES>                            // boxes of 64 rows of x
+struct FewCfg {
+  static constexpr int stage_bytes = (BOXES + 2) * kGbBox;
+  static constexpr int stages = BOXES == 1 ? 4 : 3;
+  static constexpr int smem_bytes = stages * stage_bytes;
+  static_assert(2 * (smem_bytes + 1024 + 1024) <= 228 * 1024, "two blocks on an SM");
+  static_assert(64 * BOXES * kGfPitch * 4 <= smem_bytes, "partial sums fit where the operands were");
+};
+
+struct GatedFew {
+  CUtensorMap x, gate, up;
+  __nv_bfloat16* h;
+  int rows, inner, blocks;                      // blocks: stages of the whole contraction
+};
+
+__device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ float4 lds_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int ACT, int BOXES>
+__global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_constant__ GatedFew p, unsigned* status) {
+  using C = FewCfg<BOXES>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(16) uint64_t ctl_bars[2 * C::stages + 1];
+  __shared__ uint32_t ctl_tmem_ptr;
+  __shared__ int ctl_abort;
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t full0 = smem_u32(ctl_bars), empty0 = full0 + 8u * C::stages, done_bar = empty0 + 8u * C::stages;
+  volatile uint32_t* tmem_ptr_smem = &ctl_tmem_ptr;
+  volatile int* abort_flag = &ctl_abort;
+  if ((sbase & 1023u) != 0) {   // the swizzled layouts need this alignment (all blocks have the same layout)
+    if (threadIdx.x == 0 && status != nullptr) atomicCAS(status, 0u, 6u);
+    return;
+  }
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  uint32_t ranges;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranges));
+  const uint32_t rank = cluster_rank();
+  const int n0 = int(blockIdx.x / ranges) * kGfCols;
+  const int first = int(uint64_t(p.blocks) * rank / ranges), last = int(uint64_t(p.blocks) * (rank + 1) / ranges);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::stages; ++s) {
+      mbar_init(full0 + 8u * s, 1);
+      mbar_init(empty0 + 8u * s, 1);
+    }
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 5) {
+    tmem_take(smem_u32(&ctl_tmem_ptr), 2 * kGfCols);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_ptr_smem;
+  grid_trigger();
+  grid_wait();
+
+  if (warp == 4) {
+    uint32_t s = 0, ph = 1;
+    for (int kb = first; kb < last; ++kb) {
+      if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, ph, abort_flag, status, 1u))) break;
+      if (elect_one()) {
+        const uint32_t dst = sbase + s * C::stage_bytes, fb = full0 + 8u * s;
+        mbar_expect_tx(fb, C::stage_bytes);
+        tma_load_2d(dst + BOXES * kGbBox, &p.gate, fb, n0, kb * kGbK);
+        tma_load_2d(dst + (BOXES + 1) * kGbBox, &p.up, fb, n0, kb * kGbK);
+#pragma unroll
+        for (int i = 0; i < BOXES; ++i) tma_load_2d(dst + i * kGbBox, &p.x, fb, kb * kGbK, 64 * i);
+      }
+      __syncwarp();
+      if (++s == C::stages) { s = 0; ph ^= 1u; }
+    }
+  } else if (warp == 5) {
+    // A K-major (with one box, rows 64.. of the tile are whatever lies behind it: rows of the result that nobody reads), B MN-major
+    const uint64_t desc_a0 = gated_desc(sbase), desc_b0 = gated_desc(sbase + BOXES * kGbBox);
+    const uint32_t desc_hi = uint32_t(desc_a0 >> 32), a_lo0 = uint32_t(desc_a0), b_lo0 = uint32_t(desc_b0);
+    const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(2 * kGfCols >> 3) << 17) | (uint32_t(kGfRows >> 4) << 24);
+    uint32_t s = 0, ph = 0;
+    for (int kb = first; kb < last; ++kb) {
+      if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8u * s, ph, abort_flag, status, 3u))) break;
+      __syncwarp();
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t soff = s * uint32_t(C::stage_bytes >> 4);
+#pragma unroll
+        for (int k = 0; k < kGbK / 16; ++k)
+          umma_bf16(tmem_base, (uint64_t(desc_hi) << 32) | (a_lo0 + soff + k * 2u), (uint64_t(desc_hi) << 32) | (b_lo0 + soff + k * 128u), idesc,
+                    kb > first || k > 0 ? 1u : 0u);
+        umma_commit(empty0 + 8u * s);
+      }
+      __syncwarp();
+      if (++s == C::stages) { s = 0; ph ^= 1u; }
+    }
+    // (after a wait that gave up too: nothing issued here may still be running when tensor memory is freed)
+    if (elect_one()) umma_commit(done_bar);
+    __syncwarp();
+  }
+  // every warp: the products are done, and with them the last look at the operands' shared memory
+  const bool ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0u, abort_flag, status, 5u)) && !*abort_flag;
+  __syncwarp();
+  tc_fence_after();
+  if (warp < 4 && ok && warp * 32 < p.rows) {
+    const uint32_t at = tmem_base + (uint32_t(warp * 32) << 16);
+    const int row = warp * 32 + lane;
+    uint32_t g0[32], g1[32], u0[32], u1[32];
+    tmem_ld32(at, g0);
+    tmem_ld32(at + 32u, g1);
+    tmem_ld32(at + 64u, u0);
+    tmem_ld32(at + 96u, u1);
+    tmem_wait_ld(g0);
+    tmem_wait_ld(g1);
+    tmem_wait_ld(u0);
+    tmem_wait_ld(u1);
+    if (row < p.rows) {
+      if (ranges == 1) {
+        __nv_bfloat16* to = p.h + int64_t(row) * p.inner + n0;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = 8 * (c & 3) + 2 * j;
+            const uint32_t(&g)[32] = c < 4 ? g0 : g1;
+            const uint32_t(&u)[32] = c < 4 ? u0 : u1;
+            o[j] = pack_bf16x2(gated_act<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]), gated_act<ACT>(__uint_as_float(g[i + 1])) * __uint_as_float(u[i + 1]));
+          }
+          if (n0 + 8 * c < p.inner) *reinterpret_cast<uint4*>(to + 8 * c) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      } else {
+        const uint32_t to = sbase + uint32_t(row) * (kGfPitch * 4);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const uint32_t(&v)[32] = c < 8 ? g0 : c < 16 ? g1 : c < 24 ? u0 : u1;
+          sts128(to + 16u * c, make_uint4(v[4 * (c & 7)], v[4 * (c & 7) + 1], v[4 * (c & 7) + 2], v[4 * (c & 7) + 3]));
+        }
+      }
+    }
+  }
+  if (ranges > 1) {
+    __syncwarp();
+    cluster_sync();                              // the partial sums are there
+    const int each = kGfCols / int(ranges), quads = each / 4;      // columns of this block's share, in fours
+    const int all_ok = ok;
+    for (int e = threadIdx.x; all_ok && e < p.rows * quads; e += kGfThreads) {
+      const int row = e / quads, col = int(rank) * each + 4 * (e - row * quads);
+      if (n0 + col >= p.inner) continue;
+      const uint32_t from = sbase + uint32_t(row * kGfPitch + col) * 4u;
+      float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
+      for (uint32_t r = 0; r < ranges; ++r) {
+        const uint32_t peer = map_rank(from, r);
+        const float4 a = lds_cluster(peer), b = lds_cluster(peer + 4u * kGfCols);
+        g = make_float4(g.x + a.x, g.y + a.y, g.z + a.z, g.w + a.w);
+        u = make_float4(u.x + b.x, u.y + b.y, u.z + b.z, u.w + b.w);
+      }
+      *reinterpret_cast<uint2*>(p.h + int64_t(row) * p.inner + n0 + col) =
+          make_uint2(pack_bf16x2(gated_act<ACT>(g.x) * u.x, gated_act<ACT>(g.y) * u.y), pack_bf16x2(gated_act<ACT>(g.z) * u.z, gated_act<ACT>(g.w) * u.w));
+    }
+    __syncwarp();
+    cluster_sync();                              // the partners have read this block's sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * kGfCols);
+  }
 }
 
 // ---- dG and dU -----------------------------------------------------------------------------------------------------
@@ -451,7 +649,7 @@ struct GatedSlopes {
   int64_t rows;
   int inner, chunks;
 };
-constexpr int kGsThreads = 256, kGsRows = kGsThreads / 8, kGsUnroll = 2;
+constexpr int kGsThreads = 128, kGsRows = kGsThreads / 8, kGsUnroll = 4;
 
 // A block takes 64 columns of 32 rows at a time, eight lanes a row: a row's 128 bytes of each tensor are one request, and its
 // exponents one of a few in the same sector.
@@ -460,16 +658,15 @@ __global__ void __launch_bounds__(kGsThreads) gated_slopes_kernel(const GatedSlo
   grid_trigger();
   grid_wait();
   const int lane8 = threadIdx.x & 7, r0 = threadIdx.x >> 3;
-  const int64_t groups = (p.rows + kGsRows * kGsUnroll - 1) / (kGsRows * kGsUnroll), items = groups * p.chunks;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t group = item / p.chunks;
-    const int chunk = int(item - group * p.chunks), col = chunk * 64 + lane8 * 8;
+  {
+    const uint32_t group = blockIdx.x / uint32_t(p.chunks);
+    const int chunk = int(blockIdx.x - group * uint32_t(p.chunks)), col = chunk * 64 + lane8 * 8;
     uint4 g[kGsUnroll], a[kGsUnroll], u[kGsUnroll];
     uint32_t e[kGsUnroll];
     int64_t row[kGsUnroll];
 #pragma unroll
     for (int k = 0; k < kGsUnroll; ++k) {
-      row[k] = (group * kGsUnroll + k) * kGsRows + r0;
+      row[k] = (int64_t(group) * kGsUnroll + k) * kGsRows + r0;
       if (col >= p.inner || row[k] >= p.rows) row[k] = -1;
       if (row[k] < 0) continue;
       const int64_t at = row[k] * p.inner + col;
@@ -558,12 +755,38 @@ static bool gated_aligned(const tg_gated_args* a) {
 }
 static int64_t gated_chunks(int64_t inner) { return (inner + 63) / 64; }
 
+template <int ACT, int BOXES>
+static int launch_few(const GatedFew& p, int tiles, int ranges, unsigned* status, cudaStream_t st) {
+  static std::atomic<bool> done[64];
+  using C = FewCfg<BOXES>;
+  if (int rc = allow_smem(gated_few_kernel<ACT, BOXES>, C::smem_bytes, done)) return rc;
+  TG_CUDA_CHECK(launch_early_clusters(gated_few_kernel<ACT, BOXES>, ranges, tiles * ranges, kGfThreads, C::smem_bytes, st, p, status));
+  return TG_OK;
+}
+static int run_gated_few(const tg_gated_args* a, cudaStream_t st) {
+  GatedFew p = {};
+  if (int rc = gated_map(&p.x, a->x, false, a->rows, a->cols, a->ldx, 64)) return rc;
+  if (int rc = gated_map(&p.gate, a->w_gate, false, a->cols, a->inner, a->ld_gate, 64)) return rc;
+  if (int rc = gated_map(&p.up, a->w_up, false, a->cols, a->inner, a->ld_up, 64)) return rc;
+  p.h = static_cast<__nv_bfloat16*>(a->h);
+  p.rows = int(a->rows);
+  p.inner = int(a->inner);
+  p.blocks = int((a->cols + kGbK - 1) / kGbK);
+  const int tiles = int((a->inner + kGfCols - 1) / kGfCols);
+  int ranges = 1;                                // as many as find a place at once, of four stages at least
+  while (ranges < 8 && tiles * ranges * 2 <= 2 * sm_count() && p.blocks >= 8 * ranges) ranges *= 2;
+  const bool one = a->rows <= 64;
+  if (a->act == TG_GATED_SILU) return one ? launch_few<TG_GATED_SILU, 1>(p, tiles, ranges, a->status, st) : launch_few<TG_GATED_SILU, 2>(p, tiles, ranges, a->status, st);
+  if (a->act == TG_GATED_GELU) return one ? launch_few<TG_GATED_GELU, 1>(p, tiles, ranges, a->status, st) : launch_few<TG_GATED_GELU, 2>(p, tiles, ranges, a->status, st);
+  return one ? launch_few<TG_GATED_RELU, 1>(p, tiles, ranges, a->status, st) : launch_few<TG_GATED_RELU, 2>(p, tiles, ranges, a->status, st);
+}
+
 template <int ACT, bool SAVE>
 static int run_gated_fwd(const GatedProblem& p, const GatedSaved& s, unsigned* status, cudaStream_t st) {
   static std::atomic<int> units_of[64];
   const int64_t items = int64_t(p.tiles_m) * p.tiles_n;
   int units = 0;
-  return launch_gated(gated_fwd_kernel<ACT, SAVE>, GatedCfg<SAVE ? 3 : 1, SAVE>::smem_bytes, units_of, items, items <= 4 * gemm_pairs() && p.blocks <= 64, st,
+  return launch_gated(gated_fwd_kernel<ACT, SAVE>, GatedCfg<1>::smem_bytes, units_of, items, items <= 4 * gemm_pairs() && p.blocks <= 64, st,
                       units, p, s, status);
 }
 template <bool SAVE>
@@ -590,6 +813,7 @@ extern "C" int tg_gated_linear_fwd(const tg_gated_args* a, void* stream) {
   if (!gated_aligned(a) || !aligned16(a->h) || !aligned16(a->saved_gate) || !aligned16(a->saved_up) || !aligned16(a->saved_exponents)) return TG_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
   const int64_t M = a->rows, D = a->cols, F = a->inner;
+  if (!save && M <= kGfRows) return run_gated_few(a, static_cast<cudaStream_t>(stream));
   GatedProblem p = {};
   GatedSaved s = {};
   if (int rc = gated_map(&p.a[0], a->x, false, M, D, a->ldx, 64)) return rc;
@@ -647,7 +871,7 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
   s.chunks = int(gated_chunks(F));
   const int64_t items = (M + kGsRows * kGsUnroll - 1) / (kGsRows * kGsUnroll) * s.chunks;
   auto kern = a->act == TG_GATED_SILU ? gated_slopes_kernel<TG_GATED_SILU> : a->act == TG_GATED_GELU ? gated_slopes_kernel<TG_GATED_GELU> : gated_slopes_kernel<TG_GATED_RELU>;
-  TG_CUDA_CHECK(launch_if_short(items <= 8 * sm_count(), kern, dim3(unsigned(std::min<int64_t>(items, int64_t(sm_count()) * 6))), kGsThreads, 0, st, s));
+  TG_CUDA_CHECK(launch_if_short(items <= 8 * sm_count(), kern, dim3(unsigned(items)), kGsThreads, 0, st, s));
 
   GatedProblem data = {}, weights = {};
   if (dx) {
@@ -678,7 +902,7 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
   const GatedProblem &one = data_first ? data : weights, &two = data_first ? weights : data;
   const int64_t n1 = int64_t(one.tiles_m) * one.tiles_n, n2 = both ? int64_t(two.tiles_m) * two.tiles_n : 0;
   static std::atomic<int> units_of[64];
-  using C = GatedCfg<2, false>;
+  using C = GatedCfg<2>;
   int units = 0, rounds = 0;
   if (int rc = launch_gated(gated_bwd_kernel, C::smem_bytes, units_of, n1 + n2, false, st, units)) return rc;
   if (both) two_problems_us(n1, double(one.blocks) + 3.0, n2, double(two.blocks) + 3.0, units, rounds);
