@@ -456,21 +456,20 @@ gated_bwd_kernel(const __grid_constant__ GatedProblem one, const __grid_constant
 // of the accumulator: the gate's, then the up-projection's) and one row tile, two blocks run on an SM, and where there are fewer tiles than
 // places for them the contraction is cut into up to eight ranges, a cluster's blocks one each: their partial sums meet in shared memory,
 // in the order of the ranges.  (All places busy at once is what counts: 1 x 4096 -> 11008 has 86 tiles of 128 columns for 74 pairs, 55 us there.)
+// A stage holds no more rows of x than there are, in boxes of eight at least: rows of a box that lie outside the tensor are not free
+// (1 x 4096 -> 11008 29.4 us, in boxes of 64 44.8), and more than four stages measured slower (16 x 8192 -> 8192 41.8, six 45.1).
+// 1, 16 and 128 x 8192 -> 8192 41.5, 41.8 and 46.8 us (6.5, 6.4 and 5.7 TB/s of weights).
 // Warps 0-3 epilogue, 4 TMA producer, 5 MMA issuer.
 constexpr int kGfRows = 128, kGfThreads = 192, kGfCols = 64, kGfPitch = 2 * kGfCols + 4;      // pitch of a row of partial sums, floats
-template <int BOXES>                            // boxes of 64 rows of x
-struct FewCfg {
-  static constexpr int stage_bytes = (BOXES + 2) * kGbBox;
-  static constexpr int stages = BOXES == 1 ? 4 : 3;
-  static constexpr int smem_bytes = stages * stage_bytes;
-  static_assert(2 * (smem_bytes + 1024 + 1024) <= 228 * 1024, "two blocks on an SM");
-  static_assert(64 * BOXES * kGfPitch * 4 <= smem_bytes, "partial sums fit where the operands were");
-};
+constexpr int kGfStages = 4, kGfMost = 110 * 1024;      // at most; shared memory of a block, two of which an SM has room for
+static_assert(2 * (kGfMost + 2048) <= 228 * 1024, "two blocks on an SM");
 
 struct GatedFew {
-  CUtensorMap x, gate, up;
+  CUtensorMap x, gate, up;                      // boxes of x_rows x 64, 64 x 64
   __nv_bfloat16* h;
   int rows, inner, blocks;                      // blocks: stages of the whole contraction
+  int stages;                                   // of the ring
+  int x_rows, x_boxes;                          // rows of x in a stage: boxes of a multiple of eight rows
 };
 
 __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -487,15 +486,41 @@ __device__ __forceinline__ float4 lds_cluster(uint32_t addr) {
   return v;
 }
 
-template <int ACT, int BOXES>
+// This block's share of the columns: the ranges' partial sums, all on their way at once and added up in order, then h.
+template <int ACT, int RANGES>
+__device__ __forceinline__ void few_join(const GatedFew& p, uint32_t sums, uint32_t rank, int n0) {
+  constexpr int kQuads = kGfCols / RANGES / 4;      // columns in fours
+  for (int e = threadIdx.x; e < p.rows * kQuads; e += kGfThreads) {
+    const int row = e / kQuads, col = int(rank) * 4 * kQuads + 4 * (e - row * kQuads);
+    if (n0 + col >= p.inner) continue;
+    const uint32_t from = sums + uint32_t(row * kGfPitch + col) * 4u;
+    float4 a[RANGES], b[RANGES];
+#pragma unroll
+    for (uint32_t r = 0; r < RANGES; ++r) {
+      const uint32_t peer = map_rank(from, r);
+      a[r] = lds_cluster(peer);
+      b[r] = lds_cluster(peer + 4u * kGfCols);
+    }
+    float4 g = a[0], u = b[0];
+#pragma unroll
+    for (int r = 1; r < RANGES; ++r) {
+      g = make_float4(g.x + a[r].x, g.y + a[r].y, g.z + a[r].z, g.w + a[r].w);
+      u = make_float4(u.x + b[r].x, u.y + b[r].y, u.z + b[r].z, u.w + b[r].w);
+    }
+    *reinterpret_cast<uint2*>(p.h + int64_t(row) * p.inner + n0 + col) =
+        make_uint2(pack_bf16x2(gated_act<ACT>(g.x) * u.x, gated_act<ACT>(g.y) * u.y), pack_bf16x2(gated_act<ACT>(g.z) * u.z, gated_act<ACT>(g.w) * u.w));
+  }
+}
+
+template <int ACT>
 __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_constant__ GatedFew p, unsigned* status) {
-  using C = FewCfg<BOXES>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ __align__(16) uint64_t ctl_bars[2 * C::stages + 1];
+  __shared__ __align__(16) uint64_t ctl_bars[2 * kGfStages + 1];
   __shared__ uint32_t ctl_tmem_ptr;
   __shared__ int ctl_abort;
   const uint32_t sbase = smem_u32(smem);
-  const uint32_t full0 = smem_u32(ctl_bars), empty0 = full0 + 8u * C::stages, done_bar = empty0 + 8u * C::stages;
+  const uint32_t full0 = smem_u32(ctl_bars), empty0 = full0 + 8u * kGfStages, done_bar = empty0 + 8u * kGfStages;
+  const uint32_t x_bytes = uint32_t(p.x_rows * p.x_boxes) * 128u, stage_bytes = x_bytes + 2 * kGbBox;
   volatile uint32_t* tmem_ptr_smem = &ctl_tmem_ptr;
   volatile int* abort_flag = &ctl_abort;
   if ((sbase & 1023u) != 0) {   // the swizzled layouts need this alignment (all blocks have the same layout)
@@ -509,7 +534,7 @@ __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_c
   const int n0 = int(blockIdx.x / ranges) * kGfCols;
   const int first = int(uint64_t(p.blocks) * rank / ranges), last = int(uint64_t(p.blocks) * (rank + 1) / ranges);
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::stages; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       mbar_init(full0 + 8u * s, 1);
       mbar_init(empty0 + 8u * s, 1);
     }
@@ -532,19 +557,18 @@ __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_c
     for (int kb = first; kb < last; ++kb) {
       if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, ph, abort_flag, status, 1u))) break;
       if (elect_one()) {
-        const uint32_t dst = sbase + s * C::stage_bytes, fb = full0 + 8u * s;
-        mbar_expect_tx(fb, C::stage_bytes);
-        tma_load_2d(dst + BOXES * kGbBox, &p.gate, fb, n0, kb * kGbK);
-        tma_load_2d(dst + (BOXES + 1) * kGbBox, &p.up, fb, n0, kb * kGbK);
-#pragma unroll
-        for (int i = 0; i < BOXES; ++i) tma_load_2d(dst + i * kGbBox, &p.x, fb, kb * kGbK, 64 * i);
+        const uint32_t dst = sbase + s * stage_bytes, fb = full0 + 8u * s;
+        mbar_expect_tx(fb, stage_bytes);
+        tma_load_2d(dst + x_bytes, &p.gate, fb, n0, kb * kGbK);
+        tma_load_2d(dst + x_bytes + kGbBox, &p.up, fb, n0, kb * kGbK);
+        for (int i = 0; i < p.x_boxes; ++i) tma_load_2d(dst + i * kGbBox, &p.x, fb, kb * kGbK, 64 * i);
       }
       __syncwarp();
-      if (++s == C::stages) { s = 0; ph ^= 1u; }
+      if (++s == uint32_t(p.stages)) { s = 0; ph ^= 1u; }
     }
   } else if (warp == 5) {
-    // A K-major (with one box, rows 64.. of the tile are whatever lies behind it: rows of the result that nobody reads), B MN-major
-    const uint64_t desc_a0 = gated_desc(sbase), desc_b0 = gated_desc(sbase + BOXES * kGbBox);
+    // A K-major (rows of the tile beyond those of x are whatever lies behind them in the stage: rows of the result that nobody reads), B MN-major
+    const uint64_t desc_a0 = gated_desc(sbase), desc_b0 = gated_desc(sbase + x_bytes);
     const uint32_t desc_hi = uint32_t(desc_a0 >> 32), a_lo0 = uint32_t(desc_a0), b_lo0 = uint32_t(desc_b0);
     const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(2 * kGfCols >> 3) << 17) | (uint32_t(kGfRows >> 4) << 24);
     uint32_t s = 0, ph = 0;
@@ -553,7 +577,7 @@ __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_c
       __syncwarp();
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t soff = s * uint32_t(C::stage_bytes >> 4);
+        const uint32_t soff = s * (stage_bytes >> 4);
 #pragma unroll
         for (int k = 0; k < kGbK / 16; ++k)
           umma_bf16(tmem_base, (uint64_t(desc_hi) << 32) | (a_lo0 + soff + k * 2u), (uint64_t(desc_hi) << 32) | (b_lo0 + soff + k * 128u), idesc,
@@ -561,7 +585,7 @@ __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_c
         umma_commit(empty0 + 8u * s);
       }
       __syncwarp();
-      if (++s == C::stages) { s = 0; ph ^= 1u; }
+      if (++s == uint32_t(p.stages)) { s = 0; ph ^= 1u; }
     }
     // (after a wait that gave up too: nothing issued here may still be running when tensor memory is freed)
     if (elect_one()) umma_commit(done_bar);
@@ -611,21 +635,10 @@ __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_c
   if (ranges > 1) {
     __syncwarp();
     cluster_sync();                              // the partial sums are there
-    const int each = kGfCols / int(ranges), quads = each / 4;      // columns of this block's share, in fours
-    const int all_ok = ok;
-    for (int e = threadIdx.x; all_ok && e < p.rows * quads; e += kGfThreads) {
-      const int row = e / quads, col = int(rank) * each + 4 * (e - row * quads);
-      if (n0 + col >= p.inner) continue;
-      const uint32_t from = sbase + uint32_t(row * kGfPitch + col) * 4u;
-      float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
-      for (uint32_t r = 0; r < ranges; ++r) {
-        const uint32_t peer = map_rank(from, r);
-        const float4 a = lds_cluster(peer), b = lds_cluster(peer + 4u * kGfCols);
-        g = make_float4(g.x + a.x, g.y + a.y, g.z + a.z, g.w + a.w);
-        u = make_float4(u.x + b.x, u.y + b.y, u.z + b.z, u.w + b.w);
-      }
-      *reinterpret_cast<uint2*>(p.h + int64_t(row) * p.inner + n0 + col) =
-          make_uint2(pack_bf16x2(gated_act<ACT>(g.x) * u.x, gated_act<ACT>(g.y) * u.y), pack_bf16x2(gated_act<ACT>(g.z) * u.z, gated_act<ACT>(g.w) * u.w));
+    if (ok) {
+      if (ranges == 2) few_join<ACT, 2>(p, sbase, rank, n0);
+      else if (ranges == 4) few_join<ACT, 4>(p, sbase, rank, n0);
+      else few_join<ACT, 8>(p, sbase, rank, n0);
     }
     __syncwarp();
     cluster_sync();                              // the partners have read this block's sums
@@ -755,17 +768,18 @@ static bool gated_aligned(const tg_gated_args* a) {
 }
 static int64_t gated_chunks(int64_t inner) { return (inner + 63) / 64; }
 
-template <int ACT, int BOXES>
-static int launch_few(const GatedFew& p, int tiles, int ranges, unsigned* status, cudaStream_t st) {
+template <int ACT>
+static int launch_few(const GatedFew& p, int tiles, int ranges, int smem, unsigned* status, cudaStream_t st) {
   static std::atomic<bool> done[64];
-  using C = FewCfg<BOXES>;
-  if (int rc = allow_smem(gated_few_kernel<ACT, BOXES>, C::smem_bytes, done)) return rc;
-  TG_CUDA_CHECK(launch_early_clusters(gated_few_kernel<ACT, BOXES>, ranges, tiles * ranges, kGfThreads, C::smem_bytes, st, p, status));
+  if (int rc = allow_smem(gated_few_kernel<ACT>, kGfMost, done)) return rc;
+  TG_CUDA_CHECK(launch_early_clusters(gated_few_kernel<ACT>, ranges, tiles * ranges, kGfThreads, smem, st, p, status));
   return TG_OK;
 }
 static int run_gated_few(const tg_gated_args* a, cudaStream_t st) {
   GatedFew p = {};
-  if (int rc = gated_map(&p.x, a->x, false, a->rows, a->cols, a->ldx, 64)) return rc;
+  p.x_rows = std::min(64, pow2_at_least(int(std::max<int64_t>(a->rows, 8))));
+  p.x_boxes = a->rows > 64 ? 2 : 1;
+  if (int rc = gated_map(&p.x, a->x, false, a->rows, a->cols, a->ldx, p.x_rows)) return rc;
   if (int rc = gated_map(&p.gate, a->w_gate, false, a->cols, a->inner, a->ld_gate, 64)) return rc;
   if (int rc = gated_map(&p.up, a->w_up, false, a->cols, a->inner, a->ld_up, 64)) return rc;
   p.h = static_cast<__nv_bfloat16*>(a->h);
@@ -773,12 +787,17 @@ static int run_gated_few(const tg_gated_args* a, cudaStream_t st) {
   p.inner = int(a->inner);
   p.blocks = int((a->cols + kGbK - 1) / kGbK);
   const int tiles = int((a->inner + kGfCols - 1) / kGfCols);
-  int ranges = 1;                                // as many as find a place at once, of four stages at least
-  while (ranges < 8 && tiles * ranges * 2 <= 2 * sm_count() && p.blocks >= 8 * ranges) ranges *= 2;
-  const bool one = a->rows <= 64;
-  if (a->act == TG_GATED_SILU) return one ? launch_few<TG_GATED_SILU, 1>(p, tiles, ranges, a->status, st) : launch_few<TG_GATED_SILU, 2>(p, tiles, ranges, a->status, st);
-  if (a->act == TG_GATED_GELU) return one ? launch_few<TG_GATED_GELU, 1>(p, tiles, ranges, a->status, st) : launch_few<TG_GATED_GELU, 2>(p, tiles, ranges, a->status, st);
-  return one ? launch_few<TG_GATED_RELU, 1>(p, tiles, ranges, a->status, st) : launch_few<TG_GATED_RELU, 2>(p, tiles, ranges, a->status, st);
+  // As many ranges as find a place at once, of four stages at least and of one per eight tokens, whose sums take their time to meet: 128 x 1024 -> 4096
+  // 10.5 us in one range, 12.5 in four; 128 x 4096 -> 4096 28.7 and 19.9; 16 x 1024 -> 4096 6.9 in four.
+  int ranges = 1;
+  while (ranges < 8 && tiles * ranges * 2 <= 2 * sm_count() && p.blocks >= 8 * ranges && 8 * (p.blocks / (2 * ranges)) >= a->rows) ranges *= 2;
+  const int stage = p.x_rows * p.x_boxes * 128 + 2 * kGbBox;
+  p.stages = std::min(kGfStages, kGfMost / stage);
+  const int smem = std::max(p.stages * stage, ranges > 1 ? int(a->rows) * kGfPitch * 4 : 0);
+  static_assert(kGfRows * kGfPitch * 4 <= kGfMost, "partial sums fit where the operands were");
+  if (a->act == TG_GATED_SILU) return launch_few<TG_GATED_SILU>(p, tiles, ranges, smem, a->status, st);
+  if (a->act == TG_GATED_GELU) return launch_few<TG_GATED_GELU>(p, tiles, ranges, smem, a->status, st);
+  return launch_few<TG_GATED_RELU>(p, tiles, ranges, smem, a->status, st);
 }
 
 template <int ACT, bool SAVE>
