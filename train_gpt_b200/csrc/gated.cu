@@ -145,17 +145,20 @@ struct GatedCfg {
   static_assert(stages >= 4 && smem_bytes + 1024 <= kSmemLimit, "shared-memory plan");
 };
 
+// The exponent of the power of two by which a row's 64 values are scaled down to fit fp16, from the bits of the largest magnitude: 0 up to 65504,
+// else what puts it below 2^15 (infinities and NaN count as 2^128).
+__device__ __forceinline__ uint32_t save_exponent(uint32_t m, float& scale) {
+  const uint32_t e = m >= 0x477fe000u ? (m >> 23) - 127u - 14u : 0u;
+  scale = __uint_as_float((127u - e) << 23);
+  return e;
+}
 // f16 of 64 accumulator values, scaled down by the power of two that keeps the largest (finite) one in range; returns its exponent
 __device__ __forceinline__ uint32_t save_row(const uint32_t (&v0)[32], const uint32_t (&v1)[32], uint32_t row, int lane) {
   uint32_t m = 0u;
 #pragma unroll
   for (int j = 0; j < 32; ++j) m = max_magnitude(max_magnitude(m, v0[j]), v1[j]);
-  uint32_t e = 0u;
-  float scale = 1.f;
-  if (m >= 0x477fe000u) {                       // 65504: the exponent that puts the largest below 2^15 (infinities and NaN: as 2^128)
-    e = min(m >> 23, 255u) - 127u - 14u;
-    scale = __uint_as_float((127u - e) << 23);
-  }
+  float scale;
+  const uint32_t e = save_exponent(m, scale);
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
     uint32_t o[4];
@@ -452,10 +455,10 @@ gated_bwd_kernel(const __grid_constant__ GatedProblem one, const __grid_constant
 
 // ---- few tokens ----------------------------------------------------------------------------------------------------
 
-// Up to 128 tokens without anything kept: bound by the pass over the weights, so the tiles are made for that.  A block has 64 columns of h (128
+// Up to 128 tokens: bound by the pass over the weights, so the tiles are made for that.  A block has 64 columns of h (128
 // of the accumulator: the gate's, then the up-projection's) and one row tile, two blocks run on an SM, and where there are fewer tiles than
 // places for them the contraction is cut into up to eight ranges, a cluster's blocks one each: their partial sums meet in shared memory,
-// in the order of the ranges.  (All places busy at once is what counts: 1 x 4096 -> 11008 has 86 tiles of 128 columns for 74 pairs, 55 us there.)
+// in the order of the ranges, and the blocks share the rows out.  (All places busy at once is what counts: 1 x 4096 -> 11008 has 86 tiles of 128 columns for 74 pairs, 55 us there.)
 // A stage holds no more rows of x than there are, in boxes of eight at least: rows of a box that lie outside the tensor are not free
 // (1 x 4096 -> 11008 29.4 us, in boxes of 64 44.8), and more than four stages measured slower (16 x 8192 -> 8192 41.8, six 45.1).
 // 1, 16 and 128 x 8192 -> 8192 41.5, 41.8 and 46.8 us (6.5, 6.4 and 5.7 TB/s of weights).
@@ -467,6 +470,8 @@ static_assert(2 * (kGfMost + 2048) <= 228 * 1024, "two blocks on an SM");
 struct GatedFew {
   CUtensorMap x, gate, up;                      // boxes of x_rows x 64, 64 x 64
   __nv_bfloat16* h;
+  __half *saved_gate, *saved_up;
+  uint8_t* exponents;
   int rows, inner, blocks;                      // blocks: stages of the whole contraction
   int stages;                                   // of the ring
   int x_rows, x_boxes;                          // rows of x in a stage: boxes of a multiple of eight rows
@@ -486,33 +491,55 @@ __device__ __forceinline__ float4 lds_cluster(uint32_t addr) {
   return v;
 }
 
-// This block's share of the columns: the ranges' partial sums, all on their way at once and added up in order, then h.
-template <int ACT, int RANGES>
+// This block's share of the rows, sixteen lanes each: the ranges' partial sums, all on their way at once and added up in order, then h and
+// what the backward pass needs.
+template <int ACT, bool SAVE, int RANGES>
 __device__ __forceinline__ void few_join(const GatedFew& p, uint32_t sums, uint32_t rank, int n0) {
-  constexpr int kQuads = kGfCols / RANGES / 4;      // columns in fours
-  for (int e = threadIdx.x; e < p.rows * kQuads; e += kGfThreads) {
-    const int row = e / kQuads, col = int(rank) * 4 * kQuads + 4 * (e - row * kQuads);
-    if (n0 + col >= p.inner) continue;
-    const uint32_t from = sums + uint32_t(row * kGfPitch + col) * 4u;
-    float4 a[RANGES], b[RANGES];
+  const int lane = threadIdx.x & 31, col = 4 * (lane & 15);
+  for (int i = 2 * int(threadIdx.x >> 5); i * RANGES < p.rows; i += 2 * kGfThreads / 32) {
+    const int row = (i + (lane >> 4)) * RANGES + int(rank);
+    const bool there = row < p.rows;
+    float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
+    if (there) {
+      const uint32_t from = sums + uint32_t(row * kGfPitch + col) * 4u;
+      float4 a[RANGES], b[RANGES];
 #pragma unroll
-    for (uint32_t r = 0; r < RANGES; ++r) {
-      const uint32_t peer = map_rank(from, r);
-      a[r] = lds_cluster(peer);
-      b[r] = lds_cluster(peer + 4u * kGfCols);
-    }
-    float4 g = a[0], u = b[0];
+      for (uint32_t r = 0; r < RANGES; ++r) {
+        const uint32_t peer = map_rank(from, r);
+        a[r] = lds_cluster(peer);
+        b[r] = lds_cluster(peer + 4u * kGfCols);
+      }
+      g = a[0];
+      u = b[0];
 #pragma unroll
-    for (int r = 1; r < RANGES; ++r) {
-      g = make_float4(g.x + a[r].x, g.y + a[r].y, g.z + a[r].z, g.w + a[r].w);
-      u = make_float4(u.x + b[r].x, u.y + b[r].y, u.z + b[r].z, u.w + b[r].w);
+      for (int r = 1; r < RANGES; ++r) {
+        g = make_float4(g.x + a[r].x, g.y + a[r].y, g.z + a[r].z, g.w + a[r].w);
+        u = make_float4(u.x + b[r].x, u.y + b[r].y, u.z + b[r].z, u.w + b[r].w);
+      }
     }
-    *reinterpret_cast<uint2*>(p.h + int64_t(row) * p.inner + n0 + col) =
-        make_uint2(pack_bf16x2(gated_act<ACT>(g.x) * u.x, gated_act<ACT>(g.y) * u.y), pack_bf16x2(gated_act<ACT>(g.z) * u.z, gated_act<ACT>(g.w) * u.w));
+    const bool stores = there && n0 + col < p.inner;
+    const int64_t at = int64_t(row) * p.inner + n0 + col;
+    if constexpr (SAVE) {
+      uint32_t e[2];
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const float4 v = which ? u : g;
+        uint32_t m = max_magnitude(max_magnitude(max_magnitude(max_magnitude(0u, __float_as_uint(v.x)), __float_as_uint(v.y)), __float_as_uint(v.z)), __float_as_uint(v.w));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        float scale;
+        e[which] = save_exponent(m, scale);
+        if (stores) *reinterpret_cast<uint2*>((which ? p.saved_up : p.saved_gate) + at) = make_uint2(pack_f16x2(v.x * scale, v.y * scale), pack_f16x2(v.z * scale, v.w * scale));
+      }
+      if (there && col == 0) reinterpret_cast<uint16_t*>(p.exponents)[int64_t(n0 / kGfCols) * p.rows + row] = uint16_t(e[0] | e[1] << 8);
+    }
+    if (stores)
+      *reinterpret_cast<uint2*>(p.h + at) =
+          make_uint2(pack_bf16x2(gated_act<ACT>(g.x) * u.x, gated_act<ACT>(g.y) * u.y), pack_bf16x2(gated_act<ACT>(g.z) * u.z, gated_act<ACT>(g.w) * u.w));
   }
 }
 
-template <int ACT>
+template <int ACT, bool SAVE>
 __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_constant__ GatedFew p, unsigned* status) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(16) uint64_t ctl_bars[2 * kGfStages + 1];
@@ -608,41 +635,24 @@ __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_c
     tmem_wait_ld(u0);
     tmem_wait_ld(u1);
     if (row < p.rows) {
-      if (ranges == 1) {
-        __nv_bfloat16* to = p.h + int64_t(row) * p.inner + n0;
+      const uint32_t to = sbase + uint32_t(row) * (kGfPitch * 4);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t o[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int i = 8 * (c & 3) + 2 * j;
-            const uint32_t(&g)[32] = c < 4 ? g0 : g1;
-            const uint32_t(&u)[32] = c < 4 ? u0 : u1;
-            o[j] = pack_bf16x2(gated_act<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]), gated_act<ACT>(__uint_as_float(g[i + 1])) * __uint_as_float(u[i + 1]));
-          }
-          if (n0 + 8 * c < p.inner) *reinterpret_cast<uint4*>(to + 8 * c) = make_uint4(o[0], o[1], o[2], o[3]);
-        }
-      } else {
-        const uint32_t to = sbase + uint32_t(row) * (kGfPitch * 4);
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const uint32_t(&v)[32] = c < 8 ? g0 : c < 16 ? g1 : c < 24 ? u0 : u1;
-          sts128(to + 16u * c, make_uint4(v[4 * (c & 7)], v[4 * (c & 7) + 1], v[4 * (c & 7) + 2], v[4 * (c & 7) + 3]));
-        }
+      for (int c = 0; c < 32; ++c) {
+        const uint32_t(&v)[32] = c < 8 ? g0 : c < 16 ? g1 : c < 24 ? u0 : u1;
+        sts128(to + 16u * c, make_uint4(v[4 * (c & 7)], v[4 * (c & 7) + 1], v[4 * (c & 7) + 2], v[4 * (c & 7) + 3]));
       }
     }
   }
-  if (ranges > 1) {
-    __syncwarp();
-    cluster_sync();                              // the partial sums are there
-    if (ok) {
-      if (ranges == 2) few_join<ACT, 2>(p, sbase, rank, n0);
-      else if (ranges == 4) few_join<ACT, 4>(p, sbase, rank, n0);
-      else few_join<ACT, 8>(p, sbase, rank, n0);
-    }
-    __syncwarp();
-    cluster_sync();                              // the partners have read this block's sums
+  __syncwarp();
+  cluster_sync();                              // the partial sums are there
+  if (ok) {
+    if (ranges == 1) few_join<ACT, SAVE, 1>(p, sbase, rank, n0);
+    else if (ranges == 2) few_join<ACT, SAVE, 2>(p, sbase, rank, n0);
+    else if (ranges == 4) few_join<ACT, SAVE, 4>(p, sbase, rank, n0);
+    else few_join<ACT, SAVE, 8>(p, sbase, rank, n0);
   }
+  __syncwarp();
+  cluster_sync();                              // the partners have read this block's sums
   tc_fence_before();
   __syncthreads();
   if (warp == 5) {
@@ -768,13 +778,14 @@ static bool gated_aligned(const tg_gated_args* a) {
 }
 static int64_t gated_chunks(int64_t inner) { return (inner + 63) / 64; }
 
-template <int ACT>
+template <int ACT, bool SAVE>
 static int launch_few(const GatedFew& p, int tiles, int ranges, int smem, unsigned* status, cudaStream_t st) {
   static std::atomic<bool> done[64];
-  if (int rc = allow_smem(gated_few_kernel<ACT>, kGfMost, done)) return rc;
-  TG_CUDA_CHECK(launch_early_clusters(gated_few_kernel<ACT>, ranges, tiles * ranges, kGfThreads, smem, st, p, status));
+  if (int rc = allow_smem(gated_few_kernel<ACT, SAVE>, kGfMost, done)) return rc;
+  TG_CUDA_CHECK(launch_early_clusters(gated_few_kernel<ACT, SAVE>, ranges, tiles * ranges, kGfThreads, smem, st, p, status));
   return TG_OK;
 }
+template <bool SAVE>
 static int run_gated_few(const tg_gated_args* a, cudaStream_t st) {
   GatedFew p = {};
   p.x_rows = std::min(64, pow2_at_least(int(std::max<int64_t>(a->rows, 8))));
@@ -783,6 +794,9 @@ static int run_gated_few(const tg_gated_args* a, cudaStream_t st) {
   if (int rc = gated_map(&p.gate, a->w_gate, false, a->cols, a->inner, a->ld_gate, 64)) return rc;
   if (int rc = gated_map(&p.up, a->w_up, false, a->cols, a->inner, a->ld_up, 64)) return rc;
   p.h = static_cast<__nv_bfloat16*>(a->h);
+  p.saved_gate = static_cast<__half*>(a->saved_gate);
+  p.saved_up = static_cast<__half*>(a->saved_up);
+  p.exponents = a->saved_exponents;
   p.rows = int(a->rows);
   p.inner = int(a->inner);
   p.blocks = int((a->cols + kGbK - 1) / kGbK);
@@ -793,11 +807,11 @@ static int run_gated_few(const tg_gated_args* a, cudaStream_t st) {
   while (ranges < 8 && tiles * ranges * 2 <= 2 * sm_count() && p.blocks >= 8 * ranges && 8 * (p.blocks / (2 * ranges)) >= a->rows) ranges *= 2;
   const int stage = p.x_rows * p.x_boxes * 128 + 2 * kGbBox;
   p.stages = std::min(kGfStages, kGfMost / stage);
-  const int smem = std::max(p.stages * stage, ranges > 1 ? int(a->rows) * kGfPitch * 4 : 0);
+  const int smem = std::max(p.stages * stage, int(a->rows) * kGfPitch * 4);
   static_assert(kGfRows * kGfPitch * 4 <= kGfMost, "partial sums fit where the operands were");
-  if (a->act == TG_GATED_SILU) return launch_few<TG_GATED_SILU>(p, tiles, ranges, smem, a->status, st);
-  if (a->act == TG_GATED_GELU) return launch_few<TG_GATED_GELU>(p, tiles, ranges, smem, a->status, st);
-  return launch_few<TG_GATED_RELU>(p, tiles, ranges, smem, a->status, st);
+  if (a->act == TG_GATED_SILU) return launch_few<TG_GATED_SILU, SAVE>(p, tiles, ranges, smem, a->status, st);
+  if (a->act == TG_GATED_GELU) return launch_few<TG_GATED_GELU, SAVE>(p, tiles, ranges, smem, a->status, st);
+  return launch_few<TG_GATED_RELU, SAVE>(p, tiles, ranges, smem, a->status, st);
 }
 
 template <int ACT, bool SAVE>
@@ -832,7 +846,7 @@ extern "C" int tg_gated_linear_fwd(const tg_gated_args* a, void* stream) {
   if (!gated_aligned(a) || !aligned16(a->h) || !aligned16(a->saved_gate) || !aligned16(a->saved_up) || !aligned16(a->saved_exponents)) return TG_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
   const int64_t M = a->rows, D = a->cols, F = a->inner;
-  if (!save && M <= kGfRows) return run_gated_few(a, static_cast<cudaStream_t>(stream));
+  if (M <= kGfRows) return save ? run_gated_few<true>(a, static_cast<cudaStream_t>(stream)) : run_gated_few<false>(a, static_cast<cudaStream_t>(stream));
   GatedProblem p = {};
   GatedSaved s = {};
   if (int rc = gated_map(&p.a[0], a->x, false, M, D, a->ldx, 64)) return rc;
