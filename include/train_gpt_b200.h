@@ -290,8 +290,10 @@ int tg_qk_norm_rope_bwd(const tg_qk_args* args, void* stream);
  *   status    a device word as in tg_gemm_args, or NULL
  * Backward, from the gradient g bf16 [rows, inner] of h and what was saved: dx bf16 [rows, cols] (or NULL), dw_gate and dw_up bf16 [cols, inner]
  * (both or neither).  The gradients at the two projections are rounded to bf16 once before the products.
- *   scratch   tg_gated_linear_bwd_scratch_bytes(rows, inner) bytes, 16-byte aligned, contents undefined on entry and exit
- * Deterministic. */
+ *   scratch   scratch_bytes of it, 16-byte aligned, contents undefined on entry and exit: at least 4 bytes an element of h (each half rounded up to
+ *             256); with tg_gated_linear_bwd_scratch_bytes(args) of them, few tiles of a long contraction are cut into ranges and their float32
+ *             sums added up in order (dx, dw_gate and cols of args count: results that are not wanted are not planned for)
+ * Deterministic for the same scratch_bytes. */
 #define TG_GATED_SILU 0
 #define TG_GATED_GELU 1
 #define TG_GATED_RELU 2
@@ -309,12 +311,13 @@ typedef struct tg_gated_args {
   const void* g;
   void *dx, *dw_gate, *dw_up;
   void* scratch;
+  int64_t scratch_bytes;
   int64_t rows, cols, inner;
   uint32_t* status;
 } tg_gated_args;
 int64_t tg_gated_linear_exponent_bytes(int64_t rows, int64_t inner);
 int tg_gated_linear_fwd(const tg_gated_args* args, void* stream);
-int64_t tg_gated_linear_bwd_scratch_bytes(int64_t rows, int64_t inner);
+int64_t tg_gated_linear_bwd_scratch_bytes(const tg_gated_args* args);
 int tg_gated_linear_bwd(const tg_gated_args* args, void* stream);
 
 /* No counterpart in the reference.  y = bf16(residual + keep * x * 65536 / (65536 - t)) with t = p * 65536 rounded to an integer (ties to even)

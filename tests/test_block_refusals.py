@@ -135,7 +135,7 @@ def test_rope_entries(lib):
 def _gated(**kw):
     from train_gpt_b200._lib import GatedArgs
     a = GatedArgs(x=A[0], ldx=64, w_gate=A[1], ld_gate=72, w_up=A[2], ld_up=72, act=0, h=A[3], saved_gate=A[4], saved_up=A[5], saved_exponents=A[6], g=A[7], dx=A[8],
-                  dw_gate=A[9], dw_up=A[10], scratch=A[11], rows=10, cols=64, inner=72)
+                  dw_gate=A[9], dw_up=A[10], scratch=A[11], scratch_bytes=2 * 1536, rows=10, cols=64, inner=72)
     for n, v in kw.items():
         setattr(a, n, v)
     return ctypes.byref(a)
@@ -152,13 +152,16 @@ def test_gated_entries(lib):
     for kw in (dict(x=A[0] + 2), dict(w_up=A[0] + 8), dict(ldx=68), dict(ld_gate=76), dict(saved_gate=A[0] + 2), dict(saved_exponents=A[0] + 1)):
         assert [f(_gated(**kw), None) for f in both] == [TG_ERR_ALIGN] * 2, kw
     assert lib.tg_gated_linear_fwd(_gated(h=None), None) == TG_ERR_SHAPE and lib.tg_gated_linear_fwd(_gated(h=A[0] + 2), None) == TG_ERR_ALIGN
-    for kw in (dict(g=None), dict(scratch=None), dict(dw_gate=None), dict(dw_up=None)):
+    for kw in (dict(g=None), dict(scratch=None), dict(scratch_bytes=2 * 1536 - 1), dict(dw_gate=None), dict(dw_up=None)):
         assert lib.tg_gated_linear_bwd(_gated(**kw), None) == TG_ERR_SHAPE, kw
     for kw in (dict(g=A[0] + 2), dict(scratch=A[0] + 4), dict(dx=A[0] + 2), dict(dw_up=A[0] + 2)):
         assert lib.tg_gated_linear_bwd(_gated(**kw), None) == TG_ERR_ALIGN, kw
     assert lib.tg_gated_linear_fwd(_gated(rows=0), None) == TG_OK and lib.tg_gated_linear_fwd(None, None) == TG_ERR_SHAPE
     assert lib.tg_gated_linear_exponent_bytes(10, 72) == 2 * 10 * 2 and lib.tg_gated_linear_exponent_bytes(0, 72) == 0
-    assert lib.tg_gated_linear_bwd_scratch_bytes(10, 72) == 2 * 1536 and lib.tg_gated_linear_bwd_scratch_bytes(10, 0) == 0
+    assert lib.tg_gated_linear_bwd_scratch_bytes(_gated()) == 2 * 1536 and lib.tg_gated_linear_bwd_scratch_bytes(_gated(rows=0)) == 0
+    long = dict(rows=65536, cols=512, ldx=512, inner=64, ld_gate=64, ld_up=64)      # four tiles of the weights' gradients, of 1024 stages
+    assert lib.tg_gated_linear_bwd_scratch_bytes(_gated(**long)) > 2 * 65536 * 128
+    assert lib.tg_gated_linear_bwd_scratch_bytes(_gated(**long, dw_gate=None, dw_up=None)) == 2 * 65536 * 128
 
 
 def test_dropout_entry(lib):
@@ -176,7 +179,7 @@ def test_dropout_entry(lib):
 def test_structs_have_the_headers_layout():
     from train_gpt_b200._lib import GatedArgs, QkArgs
     assert QkArgs.positions.offset == 8 * 12 and QkArgs.batch.offset == 8 * 16 and QkArgs.theta.offset == 8 * 21 and ctypes.sizeof(QkArgs) == 8 * 33
-    assert GatedArgs.h.offset == 56 and GatedArgs.rows.offset == 8 * 16 and ctypes.sizeof(GatedArgs) == 8 * 20
+    assert GatedArgs.h.offset == 56 and GatedArgs.rows.offset == 8 * 17 and ctypes.sizeof(GatedArgs) == 8 * 21
 
 
 # ---- the generator ----------------------------------------------------------------------------------------------------
@@ -195,7 +198,7 @@ def test_the_pairs_kernel_keeps_the_gemms_rules():
     before the wait for the kernel before, an arrival for a whole warp follows its __syncwarp."""
     text = re.sub(r"//[^\n]*", "", open(os.path.join(ROOT, "train_gpt_b200", "csrc", "gated.cu")).read())
     pairs, few = text[text.index("void gated_body("):text.index("gated_fwd_kernel(")], text[text.index("gated_few_kernel(const"):text.index("struct GatedSlopes")]
-    for body, take, meet, touch in ((pairs, "tmem_take_pair(", "cluster_sync();", ("tma_load", "tma_store", "exponents")), (few, "tmem_take(", "__syncthreads();", ("tma_load", "p.h"))):
+    for body, take, meet, touch in ((pairs, "tmem_take_pair(", "cluster_sync();", ("tma_load", "tma_store", "exponents")), (few, "tmem_take(", "__syncthreads();", ("tma_load", "few_join<"))):
         taken = body.index(take)
         met, trigger, wait = (body.index(s, taken) for s in (meet, "grid_trigger();", "grid_wait();"))
         assert taken < met < trigger < wait < min(body.index(s) for s in touch)

@@ -69,6 +69,26 @@ def test_long_contractions():
     _check(*_make(9000, 16, 40))
 
 
+@pytest.mark.parametrize("m,k,f", [(9000, 200, 72), (30000, 64, 520), (40, 1000, 8192), (130, 24, 16384), (20000, 2048, 40), (260, 264, 6000)])
+def test_contractions_in_ranges(m, k, f):
+    """Few tiles of a long contraction, of dx, of the weights' gradients or of both."""
+    from train_gpt_b200 import _lib
+    x, wg, wu, g = _make(m, k, f)
+    _, grads = _check(x, wg, wu, g)
+    leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+    h = kernels.gated_linear(*leaves)
+    for which in ((0,), (1, 2), (0, 1, 2)):
+        again = torch.autograd.grad(h, [leaves[i] for i in which], g, retain_graph=True)
+        d = [t.double() for t in (x, wg, wu, g)]
+        for got, want in zip(again, [ref.gated_bwd(*d[:3], "silu", d[3])[i] for i in which]):
+            _near(got, want, which)
+    assert all(torch.equal(a, b) for a, b in zip(again, grads))
+    lib = _lib.load()
+    args = _lib.GatedArgs(x=16, ldx=k, w_gate=16, ld_gate=f, w_up=16, ld_up=f, dx=16, dw_gate=16, dw_up=16, rows=m, cols=k, inner=f)
+    import ctypes
+    assert lib.tg_gated_linear_bwd_scratch_bytes(ctypes.byref(args)) > 2 * ((m * f * 2 + 255) // 256 * 256)      # (it is cut)
+
+
 def test_leading_axes_strides_and_alignment():
     x, wg, wu, g = _make(60, 64, 72)
     h, (dx, dg, du) = _check(x, wg, wu, g)

@@ -58,7 +58,7 @@ class GatedArgs(C.Structure):
     """struct tg_gated_args"""
     _fields_ = [
         ("x", _p), ("ldx", _i64), ("w_gate", _p), ("ld_gate", _i64), ("w_up", _p), ("ld_up", _i64), ("act", _i), ("h", _p),
-        ("saved_gate", _p), ("saved_up", _p), ("saved_exponents", _p), ("g", _p), ("dx", _p), ("dw_gate", _p), ("dw_up", _p), ("scratch", _p),
+        ("saved_gate", _p), ("saved_up", _p), ("saved_exponents", _p), ("g", _p), ("dx", _p), ("dw_gate", _p), ("dw_up", _p), ("scratch", _p), ("scratch_bytes", _i64),
         ("rows", _i64), ("cols", _i64), ("inner", _i64), ("status", _p),
     ]
 
@@ -92,7 +92,7 @@ SYMBOLS = {
     "tg_qk_norm_rope_bwd": (_i, [C.POINTER(QkArgs), _p]),
     "tg_gated_linear_exponent_bytes": (_i64, [_i64, _i64]),
     "tg_gated_linear_fwd": (_i, [C.POINTER(GatedArgs), _p]),
-    "tg_gated_linear_bwd_scratch_bytes": (_i64, [_i64, _i64]),
+    "tg_gated_linear_bwd_scratch_bytes": (_i64, [C.POINTER(GatedArgs)]),
     "tg_gated_linear_bwd": (_i, [C.POINTER(GatedArgs), _p]),
     "tg_dropout": (_i, [_p, _p, C.c_double, _p, C.c_uint32, _p, _i64, _p]),
     "tg_softcap_ce_fwd": (_i, [_p, _p, _f, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),

@@ -94,6 +94,10 @@ struct GatedProblem {
   CUtensorMap a[2], b[2], d[2];
   int kind, tiles_m, tiles_n, blocks;           // blocks: stages of the contraction of a tile
   int half;                                     // kGbData: its first stage that reads the second operands; kGbWeights: column tiles of dWg
+  // The contraction may be cut into ranges: item i is tile i % tiles of range i / tiles, and its float32 sums go to `partial`, 256 KB an item,
+  // in the order in which the epilogue's threads hold them (see gated_join_kernel).
+  int ranges;
+  float4* partial;
 };
 struct GatedSaved {
   CUtensorMap gate, up;
@@ -102,10 +106,22 @@ struct GatedSaved {
   int chunks;                                   // of 64 columns
 };
 
-__device__ __forceinline__ void gated_tile(const GatedProblem& p, int item, int& tm, int& tn) {
-  const int per_band = kGbBand * p.tiles_n, b = item / per_band, w = item - b * per_band, rows = min(kGbBand, p.tiles_m - b * kGbBand);
+__device__ __forceinline__ void gated_place(int tiles_m, int tiles_n, int tile, int& tm, int& tn) {
+  const int per_band = kGbBand * tiles_n, b = tile / per_band, w = tile - b * per_band, rows = min(kGbBand, tiles_m - b * kGbBand);
   tn = w / rows;
   tm = b * kGbBand + (w - tn * rows);
+}
+// item -> tile, and the stages of its range
+__device__ __forceinline__ void gated_tile(const GatedProblem& p, int item, int& tm, int& tn, int& first, int& last) {
+  first = 0;
+  last = p.blocks;
+  if (p.ranges > 1) {
+    const int tiles = p.tiles_m * p.tiles_n, range = item / tiles;
+    item -= range * tiles;
+    first = int(int64_t(p.blocks) * range / p.ranges);
+    last = int(int64_t(p.blocks) * (range + 1) / p.ranges);
+  }
+  gated_place(p.tiles_m, p.tiles_n, item, tm, tn);
 }
 
 __device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -192,9 +208,9 @@ __device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedP
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int unit = int(blockIdx.x) / 2, units = int(gridDim.x) / 2;
-  const int n1 = one.tiles_m * one.tiles_n;
+  const int n1 = one.tiles_m * one.tiles_n * one.ranges;
   const Walk walk1 = walk_alone(unit, units, n1);
-  const Walk walk2 = both ? walk_second(unit, units, n1, two.tiles_m * two.tiles_n, rounds) : Walk{0, 0, 0, 1, 0};
+  const Walk walk2 = both ? walk_second(unit, units, n1, two.tiles_m * two.tiles_n * two.ranges, rounds) : Walk{0, 0, 0, 1, 0};
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -224,10 +240,10 @@ __device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedP
     const uint32_t full_leader = map_rank(full0, 0u);
     auto produce = [&](const GatedProblem& p, const Walk& w) {
       for (int item = w.first; ok && item < w.n; item = w.next(item)) {
-        int tm, tn;
-        gated_tile(p, item, tm, tn);
+        int tm, tn, first, last;
+        gated_tile(p, item, tm, tn, first, last);
         const int m0 = (2 * tm + int(rank)) * 128;
-        for (int kb = 0; kb < p.blocks; ++kb) {
+        for (int kb = first; kb < last; ++kb) {
           ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8u * s, ph, abort_flag, status, 1u));
           if (!ok) break;
           if (elect_one()) {
@@ -280,8 +296,10 @@ __device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedP
         // descriptor step per 16 of the contraction: 32 bytes along a K-major row, 16 rows of 128 bytes otherwise
         const uint32_t a_step = a_mn ? 128u : 2u, b_step = b_mn ? 128u : 2u;
         for (int item = w.first; ok && item < w.n; item = w.next(item)) {
-          for (int kb = 0; kb < p.blocks; ++kb) {
-            ok = __all_sync(0xffffffffu, (kb > 0 || mbar_wait(tempty0 + 8u * buf, bph, abort_flag, status, 2u)) &&
+          int tm, tn, first, last;
+          gated_tile(p, item, tm, tn, first, last);
+          for (int kb = first; kb < last; ++kb) {
+            ok = __all_sync(0xffffffffu, (kb > first || mbar_wait(tempty0 + 8u * buf, bph, abort_flag, status, 2u)) &&
                                              mbar_wait(full0 + 8u * s, sph, abort_flag, status, 3u));
             if (!ok) break;
             __syncwarp();
@@ -291,9 +309,9 @@ __device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedP
 #pragma unroll
               for (int k = 0; k < kGbK / 16; ++k)
                 umma_bf16_pair(tmem_base + buf * 256u, (uint64_t(desc_hi) << 32) | (a_lo0 + soff + k * a_step),
-                               (uint64_t(desc_hi) << 32) | (b_lo0 + soff + k * b_step), idesc, kb > 0 || k > 0 ? 1u : 0u);
+                               (uint64_t(desc_hi) << 32) | (b_lo0 + soff + k * b_step), idesc, kb > first || k > 0 ? 1u : 0u);
               umma_commit_both(empty0 + 8u * s);
-              if (kb + 1 == p.blocks) umma_commit_both(tfull0 + 8u * buf);
+              if (kb + 1 == last) umma_commit_both(tfull0 + 8u * buf);
             }
             __syncwarp();
             if (++s == kStages) { s = 0; sph ^= 1u; }
@@ -333,8 +351,8 @@ __device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedP
     };
     auto finish = [&](const GatedProblem& p, const Walk& w) {
       for (int item = w.first; item < w.n; item = w.next(item)) {
-        int tm, tn;
-        gated_tile(p, item, tm, tn);
+        int tm, tn, first, last;
+        gated_tile(p, item, tm, tn, first, last);
         const int m0 = (2 * tm + int(rank)) * 128 + quarter * 32;
         ok = __all_sync(0xffffffffu, mbar_wait(tfull0 + 8u * buf, bph, abort_flag, status, 5u));
         if (!ok) break;
@@ -394,6 +412,21 @@ __device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedP
         } else {
           const int sel = p.kind == kGbWeights && tn >= p.half, n0 = (tn - (sel ? p.half : 0)) * 256 + half * 128;
           const uint32_t at = lanes + buf * 256u + uint32_t(half) * 128u;
+          if (p.ranges > 1) {           // four columns a lane, a warp's rows side by side
+            float4* to = p.partial + ((int64_t(item) * 2 + rank) * kGbWarps + warp) * 1024 + lane;
+#pragma unroll
+            for (int piece = 0; piece < 4; ++piece) {
+              uint32_t v[32];
+              tmem_ld32(at + 32u * piece, v);
+              tmem_wait_ld(v);
+              if (piece == 3) release();
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                to[(8 * piece + j) * 32] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+            }
+            if ((buf ^= 1u) == 0u) bph ^= 1u;
+            continue;
+          }
           rows_free();
 #pragma unroll
           for (int box = 0; box < 2; ++box) {
@@ -451,6 +484,39 @@ __global__ void __launch_bounds__(kGbThreads, 1) gated_fwd_kernel(const __grid_c
 __global__ void __launch_bounds__(kGbThreads, 1)
 gated_bwd_kernel(const __grid_constant__ GatedProblem one, const __grid_constant__ GatedProblem two, int both, int rounds, unsigned* status) {
   gated_body<kGbData, 0, false, GatedCfg<2>>(one, two, both != 0, rounds, GatedSaved{}, status);
+}
+
+// The ranges of a problem that was cut, added up in order.  A warp has eight columns of the 32 rows of an epilogue's warp at a time.
+struct GatedJoin {
+  const float4* partial;
+  __nv_bfloat16* d[2];
+  int kind, tiles_m, tiles_n, half, ranges;
+  int64_t rows, cols;                           // of a result; its pitch is cols
+};
+__global__ void __launch_bounds__(256) gated_join_kernel(const __grid_constant__ GatedJoin a, const __grid_constant__ GatedJoin b, int blocks_a) {
+  grid_trigger();
+  grid_wait();
+  const bool second = int(blockIdx.x) >= blocks_a;
+  const GatedJoin& p = second ? b : a;
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = int64_t(int(blockIdx.x) - (second ? blocks_a : 0)) * 8 + (threadIdx.x >> 5);      // (tile, CTA, warp, eight columns)
+  const int tiles = p.tiles_m * p.tiles_n, piece = int(unit & 15), slab = int(unit >> 4), tile = slab >> 4, rank = (slab >> 3) & 1, warp = slab & 7;
+  if (tile >= tiles) return;
+  int tm, tn;
+  gated_place(p.tiles_m, p.tiles_n, tile, tm, tn);
+  const float4* at = p.partial + int64_t(slab) * 1024 + piece * 64 + lane;
+  const int64_t step = int64_t(tiles) * 16 * 1024;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+#pragma unroll 4
+  for (int r = 0; r < p.ranges; ++r) {
+    const float4 v = __ldcg(at + r * step), w = __ldcg(at + r * step + 32);
+    x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
+    y = make_float4(y.x + w.x, y.y + w.y, y.z + w.z, y.w + w.w);
+  }
+  const int sel = p.kind == kGbWeights && tn >= p.half;
+  const int64_t row = (2 * tm + rank) * 128 + (warp & 3) * 32 + lane, col = int64_t(tn - (sel ? p.half : 0)) * 256 + (warp >> 2) * 128 + piece * 8;
+  if (row < p.rows && col < p.cols)
+    *reinterpret_cast<uint4*>(p.d[sel] + row * p.cols + col) = make_uint4(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w), pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
 }
 
 // ---- few tokens ----------------------------------------------------------------------------------------------------
@@ -861,6 +927,7 @@ extern "C" int tg_gated_linear_fwd(const tg_gated_args* a, void* stream) {
     s.chunks = int(gated_chunks(F));
   }
   p.kind = kGbForward;
+  p.ranges = 1;
   p.tiles_m = int((M + 255) / 256);
   p.tiles_n = int((F + 127) / 128);
   p.blocks = int((D + kGbK - 1) / kGbK);
@@ -868,8 +935,66 @@ extern "C" int tg_gated_linear_fwd(const tg_gated_args* a, void* stream) {
   return save ? run_gated_fwd<true>(a->act, p, s, a->status, st) : run_gated_fwd<false>(a->act, p, s, a->status, st);
 }
 
-extern "C" int64_t tg_gated_linear_bwd_scratch_bytes(int64_t rows, int64_t inner) {
-  return rows <= 0 || inner <= 0 ? 0 : 2 * ((rows * inner * 2 + 255) / 256 * 256);
+// Sizes of a problem as the launch sees them
+struct GatedTiles {
+  int64_t tiles = 0, blocks = 0, ranges = 1;
+};
+static double gated_makespan(const GatedTiles& x, const GatedTiles& y, int64_t units, int& rounds) {
+  const GatedTiles &a = x.blocks * y.ranges >= y.blocks * x.ranges ? x : y, &b = &a == &x ? y : x;
+  auto item = [](const GatedTiles& t) { return double(t.blocks) / double(t.ranges) + 3.0; };
+  rounds = 0;
+  if (a.tiles == 0 || b.tiles == 0) {
+    const GatedTiles& t = a.tiles == 0 ? b : a;
+    return double((t.tiles * t.ranges + units - 1) / units) * item(t);
+  }
+  return two_problems_us(a.tiles * a.ranges, item(a), b.tiles * b.ranges, item(b), units, rounds);
+}
+// How many ranges the contractions of dx and dW are cut into, in units of a stage (0.3 us): where whole items leave a fifth of the pairs' time
+// unused or more, into items of a third of what each pair has to do, if that gains more than the sums' way through memory and a launch cost.
+// 65536 x 512 -> 64 has four tiles of dW, of 1024 stages.
+static void gated_ranges(GatedTiles& data, GatedTiles& weights) {
+  const int64_t units = sm_count() / 2;
+  int rounds;
+  const double load = double(data.tiles * data.blocks + weights.tiles * weights.blocks) / double(units);
+  const double whole = gated_makespan(data, weights, units, rounds);
+  if (whole < 1.2 * load + 10.0) return;
+  const int64_t length = std::max<int64_t>(16, int64_t(load / 3.0));
+  double best = whole;
+  const GatedTiles x = data, y = weights;
+  for (int which = 1; which < 4; ++which) {
+    GatedTiles u = x, v = y;
+    if (which & 1) u.ranges = std::max<int64_t>(1, std::min<int64_t>(u.blocks / 8, (u.blocks + length - 1) / length));
+    if (which & 2) v.ranges = std::max<int64_t>(1, std::min<int64_t>(v.blocks / 8, (v.blocks + length - 1) / length));
+    const int64_t moved = (u.ranges > 1 ? u.tiles * u.ranges : 0) + (v.ranges > 1 ? v.tiles * v.ranges : 0);
+    if (moved == 0 || moved > 1024) continue;
+    const double time = gated_makespan(u, v, units, rounds) + 10.0 + 0.5 * double(moved);
+    if (time < best) {
+      best = time;
+      data = u;
+      weights = v;
+    }
+  }
+}
+static void gated_tiles(const tg_gated_args* a, GatedTiles& data, GatedTiles& weights) {
+  auto over = [](int64_t n, int64_t t) { return (n + t - 1) / t; };
+  if (a->dx != nullptr) {
+    data.tiles = over(a->rows, 256) * over(a->cols, 256);
+    data.blocks = 2 * over(a->inner, kGbK);
+  }
+  if (a->dw_gate != nullptr) {
+    weights.tiles = over(a->cols, 256) * 2 * over(a->inner, 256);
+    weights.blocks = over(a->rows, kGbK);
+  }
+  gated_ranges(data, weights);
+}
+static int64_t gated_half_bytes(const tg_gated_args* a) { return (a->rows * a->inner * 2 + 255) / 256 * 256; }
+static int64_t gated_partial_items(const GatedTiles& t) { return t.ranges > 1 ? t.tiles * t.ranges : 0; }
+
+extern "C" int64_t tg_gated_linear_bwd_scratch_bytes(const tg_gated_args* a) {
+  if (gated_check(a) != TG_OK || a->rows == 0) return 0;
+  GatedTiles data, weights;
+  gated_tiles(a, data, weights);
+  return 2 * gated_half_bytes(a) + (gated_partial_items(data) + gated_partial_items(weights)) * 262144;
 }
 
 extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
@@ -884,7 +1009,7 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
     return TG_OK;
   }
   const bool dx = a->dx != nullptr, dw = a->dw_gate != nullptr;
-  if (a->g == nullptr || a->saved_gate == nullptr || a->saved_up == nullptr || a->saved_exponents == nullptr || a->scratch == nullptr ||
+  if (a->g == nullptr || a->saved_gate == nullptr || a->saved_up == nullptr || a->saved_exponents == nullptr || a->scratch == nullptr || a->scratch_bytes < 2 * gated_half_bytes(a) ||
       (dx && (a->w_gate == nullptr || a->w_up == nullptr)) || (dw && a->x == nullptr))
     return TG_ERR_SHAPE;
   if (!gated_aligned(a) || !aligned16(a->g) || !aligned16(a->saved_gate) || !aligned16(a->saved_up) || !aligned16(a->saved_exponents) || !aligned16(a->dx) ||
@@ -898,7 +1023,7 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
   s.up = static_cast<const __half*>(a->saved_up);
   s.exponents = reinterpret_cast<const uint16_t*>(a->saved_exponents);
   s.dgate = static_cast<__nv_bfloat16*>(a->scratch);
-  s.dup = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(a->scratch) + tg_gated_linear_bwd_scratch_bytes(M, F) / 2);
+  s.dup = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(a->scratch) + gated_half_bytes(a));
   s.rows = M;
   s.inner = int(F);
   s.chunks = int(gated_chunks(F));
@@ -906,7 +1031,20 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
   auto kern = a->act == TG_GATED_SILU ? gated_slopes_kernel<TG_GATED_SILU> : a->act == TG_GATED_GELU ? gated_slopes_kernel<TG_GATED_GELU> : gated_slopes_kernel<TG_GATED_RELU>;
   TG_CUDA_CHECK(launch_if_short(items <= 8 * sm_count(), kern, dim3(unsigned(items)), kGsThreads, 0, st, s));
 
+  GatedTiles data_tiles, weights_tiles;
+  gated_tiles(a, data_tiles, weights_tiles);
+  if (a->scratch_bytes < tg_gated_linear_bwd_scratch_bytes(a)) data_tiles.ranges = weights_tiles.ranges = 1;
   GatedProblem data = {}, weights = {};
+  GatedJoin joins[2] = {};
+  int n_joins = 0;
+  uint8_t* partial = static_cast<uint8_t*>(a->scratch) + 2 * gated_half_bytes(a);
+  auto cut = [&](GatedProblem& p, const GatedTiles& t, void* d0, void* d1, int64_t rows, int64_t cols) {
+    p.ranges = int(t.ranges);
+    if (t.ranges == 1) return;
+    p.partial = reinterpret_cast<float4*>(partial);
+    partial += gated_partial_items(t) * 262144;
+    joins[n_joins++] = {p.partial, {static_cast<__nv_bfloat16*>(d0), static_cast<__nv_bfloat16*>(d1)}, p.kind, p.tiles_m, p.tiles_n, p.half, p.ranges, rows, cols};
+  };
   if (dx) {
     for (int i = 0; i < 2; ++i) {
       if (int rc = gated_map(&data.a[i], i ? s.dup : s.dgate, false, M, F, F, 64)) return rc;
@@ -918,6 +1056,7 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
     data.tiles_n = int((D + 255) / 256);
     data.half = int((F + kGbK - 1) / kGbK);
     data.blocks = 2 * data.half;
+    cut(data, data_tiles, a->dx, nullptr, M, D);
   }
   if (dw) {
     if (int rc = gated_map(&weights.a[0], a->x, false, M, D, a->ldx, 64)) return rc;
@@ -930,15 +1069,24 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
     weights.half = int((F + 255) / 256);
     weights.tiles_n = 2 * weights.half;
     weights.blocks = int((M + kGbK - 1) / kGbK);
+    cut(weights, weights_tiles, a->dw_gate, a->dw_up, D, F);
   }
-  const bool both = dx && dw, data_first = dx && (!dw || data.blocks >= weights.blocks);
+  // the longer items first
+  const bool both = dx && dw, data_first = dx && (!dw || data_tiles.blocks * weights_tiles.ranges >= weights_tiles.blocks * data_tiles.ranges);
   const GatedProblem &one = data_first ? data : weights, &two = data_first ? weights : data;
-  const int64_t n1 = int64_t(one.tiles_m) * one.tiles_n, n2 = both ? int64_t(two.tiles_m) * two.tiles_n : 0;
+  const int64_t n1 = int64_t(one.tiles_m) * one.tiles_n * one.ranges, n2 = both ? int64_t(two.tiles_m) * two.tiles_n * two.ranges : 0;
   static std::atomic<int> units_of[64];
   using C = GatedCfg<2>;
   int units = 0, rounds = 0;
   if (int rc = launch_gated(gated_bwd_kernel, C::smem_bytes, units_of, n1 + n2, false, st, units)) return rc;
-  if (both) two_problems_us(n1, double(one.blocks) + 3.0, n2, double(two.blocks) + 3.0, units, rounds);
-  const bool early = n1 + n2 <= 4 * units && one.blocks <= 64;
-  return launch_gated(gated_bwd_kernel, C::smem_bytes, units_of, n1 + n2, early, st, units, one, two, int(both), rounds, reinterpret_cast<unsigned*>(a->status));
+  gated_makespan(data_tiles, weights_tiles, units, rounds);
+  const bool early = n1 + n2 <= 4 * units && one.blocks / one.ranges <= 64;
+  if (int rc = launch_gated(gated_bwd_kernel, C::smem_bytes, units_of, n1 + n2, early, st, units, one, two, int(both), rounds, reinterpret_cast<unsigned*>(a->status)))
+    return rc;
+  if (n_joins > 0) {
+    auto blocks_of = [](const GatedJoin& j) { return j.ranges > 1 ? j.tiles_m * j.tiles_n * 32 : 0; };
+    const int first = blocks_of(joins[0]);
+    TG_CUDA_CHECK(launch_if_short(true, gated_join_kernel, dim3(unsigned(first + blocks_of(joins[1]))), 256, 0, st, joins[0], joins[1], first));
+  }
+  return TG_OK;
 }

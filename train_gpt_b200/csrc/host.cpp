@@ -603,7 +603,6 @@ std::array<Tensor, 3> gated_linear_bwd(const Tensor& x, const Tensor& w_gate, co
   if (want_dx) out[0] = empty(x.sizes(), at::kBFloat16, x);
   if (want_dw)
     for (int i : {1, 2}) out[i] = empty({g.cols, g.inner}, at::kBFloat16, x);
-  const Tensor scratch = empty({std::max<int64_t>(api.tg_gated_linear_bwd_scratch_bytes(g.rows, g.inner), 16)}, at::kByte, x);
   tg_gated_args a = gated_args(g);
   a.saved_gate = ptr(kept.gate);
   a.saved_up = ptr(kept.up);
@@ -612,6 +611,8 @@ std::array<Tensor, 3> gated_linear_bwd(const Tensor& x, const Tensor& w_gate, co
   a.dx = ptr(out[0]);
   a.dw_gate = ptr(out[1]);
   a.dw_up = ptr(out[2]);
+  a.scratch_bytes = std::max<int64_t>(api.tg_gated_linear_bwd_scratch_bytes(&a), 16);
+  const Tensor scratch = empty({a.scratch_bytes}, at::kByte, x);
   a.scratch = ptr(scratch);
   check(api.tg_gated_linear_bwd(&a, cur_stream()), "tg_gated_linear_bwd");
   return out;

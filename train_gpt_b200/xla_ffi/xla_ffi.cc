@@ -375,12 +375,13 @@ ffi::Error GatedLinearBwd(cudaStream_t s, BF16 x, BF16 w_gate, BF16 w_up, U8 sav
   tg_gated_args a = {};
   if (!GatedArgs(s, x, w_gate, w_up, static_cast<int64_t>(g.element_count()), status, &a) || !Have(2 * a.rows * a.inner, saved_gate, saved_up) ||
       !Have(a.rows * a.cols, *dx) || !Have(a.cols * a.inner, *dw_gate, *dw_up) ||
-      static_cast<int64_t>(exponents.element_count()) < tg_gated_linear_exponent_bytes(a.rows, a.inner) ||
-      static_cast<int64_t>(scratch->element_count()) < tg_gated_linear_bwd_scratch_bytes(a.rows, a.inner))
-    return Mismatch("TgGatedLinearBwd: g must be (rows, inner), results like x and the weights, saved buffers as TgGatedLinearFwd's, scratch tg_gated_linear_bwd_scratch_bytes");
+      static_cast<int64_t>(exponents.element_count()) < tg_gated_linear_exponent_bytes(a.rows, a.inner))
+    return Mismatch("TgGatedLinearBwd: g must be (rows, inner), results like x and the weights, saved buffers as TgGatedLinearFwd's");
   a.act = act; a.g = g.untyped_data();
   a.saved_gate = saved_gate.untyped_data(); a.saved_up = saved_up.untyped_data(); a.saved_exponents = exponents.typed_data();
   a.dx = dx->untyped_data(); a.dw_gate = dw_gate->untyped_data(); a.dw_up = dw_up->untyped_data(); a.scratch = scratch->untyped_data();
+  a.scratch_bytes = static_cast<int64_t>(scratch->element_count());
+  if (a.scratch_bytes < tg_gated_linear_bwd_scratch_bytes(&a)) return Mismatch("TgGatedLinearBwd: scratch result smaller than tg_gated_linear_bwd_scratch_bytes");
   return Check(tg_gated_linear_bwd(&a, s), "tg_gated_linear_bwd");
 }
 
