@@ -19,10 +19,17 @@ LAYER_KEYS = ("norm1", "wq", "wk", "wv", "wo", "norm2", "w_up", "w_down")      #
 TOP_KEYS = ("embed", "pos", "final_norm")                                      # model.py:47-52
 SANDWICH_KEYS = ("post1", "post2", "gate1", "gate2")                           # of blocks with a norm on both sides, which the reference lacks
 
+BLOCK_KEYS = ("w_gate", "q_norm", "k_norm")                                    # of a gated feed-forward and normed queries and keys, likewise
+
 
 def _layer_keys(layers):
-    """The keys of a layer's parameters: the reference's, and what of the sandwich norm's a model or a tree has."""
-    return LAYER_KEYS + tuple(k for k in SANDWICH_KEYS if k in layers)
+    """The keys of a layer's parameters: the reference's, and what of the sandwich norm's and of such blocks' a model or a tree has."""
+    return LAYER_KEYS + tuple(k for k in SANDWICH_KEYS + BLOCK_KEYS if k in layers)
+
+
+def _top_keys(model):
+    """A model with rotary positions has no table of them."""
+    return TOP_KEYS if model.pos is not None else tuple(k for k in TOP_KEYS if k != "pos")
 
 
 def _to_numpy(t: torch.Tensor) -> np.ndarray:
@@ -43,7 +50,7 @@ def _to_torch(a: np.ndarray, like: torch.Tensor) -> torch.Tensor:
 
 def params_tree(model) -> dict:
     """The reference's parameter pytree (model.py:46-54) from a `step.GPT`."""
-    tree = {k: _to_numpy(getattr(model, k)) for k in TOP_KEYS}
+    tree = {k: _to_numpy(getattr(model, k)) for k in _top_keys(model)}
     tree["layers"] = {k: np.stack([_to_numpy(lp[k]) for lp in model.layers]) for k in _layer_keys(model.layers[0] if model.layers else ())}
     tree["unembed"] = _to_numpy(model.unembed)
     return tree
@@ -83,7 +90,10 @@ def load_params(model, tree: dict) -> None:
         with torch.no_grad():
             dst.copy_(_to_torch(src, dst))
 
-    for k in TOP_KEYS:
+    top = tuple(k for k in TOP_KEYS if k in tree)
+    if top != _top_keys(model):
+        raise ValueError(f"checkpoint has parameters {top}, the model {_top_keys(model)}")
+    for k in top:
         put(getattr(model, k), tree[k], k)
     layers = tree["layers"]
     n = len(model.layers)

@@ -19,7 +19,9 @@ Differences from model.py that the benchmark's training configuration asks for a
 q/k/v, untied head, tanh logit cap 15 and the 0.02 / 0.02/sqrt(2L) init follow model.py.
 Beyond the reference: `block_norm="sandwich"` (a norm behind each branch too, with a gate and a scaled residual stream:
 kernels.sandwich_norm) and distillation (`GPT.top_logits` of a teacher, `Trainer.step(..., teacher=)` for its student:
-losses.capped_distillation).  Both run through autograd.
+losses.capped_distillation); rotary positions and a norm per head of queries and keys (`positions="rotary"`, `qk_norm=True`:
+kernels.qk_norm_rope), a gated feed-forward (`activation="swiglu"` and its like: kernels.gated_linear, in bf16 beside FP8 linears),
+dropout of every branch (`dropout=`: kernels.dropout).  All of them run through autograd.
 
 No per-block rematerialisation (the reference's `use_remat` trades compute for memory; 180 GB
 does not need it at these sizes).
@@ -49,7 +51,11 @@ class StepConfig:
     init_std: float = 0.02          # config.py:16
     rms_eps: float = 1e-5           # config.py:17
     logit_cap: float = 15.0         # config.py:19
-    activation: str = "gelu"        # "gelu" (the benchmark's training configuration) or "relu2" (model.py:72)
+    activation: str = "gelu"        # "gelu" (the benchmark's training configuration) or "relu2" (model.py:72); "swiglu", "geglu", "reglu": act(h w_gate) * (h w_up)
+    positions: str = "learned"      # "learned" (model.py:83), added to the embeddings; "rotary": queries and keys turned by their position
+    rope_theta: float = 10000.0     # with positions "rotary"
+    qk_norm: bool = False           # a norm with a learned scale on every head of queries and keys
+    dropout: float = 0.0            # of every branch before the residual add, where gradients are on
     mm: str = "fp8"
     mlp: str = "fused"              # "fused": activation and its gradient folded into the quantisers (FP8 mm only); "unfused"
     norm: str = "fused"
@@ -75,6 +81,8 @@ class StepConfig:
 # 0 -> 99.4, 8 -> 101.6, 16 -> 101.7, 32 -> 103.8: the all-reduce kernels themselves shrink (6.3 -> 2.8 ms summed over a
 # step) but they were hidden behind the backward pass anyway, and the GEMMs lose more than that.  So: none.
 RESERVED_SMS_DP = 0
+
+GATED = {"swiglu": "silu", "geglu": "gelu", "reglu": "relu"}       # activation -> that of kernels.gated_linear
 
 SMALL = dict(vocab_size=256, seq_len=128, d_model=128, n_layers=2, n_heads=4, head_dim=32, d_ff=512)  # config.py:32-40
 
@@ -260,6 +268,18 @@ class _FusedMLP(torch.autograd.Function):
         return dh.reshape(h.shape), None, dw_up, dw_down, None
 
 
+def _keep(like, p: float, seed, site: int):
+    """The mask of kernels.dropout as a tensor: Philox4x32-10 in 64-bit integer operations."""
+    low, piece = 0xFFFFFFFF, torch.arange((like.numel() + 7) // 8, device=like.device)
+    c, k = [piece & low, piece >> 32, torch.full_like(piece, site), torch.zeros_like(piece)], [seed & low, (seed >> 32) & low]
+    for _ in range(10):
+        a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [((b >> 32) & low) ^ c[1] ^ k[0], b & low, ((a >> 32) & low) ^ c[3] ^ k[1], a & low]
+        k = [(k[0] + 0x9E3779B9) & low, (k[1] + 0xBB67AE85) & low]
+    words = torch.stack(c, -1)
+    return (torch.stack((words & 0xFFFF, words >> 16), -1).flatten()[:like.numel()] >= round(65536 * p)).view(like.shape)
+
+
 class GPT:
     """Parameters (bf16, model.py:19-54) and forward pass."""
 
@@ -270,7 +290,14 @@ class GPT:
             raise ValueError(f"unknown residual_gate {cfg.residual_gate!r}")
         if cfg.block_norm == "pre" and (cfg.residual_gate != "none" or cfg.residual_scale != 1.0):
             raise ValueError("residual_gate and residual_scale need block_norm 'sandwich'")
+        if cfg.positions not in ("learned", "rotary"):
+            raise ValueError(f"unknown positions {cfg.positions!r}")
+        if (cfg.positions == "rotary" or cfg.qk_norm) and (cfg.head_dim % 16 or cfg.head_dim > 512):
+            raise ValueError(f"positions 'rotary' and qk_norm need a head_dim that is a multiple of 16 and at most 512, got {cfg.head_dim}")
+        if not 0.0 <= cfg.dropout <= 1.0:
+            raise ValueError(f"dropout={cfg.dropout} must be between 0 and 1")
         self.cfg = cfg
+        self.gated = cfg.activation in GATED
         g = torch.Generator(device=device).manual_seed(seed)
         std, proj_std = cfg.init_std, cfg.init_std / math.sqrt(2.0 * cfg.n_layers)   # model.py:21-22
         d, h, ff = cfg.d_model, cfg.n_heads * cfg.head_dim, cfg.d_ff
@@ -282,13 +309,17 @@ class GPT:
             return torch.nn.Parameter(torch.ones(n, device=device, dtype=torch.bfloat16))
 
         self.embed = normal((cfg.vocab_size, d))
-        self.pos = normal((cfg.seq_len, d))
+        self.pos = normal((cfg.seq_len, d)) if cfg.positions == "learned" else None
         self.layers = []
         for _ in range(cfg.n_layers):
             self.layers.append({
                 "norm1": ones(d), "wq": normal((d, h)), "wk": normal((d, h)), "wv": normal((d, h)),
                 "wo": normal((h, d), proj_std), "norm2": ones(d), "w_up": normal((d, ff)),
                 "w_down": normal((ff, d), proj_std)})
+            if self.gated:
+                self.layers[-1]["w_gate"] = normal((d, ff))
+            if cfg.qk_norm:
+                self.layers[-1].update({"q_norm": ones(cfg.head_dim), "k_norm": ones(cfg.head_dim)})
             if cfg.block_norm == "sandwich":
                 # a gate per channel starts where proj_std puts a branch's share (model.py:22); one per token at 1/2 (a zero projection)
                 gate = {"none": None, "channel": lambda: ones(d).detach() / math.sqrt(2.0 * cfg.n_layers),
@@ -298,6 +329,8 @@ class GPT:
                     self.layers[-1].update({"gate1": torch.nn.Parameter(gate()), "gate2": torch.nn.Parameter(gate())})
         self.final_norm = ones(d)
         self.unembed = normal((d, cfg.vocab_size))
+        # what the masks are drawn from; Trainer counts it up every step (a device word, so that a captured step draws new ones)
+        self.dropout_seed = torch.tensor([seed], dtype=torch.int64, device=device) if cfg.dropout > 0 else None
         self.exchange = None            # gradient buckets with a deferred exchange (data-parallel training): see _ExchangePoint
 
     def buckets(self, qkv_side_by_side: bool = False):
@@ -310,15 +343,18 @@ class GPT:
                 out.append([lp["norm1"], (lp["wq"], lp["wk"], lp["wv"]), *(v for n, v in lp.items() if n not in ("norm1", "wq", "wk", "wv"))])
             else:
                 out.append(list(lp.values()))
-        out.append([self.embed, self.pos])
+        out.append([self.embed] if self.pos is None else [self.embed, self.pos])
         return out
 
     def parameters(self):
         return [p for b in self.buckets() for p in b]
 
     def matrices(self):
-        """The parameters whose only use is an FP8 linear (model.py:63-72): wq, wk, wv, wo, w_up, w_down."""
-        return [lp[n] for lp in self.layers for n in ("wq", "wk", "wv", "wo", "w_up", "w_down")]
+        """The parameters whose only use is an FP8 linear (model.py:63-72): wq, wk, wv, wo, w_up, w_down (not w_up where it is gated)."""
+        return [lp[n] for lp in self.layers for n in self.linears()]
+
+    def linears(self):
+        return ("wq", "wk", "wv", "wo", "w_down") if self.gated else ("wq", "wk", "wv", "wo", "w_up", "w_down")
 
     # ---- the mm / norm seam (bench_fp8_norm.py:81-86) -------------------------------------
     def _mm(self, a, w, aq=None):
@@ -361,6 +397,44 @@ class GPT:
         out = kernels.sandwich_norm(x, branch, post, gamma, c.rms_eps, gate=gate, residual_scale=c.residual_scale, quantize=quantize)
         return out[0], out[1], fp8.QuantizedActivation(*out[1:]) if quantize else None
 
+    def _place(self, q, k, lp):
+        """Queries and keys (B, T, heads, head_dim) normed and rotated, as far as the configuration asks for either."""
+        c = self.cfg
+        rotary = c.head_dim if c.positions == "rotary" else 0
+        scales = (lp["q_norm"], lp["k_norm"]) if c.qk_norm else (None, None)
+        if rotary == 0 and not c.qk_norm:
+            return q, k
+        if c.norm != "torch_reference":
+            return kernels.qk_norm_rope(q, k, *scales, c.rms_eps, theta=c.rope_theta, rotary_dim=rotary)
+        angle = torch.arange(q.shape[1], device=q.device, dtype=torch.float64)[:, None, None] * c.rope_theta ** (
+            -torch.arange(0, rotary, 2, device=q.device, dtype=torch.float64) / max(rotary, 1))
+
+        def place(x, scale):
+            y = x.float()
+            if scale is not None:
+                y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + c.rms_eps) * scale.float()
+            if rotary:
+                a, b, cos, sin = y[..., :rotary // 2], y[..., rotary // 2:], angle.cos().float(), angle.sin().float()
+                y = torch.cat((a * cos - b * sin, a * sin + b * cos), -1)
+            return y.to(x.dtype)
+        return place(q, scales[0]), place(k, scales[1])
+
+    def _drop(self, branch, site, residual=None):
+        """branch dropped out and added to the residual stream, where there is one to add to."""
+        c = self.cfg
+        if c.norm != "torch_reference":
+            return kernels.dropout(branch, c.dropout, self.dropout_seed, site, residual)
+        t = round(65536 * c.dropout)
+        y = torch.where(_keep(branch, c.dropout, self.dropout_seed, site), branch.float() * (65536 / (65536 - t) if t < 65536 else 0.0), 0.0)
+        return (y if residual is None else y + residual.float()).to(branch.dtype)
+
+    def _gated(self, h, lp):
+        """act(h w_gate) * (h w_up)"""
+        c = self.cfg
+        if c.mlp == "fused" and c.norm != "torch_reference":
+            return kernels.gated_linear(h, lp["w_gate"], lp["w_up"], GATED[c.activation])
+        return {"silu": F.silu, "gelu": F.gelu, "relu": F.relu}[GATED[c.activation]](h @ lp["w_gate"]) * (h @ lp["w_up"])
+
     def _act(self, u):
         return F.gelu(u) if self.cfg.activation == "gelu" else F.relu(u) ** 2      # model.py:72
 
@@ -368,11 +442,13 @@ class GPT:
         """model.py:75-96: everything up to the unembedding GEMM (no cap)."""
         c = self.cfg
         B, T = ids.shape
-        x = self.embed[ids] + self.pos[:T]                                          # model.py:83
+        x = self.embed[ids] if self.pos is None else self.embed[ids] + self.pos[:T]  # model.py:83
         # With `residual == "fused"` a branch's output is not added where model.py adds it: it waits in
         # `branch` and the norm that follows does the add (same values: one bf16 rounding of x + branch).
         fuse = c.residual == "fused" and c.norm == "fused" and c.mm != "bf16" and c.d_model <= ops.ADD_NORM_MAX_COLS
         branch = None
+        dropped = self.dropout_seed is not None and torch.is_grad_enabled()
+        sites = iter(range(2 * c.n_layers))       # every branch draws masks of its own
 
         def norm_after(x, branch, gamma, want_q=True, behind=None):
             """(new x, h, quantised h) for `x = x + branch; h = norm(x)`; branch None: no add pending.  behind: the branch's
@@ -380,6 +456,12 @@ class GPT:
             if branch is None:
                 h, hq = self._norm(x, gamma)
                 return x, h, hq
+            if dropped and c.block_norm == "pre":
+                x = self._drop(branch, next(sites), x)
+                h, hq = self._norm(x, gamma)
+                return x, h, hq
+            if dropped:
+                branch = self._drop(branch, next(sites))
             if c.block_norm == "sandwich":
                 return self._junction(x, branch, behind[0], gamma, behind[1], behind[2], want_q)
             if not fuse:
@@ -397,6 +479,7 @@ class GPT:
             else:
                 q, k, v = (self._mm(h, lp[n], hq) for n in ("wq", "wk", "wv"))
             q, k, v = (t.view(B, T, c.n_heads, c.head_dim) for t in (q, k, v))
+            q, k = self._place(q, k, lp)
             o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True)
             if self.exchange is not None and torch.is_grad_enabled():
                 o = _ExchangePoint.apply(o, self.exchange)
@@ -404,8 +487,10 @@ class GPT:
             # the attention output feeds one linear: both its quantised forms from one read when a backward pass follows
             oq = fp8.QuantizedActivation.both(o) if (c.mm == "fp8" and torch.is_grad_enabled() and o.shape[-1] % 128 == 0) else None
             branch = self._mm(o, lp["wo"], oq)
-            x, h, hq = norm_after(x, branch, lp["norm2"], behind=(h, lp, 1))        # model.py:68, :77
-            if c.mm == "fp8" and c.mlp == "fused":
+            x, h, hq = norm_after(x, branch, lp["norm2"], want_q=not self.gated, behind=(h, lp, 1))     # model.py:68, :77
+            if self.gated:
+                branch = self._mm(self._gated(h, lp), lp["w_down"])
+            elif c.mm == "fp8" and c.mlp == "fused":
                 branch = _FusedMLP.apply(h, hq, lp["w_up"], lp["w_down"], c.activation)
             else:
                 branch = self._mm(self._act(self._mm(h, lp["w_up"], hq)), lp["w_down"])
@@ -487,10 +572,11 @@ class Trainer:
             self.model.exchange = self.buckets
         if direct:
             skip = () if (side_by_side or not fused_qkv) else ("wq", "wk", "wv")    # three slices of one GEMM result: autograd adds them
-            self.buckets.enable_direct([lp[n] for lp in self.model.layers for n in ("wq", "wk", "wv", "wo", "w_up", "w_down")
-                                        if n not in skip])
+            self.buckets.enable_direct([lp[n] for lp in self.model.layers for n in self.model.linears() if n not in skip])
         self._want_graph = bool(graph) and on_gpu
         self._graph = None
+        if self.model.dropout_seed is not None and torch.distributed.is_available() and torch.distributed.is_initialized():
+            self.model.dropout_seed.add_(torch.distributed.get_rank() << 40)         # every rank draws masks of its own
         if self._fused_opt:
             flat = None
             if cfg.flat_parameters:
@@ -511,6 +597,7 @@ class Trainer:
         c, b = self.cfg, self.buckets
         h = c.n_heads * c.head_dim
         if not (torch.device(self.device).type == "cuda" and c.block_norm == "pre" and c.mm == "fp8" and c.norm == "fused" and c.mlp == "fused" and c.qkv == "fused"
+                and c.positions == "learned" and not c.qk_norm and c.dropout == 0
                 and c.residual == "fused" and c.loss == "fused" and self._fused_opt and c.flat_parameters and c.direct_grads
                 and c.activation in ("gelu", "relu2") and c.d_model <= ops.ADD_NORM_MAX_COLS
                 and not (c.d_model % 128 or h % 128 or c.d_ff % 128)):
@@ -542,6 +629,8 @@ class Trainer:
             if out is not None:                   # (None: a parameter is frozen or has a gradient hook)
                 return out
         self.buckets.zero()
+        if self.model.dropout_seed is not None:
+            self.model.dropout_seed.add_(1)
         loss = self.model.loss(ids, targets) if teacher is None else self.model.distillation_loss(ids, targets, teacher)
         loss.backward()
         self.buckets.finish()
@@ -573,6 +662,8 @@ class Trainer:
         params = self.model.parameters()
         saved_p = [p.detach().clone() for p in params]
         saved_s = {id(t): t.clone() for t in self._opt_state_tensors()}
+        seed = self.model.dropout_seed
+        saved_seed = None if seed is None else seed.clone()
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
@@ -587,6 +678,8 @@ class Trainer:
                     t.copy_(saved_s[id(t)])
                 else:
                     t.zero_()                       # state created by the warm-up: back to its initial value
+            if seed is not None:
+                seed.copy_(saved_seed)
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
@@ -654,7 +747,7 @@ def synthetic_batch(cfg: StepConfig, batch: int, device, seed: int, learnable=Fa
 def step_flops(cfg: StepConfig, tokens: int) -> float:
     """The reference's estimator 6 * L * layer_params * tokens (bench.py:96-102)."""
     d, h, ff = cfg.d_model, cfg.n_heads * cfg.head_dim, cfg.d_ff
-    layer_params = 3 * d * h + h * d + 2 * d * ff
+    layer_params = 3 * d * h + h * d + (3 if cfg.activation in GATED else 2) * d * ff
     return 6.0 * cfg.n_layers * layer_params * tokens
 
 
