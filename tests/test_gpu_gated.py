@@ -111,6 +111,8 @@ def test_leading_axes_strides_and_alignment():
         want = kernels.gated_linear(x, wg, wu)
         for a, b, c in ((wide[:, 8:72], both[:, :72], both[:, 72:]), (shifted, wg.T.contiguous().T, wu)):
             assert torch.equal(kernels.gated_linear(a, b, c), want)
+    one = kernels.gated_linear(x[3], wg, wu)                                      # a token without a leading axis
+    assert one.shape == (72,) and torch.equal(one, kernels.gated_linear(x[3:4], wg, wu)[0])
     row = x[:1].expand(60, 64)
     assert torch.equal(kernels.gated_linear(row, wg, wu)[7:8], kernels.gated_linear(row, wg, wu)[:1])
 

@@ -833,9 +833,9 @@ static int gated_check(const tg_gated_args* a) {
   if (a->ldx < a->cols || a->ld_gate < a->inner || a->ld_up < a->inner) return TG_ERR_SHAPE;
   const int64_t most = int64_t(1) << 30;
   if (a->rows > most || a->cols > most || a->inner > most) return TG_ERR_TOO_LARGE;
-  auto tiles = [](int64_t n, int64_t t) { return (n + t - 1) / t; };
+  auto tiles = [](int64_t n, int64_t t) { return (n + t - 1) / t; };      // (every grid and every item number fits an int)
   if (tiles(a->rows, 256) * tiles(a->inner, 128) > INT32_MAX / 2 || tiles(a->rows, 256) * tiles(a->cols, 256) > INT32_MAX / 2 ||
-      2 * tiles(a->cols, 256) * tiles(a->inner, 256) > INT32_MAX / 2)
+      2 * tiles(a->cols, 256) * tiles(a->inner, 256) > INT32_MAX / 2 || tiles(a->rows, 64) * tiles(a->inner, 64) > INT32_MAX)
     return TG_ERR_TOO_LARGE;
   return TG_OK;
 }

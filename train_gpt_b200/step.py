@@ -489,7 +489,8 @@ class GPT:
             branch = self._mm(o, lp["wo"], oq)
             x, h, hq = norm_after(x, branch, lp["norm2"], want_q=not self.gated, behind=(h, lp, 1))     # model.py:68, :77
             if self.gated:
-                branch = self._mm(self._gated(h, lp), lp["w_down"])
+                a = self._gated(h, lp)
+                branch = self._mm(a, lp["w_down"], fp8.QuantizedActivation.both(a) if c.mm == "fp8" and torch.is_grad_enabled() and c.d_ff % 128 == 0 else None)
             elif c.mm == "fp8" and c.mlp == "fused":
                 branch = _FusedMLP.apply(h, hq, lp["w_up"], lp["w_down"], c.activation)
             else:
