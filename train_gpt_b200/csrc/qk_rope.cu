@@ -15,8 +15,8 @@
 // warps where there are few tokens.
 //
 // Pieces come through slots in shared memory by cp.async, rounds of heads ahead and across tokens, so that a warp never waits for a whole
-// round trip; a lane reads only what it fetched itself.  32768 tokens (of 32 + 8 heads of 128 / 16 + 16 heads of 64): forward 108 / 48.5 us (6.2 / 5.5
-// TB/s), rotation alone 117, backward 166 / 76.5 (6.1 / 5.3 TB/s); loads straight into registers 118 / 52, 107, 206 / 92.
+// round trip; a lane reads only what it fetched itself.  32768 tokens (of 32 + 8 heads of 128 / 16 + 16 heads of 64): forward 107 / 48.5 us (6.3 / 5.5
+// TB/s), backward 164 / 76 (6.1 / 5.3 TB/s); loads straight into registers 118 / 52 and 206 / 92.
 #include <math.h>
 
 #include <algorithm>
@@ -155,7 +155,7 @@ __device__ __forceinline__ void qk_scale(const QkPart& q, const QkLane<G, INTER>
 }
 
 // Warps of a block, of which an SM has one: a grid of small blocks that leaves room for more of them is spread unevenly where the launch before it
-// ends, and the SM with most of them ends last (32768 tokens of 40 heads of 128, rotated alone: 123 us in blocks of four warps, 117 so).  Twelve backward:
+// ends, and the SM with most of them ends last (32768 tokens of 40 heads of 128, rotated alone through slots: 123 us in blocks of four warps, 117 so).  Twelve backward:
 // with 164 registers that is what fits; at sixteen the sums spill (32 x 1024 tokens of 32 heads of 64: 76 us, 112 with spills).
 constexpr int kQkFwdWarps = 16, kQkBwdWarps = 12, kQkFewWarps = 4;
 // Slots of a warp: more measured slower (forward with eight 110 us for 108 at 32768 tokens of 40 heads of 128, backward with seven 170 for 166).
@@ -243,7 +243,7 @@ struct QkStream {
   }
 };
 
-template <int G, bool NORM, bool INTER>
+template <int G, bool INTER>
 __global__ void __launch_bounds__(kQkFwdWarps * 32, 1) qk_fwd_kernel(const __grid_constant__ QkParams p) {
   extern __shared__ __align__(16) uint8_t s_qk[];
   constexpr int RW = 32 / G;
@@ -270,14 +270,12 @@ __global__ void __launch_bounds__(kQkFwdWarps * 32, 1) qk_fwd_kernel(const __gri
       const int64_t out_step = int64_t(p.dim) * next;
       QkTurn a;
       qk_turn(l, s_at.cs, a);
-      if constexpr (NORM) {                    // the scale goes into the coefficients
-        float2 v[8];
-        qk_scale(q, l, v);
+      float2 w[8];                             // the scale goes into the coefficients
+      qk_scale(q, l, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          a.from[j] = __fmul2_rn(a.from[j], v[j]);
-          a.across[j] = __fmul2_rn(a.across[j], qk_other<INTER>(v, j));
-        }
+      for (int j = 0; j < 8; ++j) {
+        a.from[j] = __fmul2_rn(a.from[j], w[j]);
+        a.across[j] = __fmul2_rn(a.across[j], qk_other<INTER>(w, j));
       }
 #pragma unroll 1
       for (int round = 0; round < q.rounds; ++round) {
@@ -285,27 +283,82 @@ __global__ void __launch_bounds__(kQkFwdWarps * 32, 1) qk_fwd_kernel(const __gri
         // (a lane of a head that does not exist works on what its slot held before: its sums stay in its group, and nothing is stored)
         float2 v[8];
         qk_unpack(lds128(slot), lds128(slot + 512), v);
-        if constexpr (NORM) {
-          float2 s2 = __fmul2_rn(v[0], v[0]), t2 = __fmul2_rn(v[1], v[1]);
+        float2 s2 = __fmul2_rn(v[0], v[0]), t2 = __fmul2_rn(v[1], v[1]);
 #pragma unroll
-          for (int j = 2; j < 8; j += 2) {
-            s2 = __ffma2_rn(v[j], v[j], s2);
-            t2 = __ffma2_rn(v[j + 1], v[j + 1], t2);
-          }
-          const float s = qk_sum<G>((s2.x + t2.x) + (s2.y + t2.y));
-          const float2 rn = qk_splat(__frsqrt_rn(fmaf(s, inv_dim, p.eps)));
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = __fmul2_rn(v[j], rn);
+        for (int j = 2; j < 8; j += 2) {
+          s2 = __ffma2_rn(v[j], v[j], s2);
+          t2 = __ffma2_rn(v[j + 1], v[j + 1], t2);
         }
+        const float s = qk_sum<G>((s2.x + t2.x) + (s2.y + t2.y));
+        const float2 rn = qk_splat(__frsqrt_rn(fmaf(s, inv_dim, p.eps)));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __fmul2_rn(v[j], rn);
         if (l.rot) {
           qk_rotate<INTER>(v, a);
-        } else if (NORM) {
+        } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = __fmul2_rn(v[j], a.from[j]);
         }
         if (l.on && head < q.heads) qk_store(out, delta, v);
         out += out_step;
         head += next;
+      }
+    }
+  }
+}
+
+// The rotation alone (without scales, and backward without them): nothing waits for a sum, and loads straight into registers, four rounds at a time in
+// blocks of four warps, four of them at a time on an SM, are ahead of the slots: 32768 tokens of 40 heads of 128 105 us (6.4 TB/s), 117 through slots;
+// two rounds at a time 107, one 116.
+constexpr int kQkTurnWarps = 4, kQkTurnRounds = 4, kQkTurnPerSm = 8;
+template <int G, bool INTER>
+__global__ void __launch_bounds__(kQkTurnWarps * 32, kQkTurnPerSm / 2) qk_turn_kernel(const __grid_constant__ QkParams p) {
+  extern __shared__ __align__(16) uint8_t s_qk[];
+  constexpr int RW = 32 / G, U = kQkTurnRounds;
+  const QkLane<G, INTER> l(p);
+  const QkShared s_at(s_qk, p.rotary, l.warp, kQkTurnWarps);
+  for (int i = threadIdx.x; i < p.rotary / 2; i += blockDim.x) s_at.turns[i] = p.turns[i];
+  __syncthreads();
+  grid_trigger();
+  grid_wait();
+  const int delta = l.hi - l.lo, next = p.splits * RW;
+  const uint64_t items = uint64_t(p.n_tokens) * uint32_t(p.splits), step = uint64_t(gridDim.x) * kQkTurnWarps;
+  for (uint64_t item = uint64_t(blockIdx.x) * kQkTurnWarps + l.warp; item < items; item += step) {
+    const uint32_t n = p.splits == 1 ? uint32_t(item) : uint32_t(item / uint32_t(p.splits));
+    const uint32_t b = n / p.tokens, t = n - b * p.tokens;
+    const int first = int(item - uint64_t(n) * uint32_t(p.splits)) * RW + l.row;
+    QkTurn a;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const QkPart& q = p.part[i];
+      int head = first;
+      const __nv_bfloat16* in = q.x.at + (int64_t(b) * q.x.batch + int64_t(t) * q.x.token + int64_t(head) * q.x.head + l.lo);
+      __nv_bfloat16* out = q.out + (int64_t(n) * q.heads + head) * p.dim + l.lo;
+      const int64_t in_step = q.x.head * next, out_step = int64_t(p.dim) * next;
+      for (int round = 0; round < q.rounds; round += U) {
+        uint4 x[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          x[u][0] = x[u][1] = make_uint4(0u, 0u, 0u, 0u);
+          if (l.on && head + u * next < q.heads) {        // (a round beyond the last has no heads)
+            x[u][0] = ld_stream_v4(in);
+            x[u][1] = ld_stream_v4(in + delta);
+          }
+          in += in_step;
+        }
+        if (i == 0 && round == 0) {
+          qk_angles(p, l.lane, s_at.turns, s_at.cs, b, t);
+          qk_turn(l, s_at.cs, a);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float2 v[8];
+          qk_unpack(x[u][0], x[u][1], v);
+          if (l.rot) qk_rotate<INTER>(v, a);
+          if (l.on && head < q.heads) qk_store(out, delta, v);
+          out += out_step;
+          head += next;
+        }
       }
     }
   }
@@ -427,21 +480,23 @@ __global__ void __launch_bounds__(1024) qk_scale_reduce_kernel(const float* part
 
 static int qk_group(int dim) { return std::max(2, pow2_at_least(dim / 16)); }
 
-// How many warps share a token, so that few tokens still give every SM some, and the launch: a block per SM, or small ones where there is less
-// than one for each.
+// How many warps share a token, so that few tokens still give every SM some, and the launch: as many blocks as an SM has of them, or small ones
+// where there is less.
 struct QkGeom {
   int splits, rounds[2], warps, blocks;
 };
-static QkGeom qk_geom(const tg_qk_args* a, int warps) {
+static QkGeom qk_geom(const tg_qk_args* a, int warps, int blocks_per_sm) {
   const int rw = 32 / qk_group(a->dim), all[2] = {(a->heads + rw - 1) / rw, (a->kv_heads + rw - 1) / rw};
-  const int64_t n = a->batch * a->tokens, sms = sm_count();
+  const int64_t n = a->batch * a->tokens, most = int64_t(sm_count()) * blocks_per_sm * warps;
   QkGeom g;
-  g.splits = int(std::max<int64_t>(1, std::min<int64_t>(std::max(all[0], all[1]), sms * warps / std::max<int64_t>(n, 1))));
+  g.splits = int(std::max<int64_t>(1, std::min<int64_t>(std::max(all[0], all[1]), most / std::max<int64_t>(n, 1))));
   for (int i = 0; i < 2; ++i) g.rounds[i] = (all[i] + g.splits - 1) / g.splits;
-  g.warps = n * g.splits < sms * warps ? kQkFewWarps : warps;
-  g.blocks = int(std::min<int64_t>((n * g.splits + g.warps - 1) / g.warps, g.warps == warps ? sms : int64_t(INT32_MAX)));
+  g.warps = n * g.splits < most ? std::min(warps, kQkFewWarps) : warps;
+  g.blocks = int(std::min<int64_t>(n * g.splits, most) / g.warps + (std::min<int64_t>(n * g.splits, most) % g.warps != 0));
   return g;
 }
+static QkGeom qk_geom_fwd(const tg_qk_args* a) { return a->q_scale != nullptr ? qk_geom(a, kQkFwdWarps, 1) : qk_geom(a, kQkTurnWarps, kQkTurnPerSm); }
+static QkGeom qk_geom_bwd(const tg_qk_args* a) { return a->q_scale != nullptr ? qk_geom(a, kQkBwdWarps, 1) : qk_geom(a, kQkTurnWarps, kQkTurnPerSm); }
 
 static bool qk_sizes_ok(const tg_qk_args* a) {
   return a->batch >= 0 && a->tokens >= 0 && a->heads >= 1 && a->kv_heads >= 1 && a->dim >= 16 && a->dim % 16 == 0 && a->rotary_dim >= 0 &&
@@ -479,19 +534,20 @@ static QkParams qk_params(const tg_qk_args* a, const QkGeom& g, bool backward) {
   return p;
 }
 
-template <int G, bool NORM, bool INTER>
+template <int G, bool INTER>
 static int launch_qk_fwd(const QkParams& p, const QkGeom& g, cudaStream_t st) {
   static std::atomic<bool> done[64];
   constexpr int most = kQkMaxDim * 4 * (1 + kQkFwdWarps) + kQkFwdWarps * kQkFwdSlots * 1024;
   static_assert(most <= 227 * 1024, "slots exceed shared memory");
-  if (int rc = allow_smem(qk_fwd_kernel<G, NORM, INTER>, most, done)) return rc;
-  TG_CUDA_CHECK(launch_early(qk_fwd_kernel<G, NORM, INTER>, g.blocks, g.warps * 32, qk_shared_bytes(p.rotary, g.warps, kQkFwdSlots * 1024), st, p));
+  if (int rc = allow_smem(qk_fwd_kernel<G, INTER>, most, done)) return rc;
+  TG_CUDA_CHECK(launch_early(qk_fwd_kernel<G, INTER>, g.blocks, g.warps * 32, qk_shared_bytes(p.rotary, g.warps, kQkFwdSlots * 1024), st, p));
   return TG_OK;
 }
 template <int G>
 static int launch_qk_fwd(const QkParams& p, const QkGeom& g, bool norm, bool inter, cudaStream_t st) {
-  if (norm) return inter ? launch_qk_fwd<G, true, true>(p, g, st) : launch_qk_fwd<G, true, false>(p, g, st);
-  return inter ? launch_qk_fwd<G, false, true>(p, g, st) : launch_qk_fwd<G, false, false>(p, g, st);
+  if (norm) return inter ? launch_qk_fwd<G, true>(p, g, st) : launch_qk_fwd<G, false>(p, g, st);
+  TG_CUDA_CHECK(launch_early(inter ? qk_turn_kernel<G, true> : qk_turn_kernel<G, false>, g.blocks, g.warps * 32, qk_shared_bytes(p.rotary, g.warps, 0), st, p));
+  return TG_OK;
 }
 template <int G, bool INTER>
 static int launch_qk_bwd(const QkParams& p, const QkGeom& g, cudaStream_t st) {
@@ -525,7 +581,7 @@ extern "C" int tg_qk_norm_rope_fwd(const tg_qk_args* a, void* stream) {
       !qk_strides_ok(a->q_stride) || !qk_strides_ok(a->k_stride))
     return TG_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
-  const QkGeom g = qk_geom(a, kQkFwdWarps);
+  const QkGeom g = qk_geom_fwd(a);
   const QkParams p = qk_params(a, g, false);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool norm = a->q_scale != nullptr, inter = a->interleaved != 0;
@@ -540,7 +596,7 @@ extern "C" int tg_qk_norm_rope_fwd(const tg_qk_args* a, void* stream) {
 
 extern "C" int64_t tg_qk_norm_rope_bwd_scratch_bytes(const tg_qk_args* a) {
   if (qk_check(a) != TG_OK || a->batch == 0 || a->tokens == 0 || a->q_scale == nullptr) return 0;
-  return int64_t(qk_geom(a, kQkBwdWarps).blocks) * 2 * a->dim * int64_t(sizeof(float));
+  return int64_t(qk_geom_bwd(a).blocks) * 2 * a->dim * int64_t(sizeof(float));
 }
 
 extern "C" int tg_qk_norm_rope_bwd(const tg_qk_args* a, void* stream) {
@@ -562,7 +618,7 @@ extern "C" int tg_qk_norm_rope_bwd(const tg_qk_args* a, void* stream) {
                !qk_strides_ok(a->q_stride) || !qk_strides_ok(a->k_stride)))
     return TG_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
-  const QkGeom g = qk_geom(a, norm ? kQkBwdWarps : kQkFwdWarps);
+  const QkGeom g = qk_geom_bwd(a);
   const QkParams p = qk_params(a, g, true);
   int rc = TG_OK;
   switch (qk_group(a->dim)) {
