@@ -284,7 +284,7 @@ int tg_qk_norm_rope_bwd(const tg_qk_args* args, void* stream);
 /* No counterpart in the reference.  h = act(x w_gate) * (x w_up) in bf16 with float32 accumulation and one rounding: both projections, the
  * activation and the product in one kernel.
  *   x         bf16 [rows, cols], row pitch ldx;  w_gate, w_up  bf16 [cols, inner], row pitches ld_gate, ld_up;  h bf16 [rows, inner]
- *             cols, inner and the pitches multiples of 8, pointers 16-byte aligned, sizes up to 2^30
+ *             cols, inner and the pitches multiples of 8, pointers 16-byte aligned; rows up to 2^30, cols and inner up to 2^26
  *   saved_gate, saved_up, saved_exponents   what the backward pass needs, all or none: [rows, inner] of 16 bits each and
  *             tg_gated_linear_exponent_bytes(rows, inner) bytes; 16-byte aligned
  *   status    a device word as in tg_gemm_args, or NULL

@@ -147,7 +147,7 @@ def test_gated_entries(lib):
     for kw in (dict(rows=-1), dict(cols=60), dict(inner=60), dict(cols=0), dict(inner=0), dict(act=3), dict(act=-1), dict(ldx=56), dict(ld_gate=64), dict(ld_up=64),
                dict(saved_gate=None), dict(saved_up=None), dict(saved_exponents=None), dict(x=None), dict(w_gate=None), dict(w_up=None)):
         assert [f(_gated(**kw), None) for f in both] == [TG_ERR_SHAPE] * 2, kw
-    for kw in (dict(rows=2 ** 30 + 1), dict(cols=2 ** 30 + 8, ldx=2 ** 30 + 8), dict(rows=2 ** 30, inner=2 ** 30, ld_gate=2 ** 30, ld_up=2 ** 30)):
+    for kw in (dict(rows=2 ** 30 + 1), dict(cols=2 ** 26 + 8, ldx=2 ** 26 + 8), dict(inner=2 ** 26 + 8, ld_gate=2 ** 27, ld_up=2 ** 27), dict(rows=2 ** 30, inner=2 ** 26, ld_gate=2 ** 26, ld_up=2 ** 26)):
         assert [f(_gated(**kw), None) for f in both] == [TG_ERR_TOO_LARGE] * 2, kw
     for kw in (dict(x=A[0] + 2), dict(w_up=A[0] + 8), dict(ldx=68), dict(ld_gate=76), dict(saved_gate=A[0] + 2), dict(saved_exponents=A[0] + 1)):
         assert [f(_gated(**kw), None) for f in both] == [TG_ERR_ALIGN] * 2, kw

@@ -831,8 +831,8 @@ static int gated_check(const tg_gated_args* a) {
   if (a == nullptr || a->rows < 0 || a->cols < 8 || a->inner < 8 || a->cols % 8 != 0 || a->inner % 8 != 0) return TG_ERR_SHAPE;
   if (a->act != TG_GATED_SILU && a->act != TG_GATED_GELU && a->act != TG_GATED_RELU) return TG_ERR_SHAPE;
   if (a->ldx < a->cols || a->ld_gate < a->inner || a->ld_up < a->inner) return TG_ERR_SHAPE;
-  const int64_t most = int64_t(1) << 30;
-  if (a->rows > most || a->cols > most || a->inner > most) return TG_ERR_TOO_LARGE;
+  // (a tile's contraction stays far below what its barriers' waits are bounded by)
+  if (a->rows > int64_t(1) << 30 || a->cols > int64_t(1) << 26 || a->inner > int64_t(1) << 26) return TG_ERR_TOO_LARGE;
   auto tiles = [](int64_t n, int64_t t) { return (n + t - 1) / t; };      // (every grid and every item number fits an int)
   if (tiles(a->rows, 256) * tiles(a->inner, 128) > INT32_MAX / 2 || tiles(a->rows, 256) * tiles(a->cols, 256) > INT32_MAX / 2 ||
       2 * tiles(a->cols, 256) * tiles(a->inner, 256) > INT32_MAX / 2 || tiles(a->rows, 64) * tiles(a->inner, 64) > INT32_MAX)
@@ -1017,6 +1017,10 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
     return TG_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
   if (!dx && !dw) return TG_OK;
+  GatedTiles data_tiles, weights_tiles;
+  gated_tiles(a, data_tiles, weights_tiles);
+  if (a->scratch_bytes < tg_gated_linear_bwd_scratch_bytes(a)) data_tiles.ranges = weights_tiles.ranges = 1;
+  if (weights_tiles.blocks / weights_tiles.ranges > 1 << 21) return TG_ERR_TOO_LARGE;
   GatedSlopes s = {};
   s.g = static_cast<const __nv_bfloat16*>(a->g);
   s.gate = static_cast<const __half*>(a->saved_gate);
@@ -1031,9 +1035,6 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
   auto kern = a->act == TG_GATED_SILU ? gated_slopes_kernel<TG_GATED_SILU> : a->act == TG_GATED_GELU ? gated_slopes_kernel<TG_GATED_GELU> : gated_slopes_kernel<TG_GATED_RELU>;
   TG_CUDA_CHECK(launch_if_short(items <= 8 * sm_count(), kern, dim3(unsigned(items)), kGsThreads, 0, st, s));
 
-  GatedTiles data_tiles, weights_tiles;
-  gated_tiles(a, data_tiles, weights_tiles);
-  if (a->scratch_bytes < tg_gated_linear_bwd_scratch_bytes(a)) data_tiles.ranges = weights_tiles.ranges = 1;
   GatedProblem data = {}, weights = {};
   GatedJoin joins[2] = {};
   int n_joins = 0;
