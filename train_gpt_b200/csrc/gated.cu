@@ -521,8 +521,8 @@ __global__ void __launch_bounds__(256) gated_join_kernel(const __grid_constant__
 
 // ---- few tokens ----------------------------------------------------------------------------------------------------
 
-// Up to 128 tokens: bound by the pass over the weights, so the tiles are made for that.  A block has 64 columns of h (128
-// of the accumulator: the gate's, then the up-projection's) and one row tile, two blocks run on an SM, and where there are fewer tiles than
+// Few tokens are bound by the pass over the weights, so the tiles are made for that (and small problems, which are launches and ramps, have more of
+// them to share out; few_plan).  A block has 128 rows and 64 columns of h (128 of the accumulator: the gate's, then the up-projection's), two blocks run on an SM, and where there are fewer tiles than
 // places for them the contraction is cut into up to eight ranges, a cluster's blocks one each: their partial sums meet in shared memory,
 // in the order of the ranges, and the blocks share the rows out.  (All places busy at once is what counts: 1 x 4096 -> 11008 has 86 tiles of 128 columns for 74 pairs, 55 us there.)
 // A stage holds no more rows of x than there are, in boxes of eight at least: rows of a box that lie outside the tensor are not free
@@ -539,6 +539,7 @@ struct GatedFew {
   __half *saved_gate, *saved_up;
   uint8_t* exponents;
   int rows, inner, blocks;                      // blocks: stages of the whole contraction
+  int tiles_m;                                  // row tiles, the blocks of a column tile's side by side
   int stages;                                   // of the ring
   int x_rows, x_boxes;                          // rows of x in a stage: boxes of a multiple of eight rows
 };
@@ -560,11 +561,12 @@ __device__ __forceinline__ float4 lds_cluster(uint32_t addr) {
 // This block's share of the rows, sixteen lanes each: the ranges' partial sums, all on their way at once and added up in order, then h and
 // what the backward pass needs.
 template <int ACT, bool SAVE, int RANGES>
-__device__ __forceinline__ void few_join(const GatedFew& p, uint32_t sums, uint32_t rank, int n0) {
+__device__ __forceinline__ void few_join(const GatedFew& p, uint32_t sums, uint32_t rank, int m0, int n0) {
   const int lane = threadIdx.x & 31, col = 4 * (lane & 15);
-  for (int i = 2 * int(threadIdx.x >> 5); i * RANGES < p.rows; i += 2 * kGfThreads / 32) {
+  const int rows = min(kGfRows, p.rows - m0);
+  for (int i = 2 * int(threadIdx.x >> 5); i * RANGES < rows; i += 2 * kGfThreads / 32) {
     const int row = (i + (lane >> 4)) * RANGES + int(rank);
-    const bool there = row < p.rows;
+    const bool there = row < rows;
     float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
     if (there) {
       const uint32_t from = sums + uint32_t(row * kGfPitch + col) * 4u;
@@ -584,7 +586,7 @@ __device__ __forceinline__ void few_join(const GatedFew& p, uint32_t sums, uint3
       }
     }
     const bool stores = there && n0 + col < p.inner;
-    const int64_t at = int64_t(row) * p.inner + n0 + col;
+    const int64_t at = int64_t(m0 + row) * p.inner + n0 + col;
     if constexpr (SAVE) {
       uint32_t e[2];
 #pragma unroll
@@ -597,7 +599,7 @@ __device__ __forceinline__ void few_join(const GatedFew& p, uint32_t sums, uint3
         e[which] = save_exponent(m, scale);
         if (stores) *reinterpret_cast<uint2*>((which ? p.saved_up : p.saved_gate) + at) = make_uint2(pack_f16x2(v.x * scale, v.y * scale), pack_f16x2(v.z * scale, v.w * scale));
       }
-      if (there && col == 0) reinterpret_cast<uint16_t*>(p.exponents)[int64_t(n0 / kGfCols) * p.rows + row] = uint16_t(e[0] | e[1] << 8);
+      if (there && col == 0) reinterpret_cast<uint16_t*>(p.exponents)[int64_t(n0 / kGfCols) * p.rows + m0 + row] = uint16_t(e[0] | e[1] << 8);
     }
     if (stores)
       *reinterpret_cast<uint2*>(p.h + at) =
@@ -624,7 +626,7 @@ __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_c
   uint32_t ranges;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranges));
   const uint32_t rank = cluster_rank();
-  const int n0 = int(blockIdx.x / ranges) * kGfCols;
+  const int tile = int(blockIdx.x / ranges), n0 = tile / p.tiles_m * kGfCols, m0 = (tile - tile / p.tiles_m * p.tiles_m) * kGfRows;
   const int first = int(uint64_t(p.blocks) * rank / ranges), last = int(uint64_t(p.blocks) * (rank + 1) / ranges);
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -654,7 +656,7 @@ __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_c
         mbar_expect_tx(fb, stage_bytes);
         tma_load_2d(dst + x_bytes, &p.gate, fb, n0, kb * kGbK);
         tma_load_2d(dst + x_bytes + kGbBox, &p.up, fb, n0, kb * kGbK);
-        for (int i = 0; i < p.x_boxes; ++i) tma_load_2d(dst + i * kGbBox, &p.x, fb, kb * kGbK, 64 * i);
+        for (int i = 0; i < p.x_boxes; ++i) tma_load_2d(dst + i * kGbBox, &p.x, fb, kb * kGbK, m0 + 64 * i);
       }
       __syncwarp();
       if (++s == uint32_t(p.stages)) { s = 0; ph ^= 1u; }
@@ -688,7 +690,7 @@ __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_c
   const bool ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0u, abort_flag, status, 5u)) && !*abort_flag;
   __syncwarp();
   tc_fence_after();
-  if (warp < 4 && ok && warp * 32 < p.rows) {
+  if (warp < 4 && ok && m0 + warp * 32 < p.rows) {
     const uint32_t at = tmem_base + (uint32_t(warp * 32) << 16);
     const int row = warp * 32 + lane;
     uint32_t g0[32], g1[32], u0[32], u1[32];
@@ -700,7 +702,7 @@ __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_c
     tmem_wait_ld(g1);
     tmem_wait_ld(u0);
     tmem_wait_ld(u1);
-    if (row < p.rows) {
+    if (m0 + row < p.rows) {
       const uint32_t to = sbase + uint32_t(row) * (kGfPitch * 4);
 #pragma unroll
       for (int c = 0; c < 32; ++c) {
@@ -712,10 +714,10 @@ __global__ void __launch_bounds__(kGfThreads, 2) gated_few_kernel(const __grid_c
   __syncwarp();
   cluster_sync();                              // the partial sums are there
   if (ok) {
-    if (ranges == 1) few_join<ACT, SAVE, 1>(p, sbase, rank, n0);
-    else if (ranges == 2) few_join<ACT, SAVE, 2>(p, sbase, rank, n0);
-    else if (ranges == 4) few_join<ACT, SAVE, 4>(p, sbase, rank, n0);
-    else few_join<ACT, SAVE, 8>(p, sbase, rank, n0);
+    if (ranges == 1) few_join<ACT, SAVE, 1>(p, sbase, rank, m0, n0);
+    else if (ranges == 2) few_join<ACT, SAVE, 2>(p, sbase, rank, m0, n0);
+    else if (ranges == 4) few_join<ACT, SAVE, 4>(p, sbase, rank, m0, n0);
+    else few_join<ACT, SAVE, 8>(p, sbase, rank, m0, n0);
   }
   __syncwarp();
   cluster_sync();                              // the partners have read this block's sums
@@ -844,6 +846,31 @@ static bool gated_aligned(const tg_gated_args* a) {
 }
 static int64_t gated_chunks(int64_t inner) { return (inner + 63) / 64; }
 
+// Whether that kernel takes a problem, and how.
+struct FewPlan {
+  int tiles_m = 1, tiles = 0, ranges = 1;
+  bool takes = false;
+};
+static FewPlan few_plan(const tg_gated_args* a) {
+  FewPlan f;
+  const int64_t tiles_m = (a->rows + kGfRows - 1) / kGfRows, tiles = tiles_m * ((a->inner + kGfCols - 1) / kGfCols), blocks = (a->cols + kGbK - 1) / kGbK;
+  const int64_t places = 2 * sm_count(), rows = std::min<int64_t>(a->rows, kGfRows);
+  if (a->rows > 64 && tiles > places) return f;
+  // As many ranges as find a place at once, of four stages at least and of one per eight tokens, whose sums take their time to meet: 128 x 1024 -> 4096
+  // 10.5 us in one range, 12.5 in four; 128 x 4096 -> 4096 28.7 and 19.9; 16 x 1024 -> 4096 6.9 in four.
+  while (f.ranges < 8 && tiles * f.ranges * 2 <= places && blocks >= 8 * f.ranges && 8 * (blocks / (2 * f.ranges)) >= rows) f.ranges *= 2;
+  f.tiles_m = int(tiles_m);
+  f.tiles = int(tiles);
+  // Beyond 64 tokens by what the two take, in microseconds (a stage costs a block 0.2 with few of them and 0.45 with 128 and more, a pair's tile
+  // 0.3): 1024 x 8192 -> 1024 32.8 here, 43 on pairs; 256 x 4096 -> 4096 21.5 and 25; 512 x 2048 -> 2048 13.5 and 14.8, 768 18.6 and 15.8; 300 x
+  // 1024 -> 1024 7.9 and 9.2; 129 x 1024 -> 4096 11.2 and 10.1.
+  const int64_t pair_tiles = (a->rows + 255) / 256 * ((a->inner + 127) / 128), pairs = sm_count() / 2;
+  const double stage = 0.14 + 0.31 * std::min(1.0, double(tiles * f.ranges) / 128.0);
+  const double here = 4.0 + (f.ranges > 1 ? 1.5 : 0.0) + stage * double(blocks) / f.ranges;
+  const double on_pairs = 4.3 + 0.3 * double((pair_tiles + pairs - 1) / pairs * (blocks + 3));
+  f.takes = a->rows <= 64 || here < on_pairs;
+  return f;
+}
 template <int ACT, bool SAVE>
 static int launch_few(const GatedFew& p, int tiles, int ranges, int smem, unsigned* status, cudaStream_t st) {
   static std::atomic<bool> done[64];
@@ -866,14 +893,12 @@ static int run_gated_few(const tg_gated_args* a, cudaStream_t st) {
   p.rows = int(a->rows);
   p.inner = int(a->inner);
   p.blocks = int((a->cols + kGbK - 1) / kGbK);
-  const int tiles = int((a->inner + kGfCols - 1) / kGfCols);
-  // As many ranges as find a place at once, of four stages at least and of one per eight tokens, whose sums take their time to meet: 128 x 1024 -> 4096
-  // 10.5 us in one range, 12.5 in four; 128 x 4096 -> 4096 28.7 and 19.9; 16 x 1024 -> 4096 6.9 in four.
-  int ranges = 1;
-  while (ranges < 8 && tiles * ranges * 2 <= 2 * sm_count() && p.blocks >= 8 * ranges && 8 * (p.blocks / (2 * ranges)) >= a->rows) ranges *= 2;
+  const FewPlan plan = few_plan(a);
+  p.tiles_m = plan.tiles_m;
+  const int tiles = plan.tiles, ranges = plan.ranges, rows = int(std::min<int64_t>(a->rows, kGfRows));
   const int stage = p.x_rows * p.x_boxes * 128 + 2 * kGbBox;
   p.stages = std::min(kGfStages, kGfMost / stage);
-  const int smem = std::max(p.stages * stage, int(a->rows) * kGfPitch * 4);
+  const int smem = std::max(p.stages * stage, rows * kGfPitch * 4);
   static_assert(kGfRows * kGfPitch * 4 <= kGfMost, "partial sums fit where the operands were");
   if (a->act == TG_GATED_SILU) return launch_few<TG_GATED_SILU, SAVE>(p, tiles, ranges, smem, a->status, st);
   if (a->act == TG_GATED_GELU) return launch_few<TG_GATED_GELU, SAVE>(p, tiles, ranges, smem, a->status, st);
@@ -912,7 +937,7 @@ extern "C" int tg_gated_linear_fwd(const tg_gated_args* a, void* stream) {
   if (!gated_aligned(a) || !aligned16(a->h) || !aligned16(a->saved_gate) || !aligned16(a->saved_up) || !aligned16(a->saved_exponents)) return TG_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
   const int64_t M = a->rows, D = a->cols, F = a->inner;
-  if (M <= kGfRows) return save ? run_gated_few<true>(a, static_cast<cudaStream_t>(stream)) : run_gated_few<false>(a, static_cast<cudaStream_t>(stream));
+  if (few_plan(a).takes) return save ? run_gated_few<true>(a, static_cast<cudaStream_t>(stream)) : run_gated_few<false>(a, static_cast<cudaStream_t>(stream));
   GatedProblem p = {};
   GatedSaved s = {};
   if (int rc = gated_map(&p.a[0], a->x, false, M, D, a->ldx, 64)) return rc;
