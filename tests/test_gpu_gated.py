@@ -205,6 +205,46 @@ def test_few_tokens_in_graphs():
     ops.check_status()
 
 
+@pytest.mark.parametrize("m,k,f", [(16, 1024, 1024), (300, 1024, 1024), (700, 512, 704)])
+def test_two_streams_and_two_graphs_at_once(m, k, f):
+    """A column tile's rows in one and in several blocks, the contraction in ranges: nothing is shared between calls."""
+    x, wg, wu, _ = _make(m, k, f)
+    xs = [x, x.flip(0).contiguous()]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in xs], [], []
+    with torch.no_grad():
+        want = [kernels.gated_linear(v, wg, wu) for v in xs]
+        for v in xs:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                outs.append(kernels.gated_linear(v, wg, wu))
+        for h in outs:
+            h.fill_(float("nan"))
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        for _ in range(20):
+            for s, g in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    g.replay()
+        alone = []
+        for s, v in zip(streams, xs):
+            with torch.cuda.stream(s):
+                alone.append([kernels.gated_linear(v, wg, wu) for _ in range(5)])
+        torch.cuda.synchronize()
+    assert all(torch.equal(h, w) for h, w in zip(outs, want)) and all(torch.equal(h, w) for hs, w in zip(alone, want) for h in hs)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("m", [5, 100, 300])
+def test_rows_that_share_memory(m):
+    """Expanded and overlapping rows, a column slice with a step."""
+    x, wg, wu, _ = _make(m, 64, 128)
+    wide = _make(m, 128, 128)[0]
+    long = _make(m + 8, 64, 8)[0].flatten()
+    for a, b in ((x[:1].expand(m, 64), wg), (long.as_strided((m, 64), (8, 1)), wg), (wide[:, ::2], wg), (x, wg[:1].expand(64, 128)), (x, wg.t().contiguous().t())):
+        with torch.no_grad():
+            assert torch.equal(kernels.gated_linear(a, b, wu), kernels.gated_linear(a.contiguous(), b.contiguous(), wu))
+
+
 def test_large_negative_gates_and_infinities():
     """silu and gelu go to 0 on the left, not to not-a-number; what is not finite stays in its row."""
     x, wg, wu, g = _make(40, 64, 64)
