@@ -289,10 +289,12 @@ int tg_qk_norm_rope_bwd(const tg_qk_args* args, void* stream);
  *             tg_gated_linear_exponent_bytes(rows, inner) bytes; 16-byte aligned
  *   status    a device word as in tg_gemm_args, or NULL
  * Backward, from the gradient g bf16 [rows, inner] of h and what was saved: dx bf16 [rows, cols] (or NULL), dw_gate and dw_up bf16 [cols, inner]
- * (both or neither).  The gradients at the two projections are rounded to bf16 once before the products.
+ * (both or neither).  The gradients at the two projections are rounded to bf16 once before the products (small problems: to the
+ * sum of two bf16).
  *   scratch   scratch_bytes of it, 16-byte aligned, contents undefined on entry and exit: at least 4 bytes an element of h (each half rounded up to
- *             256); with tg_gated_linear_bwd_scratch_bytes(args) of them, few tiles of a long contraction are cut into ranges and their float32
- *             sums added up in order (dx, dw_gate and cols of args count: results that are not wanted are not planned for)
+ *             256); with tg_gated_linear_bwd_scratch_bytes(args) of them, small problems have their second pieces, and few tiles of a long
+ *             contraction are cut into ranges, their float32 sums added up in order (dx, dw_gate and cols of args count: results that are not
+ *             wanted are not planned for)
  * Deterministic for the same scratch_bytes. */
 #define TG_GATED_SILU 0
 #define TG_GATED_GELU 1

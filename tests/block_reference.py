@@ -69,8 +69,8 @@ def gated(x, wg, wu, name):
     return h, BF * h.abs() + (1.2 * dg + 2.0 ** -20 * g.abs()) * (u.abs() + du) + a.abs() * du + 1e-38
 
 
-def gated_bwd(x, wg, wu, name, grad):
-    """[(dx, how far it may be off), ...] for x and both weights"""
+def gated_bwd(x, wg, wu, name, grad, pieces=1):
+    """[(dx, how far it may be off), ...] for x and both weights; pieces: of bf16 that the gradients at the projections are the sum of"""
     k, (m, f) = x.shape[1], grad.shape
     g, u = x @ wg, x @ wu
     # what the projections are when the backward pass sees them: accumulated, then in fp16 (2^-24: its smallest steps)
@@ -78,12 +78,13 @@ def gated_bwd(x, wg, wu, name, grad):
     a, da = act(g, name)
     bend = (g.abs() <= eg).double() if name == "relu" else 0.8 * eg + 2.0 ** -20 * (1 + g.abs())       # of the derivative
     dg, du = grad * u * da, grad * a
-    err_g = BF * dg.abs() + grad.abs() * (bend * (u.abs() + eu) + 1.2 * eu)
-    err_u = BF * du.abs() + grad.abs() * (1.2 * eg + 2.0 ** -20 * g.abs())
+    r = BF ** pieces                            # (the second is of what the first left, at most BF of it)
+    err_g = r * dg.abs() + grad.abs() * (bend * (u.abs() + eu) + 1.2 * eu)
+    err_u = r * du.abs() + grad.abs() * (1.2 * eg + 2.0 ** -20 * g.abs())
 
     def total(value, parts, n):
         """`value` of products a @ b whose second factor may be off by e, n terms in all"""
-        return value, 1.01 * BF * value.abs() + sum(1.01 * (p.abs() @ e) + n * F32 * (p.abs() @ q.abs()) for p, q, e in parts) + 1e-38
+        return value, 1.01 * BF * value.abs() + sum(1.01 * (p.abs() @ e) + pieces * n * F32 * (p.abs() @ q.abs()) for p, q, e in parts) + 1e-38
 
     dx = (dg @ wg.T + du @ wu.T).T
     dx, e = total(dx, [(wg, dg.T, err_g.T), (wu, du.T, err_u.T)], 2 * f)

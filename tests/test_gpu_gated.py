@@ -245,6 +245,54 @@ def test_rows_that_share_memory(m):
             assert torch.equal(kernels.gated_linear(a, b, wu), kernels.gated_linear(a.contiguous(), b.contiguous(), wu))
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("m,k,f", [(1, 8, 8), (56, 64, 64), (34, 80, 136), (65, 72, 72), (128, 128, 512), (130, 1000, 264), (2, 6488, 136), (500, 40, 1048)])
+def test_small_problems_have_the_gradients_in_two_pieces(act, m, k, f):
+    x, wg, wu, g = _make(m, k, f)
+    leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+    grads = torch.autograd.grad(kernels.gated_linear(*leaves, act), leaves, g)
+    for got, want, name in zip(grads, ref.gated_bwd(*[t.double() for t in (x, wg, wu)], act, g.double(), 2), ("dx", "dw_gate", "dw_up")):
+        _near(got, want, name)
+
+
+def test_an_infinite_gradient_stays_one():
+    """Its second piece is zero, not the not-a-number that is left of it."""
+    x, wg, wu, g = _make(40, 64, 72)
+    g[3, 5] = float("inf")
+    leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+    dx, dg, du = torch.autograd.grad(kernels.gated_linear(*leaves), leaves, g)
+    want = x[3].double() * torch.nn.functional.silu(x[3].double() @ wg.double())[5]
+    assert torch.equal(du[:, 5].isposinf(), want > 0) and torch.equal(du[:, 5].isneginf(), want < 0)
+    rest = torch.ones(72, dtype=torch.bool, device="cuda")
+    rest[5] = False
+    assert torch.isfinite(du[:, rest]).all() and torch.isfinite(dg[:, rest]).all()
+    rows = torch.ones(40, dtype=torch.bool, device="cuda")
+    rows[3] = False
+    assert torch.isfinite(dx[rows]).all() and not torch.isfinite(dx[3]).any()
+
+
+@pytest.mark.parametrize("m,k,f", [(40, 64, 72), (300, 64, 264), (24, 4096, 64)])
+def test_the_least_scratch_does(m, k, f):
+    """The C entry with room for one piece alone."""
+    from train_gpt_b200 import _lib
+    import ctypes
+    lib, (x, wg, wu, g) = _lib.load(), _make(m, k, f)
+    half = (m * f * 2 + 255) // 256 * 256
+    h, kept = torch.empty_like(g), torch.empty(2, m, f, device="cuda", dtype=torch.float16)
+    exponents = torch.empty(lib.tg_gated_linear_exponent_bytes(m, f), device="cuda", dtype=torch.uint8)
+    out = [torch.empty_like(t) for t in (x, wg, wu)]
+    scratch = torch.full((2 * half + 256,), 0x7F, device="cuda", dtype=torch.uint8)
+    args = _lib.GatedArgs(x=x.data_ptr(), ldx=k, w_gate=wg.data_ptr(), ld_gate=f, w_up=wu.data_ptr(), ld_up=f, act=_lib.TG_GATED["silu"], h=h.data_ptr(),
+                          saved_gate=kept[0].data_ptr(), saved_up=kept[1].data_ptr(), saved_exponents=exponents.data_ptr(), g=g.data_ptr(), dx=out[0].data_ptr(),
+                          dw_gate=out[1].data_ptr(), dw_up=out[2].data_ptr(), scratch=scratch.data_ptr(), scratch_bytes=2 * half, rows=m, cols=k, inner=f)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.tg_gated_linear_fwd(ctypes.byref(args), stream) == 0 and lib.tg_gated_linear_bwd(ctypes.byref(args), stream) == 0
+    torch.cuda.synchronize()
+    for got, want, name in zip(out, ref.gated_bwd(*[t.double() for t in (x, wg, wu)], "silu", g.double()), ("dx", "dw_gate", "dw_up")):
+        _near(got, want, name)
+    assert (scratch[2 * half:] == 0x7F).all()
+
+
 def test_large_negative_gates_and_infinities():
     """silu and gelu go to 0 on the left, not to not-a-number; what is not finite stays in its row."""
     x, wg, wu, g = _make(40, 64, 64)

@@ -6,7 +6,7 @@
 //
 //     dG = g U act'(G),  dU = g act(G),    dx = dG Wg^T + dU Wu^T,    dWg = x^T dG,  dWu = x^T dU
 //
-// one pass for dG and dU and one launch for the three products.  Products are bf16 tcgen05.mma on pairs of SMs (cta_group::2) with float32
+// one pass for dG and dU, in bf16 (of small problems as the sum of two), and one launch for the three products.  Products are bf16 tcgen05.mma on pairs of SMs (cta_group::2) with float32
 // accumulators in tensor memory; no operand is transposed in memory, the descriptors carry the major-ness.  A cluster of two CTAs has a
 // tile of 256 rows and 256 accumulator columns: CTA r owns rows 128 r.. of it and loads them of A, and half of the 256 rows of B.
 //   forward   A = x, B: the first CTA loads 128 columns of Wg, the second the same of Wu.  Accumulator columns 0-127 are then G and 128-255
@@ -30,6 +30,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "cluster.cuh"
 #include "common.cuh"
@@ -94,6 +95,8 @@ struct GatedProblem {
   CUtensorMap a[2], b[2], d[2];
   int kind, tiles_m, tiles_n, blocks;           // blocks: stages of the contraction of a tile
   int half;                                     // kGbData: its first stage that reads the second operands; kGbWeights: column tiles of dWg
+  // dG and dU may have a second piece (see gated_slopes_kernel), `low` rows behind the first: stages from `piece` on read that one.
+  int piece, low;
   // The contraction may be cut into ranges: item i is tile i % tiles of range i / tiles, and its float32 sums go to `partial`, 256 KB an item,
   // in the order in which the epilogue's threads hold them (see gated_join_kernel).
   int ranges;
@@ -259,18 +262,22 @@ __device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedP
                 tma_load_2d_pair(dst + (2 + i) * kGbBox, &p.b[rank], fb, n0 + 64 * i, k0);
               }
             } else if (p.kind == kGbData) {
-              const int sel = kb >= p.half, k0 = (kb - (sel ? p.half : 0)) * kGbK, n0 = tn * 256 + int(rank) * 128;
+              const bool second = kb >= p.piece;
+              const int stage = kb - (second ? p.piece : 0), sel = stage >= p.half, k0 = (stage - (sel ? p.half : 0)) * kGbK, n0 = tn * 256 + int(rank) * 128;
+              const int a0 = m0 + (second ? p.low : 0);
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                tma_load_2d_pair(dst + i * kGbBox, &p.a[sel], fb, k0, m0 + 64 * i);
+                tma_load_2d_pair(dst + i * kGbBox, &p.a[sel], fb, k0, a0 + 64 * i);
                 tma_load_2d_pair(dst + (2 + i) * kGbBox, &p.b[sel], fb, k0, n0 + 64 * i);
               }
             } else {
-              const int sel = tn >= p.half, k0 = kb * kGbK, n0 = (tn - (sel ? p.half : 0)) * 256 + int(rank) * 128;
+              const bool second = kb >= p.piece;
+              const int sel = tn >= p.half, k0 = (kb - (second ? p.piece : 0)) * kGbK, n0 = (tn - (sel ? p.half : 0)) * 256 + int(rank) * 128;
+              const int b0 = k0 + (second ? p.low : 0);
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
                 tma_load_2d_pair(dst + i * kGbBox, &p.a[0], fb, m0 + 64 * i, k0);
-                tma_load_2d_pair(dst + (2 + i) * kGbBox, &p.b[sel], fb, n0 + 64 * i, k0);
+                tma_load_2d_pair(dst + (2 + i) * kGbBox, &p.b[sel], fb, n0 + 64 * i, b0);
               }
             }
           }
@@ -737,14 +744,21 @@ struct GatedSlopes {
   const __half *gate, *up;
   const uint16_t* exponents;
   __nv_bfloat16 *dgate, *dup;
-  int64_t rows;
+  int64_t rows, low;                            // low: rows from the first pieces to the second ones, 0 for none
   int inner, chunks;
 };
 constexpr int kGsThreads = 128, kGsRows = kGsThreads / 8, kGsUnroll = 4;
 
-// A block takes 64 columns of 32 rows at a time, eight lanes a row: a row's 128 bytes of each tensor are one request, and its
+// what is left of two values beside their bf16 (of an infinity or not-a-number nothing)
+__device__ __forceinline__ uint32_t second_piece(float2 v, uint32_t first) {
+  const float2 f = bf16x2_unpack(first);
+  return pack_bf16x2(fabsf(f.x) < INFINITY ? v.x - f.x : 0.f, fabsf(f.y) < INFINITY ? v.y - f.y : 0.f);
+}
+// A block takes 64 columns of 64 rows, eight lanes a row: a row's 128 bytes of each tensor are one request, and its
 // exponents one of a few in the same sector.
-template <int ACT>
+// TWO: dG and dU as the sum of two bf16, what the first leaves of them rounded in the second, for small problems (gated_low); rows up to the
+// second pieces are zeros, since stages of dW run on into them.
+template <int ACT, bool TWO>
 __global__ void __launch_bounds__(kGsThreads) gated_slopes_kernel(const GatedSlopes p) {
   grid_trigger();
   grid_wait();
@@ -758,8 +772,15 @@ __global__ void __launch_bounds__(kGsThreads) gated_slopes_kernel(const GatedSlo
 #pragma unroll
     for (int k = 0; k < kGsUnroll; ++k) {
       row[k] = (int64_t(group) * kGsUnroll + k) * kGsRows + r0;
-      if (col >= p.inner || row[k] >= p.rows) row[k] = -1;
+      if (col >= p.inner || row[k] >= (TWO ? p.low : p.rows)) row[k] = -1;
       if (row[k] < 0) continue;
+      if constexpr (TWO) {
+        if (row[k] >= p.rows) {
+          g[k] = a[k] = u[k] = make_uint4(0u, 0u, 0u, 0u);
+          e[k] = 0u;
+          continue;
+        }
+      }
       const int64_t at = row[k] * p.inner + col;
       g[k] = ld_stream_v4(p.g + at);
       a[k] = ld_stream_v4(p.gate + at);
@@ -770,19 +791,29 @@ __global__ void __launch_bounds__(kGsThreads) gated_slopes_kernel(const GatedSlo
     for (int k = 0; k < kGsUnroll; ++k) {
       if (row[k] < 0) continue;
       const float sa = __uint_as_float((127u + (e[k] & 255u)) << 23), su = __uint_as_float((127u + (e[k] >> 8)) << 23);
-      uint32_t og[4], ou[4];
+      uint32_t og[4], ou[4], lg[4], lu[4];
       const uint32_t *gw = &g[k].x, *aw = &a[k].x, *uw = &u[k].x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 gv = bf16x2_unpack(gw[j]);
         const float2 av = __half22float2(*reinterpret_cast<const __half2*>(&aw[j])), uv = __half22float2(*reinterpret_cast<const __half2*>(&uw[j]));
         const float2 s0 = gated_act_slope<ACT>(av.x * sa), s1 = gated_act_slope<ACT>(av.y * sa);
-        og[j] = pack_bf16x2(gv.x * (uv.x * su) * s0.y, gv.y * (uv.y * su) * s1.y);
-        ou[j] = pack_bf16x2(gv.x * s0.x, gv.y * s1.x);
+        const float2 dg = make_float2(gv.x * (uv.x * su) * s0.y, gv.y * (uv.y * su) * s1.y), du = make_float2(gv.x * s0.x, gv.y * s1.x);
+        og[j] = pack_bf16x2(dg.x, dg.y);
+        ou[j] = pack_bf16x2(du.x, du.y);
+        if constexpr (TWO) {
+          lg[j] = second_piece(dg, og[j]);
+          lu[j] = second_piece(du, ou[j]);
+        }
       }
       const int64_t at = row[k] * p.inner + col;
       *reinterpret_cast<uint4*>(p.dgate + at) = make_uint4(og[0], og[1], og[2], og[3]);
       *reinterpret_cast<uint4*>(p.dup + at) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+      if constexpr (TWO) {
+        const int64_t behind = at + p.low * p.inner;
+        *reinterpret_cast<uint4*>(p.dgate + behind) = make_uint4(lg[0], lg[1], lg[2], lg[3]);
+        *reinterpret_cast<uint4*>(p.dup + behind) = make_uint4(lu[0], lu[1], lu[2], lu[3]);
+      }
     }
   }
 }
@@ -960,6 +991,13 @@ extern "C" int tg_gated_linear_fwd(const tg_gated_args* a, void* stream) {
   return save ? run_gated_fwd<true>(a->act, p, s, a->status, st) : run_gated_fwd<false>(a->act, p, s, a->status, st);
 }
 
+// Where dG and dU have two pieces: up to so many stages of the products with one, per pair of SMs.  A single rounding to bf16 makes dx and dW the root
+// of two of a float32 gradient's error off where errors average out; small problems have few roundings that count, and 9 in 100 of them were off by more
+// than 1.5 times, up to 2.5.  With two, what is left is the results' own rounding, and the products there are short next to the launches (forward and
+// backward, us): 34 x 80 x 136 10.5 -> 13.3, 128 x 128 x 512 17.4 -> 20.7, 128 x 1024 x 1024 26.6 -> 30.6.  Past that it costs too much: at 16 stages 8 x 1024 x
+// 4096 26.5 -> 35.8, 1024 x 1024 x 1024 30.5 -> 41.
+constexpr int64_t kGatedTwoStages = 4;
+
 // Sizes of a problem as the launch sees them
 struct GatedTiles {
   int64_t tiles = 0, blocks = 0, ranges = 1;
@@ -1000,26 +1038,34 @@ static void gated_ranges(GatedTiles& data, GatedTiles& weights) {
     }
   }
 }
-static void gated_tiles(const tg_gated_args* a, GatedTiles& data, GatedTiles& weights) {
+// Rows from the first pieces of dG and dU to the second ones, 0 where one piece does: by the sizes alone, not by which gradients are asked for.
+static int64_t gated_low(const tg_gated_args* a) {
+  auto over = [](int64_t n, int64_t t) { return (n + t - 1) / t; };
+  const int64_t data = over(a->rows, 256) * over(a->cols, 256) * 2 * over(a->inner, kGbK), weights = over(a->cols, 256) * 2 * over(a->inner, 256) * over(a->rows, kGbK);
+  return data + weights <= kGatedTwoStages * (sm_count() / 2) ? over(a->rows, kGbK) * kGbK : 0;
+}
+static void gated_tiles(const tg_gated_args* a, bool two, GatedTiles& data, GatedTiles& weights) {
   auto over = [](int64_t n, int64_t t) { return (n + t - 1) / t; };
   if (a->dx != nullptr) {
     data.tiles = over(a->rows, 256) * over(a->cols, 256);
-    data.blocks = 2 * over(a->inner, kGbK);
+    data.blocks = (two ? 4 : 2) * over(a->inner, kGbK);
   }
   if (a->dw_gate != nullptr) {
     weights.tiles = over(a->cols, 256) * 2 * over(a->inner, 256);
-    weights.blocks = over(a->rows, kGbK);
+    weights.blocks = (two ? 2 : 1) * over(a->rows, kGbK);
   }
   gated_ranges(data, weights);
 }
-static int64_t gated_half_bytes(const tg_gated_args* a) { return (a->rows * a->inner * 2 + 255) / 256 * 256; }
+// of dG, and of dU
+static int64_t gated_half_bytes(const tg_gated_args* a, int64_t low) { return ((low > 0 ? 2 * low : a->rows) * a->inner * 2 + 255) / 256 * 256; }
 static int64_t gated_partial_items(const GatedTiles& t) { return t.ranges > 1 ? t.tiles * t.ranges : 0; }
 
 extern "C" int64_t tg_gated_linear_bwd_scratch_bytes(const tg_gated_args* a) {
   if (gated_check(a) != TG_OK || a->rows == 0) return 0;
   GatedTiles data, weights;
-  gated_tiles(a, data, weights);
-  return 2 * gated_half_bytes(a) + (gated_partial_items(data) + gated_partial_items(weights)) * 262144;
+  const int64_t low = gated_low(a);
+  gated_tiles(a, low > 0, data, weights);
+  return 2 * gated_half_bytes(a, low) + (gated_partial_items(data) + gated_partial_items(weights)) * 262144;
 }
 
 extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
@@ -1034,7 +1080,7 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
     return TG_OK;
   }
   const bool dx = a->dx != nullptr, dw = a->dw_gate != nullptr;
-  if (a->g == nullptr || a->saved_gate == nullptr || a->saved_up == nullptr || a->saved_exponents == nullptr || a->scratch == nullptr || a->scratch_bytes < 2 * gated_half_bytes(a) ||
+  if (a->g == nullptr || a->saved_gate == nullptr || a->saved_up == nullptr || a->saved_exponents == nullptr || a->scratch == nullptr || a->scratch_bytes < 2 * gated_half_bytes(a, 0) ||
       (dx && (a->w_gate == nullptr || a->w_up == nullptr)) || (dw && a->x == nullptr))
     return TG_ERR_SHAPE;
   if (!gated_aligned(a) || !aligned16(a->g) || !aligned16(a->saved_gate) || !aligned16(a->saved_up) || !aligned16(a->saved_exponents) || !aligned16(a->dx) ||
@@ -1043,8 +1089,10 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
   if (int rc = check_arch()) return rc;
   if (!dx && !dw) return TG_OK;
   GatedTiles data_tiles, weights_tiles;
-  gated_tiles(a, data_tiles, weights_tiles);
-  if (a->scratch_bytes < tg_gated_linear_bwd_scratch_bytes(a)) data_tiles.ranges = weights_tiles.ranges = 1;
+  const bool all = a->scratch_bytes >= tg_gated_linear_bwd_scratch_bytes(a);
+  const int64_t low = all ? gated_low(a) : 0, half_bytes = gated_half_bytes(a, low);
+  gated_tiles(a, low > 0, data_tiles, weights_tiles);
+  if (!all) data_tiles.ranges = weights_tiles.ranges = 1;
   if (weights_tiles.blocks / weights_tiles.ranges > 1 << 21) return TG_ERR_TOO_LARGE;
   GatedSlopes s = {};
   s.g = static_cast<const __nv_bfloat16*>(a->g);
@@ -1052,18 +1100,23 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
   s.up = static_cast<const __half*>(a->saved_up);
   s.exponents = reinterpret_cast<const uint16_t*>(a->saved_exponents);
   s.dgate = static_cast<__nv_bfloat16*>(a->scratch);
-  s.dup = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(a->scratch) + gated_half_bytes(a));
+  s.dup = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(a->scratch) + half_bytes);
   s.rows = M;
+  s.low = low;
   s.inner = int(F);
   s.chunks = int(gated_chunks(F));
   const int64_t items = (M + kGsRows * kGsUnroll - 1) / (kGsRows * kGsUnroll) * s.chunks;
-  auto kern = a->act == TG_GATED_SILU ? gated_slopes_kernel<TG_GATED_SILU> : a->act == TG_GATED_GELU ? gated_slopes_kernel<TG_GATED_GELU> : gated_slopes_kernel<TG_GATED_RELU>;
+  static_assert(kGsRows * kGsUnroll == kGbK, "a block's rows end where the second pieces begin");
+  auto slopes = [&](auto act) { return low > 0 ? gated_slopes_kernel<act.value, true> : gated_slopes_kernel<act.value, false>; };
+  auto kern = a->act == TG_GATED_SILU   ? slopes(std::integral_constant<int, TG_GATED_SILU>())
+              : a->act == TG_GATED_GELU ? slopes(std::integral_constant<int, TG_GATED_GELU>())
+                                        : slopes(std::integral_constant<int, TG_GATED_RELU>());
   TG_CUDA_CHECK(launch_if_short(items <= 8 * sm_count(), kern, dim3(unsigned(items)), kGsThreads, 0, st, s));
 
   GatedProblem data = {}, weights = {};
   GatedJoin joins[2] = {};
   int n_joins = 0;
-  uint8_t* partial = static_cast<uint8_t*>(a->scratch) + 2 * gated_half_bytes(a);
+  uint8_t* partial = static_cast<uint8_t*>(a->scratch) + 2 * half_bytes;
   auto cut = [&](GatedProblem& p, const GatedTiles& t, void* d0, void* d1, int64_t rows, int64_t cols) {
     p.ranges = int(t.ranges);
     if (t.ranges == 1) return;
@@ -1073,7 +1126,7 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
   };
   if (dx) {
     for (int i = 0; i < 2; ++i) {
-      if (int rc = gated_map(&data.a[i], i ? s.dup : s.dgate, false, M, F, F, 64)) return rc;
+      if (int rc = gated_map(&data.a[i], i ? s.dup : s.dgate, false, low > 0 ? 2 * low : M, F, F, 64)) return rc;
       if (int rc = gated_map(&data.b[i], i ? a->w_up : a->w_gate, false, D, F, i ? a->ld_up : a->ld_gate, 64)) return rc;
     }
     if (int rc = gated_map(&data.d[0], a->dx, false, M, D, D, 32)) return rc;
@@ -1081,20 +1134,24 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
     data.tiles_m = int((M + 255) / 256);
     data.tiles_n = int((D + 255) / 256);
     data.half = int((F + kGbK - 1) / kGbK);
-    data.blocks = 2 * data.half;
+    data.piece = 2 * data.half;
+    data.low = int(low);
+    data.blocks = int(data_tiles.blocks);
     cut(data, data_tiles, a->dx, nullptr, M, D);
   }
   if (dw) {
     if (int rc = gated_map(&weights.a[0], a->x, false, M, D, a->ldx, 64)) return rc;
     for (int i = 0; i < 2; ++i) {
-      if (int rc = gated_map(&weights.b[i], i ? s.dup : s.dgate, false, M, F, F, 64)) return rc;
+      if (int rc = gated_map(&weights.b[i], i ? s.dup : s.dgate, false, low > 0 ? 2 * low : M, F, F, 64)) return rc;
       if (int rc = gated_map(&weights.d[i], i ? a->dw_up : a->dw_gate, false, D, F, F, 32)) return rc;
     }
     weights.kind = kGbWeights;
     weights.tiles_m = int((D + 255) / 256);
     weights.half = int((F + 255) / 256);
     weights.tiles_n = 2 * weights.half;
-    weights.blocks = int((M + kGbK - 1) / kGbK);
+    weights.piece = int((M + kGbK - 1) / kGbK);
+    weights.low = int(low);
+    weights.blocks = int(weights_tiles.blocks);
     cut(weights, weights_tiles, a->dw_gate, a->dw_up, D, F);
   }
   // the longer items first
