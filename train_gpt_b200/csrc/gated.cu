@@ -18,7 +18,8 @@
 //
 // What the forward pass keeps for the backward one is G and U in 16 bits.  bf16 there would cost dx and dW half as much precision again as
 // the rounding of dG and dU (which the tensor cores need) does: fp16 has three more bits, and a power of two per 64 columns of a row
-// (a byte each, 0 but where one of them is beyond 65504) gives it bf16's range.
+// (a byte each) that puts the largest of them below 2^15 makes up for its range: half a step is 2^-11 of a value, but 2^-39 of the largest
+// of its 64 at least, so that values below 2^-28 of that one have fewer bits than 11, and what is below 2^-40 of it is kept as 0.
 //
 // Warp roles of a CTA (320 threads): 0-7 epilogue (warp w reads TMEM lanes 32 (w % 4).., half w / 4 of the columns), 8 TMA producer,
 // 9 MMA issuer (in the first CTA).  Two accumulators take turns, so a tile's epilogue runs beside the next tile's products; results leave
@@ -164,14 +165,16 @@ struct GatedCfg {
   static_assert(stages >= 4 && smem_bytes + 1024 <= kSmemLimit, "shared-memory plan");
 };
 
-// The exponent of the power of two by which a row's 64 values are scaled down to fit fp16, from the bits of the largest magnitude: 0 up to 65504,
-// else what puts it below 2^15 (infinities and NaN count as 2^128).
+// What a row's 64 values are scaled by to be kept, from the bits of the largest magnitude: the power of two that puts it into [2^14, 2^15), up or
+// down (2^126 at most, for values below 2^-112 and a row of zeros; infinities and NaN count as 2^128).  Returns the exponent field of the float
+// that undoes it.
 __device__ __forceinline__ uint32_t save_exponent(uint32_t m, float& scale) {
-  const uint32_t e = m >= 0x477fe000u ? (m >> 23) - 127u - 14u : 0u;
-  scale = __uint_as_float((127u - e) << 23);
-  return e;
+  const uint32_t e = max(m >> 23, 15u);
+  scale = __uint_as_float((268u - e) << 23);
+  return e - 14u;
 }
-// f16 of 64 accumulator values, scaled down by the power of two that keeps the largest (finite) one in range; returns its exponent
+__device__ __forceinline__ float saved_scale(uint32_t field) { return __uint_as_float(field << 23); }
+// f16 of 64 accumulator values, scaled; returns the exponent field
 __device__ __forceinline__ uint32_t save_row(const uint32_t (&v0)[32], const uint32_t (&v1)[32], uint32_t row, int lane) {
   uint32_t m = 0u;
 #pragma unroll
@@ -790,7 +793,7 @@ __global__ void __launch_bounds__(kGsThreads) gated_slopes_kernel(const GatedSlo
 #pragma unroll
     for (int k = 0; k < kGsUnroll; ++k) {
       if (row[k] < 0) continue;
-      const float sa = __uint_as_float((127u + (e[k] & 255u)) << 23), su = __uint_as_float((127u + (e[k] >> 8)) << 23);
+      const float sa = saved_scale(e[k] & 255u), su = saved_scale(e[k] >> 8);
       uint32_t og[4], ou[4], lg[4], lu[4];
       const uint32_t *gw = &g[k].x, *aw = &a[k].x, *uw = &u[k].x;
 #pragma unroll
