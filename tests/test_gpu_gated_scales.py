@@ -104,3 +104,17 @@ def test_zeros():
             dx, _, _ = _grads(x, wg, wu, act, g)
             _, dg, du = _grads(torch.zeros_like(x), wg, wu, act, g)
             assert not dx[1].any() and not dg.any() and not du.any()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("m,k,f", SIZES)
+def test_what_is_not_finite_stays_in_its_column(m, k, f, value, act):
+    x, wg, wu, g = _make(m, k, f)
+    wg, wu = wg.clone(), wu.clone()
+    wg[3, 7] = wu[5, 9] = wu[1, 66] = value
+    columns = torch.ones(f, dtype=torch.bool, device="cuda")
+    columns[[7, 9, 66]] = False
+    _check(x, wg, wu, act, g, columns)
+    dx, dg, du = _grads(x, wg, wu, act, g)
+    assert not torch.isfinite(dg[:, 9]).any() and not torch.isfinite(dg[:, 66]).any()

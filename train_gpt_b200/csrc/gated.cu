@@ -18,7 +18,7 @@
 //
 // What the forward pass keeps for the backward one is G and U in 16 bits.  bf16 there would cost dx and dW half as much precision again as
 // the rounding of dG and dU (which the tensor cores need) does: fp16 has three more bits, and a power of two per 64 columns of a row
-// (a byte each) that puts the largest of them below 2^15 makes up for its range: half a step is 2^-11 of a value, but 2^-39 of the largest
+// (a byte each) that puts the largest of them below 2^15 makes up for its range: half a step is 2^-11 of a value, but 2^-39 of the largest (finite)
 // of its 64 at least, so that values below 2^-28 of that one have fewer bits than 11, and what is below 2^-40 of it is kept as 0.
 //
 // Warp roles of a CTA (320 threads): 0-7 epilogue (warp w reads TMEM lanes 32 (w % 4).., half w / 4 of the columns), 8 TMA producer,
@@ -150,7 +150,9 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint32_t max_magnitude(uint32_t m, uint32_t bits) { return max(m, bits & 0x7fffffffu); }
+// The running maximum of magnitudes by a float's bits: without the sign, and a step of the exponent up, which takes infinities and NaN past 2^32,
+// below every finite value.
+__device__ __forceinline__ uint32_t max_magnitude(uint32_t m, uint32_t bits) { return max(m, 2u * bits + 0x01000000u); }
 
 // Sixteen bytes of this lane's staging row: chunk c of its 128 bytes, swizzled
 __device__ __forceinline__ void stage16(uint32_t row, int lane, int c, uint4 v) { sts128(row + (uint32_t(c ^ (lane & 7)) << 4), v); }
@@ -165,13 +167,12 @@ struct GatedCfg {
   static_assert(stages >= 4 && smem_bytes + 1024 <= kSmemLimit, "shared-memory plan");
 };
 
-// What a row's 64 values are scaled by to be kept, from the bits of the largest magnitude: the power of two that puts it into [2^14, 2^15), up or
-// down (2^126 at most, for values below 2^-112 and a row of zeros; infinities and NaN count as 2^128).  Returns the exponent field of the float
-// that undoes it.
+// What a row's 64 values are scaled by to be kept, from max_magnitude over them: the power of two that puts the largest finite one into [2^14, 2^15), up or
+// down (2^126 at most, for values below 2^-112 and a row of zeros).  Returns the exponent field of the float that undoes it.
 __device__ __forceinline__ uint32_t save_exponent(uint32_t m, float& scale) {
-  const uint32_t e = max(m >> 23, 15u);
-  scale = __uint_as_float((268u - e) << 23);
-  return e - 14u;
+  const uint32_t e = max(m >> 24, 16u);          // the largest's exponent field, and one
+  scale = __uint_as_float((269u - e) << 23);
+  return e - 15u;
 }
 __device__ __forceinline__ float saved_scale(uint32_t field) { return __uint_as_float(field << 23); }
 // f16 of 64 accumulator values, scaled; returns the exponent field
