@@ -118,3 +118,14 @@ def test_what_is_not_finite_stays_in_its_column(m, k, f, value, act):
     _check(x, wg, wu, act, g, columns)
     dx, dg, du = _grads(x, wg, wu, act, g)
     assert not torch.isfinite(dg[:, 9]).any() and not torch.isfinite(dg[:, 66]).any()
+
+
+@pytest.mark.parametrize("m,k,f", SIZES)
+def test_a_positive_gate_keeps_its_slope(m, k, f):
+    """relu: beside one that is 2^45 times as large, too."""
+    x, wg, wu, g = _make(m, k, f)
+    wg = wg.clone()
+    wg[:, ::64] *= 2.0 ** 45
+    _, (want, most), _ = _want(*[t.double() for t in (x, wg, wu)], "relu", g.double())
+    _, got, _ = _grads(x, wg, wu, "relu", g)
+    assert ((got.double() - want).abs() <= most).all() and float(most.norm()) <= 0.5 * float(want.norm())

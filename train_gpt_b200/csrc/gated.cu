@@ -175,7 +175,13 @@ __device__ __forceinline__ uint32_t save_exponent(uint32_t m, float& scale) {
   return e - 15u;
 }
 __device__ __forceinline__ float saved_scale(uint32_t field) { return __uint_as_float(field << 23); }
+// relu's gate (POSITIVE): what is above 0 stays so, since the slope goes by that
+template <bool POSITIVE>
+__device__ __forceinline__ float save_scaled(float v, float scale) {
+  return POSITIVE && v > 0.f ? fmaxf(v * scale, 0x1p-24f) : v * scale;
+}
 // f16 of 64 accumulator values, scaled; returns the exponent field
+template <bool POSITIVE>
 __device__ __forceinline__ uint32_t save_row(const uint32_t (&v0)[32], const uint32_t (&v1)[32], uint32_t row, int lane) {
   uint32_t m = 0u;
 #pragma unroll
@@ -189,7 +195,7 @@ __device__ __forceinline__ uint32_t save_row(const uint32_t (&v0)[32], const uin
     for (int j = 0; j < 4; ++j) {
       const int at = 8 * c + 2 * j;
       const float lo = __uint_as_float(at < 32 ? v0[at & 31] : v1[at & 31]), hi = __uint_as_float(at < 32 ? v0[(at + 1) & 31] : v1[(at + 1) & 31]);
-      o[j] = pack_f16x2(lo * scale, hi * scale);
+      o[j] = pack_f16x2(save_scaled<POSITIVE>(lo, scale), save_scaled<POSITIVE>(hi, scale));
     }
     stage16(row, lane, c, make_uint4(o[0], o[1], o[2], o[3]));
   }
@@ -394,9 +400,9 @@ __device__ __forceinline__ void gated_body(const GatedProblem& one, const GatedP
               }
               rows_free();
             };
-            const uint32_t eg = save_row(g0, g1, row, lane);
+            const uint32_t eg = save_row<ACT == TG_GATED_RELU>(g0, g1, row, lane);
             send(&saved.gate);
-            const uint32_t eu = save_row(u0, u1, row, lane);
+            const uint32_t eu = save_row<false>(u0, u1, row, lane);
             send(&saved.up);
             if (m0 + lane < saved.rows && n0 / 64 < saved.chunks)
               reinterpret_cast<uint16_t*>(saved.exponents)[int64_t(n0 / 64) * saved.rows + m0 + lane] = uint16_t(eg | eu << 8);
@@ -608,7 +614,8 @@ __device__ __forceinline__ void few_join(const GatedFew& p, uint32_t sums, uint3
         for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         float scale;
         e[which] = save_exponent(m, scale);
-        if (stores) *reinterpret_cast<uint2*>((which ? p.saved_up : p.saved_gate) + at) = make_uint2(pack_f16x2(v.x * scale, v.y * scale), pack_f16x2(v.z * scale, v.w * scale));
+        auto kept = [&](float w) { return ACT == TG_GATED_RELU && which == 0 ? save_scaled<true>(w, scale) : save_scaled<false>(w, scale); };
+        if (stores) *reinterpret_cast<uint2*>((which ? p.saved_up : p.saved_gate) + at) = make_uint2(pack_f16x2(kept(v.x), kept(v.y)), pack_f16x2(kept(v.z), kept(v.w)));
       }
       if (there && col == 0) reinterpret_cast<uint16_t*>(p.exponents)[int64_t(n0 / kGfCols) * p.rows + m0 + row] = uint16_t(e[0] | e[1] << 8);
     }
