@@ -1644,19 +1644,20 @@ Pair qk_norm_rope(const Tensor& q, const Tensor& k, const std::optional<Tensor>&
 }
 
 struct GatedLinearBackward : public Node {
-  SavedVariable x, w_gate, w_up;
-  GatedKept kept;
+  SavedVariable x, w_gate, w_up, kept_gate, kept_up, kept_exponents;      // (all of them, so that hooks on what is saved see them)
+  bool released = false;
   int act = 0;
   std::string name() const override { return "GatedLinearBackward"; }
   void release_variables() override {
-    for (SavedVariable* v : {&x, &w_gate, &w_up}) v->reset_data();
-    kept = GatedKept();
+    for (SavedVariable* v : {&x, &w_gate, &w_up, &kept_gate, &kept_up, &kept_exponents}) v->reset_data();
+    released = true;
   }
   variable_list apply(variable_list&& grads) override {
     variable_list out(3);
     if (!grads[0].defined()) return out;
-    if (!kept.gate.defined()) backward_twice();
+    if (released) backward_twice();
     const Tensor a = x.unpack(), b = w_gate.unpack(), c = w_up.unpack();
+    const GatedKept kept = {kept_gate.unpack(), kept_up.unpack(), kept_exponents.unpack()};
     {
       at::AutoDispatchBelowADInplaceOrView below;
       auto d = gated_linear_bwd(a, b, c, act, kept, to(grads[0], at::kBFloat16), task_should_compute_output(0),
@@ -1682,7 +1683,9 @@ Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, i
   node->x = SavedVariable(x, false);
   node->w_gate = SavedVariable(w_gate, false);
   node->w_up = SavedVariable(w_up, false);
-  node->kept = std::move(kept);
+  node->kept_gate = SavedVariable(kept.gate, false);
+  node->kept_up = SavedVariable(kept.up, false);
+  node->kept_exponents = SavedVariable(kept.exponents, false);
   node->act = act;
   torch::autograd::set_history(h, node);
   return h;
