@@ -294,6 +294,8 @@ class GPT:
             raise ValueError(f"unknown positions {cfg.positions!r}")
         if (cfg.positions == "rotary" or cfg.qk_norm) and (cfg.head_dim % 16 or cfg.head_dim > 512):
             raise ValueError(f"positions 'rotary' and qk_norm need a head_dim that is a multiple of 16 and at most 512, got {cfg.head_dim}")
+        if cfg.activation not in ("gelu", "relu2", *GATED):
+            raise ValueError(f"unknown activation {cfg.activation!r}")
         if not 0.0 <= cfg.dropout <= 1.0:
             raise ValueError(f"dropout={cfg.dropout} must be between 0 and 1")
         self.cfg = cfg
