@@ -7,7 +7,7 @@
 // (2 i, 2 i + 1), interleaved -- by the angle t theta^(-2 i / rotary), i < rotary / 2; elements beyond `rotary` are not rotated.  Without
 // scales there is no norm: y = R(t) x, and its backward pass is R(-t) g.  Float32 between the loads and the one rounding.  Angles are counted
 // in turns, in 64 bits until whole turns are off: float32 would lose the place of a token far into a context (position 10^6 has an error of
-// 0.06 rad in it).
+// 0.06 rad in it).  Two roundings of 2^-53 on the way to the turn and float32 behind it: an angle a is off by |a| 2^-52 + 2^-23 rad at most.
 //
 // A pass is bound by memory (4 bytes an element forward, 6 backward), so the rest is kept small: a warp takes a token; its lanes
 // work out the rotary / 2 sines and cosines once, and every head of queries and of keys uses them from registers.  A head is a group of lanes, a power of two,
@@ -527,10 +527,11 @@ static QkParams qk_params(const tg_qk_args* a, const QkGeom& g, bool backward) {
   p.eps = a->eps;
   p.sign = backward ? -1.f : 1.f;
   p.partial = static_cast<float*>(a->scratch);
-  // every eighth angle's step by a power, the ones between by products: an error of 8 2^-53 at most
-  const double step = p.rotary > 0 ? pow(a->theta, -2.0 / p.rotary) : 1.0;
-  for (int i = 0; i < p.rotary / 2; ++i)
-    p.turns[i] = i % 8 == 0 ? pow(a->theta, -2.0 * i / p.rotary) / 6.283185307179586476925 : p.turns[i - 1] * step;
+  // One power and products: in 64-bit mantissas, so that of 255 products and the step's own error less than 2^-55 is left beside the one
+  // rounding to double (powers of doubles for every eighth and products between them were off by up to 9 2^-53).
+  const long double step = p.rotary > 0 ? powl(static_cast<long double>(a->theta), -2.0L / p.rotary) : 1.0L;
+  long double turns = 1.0L / 6.283185307179586476925286766559L;
+  for (int i = 0; i < p.rotary / 2; ++i, turns *= step) p.turns[i] = double(turns);
   return p;
 }
 
