@@ -1083,9 +1083,10 @@ Pair fp8_backward(const Tensor& a, const Tensor& b, const Tensor& g_, at::IntArr
                   at::ScalarType b_dtype, int64_t k, int64_t n, const BackwardIn& in) {
   Tensor da, db;
   if (in.mode == kSte) {
-    // (the engine's thread may not have touched the device yet, and cuBLAS wants a context when it makes its handle)
+    // (the engine's thread may not have touched the device yet, and cuBLAS wants a context when it makes its handle: setting the device makes
+    // it, also under a capture, which the customary cudaFree(nullptr) ends)
     const c10::cuda::CUDAGuard guard(g_.device());
-    cudaFree(nullptr);
+    cudaSetDevice(g_.get_device());
     const Tensor g2 = to(g_.dim() == 2 ? g_ : g_.reshape({-1, n}), at::kBFloat16);
     if (in.want_a) da = at::mm(g2, to(b, at::kBFloat16).t());                                 // fp8.py:96 (cuBLAS bf16)
     if (in.want_b) db = at::mm(to(a.dim() == 2 ? a : a.reshape({-1, k}), at::kBFloat16).t(), g2);                // fp8.py:97
