@@ -109,5 +109,6 @@ def dropout(x, p: float, seed: torch.Tensor, site: int = 0, residual=None):
     x bf16 of any shape, residual None or like x; 0 <= p <= 1 (0 keeps everything); seed an int64 CUDA tensor of one element, so that a captured graph
     draws new masks when it changes; site an integer in [0, 2^32), another one for every place of a model that drops out.  The mask depends on
     an element's place in the contiguous order of x alone.  Differentiable once, in reverse mode, in x and residual: the backward
-    pass draws the mask again, so the seed must not change before it (an error)."""
+    pass draws the mask again, so the seed must not change before it (an error; a graph of one's own whose replay changes it is not noticed:
+    torch.autograd.graph.increment_version(seed) behind the replay makes it one)."""
     return ops._host().dropout(x, p, seed, site, residual)

@@ -707,6 +707,8 @@ class Trainer:
                 if kept is not None:
                     kept.copy_(new)
         self._graph.replay()
+        if self.model.dropout_seed is not None:
+            torch.autograd.graph.increment_version(self.model.dropout_seed)    # (a loss that is still alive drew its masks from the old one)
         return self._loss, self._gnorm
 
 
