@@ -20,7 +20,8 @@ q/k/v, untied head, tanh logit cap 15 and the 0.02 / 0.02/sqrt(2L) init follow m
 Beyond the reference: `block_norm="sandwich"` (a norm behind each branch too, with a gate and a scaled residual stream:
 kernels.sandwich_norm) and distillation (`GPT.top_logits` of a teacher, `Trainer.step(..., teacher=)` for its student:
 losses.capped_distillation); rotary positions and a norm per head of queries and keys (`positions="rotary"`, `qk_norm=True`:
-kernels.qk_norm_rope), a gated feed-forward (`activation="swiglu"` and its like: kernels.gated_linear, in bf16 beside FP8 linears),
+kernels.qk_norm_rope), a gated feed-forward (`activation="swiglu"` and its like: kernels.gated_linear, in bf16 beside FP8 linears; with
+`mlp="unfused"` its projections are linears like the others),
 dropout of every branch (`dropout=`: kernels.dropout).  All of them run through autograd.
 
 No per-block rematerialisation (the reference's `use_remat` trades compute for memory; 180 GB
@@ -57,7 +58,8 @@ class StepConfig:
     qk_norm: bool = False           # a norm with a learned scale on every head of queries and keys
     dropout: float = 0.0            # of every branch before the residual add, where gradients are on
     mm: str = "fp8"
-    mlp: str = "fused"              # "fused": activation and its gradient folded into the quantisers (FP8 mm only); "unfused"
+    mlp: str = "fused"              # "fused": activation and its gradient folded into the quantisers (FP8 mm only), gated: kernels.gated_linear in bf16;
+                                    # "unfused": every projection by `mm`, torch's operators between them
     norm: str = "fused"
     qkv: str = "fused"              # "fused": one dgrad GEMM contracts over the gradients of q, k and v (FP8 mm, norm "fused"); "separate"
     residual: str = "fused"         # "fused": the residual add runs inside the norm after it, its gradient fan-in inside that
@@ -352,11 +354,14 @@ class GPT:
         return [p for b in self.buckets() for p in b]
 
     def matrices(self):
-        """The parameters whose only use is an FP8 linear (model.py:63-72): wq, wk, wv, wo, w_up, w_down (not w_up where it is gated)."""
+        """The parameters whose only use is an FP8 linear (model.py:63-72): wq, wk, wv, wo, w_up, w_down, and w_gate (not w_up and w_gate where
+        they are one kernel's)."""
         return [lp[n] for lp in self.layers for n in self.linears()]
 
     def linears(self):
-        return ("wq", "wk", "wv", "wo", "w_down") if self.gated else ("wq", "wk", "wv", "wo", "w_up", "w_down")
+        if self.gated and self.cfg.mlp == "fused":
+            return ("wq", "wk", "wv", "wo", "w_down")
+        return ("wq", "wk", "wv", "wo", "w_up", "w_down") + (("w_gate",) if self.gated else ())
 
     # ---- the mm / norm seam (bench_fp8_norm.py:81-86) -------------------------------------
     def _mm(self, a, w, aq=None):
@@ -430,12 +435,13 @@ class GPT:
         y = torch.where(_keep(branch, c.dropout, self.dropout_seed, site), branch.float() * (65536 / (65536 - t) if t < 65536 else 0.0), 0.0)
         return (y if residual is None else y + residual.float()).to(branch.dtype)
 
-    def _gated(self, h, lp):
+    def _gated(self, h, lp, hq=None):
         """act(h w_gate) * (h w_up)"""
         c = self.cfg
         if c.mlp == "fused" and c.norm != "torch_reference":
             return kernels.gated_linear(h, lp["w_gate"], lp["w_up"], GATED[c.activation])
-        return {"silu": F.silu, "gelu": F.gelu, "relu": F.relu}[GATED[c.activation]](h @ lp["w_gate"]) * (h @ lp["w_up"])
+        gate, up = (h @ lp[n] if c.mlp == "fused" else self._mm(h, lp[n], hq) for n in ("w_gate", "w_up"))
+        return {"silu": F.silu, "gelu": F.gelu, "relu": F.relu}[GATED[c.activation]](gate) * up
 
     def _act(self, u):
         return F.gelu(u) if self.cfg.activation == "gelu" else F.relu(u) ** 2      # model.py:72
@@ -489,9 +495,9 @@ class GPT:
             # the attention output feeds one linear: both its quantised forms from one read when a backward pass follows
             oq = fp8.QuantizedActivation.both(o) if (c.mm == "fp8" and torch.is_grad_enabled() and o.shape[-1] % 128 == 0) else None
             branch = self._mm(o, lp["wo"], oq)
-            x, h, hq = norm_after(x, branch, lp["norm2"], want_q=not self.gated, behind=(h, lp, 1))     # model.py:68, :77
+            x, h, hq = norm_after(x, branch, lp["norm2"], want_q="w_up" in self.linears(), behind=(h, lp, 1))     # model.py:68, :77
             if self.gated:
-                a = self._gated(h, lp)
+                a = self._gated(h, lp, hq)
                 branch = self._mm(a, lp["w_down"], fp8.QuantizedActivation.both(a) if c.mm == "fp8" and torch.is_grad_enabled() and c.d_ff % 128 == 0 else None)
             elif c.mm == "fp8" and c.mlp == "fused":
                 branch = _FusedMLP.apply(h, hq, lp["w_up"], lp["w_down"], c.activation)
