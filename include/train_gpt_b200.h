@@ -256,6 +256,7 @@ int tg_sandwich_norm_bwd(const void* x_new, const void* branch, const void* post
  *   positions int32 (or int64 if positions_64) with a stride per batch and per token, or NULL: a token's place in its sequence.  An angle a (in
  *             radians, whole turns included) is off by |a| 2^-52 + 2^-23 at most; the first term is the larger beyond 2^29
  *   dim, rotary_dim multiples of 16, 16 <= dim <= 512, 0 <= rotary_dim <= dim; batch * tokens < 2^31
+ *   theta     finite, at least 1e-30 (angles by a far smaller one are not finite numbers)
  * Backward, from the gradients g_q, g_k of the outputs (strides as above): q_out and k_out receive the gradients of q and k, dq_scale and
  * dk_scale bf16 [dim] those of the scales.  Without scales q and k are not read.
  *   scratch   tg_qk_norm_rope_bwd_scratch_bytes(args) bytes, 16-byte aligned, contents undefined on entry and exit

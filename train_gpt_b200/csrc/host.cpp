@@ -401,7 +401,7 @@ void need_rope(const Tensor& q, const Tensor& k, const std::optional<Tensor>& q_
   if (d % 16 || d == 0 || d > 512) throw py::value_error(cat("dim=", d, " must be a multiple of 16 and at most 512"));
   if (rotary % 16 || rotary < 0 || rotary > d) throw py::value_error(cat("rotary_dim=", rotary, " must be a multiple of 16 between 0 and dim=", d));
   if (q.size(-2) == 0 || k.size(-2) == 0) throw py::value_error("q and k must have heads");
-  if (!(theta > 0 && theta <= 1e30)) throw py::value_error(cat("theta=", theta, " must be positive"));
+  if (!(theta >= 1e-30 && theta <= 1e30)) throw py::value_error(cat("theta=", theta, " must be between 1e-30 and 1e30"));
   if (q_scale.has_value() != k_scale.has_value()) throw py::value_error("q_scale and k_scale: both or neither");
   if (q_scale) {
     need_gamma(*q_scale, d);

@@ -500,7 +500,7 @@ static QkGeom qk_geom_bwd(const tg_qk_args* a) { return a->q_scale != nullptr ? 
 
 static bool qk_sizes_ok(const tg_qk_args* a) {
   return a->batch >= 0 && a->tokens >= 0 && a->heads >= 1 && a->kv_heads >= 1 && a->dim >= 16 && a->dim % 16 == 0 && a->rotary_dim >= 0 &&
-         a->rotary_dim % 16 == 0 && a->rotary_dim <= a->dim && a->theta > 0.0 && isfinite(a->theta) && (a->q_scale == nullptr) == (a->k_scale == nullptr);
+         a->rotary_dim % 16 == 0 && a->rotary_dim <= a->dim && a->theta >= 1e-30 && isfinite(a->theta) && (a->q_scale == nullptr) == (a->k_scale == nullptr);
 }
 static bool qk_too_large(const tg_qk_args* a) {
   return a->dim > kQkMaxDim || a->heads > 65536 || a->kv_heads > 65536 || (a->tokens > 0 && a->batch >= (int64_t(1) << 31) / a->tokens);

@@ -79,7 +79,7 @@ def qk_norm_rope(q, k, q_scale, k_scale, eps: float, positions=None, *, theta: f
     q (..., H, D), k (..., K, D) bf16 with the same leading axes, any strides (column slices of one projection and transposed tensors are
     read as they lie where heads begin at 16-byte boundaries with unit stride along D); D a multiple of 16 up to 512.  q_scale, k_scale
     (D,) bf16, or both None for the rotation without a norm.  R(t) turns the pair (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with `interleaved`,
-    by t * theta^(-2 i / rotary_dim); rotary_dim (default D, a multiple of 16, 0 for none) is the part of a head that is rotated.
+    by t * theta^(-2 i / rotary_dim), theta from 1e-30 to 1e30; rotary_dim (default D, a multiple of 16, 0 for none) is the part of a head that is rotated.
     positions int32 or int64, expandable to the leading axes: a token's t, |t| < 2^31; None: its place along the last of them.
 
     Returns (q', k'), contiguous.  Differentiable once, in reverse mode, in q, k and the scales; the backward pass keeps q and k
