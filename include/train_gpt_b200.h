@@ -296,6 +296,7 @@ int tg_qk_norm_rope_bwd(const tg_qk_args* args, void* stream);
  *             256); with tg_gated_linear_bwd_scratch_bytes(args) of them, small problems have their second pieces, and few tiles of a long
  *             contraction are cut into ranges, their float32 sums added up in order (dx, dw_gate and cols of args count: results that are not
  *             wanted are not planned for)
+ *             With fewer, rows of the weights' gradients up to 2^27 (TG_ERR_TOO_LARGE beyond)
  * Deterministic for the same scratch_bytes. */
 #define TG_GATED_SILU 0
 #define TG_GATED_GELU 1

@@ -24,3 +24,26 @@ def test_bases_whose_angles_are_no_numbers(lib, theta):
     a = QkArgs(q=4096, k=8192, q_stride=s, k_stride=s, q_out=12288, k_out=16384, batch=2, tokens=3, heads=4, kv_heads=4, dim=64, rotary_dim=64, theta=theta, g_q=20480,
                g_k=24576, g_q_stride=s, g_k_stride=s)
     assert lib.tg_qk_norm_rope_fwd(ctypes.byref(a), None) == lib.tg_qk_norm_rope_bwd(ctypes.byref(a), None) == TG_ERR_SHAPE
+
+
+def _gated(rows, scratch_bytes, **kw):
+    from train_gpt_b200._lib import GatedArgs
+    a = [4096 * (i + 1) for i in range(12)]
+    g = GatedArgs(x=a[0], ldx=8, w_gate=a[1], ld_gate=8, w_up=a[2], ld_up=8, act=0, h=a[3], saved_gate=a[4], saved_up=a[5], saved_exponents=a[6], g=a[7], dx=a[8], dw_gate=a[9],
+                  dw_up=a[10], scratch=a[11], scratch_bytes=scratch_bytes, rows=rows, cols=8, inner=8)
+    for n, v in kw.items():
+        setattr(g, n, v)
+    return ctypes.byref(g)
+
+
+def test_rows_of_the_weights_gradients_with_the_least_scratch(lib):
+    """One item's stages have a limit, 2^27 rows, that the ranges of the whole scratch keep: the refusal needs no device."""
+    from train_gpt_b200._lib import TG_ERR_ARCH, TG_ERR_CUDA, TG_ERR_TOO_LARGE
+    for rows in (2 ** 27 + 64, 2 ** 30):
+        least = 2 * rows * 16
+        assert lib.tg_gated_linear_bwd(_gated(rows, least), None) == TG_ERR_TOO_LARGE
+        assert lib.tg_gated_linear_bwd_scratch_bytes(_gated(rows, 0)) > least
+    if not torch.cuda.is_available():               # (what is not refused would be launched: without a device it fails behind the checks)
+        for rows, scratch, kw in ((2 ** 27, 2 ** 32, {}), (2 ** 30, 2 ** 35, dict(dw_gate=None, dw_up=None)),
+                                  (2 ** 30, lib.tg_gated_linear_bwd_scratch_bytes(_gated(2 ** 30, 0)), {})):
+            assert lib.tg_gated_linear_bwd(_gated(rows, scratch, **kw), None) in (TG_ERR_ARCH, TG_ERR_CUDA), (rows, kw)

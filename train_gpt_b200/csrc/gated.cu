@@ -1097,14 +1097,15 @@ extern "C" int tg_gated_linear_bwd(const tg_gated_args* a, void* stream) {
   if (!gated_aligned(a) || !aligned16(a->g) || !aligned16(a->saved_gate) || !aligned16(a->saved_up) || !aligned16(a->saved_exponents) || !aligned16(a->dx) ||
       !aligned16(a->dw_gate) || !aligned16(a->dw_up) || !aligned16(a->scratch))
     return TG_ERR_ALIGN;
-  if (int rc = check_arch()) return rc;
-  if (!dx && !dw) return TG_OK;
   GatedTiles data_tiles, weights_tiles;
   const bool all = a->scratch_bytes >= tg_gated_linear_bwd_scratch_bytes(a);
   const int64_t low = all ? gated_low(a) : 0, half_bytes = gated_half_bytes(a, low);
   gated_tiles(a, low > 0, data_tiles, weights_tiles);
   if (!all) data_tiles.ranges = weights_tiles.ranges = 1;
+  // (an item's stages stay far below what its barriers' waits are bounded by: 0.6 s here; the ranges see to that, without them rows do up to 2^27)
   if (weights_tiles.blocks / weights_tiles.ranges > 1 << 21) return TG_ERR_TOO_LARGE;
+  if (int rc = check_arch()) return rc;
+  if (!dx && !dw) return TG_OK;
   GatedSlopes s = {};
   s.g = static_cast<const __nv_bfloat16*>(a->g);
   s.gate = static_cast<const __half*>(a->saved_gate);
