@@ -47,3 +47,11 @@ def test_rows_of_the_weights_gradients_with_the_least_scratch(lib):
         for rows, scratch, kw in ((2 ** 27, 2 ** 32, {}), (2 ** 30, 2 ** 35, dict(dw_gate=None, dw_up=None)),
                                   (2 ** 30, lib.tg_gated_linear_bwd_scratch_bytes(_gated(2 ** 30, 0)), {})):
             assert lib.tg_gated_linear_bwd(_gated(rows, scratch, **kw), None) in (TG_ERR_ARCH, TG_ERR_CUDA), (rows, kw)
+
+
+@pytest.mark.parametrize("rows,cols,inner,want", [(65536, 512, 64, 63963136), (2 ** 20, 64, 64, 315621376), (2 ** 20, 1024, 64, 316669952), (2 ** 24, 64, 64, 4341628928),
+                                                  (2 ** 27, 64, 64, 34406400000), (128, 128, 512, 1048576), (32768, 1024, 4096, 536870912)])
+def test_the_plans_of_long_contractions(lib, rows, cols, inner, want):
+    """The search for the best order of two problems looks no further than where the second has been taken up whole: these are the plans that it made when it did."""
+    a = _gated(rows, 0, cols=cols, ldx=cols, inner=inner, ld_gate=inner, ld_up=inner)
+    assert lib.tg_gated_linear_bwd_scratch_bytes(a) == want

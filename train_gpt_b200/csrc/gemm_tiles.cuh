@@ -182,6 +182,7 @@ inline double two_problems_us(int64_t n1, double t1, int64_t n2, double t2, int6
       best = us;
       rounds = e;
     }
+    if (rest == 0) break;      // (more rounds than take up the whole second problem only last longer)
   }
   return double(n1 / units) * t1 + best;
 }
