@@ -527,11 +527,19 @@ static QkParams qk_params(const tg_qk_args* a, const QkGeom& g, bool backward) {
   p.eps = a->eps;
   p.sign = backward ? -1.f : 1.f;
   p.partial = static_cast<float*>(a->scratch);
-  // One power and products: in 64-bit mantissas, so that of 255 products and the step's own error less than 2^-55 is left beside the one
-  // rounding to double (powers of doubles for every eighth and products between them were off by up to 9 2^-53).
-  const long double step = p.rotary > 0 ? powl(static_cast<long double>(a->theta), -2.0L / p.rotary) : 1.0L;
-  long double turns = 1.0L / 6.283185307179586476925286766559L;
-  for (int i = 0; i < p.rotary / 2; ++i, turns *= step) p.turns[i] = double(turns);
+  // A step by a power, corrected by one of Newton's for theta step^n = 1, and products, in 64-bit mantissas: of 255 of them less than 2^-55 is left beside
+  // the one rounding to double (1.04 2^-53 in all, measured).  0.08 us for 64 turns; by powl 0.34, by powers of doubles for every eighth and products
+  // between them 0.15 and off by up to 9 2^-53.
+  const int n = p.rotary / 2;
+  if (n > 0) {
+    long double step = pow(a->theta, -1.0 / n), all = 1.0L, square = step, turns = 1.0L / 6.283185307179586476925286766559L;
+    for (int bits = n;; square *= square) {
+      if (bits & 1) all *= square;
+      if ((bits >>= 1) == 0) break;
+    }
+    step += step * (1.0L - a->theta * all) / n;
+    for (int i = 0; i < n; ++i, turns *= step) p.turns[i] = double(turns);
+  }
   return p;
 }
 
