@@ -1002,11 +1002,11 @@ extern "C" int tg_gated_linear_fwd(const tg_gated_args* a, void* stream) {
   return save ? run_gated_fwd<true>(a->act, p, s, a->status, st) : run_gated_fwd<false>(a->act, p, s, a->status, st);
 }
 
-// Where dG and dU have two pieces: up to so many stages of the products with one, per pair of SMs.  A single rounding to bf16 makes dx and dW the root
-// of two of a float32 gradient's error off where errors average out; small problems have few roundings that count, and 9 in 100 of them were off by more
-// than 1.5 times, up to 2.5.  With two, what is left is the results' own rounding, and the products there are short next to the launches (forward and
-// backward, us): 34 x 80 x 136 10.5 -> 13.3, 128 x 128 x 512 17.4 -> 20.7, 128 x 1024 x 1024 26.6 -> 30.6.  Past that it costs too much: at 16 stages 8 x 1024 x
-// 4096 26.5 -> 35.8, 1024 x 1024 x 1024 30.5 -> 41.
+// Where dG and dU have two pieces: up to so many stages of the products with one, per pair of SMs.  With one, dx and dW have that rounding's error beside their
+// own, as large in 2-norm where many terms average it (so the root of two of what a float32 form is off); where a few terms decide a result, as in small
+// problems, up to 2.5 times.  With two they have their own rounding alone, so two are taken where the products are short next to the launches (forward and
+// backward, us): 34 x 80 x 136 10.5 -> 13.3, 128 x 128 x 512 17.4 -> 20.7, 128 x 1024 x 1024 26.6 -> 30.6.  Past that it costs too much for a factor that
+// averages: at 16 stages 8 x 1024 x 4096 26.5 -> 35.8, 1024 x 1024 x 1024 30.5 -> 41.  (A pair has the stages that a B200's 74 leave it.)
 constexpr int64_t kGatedTwoStages = 4;
 
 // Sizes of a problem as the launch sees them
